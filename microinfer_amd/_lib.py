@@ -25,8 +25,8 @@ _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
 
-# (restype, argtypes) of every entry point declared in include/mi_attn.h and
-# include/mi_model.h.
+# (restype, argtypes) of every entry point declared in include/mi_attn.h,
+# include/mi_model.h and include/mi_fork.h.
 SIGNATURES = {
     "mi_last_error": (ctypes.c_char_p, []),
     "mi_abi_version": (_I32, []),
@@ -110,6 +110,17 @@ SIGNATURES = {
     "mi_rms_norm_residual": (
         _I32, [_P, _I64, _P, _I64, _P, _F32, _P, _I64, _P, _I64, _I32, _I32, _I32, _P]),
     "mi_silu_mul": (_I32, [_P, _I64, _P, _I64, _I32, _I32, _I32, _P]),
+    "mi_kv_copy_blocks": (
+        _I32,
+        [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
+         _P],
+    ),
+    "mi_token_logprobs_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
+    "mi_token_logprobs": (
+        _I32,
+        [_P, _I64, _I32, _I32, _I32, _P, _P, _I64, _I32, _P, _P, _P, _P, _I32, _P, _I64, _P,
+         _P],
+    ),
 }
 
 _lock = threading.Lock()

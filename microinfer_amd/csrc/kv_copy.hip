@@ -1,0 +1,334 @@
+// Copies of cache pages within a K/V pool, all layers in one launch: forked
+// sequences' partial pages, beams that change parents, compaction.
+//
+// A parallel assignment K[dst_i] = K'[src_i] (K' the pool before the call).
+// The pairs come from the host's block manager, so they are ordered there:
+// a pair whose destination nobody else reads is independent of the rest and
+// runs anywhere; the others form groups that one thread per 16-byte word
+// walks in an order in which every block is read before it is overwritten (a
+// chain from its end, a cycle with its first word kept in registers). Only
+// words at the same place of a page depend on each other, so no thread waits
+// for another. The lists travel in the kernel's arguments: no upload and
+// nothing to keep alive.
+//
+// Bound by memory: every row is read and written once.
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
+#include "mi_common.h"
+#include "mi_fork.h"
+
+namespace mi {
+namespace {
+
+// The rows of a page as three nested dimensions, fastest first: tokens, KV
+// heads and K/V in the order of their strides, so that neighbouring lanes
+// touch neighbouring memory in every layout.
+struct PageShape {
+  int64_t stride[3];  // bytes
+  uint32_t size[3];
+  int32_t token_dim;  // which of the three counts tokens
+  uint32_t words_per_row;
+  uint32_t words;  // words of a page, K and V
+  int64_t layer_stride, block_stride;  // bytes
+};
+
+struct CopyOp {
+  int32_t src, dst, tokens;
+};
+
+// 3.6 KB of the 4 KB that a launch's arguments may take.
+constexpr int kMaxOps = 256;
+struct CopyList {
+  CopyOp op[kMaxOps];
+};
+// Groups of dependent copies: group g is ops [start[g], start[g + 1]). dst = -1
+// keeps the source's word, src = -1 writes the kept word.
+struct GroupList {
+  CopyOp op[kMaxOps];
+  uint16_t start[kMaxOps + 1];
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 4;
+
+// Byte offset of word w inside a page, and its token row.
+__device__ __forceinline__ int64_t word_offset(const PageShape& p, uint32_t w, int word_bytes,
+                                               int* token) {
+  const uint32_t row = w / p.words_per_row;
+  const uint32_t col = w - row * p.words_per_row;
+  const uint32_t r1 = row / p.size[0];
+  const uint32_t i0 = row - r1 * p.size[0];
+  const uint32_t i2 = r1 / p.size[1];
+  const uint32_t i1 = r1 - i2 * p.size[1];
+  *token = p.token_dim == 0 ? i0 : p.token_dim == 1 ? i1 : i2;
+  return i0 * p.stride[0] + i1 * p.stride[1] + i2 * p.stride[2] +
+         static_cast<int64_t>(col) * word_bytes;
+}
+
+// One slice of one pair's page in one layer: a workgroup.
+template <typename W>
+__global__ __launch_bounds__(kCopyThreads) void kv_copy_kernel(char* base, const PageShape p,
+                                                              const CopyList list, int slices) {
+  const int pair = blockIdx.x / slices;
+  const int slice = blockIdx.x - pair * slices;
+  const CopyOp op = list.op[pair];
+  char* layer = base + blockIdx.y * p.layer_stride;
+  const char* from = layer + op.src * p.block_stride;
+  char* to = layer + op.dst * p.block_stride;
+  W v[kCopyUnroll];
+  int64_t off[kCopyUnroll];
+  bool there[kCopyUnroll];
+#pragma unroll
+  for (int u = 0; u < kCopyUnroll; ++u) {
+    const uint32_t w = (slice * kCopyUnroll + u) * kCopyThreads + threadIdx.x;
+    int token;
+    off[u] = word_offset(p, w, sizeof(W), &token);
+    there[u] = w < p.words && token < op.tokens;
+    if (there[u]) v[u] = *reinterpret_cast<const W*>(from + off[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kCopyUnroll; ++u)
+    if (there[u]) *reinterpret_cast<W*>(to + off[u]) = v[u];
+}
+
+// Dependent copies: a thread per word of the page walks its group's ops.
+template <typename W>
+__global__ __launch_bounds__(kCopyThreads) void kv_copy_group_kernel(char* base,
+                                                                    const PageShape p,
+                                                                    const GroupList list,
+                                                                    int slices) {
+  const int group = blockIdx.x / slices;
+  const uint32_t w = (blockIdx.x - group * slices) * kCopyThreads + threadIdx.x;
+  if (w >= p.words) return;
+  int token;
+  char* at = base + blockIdx.y * p.layer_stride + word_offset(p, w, sizeof(W), &token);
+  W kept{};
+  for (int i = list.start[group]; i < list.start[group + 1]; ++i) {
+    const CopyOp op = list.op[i];
+    if (token >= op.tokens) continue;
+    W v = kept;
+    if (op.src >= 0) v = *reinterpret_cast<const W*>(at + op.src * p.block_stride);
+    if (op.dst >= 0)
+      *reinterpret_cast<W*>(at + op.dst * p.block_stride) = v;
+    else
+      kept = v;
+  }
+}
+
+// The pairs in launch order: independent ones, and groups of dependent ones.
+struct Order {
+  std::vector<CopyOp> single;
+  std::vector<std::vector<CopyOp>> groups;  // in order; a cycle's ops are its last
+  std::vector<size_t> whole_from;           // per group: ops from here on share a launch
+};
+
+// Orders `ops` (distinct destinations, src != dst); into[b] is 1 + the index of
+// the op that writes block b, 0 if none does.
+void order_pairs(const std::vector<CopyOp>& ops, const std::vector<int32_t>& into, Order* out) {
+  const int n = static_cast<int>(ops.size());
+  // readers[i]: how many ops still to run read the block that op i writes.
+  std::vector<int32_t> readers(n, 0), group(n);
+  for (int i = 0; i < n; ++i) group[i] = i;
+  auto root = [&](int i) {
+    while (group[i] != i) i = group[i] = group[group[i]];
+    return i;
+  };
+  for (int i = 0; i < n; ++i) {
+    const int writer = into[ops[i].src] - 1;
+    if (writer < 0) continue;
+    ++readers[writer];
+    group[root(i)] = root(writer);
+  }
+  std::vector<int32_t> members(n, 0), place(n, -1);
+  for (int i = 0; i < n; ++i) ++members[root(i)];
+  auto put = [&](const CopyOp& op, int i) {
+    const int r = root(i);
+    if (place[r] < 0) {
+      place[r] = static_cast<int32_t>(out->groups.size());
+      out->groups.emplace_back();
+      out->whole_from.push_back(SIZE_MAX);
+    }
+    out->groups[place[r]].push_back(op);
+  };
+  std::vector<int32_t> ready;
+  std::vector<char> done(n, 0);
+  for (int i = 0; i < n; ++i)
+    if (readers[i] == 0) ready.push_back(i);
+  for (size_t at = 0; at < ready.size(); ++at) {
+    const int i = ready[at];
+    done[i] = 1;
+    if (members[root(i)] == 1)
+      out->single.push_back(ops[i]);
+    else
+      put(ops[i], i);
+    const int writer = into[ops[i].src] - 1;
+    if (writer >= 0 && --readers[writer] == 0) ready.push_back(writer);
+  }
+  // What is left are cycles, whose other readers have run: keep the block
+  // that op i writes, copy into it from behind until its reader is reached.
+  for (int i = 0; i < n; ++i) {
+    if (done[i]) continue;
+    put(CopyOp{ops[i].dst, -1, INT32_MAX}, i);
+    out->whole_from[place[root(i)]] = out->groups[place[root(i)]].size() - 1;
+    for (int j = i; !done[j]; j = into[ops[j].src] - 1) {
+      done[j] = 1;
+      CopyOp op = ops[j];
+      if (op.src == ops[i].dst) op.src = -1;
+      put(op, j);
+    }
+  }
+}
+
+template <typename W>
+int32_t launch_copies(char* base, const PageShape& shape, int32_t layers, const Order& order,
+                      hipStream_t stream) {
+  PageShape p = shape;
+  const uint32_t row_words = p.words_per_row / sizeof(W);  // words_per_row holds bytes here
+  p.words_per_row = row_words;
+  p.words = row_words * p.size[0] * p.size[1] * p.size[2];
+  const int per = kCopyThreads * kCopyUnroll;
+  const int slices = static_cast<int>((p.words + per - 1) / per);
+  for (size_t i = 0; i < order.single.size(); i += kMaxOps) {
+    const int n = static_cast<int>(std::min<size_t>(kMaxOps, order.single.size() - i));
+    CopyList list;
+    std::copy_n(order.single.begin() + i, n, list.op);
+    kv_copy_kernel<W><<<dim3(n * slices, layers), kCopyThreads, 0, stream>>>(base, p, list,
+                                                                           slices);
+    const int32_t status = check_launch("mi_kv_copy_blocks");
+    if (status != MI_OK) return status;
+  }
+  const int thin = static_cast<int>((p.words + kCopyThreads - 1) / kCopyThreads);
+  GroupList list;
+  int ops = 0, groups = 0;
+  auto flush = [&]() {
+    if (ops == 0) return static_cast<int32_t>(MI_OK);
+    if (list.start[groups] != ops) list.start[++groups] = static_cast<uint16_t>(ops);
+    kv_copy_group_kernel<W><<<dim3(groups * thin, layers), kCopyThreads, 0, stream>>>(base, p,
+                                                                                    list, thin);
+    ops = groups = 0;
+    return check_launch("mi_kv_copy_blocks");
+  };
+  list.start[0] = 0;
+  for (size_t g = 0; g < order.groups.size(); ++g) {
+    const std::vector<CopyOp>& all = order.groups[g];
+    for (size_t i = 0; i < all.size();) {
+      // A cycle goes whole; other ops one by one, in order over the launches.
+      const size_t take = i == order.whole_from[g] ? all.size() - i : 1;
+      if (ops + take > static_cast<size_t>(kMaxOps)) {
+        const int32_t status = flush();
+        if (status != MI_OK) return status;
+      }
+      for (size_t k = 0; k < take; ++k) list.op[ops++] = all[i++];
+    }
+    list.start[++groups] = static_cast<uint16_t>(ops);
+  }
+  return flush();
+}
+
+int32_t copy_blocks(char* keys, char* values, int64_t layer_stride, int64_t block_stride,
+                    int64_t token_stride, int64_t head_stride, const int32_t* src,
+                    const int32_t* dst, const int32_t* tokens, int32_t num_pairs,
+                    int32_t num_layers, int32_t num_kv_heads, int32_t row_bytes,
+                    int32_t block_size, int32_t num_blocks, hipStream_t stream) {
+  std::vector<CopyOp> ops;
+  ops.reserve(num_pairs);
+  std::vector<int32_t> into(num_blocks, 0);
+  std::vector<char> written(num_blocks, 0);
+  for (int32_t i = 0; i < num_pairs; ++i) {
+    const int32_t n = tokens == nullptr ? block_size : tokens[i];
+    if (src[i] < 0 || src[i] >= num_blocks || dst[i] < 0 || dst[i] >= num_blocks)
+      return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: block id outside the pool");
+    if (n < 0 || n > block_size)
+      return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: tokens outside the block");
+    if (written[dst[i]])
+      return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: a block is written twice");
+    written[dst[i]] = 1;
+    if (n == 0 || src[i] == dst[i]) continue;
+    ops.push_back(CopyOp{src[i], dst[i], n});
+    into[dst[i]] = static_cast<int32_t>(ops.size());
+  }
+  if (ops.empty()) return MI_OK;
+  Order order;
+  bool free_order = true;
+  for (const CopyOp& op : ops) free_order = free_order && into[op.src] == 0;
+  if (free_order)
+    order.single.swap(ops);
+  else
+    order_pairs(ops, into, &order);
+  for (size_t g = 0; g < order.groups.size(); ++g)
+    if (order.whole_from[g] != SIZE_MAX &&
+        order.groups[g].size() - order.whole_from[g] > static_cast<size_t>(kMaxOps))
+      return fail(MI_ERR_UNSUPPORTED, "mi_kv_copy_blocks: a cycle of more than 255 blocks");
+
+  // Tokens, KV heads and K/V by their stride.
+  struct Dim {
+    int64_t stride;
+    uint32_t size;
+    bool token;
+  } dims[3] = {{token_stride, static_cast<uint32_t>(block_size), true},
+               {head_stride, static_cast<uint32_t>(num_kv_heads), false},
+               {values - keys, 2, false}};
+  std::stable_sort(dims, dims + 3, [](const Dim& a, const Dim& b) {
+    return std::abs(a.stride) < std::abs(b.stride);
+  });
+  PageShape p;
+  p.token_dim = 0;
+  for (int i = 0; i < 3; ++i) {
+    p.stride[i] = dims[i].stride;
+    p.size[i] = dims[i].size;
+    if (dims[i].token) p.token_dim = i;
+  }
+  p.words_per_row = row_bytes;
+  p.layer_stride = layer_stride;
+  p.block_stride = block_stride;
+  const uint64_t bits = static_cast<uint64_t>(row_bytes) | layer_stride | block_stride |
+                        token_stride | head_stride | reinterpret_cast<uintptr_t>(keys) |
+                        reinterpret_cast<uintptr_t>(values);
+  if ((bits & 15u) == 0) return launch_copies<uint4>(keys, p, num_layers, order, stream);
+  if ((bits & 3u) == 0) return launch_copies<uint32_t>(keys, p, num_layers, order, stream);
+  return launch_copies<uint16_t>(keys, p, num_layers, order, stream);
+}
+
+}  // namespace
+}  // namespace mi
+
+extern "C" int32_t mi_kv_copy_blocks(void* key_cache, void* value_cache, int64_t layer_stride,
+                                     int64_t block_stride, int64_t token_stride,
+                                     int64_t head_stride, const int32_t* src,
+                                     const int32_t* dst, const int32_t* tokens,
+                                     int32_t num_pairs, int32_t num_layers,
+                                     int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t block_size, int32_t num_blocks, int32_t dtype,
+                                     void* stream) {
+  using namespace mi;
+  clear_error();
+  if (!valid_dtype(dtype)) return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: bad dtype");
+  if (num_pairs < 0 || num_layers <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      block_size <= 0 || num_blocks <= 0)
+    return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: invalid sizes");
+  if (layer_stride < 0 || block_stride < 0 || token_stride < 0 || head_stride < 0)
+    return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: negative stride");
+  const int64_t es = static_cast<int64_t>(dtype_size(dtype));
+  // Word indexes and the launch's grid stay within 32 bits.
+  if (static_cast<int64_t>(num_kv_heads) * block_size > (int64_t(1) << 24) ||
+      head_dim > (1 << 14) ||
+      2 * es * head_dim * num_kv_heads * block_size > (int64_t(1) << 28) || num_layers > 65535)
+    return fail(MI_ERR_UNSUPPORTED, "mi_kv_copy_blocks: page or layer count too large");
+  if (num_pairs == 0) return MI_OK;
+  if (!key_cache || !value_cache || !src || !dst)
+    return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: null pointer");
+  if (reinterpret_cast<uintptr_t>(key_cache) % es || reinterpret_cast<uintptr_t>(value_cache) % es)
+    return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: misaligned pointer");
+  try {
+    return copy_blocks(static_cast<char*>(key_cache), static_cast<char*>(value_cache),
+                       layer_stride * es, block_stride * es, token_stride * es, head_stride * es,
+                       src, dst, tokens, num_pairs, num_layers, num_kv_heads,
+                       static_cast<int32_t>(head_dim * es), block_size, num_blocks,
+                       static_cast<hipStream_t>(stream));
+  } catch (const std::bad_alloc&) {
+    return fail(MI_ERR_HIP, "mi_kv_copy_blocks: out of host memory");
+  }
+}

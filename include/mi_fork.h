@@ -46,6 +46,51 @@ int32_t mi_kv_copy_blocks(void* key_cache, void* value_cache, int64_t layer_stri
                           int32_t dtype, void* stream);
 
 /*
+ * Decode attention of sequences that share their first blocks: the result of
+ * mi_paged_decode with the same tables and lengths (up to rounding), with the
+ * blocks that a group of sequences shares read once for all of it.
+ *
+ * Group g is the sequences [group_starts[g], group_starts[g + 1]) (rising;
+ * sequences outside every group are on their own), whose tables hold the same
+ * ids in their first shared_blocks[g] columns; only whole blocks within every
+ * one of the group's contexts count (the rest of shared_blocks[g] is not
+ * taken as shared). A group of one shares nothing. Groups that break these
+ * rules give wrong attention, never an access out of bounds.
+ *
+ * mi_shared_decode_plan makes a step's plan on the device from int32 device
+ * arrays (context_lens [num_seqs], group_starts [num_groups + 1],
+ * shared_blocks [num_groups]); mi_shared_decode runs a layer with it, so one
+ * plan serves all layers of a step. A negative or too large block id is
+ * masked; sequences of context 0 give zeros. Both are capture-safe.
+ *
+ * plan: mi_shared_decode_plan_bytes() bytes, 32-byte aligned; workspace:
+ * mi_shared_decode_workspace_bytes() bytes, 16-byte aligned, no
+ * initialisation, its own for calls that may run concurrently. Both sizes
+ * depend on their arguments only. bf16/f16, head_dim 128, at most 16 query
+ * heads per KV head, block_size >= 16 and a power of two, at most 4096
+ * sequences (MI_ERR_UNSUPPORTED otherwise: mi_paged_decode takes those).
+ * query and the caches 16-byte aligned, with strides of whole 16-byte vectors.
+ */
+int64_t mi_shared_decode_plan_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads);
+int64_t mi_shared_decode_workspace_bytes(int32_t num_seqs, int32_t num_q_heads,
+                                         int32_t num_kv_heads);
+int32_t mi_shared_decode_plan(const int32_t* context_lens, int32_t num_seqs,
+                              const int32_t* group_starts, const int32_t* shared_blocks,
+                              int32_t num_groups, int32_t num_q_heads, int32_t num_kv_heads,
+                              int32_t head_dim, int32_t block_size, int32_t block_table_width,
+                              int32_t dtype, void* plan, int64_t plan_bytes, void* stream);
+int32_t mi_shared_decode(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* key_cache, const void* value_cache,
+                         int64_t cache_block_stride, int64_t cache_token_stride,
+                         int64_t cache_head_stride, const int32_t* block_tables,
+                         int64_t block_table_stride, int32_t block_table_width,
+                         const void* plan, int64_t plan_bytes, void* out,
+                         int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                         int64_t workspace_bytes, int32_t num_seqs, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         int32_t num_blocks, float scale, int32_t dtype, void* stream);
+
+/*
  * Log probabilities of given tokens, the entropy and the best alternatives of
  * each row of logits, in one launch. With x = logits[r] / temperatures[r] (1
  * where temperatures is NULL) and p = softmax(x), in float32:

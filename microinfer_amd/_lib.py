@@ -115,6 +115,17 @@ SIGNATURES = {
         [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
          _P],
     ),
+    "mi_shared_decode_plan_bytes": (_I64, [_I32, _I32, _I32]),
+    "mi_shared_decode_workspace_bytes": (_I64, [_I32, _I32, _I32]),
+    "mi_shared_decode_plan": (
+        _I32,
+        [_P, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P],
+    ),
+    "mi_shared_decode": (
+        _I32,
+        [_P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I32, _P, _I64, _P, _I64, _I64, _P,
+         _I64, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P],
+    ),
     "mi_token_logprobs_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
     "mi_token_logprobs": (
         _I32,

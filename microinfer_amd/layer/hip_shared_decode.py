@@ -1,0 +1,150 @@
+"""Paged decode of sequences that share their first pages, on the HIP library.
+
+``hip_shared_decode`` is ``hip_paged_decode`` for continuations of common
+prompts (forks of a request, a system prompt): the pages that a group of
+sequences shares are read once for the whole group instead of once for each
+of its sequences. Groups are consecutive sequences of the batch;
+``shared_decode_plan`` lays out a step's work on the device from the lengths
+and groups, and every layer of the step uses that plan.
+
+16-bit caches with head_dim 128, up to 16 query heads per KV head and blocks
+of at least 16 have a kernel of their own; every other shape that
+``hip_paged_decode`` takes runs on it, with the same result.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from microinfer_amd import _lib
+from microinfer_amd.layer.hip_paged_attention import (_check_caches, _index32,
+                                                      _inner_contiguous, _is_pow2, decode_plan,
+                                                      hip_paged_decode)
+
+MAX_SEQS = 4096
+
+
+@dataclass(frozen=True)
+class SharedDecodePlan:
+    """One step's work (``shared_decode_plan``), for calls of its sizes."""
+
+    buffer: torch.Tensor
+    shared: bool  # False: a ``decode_plan`` for ``hip_paged_decode``
+    sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
+
+
+def supported_shared_decode(num_q_heads: int, num_kv_heads: int, head_dim: int,
+                            dtype: torch.dtype, block_size: int, num_seqs: int) -> bool:
+    """Whether sequences of this shape read shared pages once."""
+    return (dtype in (torch.float16, torch.bfloat16) and head_dim == 128
+            and num_q_heads <= 16 * num_kv_heads and block_size >= 16
+            and 0 < num_seqs <= MAX_SEQS)
+
+
+def shared_decode_plan(context_lens: torch.Tensor, group_starts: torch.Tensor,
+                       shared_blocks: torch.Tensor, *, num_q_heads: int, num_kv_heads: int,
+                       head_dim: int, dtype: torch.dtype, block_size: int,
+                       block_table_width: int) -> SharedDecodePlan:
+    """The plan of one decode step, from device tensors alone (capture-safe).
+
+    Group g is the sequences ``group_starts[g] : group_starts[g + 1]``; the
+    first ``shared_blocks[g]`` columns of their block tables are equal. Shared
+    blocks that are not whole in every context of the group are read by each
+    sequence for itself, as are those of a group of one and of sequences
+    outside every group.
+    """
+    _lib.require_device(context_lens, group_starts, shared_blocks, what="shared_decode_plan")
+    if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
+        raise ValueError("Hq must be divisible by Hkv")
+    if not _is_pow2(block_size):
+        raise ValueError("paged kernels require a power-of-two block size")
+    if context_lens.ndim != 1 or group_starts.ndim != 1 or shared_blocks.ndim != 1:
+        raise ValueError("context_lens, group_starts and shared_blocks must be 1-D")
+    groups = shared_blocks.numel()
+    if group_starts.numel() != groups + 1 and (groups or group_starts.numel()):
+        raise ValueError("group_starts must have one entry more than shared_blocks")
+    if any(t.device != context_lens.device for t in (group_starts, shared_blocks)):
+        raise ValueError("context_lens, group_starts and shared_blocks must share a device")
+    num_seqs = context_lens.numel()
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size,
+             block_table_width)
+    if not supported_shared_decode(num_q_heads, num_kv_heads, head_dim, dtype, block_size,
+                                   num_seqs):
+        heads = None
+        if num_q_heads > 16 * num_kv_heads or head_dim != 128 or dtype == torch.float32 \
+                or block_size < 16:
+            heads = (num_q_heads, head_dim, dtype)
+        return SharedDecodePlan(
+            decode_plan(context_lens, num_kv_heads=num_kv_heads, block_size=block_size,
+                        block_table_width=block_table_width, heads=heads), False, sizes)
+    context_lens, group_starts, shared_blocks = (
+        _index32(t) for t in (context_lens, group_starts, shared_blocks))
+    lib = _lib.load()
+    with torch.cuda.device(context_lens.device):
+        nbytes = lib.mi_shared_decode_plan_bytes(num_seqs, num_q_heads, num_kv_heads)
+        buffer = torch.empty(nbytes, dtype=torch.uint8, device=context_lens.device)
+        status = lib.mi_shared_decode_plan(
+            context_lens.data_ptr(), num_seqs, group_starts.data_ptr(), shared_blocks.data_ptr(),
+            groups, num_q_heads, num_kv_heads, head_dim, block_size, block_table_width,
+            _lib.dtype_code(dtype), buffer.data_ptr(), nbytes,
+            _lib.stream_handle(context_lens.device))
+    _lib.check(status, "mi_shared_decode_plan")
+    return SharedDecodePlan(buffer, True, sizes)
+
+
+def hip_shared_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                      block_tables: torch.Tensor, context_lens: torch.Tensor, *,
+                      plan: SharedDecodePlan, scale: float | None = None) -> torch.Tensor:
+    """Decode one query row per sequence; ``hip_paged_decode``'s arguments and
+    result, with ``plan`` from ``shared_decode_plan`` for these lengths.
+
+    The caches hold the step's K/V rows already. Without a plan there are no
+    groups to share pages in: call ``hip_paged_decode``.
+    """
+    if query.ndim != 3:
+        raise ValueError("query must have shape [requests, Hq, D]")
+    if key_cache.ndim != 4:
+        raise ValueError("key_cache must have shape [blocks, B, Hkv, D]")
+    num_seqs, num_q_heads, head_dim = query.shape
+    num_blocks, block_size, num_kv_heads, kv_dim = key_cache.shape
+    if kv_dim != head_dim:
+        raise ValueError("query and cache head dimensions differ")
+    if query.device != key_cache.device or query.dtype != key_cache.dtype:
+        raise ValueError("query and cache must share device/dtype")
+    if block_tables.ndim != 2 or block_tables.shape[0] != num_seqs:
+        raise ValueError("block_tables must have one row per request")
+    if context_lens.numel() != num_seqs:
+        raise ValueError("context_lens must have one entry per request")
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, query.dtype, block_size,
+             block_tables.shape[1])
+    if not isinstance(plan, SharedDecodePlan) or plan.sizes != sizes:
+        raise ValueError("plan must come from shared_decode_plan() for this call's sizes")
+    _lib.require_device(query, block_tables, context_lens, what="hip_shared_decode")
+    if plan.buffer.device != query.device or block_tables.device != query.device:
+        raise ValueError("plan and block_tables must be on the query's device")
+    key_cache, value_cache = _check_caches(key_cache, value_cache)
+    query = _inner_contiguous(query)
+    if not plan.shared:
+        return hip_paged_decode(query, key_cache, value_cache, block_tables, context_lens,
+                                scale=scale, plan=plan.buffer if num_seqs else None)
+    block_tables = _index32(block_tables)
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    lib = _lib.load()
+    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    with torch.cuda.device(query.device):
+        ws_bytes = lib.mi_shared_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads)
+        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device)
+        status = lib.mi_shared_decode(
+            query.data_ptr(), query.stride(0), query.stride(1), key_cache.data_ptr(),
+            value_cache.data_ptr(), *key_cache.stride()[:3], block_tables.data_ptr(),
+            block_tables.stride(0), block_tables.shape[1], plan.buffer.data_ptr(),
+            plan.buffer.numel(), out.data_ptr(), out.stride(0), out.stride(1),
+            workspace.data_ptr(), ws_bytes, num_seqs, num_q_heads, num_kv_heads, head_dim,
+            block_size, num_blocks, float(scale), _lib.dtype_code(query.dtype),
+            _lib.stream_handle(query.device))
+    _lib.check(status, "mi_shared_decode")
+    return out

@@ -1,0 +1,283 @@
+"""Decode over shared pages (mi_shared_decode via layer.hip_shared_decode)
+against float64 attention over each sequence's own table.
+
+Tolerance: the weights p round to the cache's type before the product with V,
+off by at most half a step h = eps / 2 each, and their sum adds the rounded
+ones, which moves an output by at most h * sum p |v - out| / sum p <= h (A +
+|out|) with A = sum p |v| / sum p; the output rounds once more, h |out|. The
+scores are float32 sums of 128 products, a few 2^-24 of values up to some tens,
+which move a weight by less than 2^-15 of itself.
+"""
+
+import math
+import random
+
+import pytest
+import torch
+
+from microinfer_amd.layer.hip_paged_attention import hip_paged_decode
+from microinfer_amd.layer.hip_shared_decode import (SharedDecodePlan, hip_shared_decode,
+                                                    shared_decode_plan)
+from microinfer_amd.runner import capture_graph
+from microinfer_amd.worker.kv_cache import KVCache
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+
+
+def _ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def _assert_close(out, q, keys, values, tables, contexts, scale):
+    """``out`` against float64 attention, rows of invalid blocks left out."""
+    half = torch.finfo(q.dtype).eps / 2
+    blocks, block, hkv, dim = keys.shape
+    share = q.shape[1] // hkv
+    assert out.shape == q.shape and out.dtype == q.dtype
+    for s, c in enumerate(contexts):
+        ids = tables[s, : -(-c // block)].long()
+        there = ((ids >= 0) & (ids < blocks)).repeat_interleave(block)[:c]
+        ids = ids.clamp(0, blocks - 1)
+        k = keys[ids].flatten(0, 1)[:c][there].double().transpose(0, 1).contiguous()
+        v = values[ids].flatten(0, 1)[:c][there].double().transpose(0, 1).contiguous()
+        if k.shape[1] == 0:
+            assert not out[s].any()
+            continue
+        p = torch.softmax(torch.matmul(q[s].double().view(hkv, share, dim),
+                                       k.transpose(1, 2).contiguous()) * scale, -1)
+        want = torch.matmul(p, v).view(-1, dim)
+        size = torch.matmul(p, v.abs()).view(-1, dim)
+        tol = half * (size + 2 * want.abs()) + 2.0 ** -15 * size
+        err = (out[s].double() - want).abs()
+        assert (err <= tol).all(), f"sequence {s}: {(err / tol).max()} times the tolerance"
+
+
+class Batch:
+    """Random tables whose groups share their first pages."""
+
+    def __init__(self, groups, *, hq=16, hkv=8, dim=128, block=16, dtype=torch.bfloat16,
+                 layout="paired", seed=0, extra=2, width_extra=0):
+        rng = random.Random(seed)
+        self.block = block
+        self.contexts, self.starts, self.shared, rows = [], [0], [], []
+        pages = sum(shared + sum(-(-c // block) for c in ctx) for shared, ctx in groups) + extra
+        ids = rng.sample(range(pages), pages)
+        for shared, ctx in groups:
+            head = [ids.pop() for _ in range(shared)]
+            for c in ctx:
+                need = -(-c // block)
+                rows.append((head + [ids.pop() for _ in range(max(0, need - shared))])
+                            [:max(need, shared)])
+            self.contexts += ctx
+            self.starts.append(len(self.contexts))
+            self.shared.append(shared)
+        width = max(max(map(len, rows)), 1) + width_extra
+        self.tables = _ints([r + [-1] * (width - len(r)) for r in rows])
+        cache = KVCache(1, pages, block, hkv, dim, dtype=dtype, device=DEV, layout=layout)
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        cache.keys.copy_(torch.randn(cache.keys.shape, generator=gen, device=DEV))
+        cache.values.copy_(torch.randn(cache.values.shape, generator=gen, device=DEV))
+        self.keys, self.values = cache.keys[0], cache.values[0]
+        self.q = torch.randn(len(rows), hq, dim, generator=gen, device=DEV).to(dtype)
+
+    def plan(self, starts=None, shared=None, contexts=None):
+        return shared_decode_plan(
+            _ints(self.contexts) if contexts is None else contexts,
+            _ints(self.starts if starts is None else starts),
+            _ints(self.shared if shared is None else shared), num_q_heads=self.q.shape[1],
+            num_kv_heads=self.keys.shape[2], head_dim=self.q.shape[2], dtype=self.q.dtype,
+            block_size=self.block, block_table_width=self.tables.shape[1])
+
+    def run(self, plan=None, scale=None):
+        return hip_shared_decode(self.q, self.keys, self.values, self.tables,
+                                 _ints(self.contexts), plan=plan or self.plan(), scale=scale)
+
+    def check(self, plan=None, scale=None):
+        out = self.run(plan, scale)
+        scale = self.q.shape[2] ** -0.5 if scale is None else scale
+        _assert_close(out, self.q, self.keys, self.values, self.tables, self.contexts, scale)
+        return out
+
+
+def _tails(prefix, n, most, seed):
+    rng = random.Random(seed)
+    return [prefix + rng.randint(1, most) for _ in range(n)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv", [(16, 8), (32, 8), (8, 8), (12, 4), (64, 4), (40, 8), (2, 1)])
+def test_groups_of_every_size(dtype, hq, hkv):
+    groups = [(37, _tails(592, 4, 50, 1)), (2, _tails(32, 1, 100, 2)),
+              (70, _tails(1120, 21, 90, 3)), (1, _tails(16, 2, 20, 4)),
+              (0, _tails(0, 3, 700, 5)), (9, _tails(144, 70, 33, 6))]
+    Batch(groups, hq=hq, hkv=hkv, dtype=dtype, seed=hq + hkv).check()
+
+
+@pytest.mark.parametrize("block", [16, 32, 256])
+@pytest.mark.parametrize("layout", ["paired", "head_major", "token_major"])
+def test_block_sizes_and_layouts(block, layout):
+    groups = [(5, _tails(5 * block, 6, 3 * block, 1)), (1, _tails(block, 3, 5, 2))]
+    Batch(groups, block=block, layout=layout, seed=block, width_extra=3).check()
+
+
+def test_a_long_prefix_and_many_sequences():
+    Batch([(500, _tails(8000, 16, 300, 1))], hq=32).check()
+    Batch([(40, _tails(640, 3, 9, s)) for s in range(150)], hq=8, seed=3).check()
+    Batch([(2, _tails(32, 1000, 3, 9))], hkv=1, hq=2, seed=4).check()
+
+
+def test_contexts_at_the_ends_of_pages():
+    # Nothing behind the shared pages, one position behind, one position in all.
+    Batch([(4, [64, 64, 65, 80]), (1, [16, 16]), (0, [1, 1, 2])]).check()
+
+
+def test_shared_pages_that_do_not_fit_every_context():
+    # 10 columns agree, but one sequence ends inside the third page: two count.
+    batch = Batch([(10, [400, 45, 161, 160]), (3, [48, 0, 50])])
+    out = batch.check()
+    assert not out[5].any()  # no position: zeros
+    same = batch.check(batch.plan(shared=[2, 0]))
+    assert torch.equal(out, same)
+    # Fewer columns than agree, negative and none.
+    batch.check(batch.plan(shared=[1, -5]))
+    batch.check(batch.plan(shared=[0, 2 ** 30]))
+
+
+def test_sequences_outside_every_group():
+    batch = Batch([(6, _tails(96, 5, 40, 1)), (8, _tails(128, 4, 40, 2))])
+    batch.check(batch.plan(starts=[5, 9], shared=[8]))
+    batch.check(batch.plan(starts=[1, 4], shared=[6]))
+    batch.check(batch.plan(starts=[0], shared=[]))
+    batch.check(batch.plan(starts=[], shared=[]))
+    batch.check(batch.plan(starts=[0, 5, 5, 5, 900], shared=[6, 3, 3, 8]))
+
+
+def test_invalid_blocks_are_masked_and_stale_rows_never_read():
+    batch = Batch([(6, _tails(96, 5, 40, 1)), (2, [40, 40, 33])], extra=3)
+    used = {b for row, c in zip(batch.tables.tolist(), batch.contexts)
+            for b in row[: -(-c // batch.block)]}
+    spare = next(b for b in range(batch.keys.shape[0]) if b not in used)
+    for pool in (batch.keys, batch.values):
+        pool[spare] = math.nan
+        for row, c in zip(batch.tables.tolist(), batch.contexts):
+            if c % batch.block:  # rows behind the last position
+                pool[row[c // batch.block], c % batch.block:] = math.nan
+    batch.tables[:5, 2] = -1                 # inside the shared pages
+    batch.tables[1, 6] = batch.keys.shape[0]  # a whole page of one sequence's own
+    batch.tables[5:, :] = -1                 # nothing left at all
+    batch.check()
+
+
+def test_large_scores_and_scale():
+    batch = Batch([(20, _tails(320, 9, 60, 1))])
+    batch.q *= 20
+    batch.check(scale=0.11)
+    batch.check(scale=0.0)
+
+
+def test_strided_queries_and_tables():
+    batch = Batch([(20, _tails(320, 9, 60, 1))])
+    wide = torch.randn(9, 40, 128, device=DEV).to(torch.bfloat16)
+    batch.q = wide[:, 4:20]
+    wide_tables = torch.full((9, batch.tables.shape[1] + 5), -1, dtype=torch.int32, device=DEV)
+    wide_tables[:, :-5] = batch.tables
+    batch.tables = wide_tables[:, : batch.tables.shape[1]]
+    batch.check()
+
+
+def test_offsets_past_32_bits():
+    batch = Batch([(3, [50, 60, 49])])
+    pool = KVCache(1, 2 * 65536, 16, 8, 128, dtype=torch.bfloat16, device=DEV)  # 8 GiB
+    shift = pool.num_blocks - batch.keys.shape[0]
+    pool.keys[0, shift:] = batch.keys
+    pool.values[0, shift:] = batch.values
+    want = batch.run()
+    batch.keys, batch.values = pool.keys[0], pool.values[0]
+    batch.tables = torch.where(batch.tables >= 0, batch.tables + shift, batch.tables)
+    assert torch.equal(batch.run(), want)
+
+
+def test_repeatable_and_on_another_stream():
+    batch = Batch([(60, _tails(960, 12, 200, 1))])
+    first = batch.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = batch.run()
+    torch.cuda.synchronize()
+    assert torch.equal(first, again) and torch.equal(first, batch.run())
+
+
+def test_captured_steps_follow_the_lengths_and_groups():
+    batch = Batch([(20, _tails(320, 4, 100, 1)), (4, _tails(64, 4, 100, 2))])
+    contexts, starts, shared = (_ints(x) for x in (batch.contexts, batch.starts, batch.shared))
+    sizes = dict(num_q_heads=16, num_kv_heads=8, head_dim=128, dtype=torch.bfloat16,
+                 block_size=16, block_table_width=batch.tables.shape[1])
+
+    def step():
+        plan = shared_decode_plan(contexts, starts, shared, **sizes)
+        return hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables, contexts,
+                                 plan=plan)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with capture_graph(graph, stream=side):
+        out = step()
+    most = list(batch.contexts)
+    for replay, (groups, pages) in enumerate([([0, 4, 8], [20, 4]), ([0, 3, 8], [20, 0]),
+                                              ([4, 8, 8], [3, 1]), ([0, 4, 8], [20, 4])]):
+        batch.contexts = [c - 7 * replay for c in most]
+        contexts.copy_(_ints(batch.contexts))
+        starts.copy_(_ints(groups))
+        shared.copy_(_ints(pages))
+        eager = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        _assert_close(out, batch.q, batch.keys, batch.values, batch.tables, batch.contexts,
+                      128 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,dim,block,hq,hkv", [
+    (torch.float32, 128, 16, 4, 2), (torch.bfloat16, 64, 16, 4, 2), (torch.float16, 128, 8, 4, 2),
+])
+def test_other_shapes_take_the_ordinary_kernels(dtype, dim, block, hq, hkv):
+    batch = Batch([(6, _tails(6 * block, 5, 40, 1))], dtype=dtype, dim=dim, block=block, hq=hq,
+                  hkv=hkv)
+    plan = batch.plan()
+    assert not plan.shared
+    want = hip_paged_decode(batch.q, batch.keys, batch.values, batch.tables,
+                            _ints(batch.contexts))
+    assert torch.equal(batch.run(plan), want)
+
+
+def test_no_sequences():
+    batch = Batch([(3, [50, 60])])
+    plan = shared_decode_plan(_ints([]), _ints([0]), _ints([]), num_q_heads=16, num_kv_heads=8,
+                              head_dim=128, dtype=torch.bfloat16, block_size=16,
+                              block_table_width=4)
+    out = hip_shared_decode(batch.q[:0], batch.keys, batch.values, batch.tables[:0, :4],
+                            _ints([]), plan=plan)
+    assert out.shape == (0, 16, 128)
+
+
+def test_refusals():
+    batch = Batch([(3, [50, 60])])
+    plan = batch.plan()
+    for bad in (None, plan.buffer, SharedDecodePlan(plan.buffer, True, ())):
+        with pytest.raises(ValueError, match="plan"):
+            hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables,
+                              _ints(batch.contexts), plan=bad)
+    with pytest.raises(ValueError, match="plan"):
+        hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables[:, :-1],
+                          _ints(batch.contexts), plan=plan)
+    with pytest.raises(ValueError, match="one entry"):
+        batch.plan(starts=[0, 1, 2])
+    with pytest.raises(ValueError, match="entry per request"):
+        hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables, _ints([1]), plan=plan)

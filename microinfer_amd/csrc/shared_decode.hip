@@ -63,20 +63,27 @@ struct SharedMfma<F16> {
 constexpr int kD = 128;         // head_dim
 constexpr int kTile = 16;       // positions per tile
 constexpr int kMaxRows = 64;    // query rows of an item
+constexpr int kFewRows = 16;    // up to here the waves split the positions, not the rows
 constexpr int kMaxGroup = 16;   // query heads per KV head
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kSlots = 4;       // ring slots of a wave
 constexpr int kRowBytes = kD * 2;
-constexpr int kHalfBytes = kTile * kRowBytes;
-constexpr int kSlotBytes = 2 * kHalfBytes;  // K then V of a tile
+constexpr int kHalfBytes = kTile * kRowBytes;  // K (or V) of a tile
+constexpr int kTileBytes = 2 * kHalfBytes;     // K then V
 constexpr int kLoadBytes = kWave * 16;
 constexpr int kLoadsPerHalf = kHalfBytes / kLoadBytes;
 constexpr int kLoadsPerTile = 2 * kLoadsPerHalf;
+// 64 KiB of tiles in flight per workgroup, two workgroups per CU.
+constexpr int kRingBytes = 64 * 1024;
+constexpr int kSlots = kRingBytes / (kWaves * kTileBytes);  // few rows: slots per wave
+constexpr int kStageTiles = 2;                              // many rows: tiles per stage
+constexpr int kStageBytes = kStageTiles * kTileBytes;
+constexpr int kStages = kRingBytes / kStageBytes;
 constexpr int kAccStride = kD + 4;  // floats: rows of a wave's sums, 4 banks apart
-constexpr int kRegionBytes = std::max(kSlots * kSlotBytes, kMaxRows * kAccStride * 4);
 constexpr int kRescaleSlack = 15;
-static_assert((kSlots - 1) * kLoadsPerTile <= 63, "vmcnt immediate");
+static_assert(kSlots == 2 && kStages == 4, "the waits count these");
+static_assert(kFewRows * kAccStride * 4 <= kSlots * kTileBytes, "a wave's sums fit its slots");
+static_assert(kStageTiles * 2 == kWaves, "a stage is one half-tile per wave");
 
 // A piece of work, for every KV head: the rows of sequences [seq, seq + seqs)
 // over positions [begin, end) of sequence seq's table. Its row r is partial
@@ -299,218 +306,252 @@ struct SharedArgs {
 __device__ __forceinline__ int swz_k(int r) { return r & 15; }
 __device__ __forceinline__ int swz_v(int r) { return 2 * (r & 7); }
 
-// One item with up to 16 MT query rows. Wave w takes tiles w, w + kWaves, ...
-// of the positions, all rows of each, so a K/V row is read by one wave only.
-template <typename E, int MT>
-__device__ __forceinline__ void run_item(const SharedArgs& a, const SharedItem& it, int kv_head,
-                                         char* s_ring, float (*s_m)[kMaxRows],
-                                         float (*s_l)[kMaxRows]) {
+struct Lds {
+  __attribute__((aligned(16))) char ring[kRingBytes];
+  __attribute__((aligned(16))) char q[kFewRows * kRowBytes];
+  float m[kWaves][kFewRows], l[kWaves][kFewRows];
+};
+
+// What the loops below share: the lane's place in the MFMA tiles, its offsets
+// in the direct loads of a half-tile (load u puts lane i's 16 bytes at LDS row
+// 4 u + i / 16), and the block table.
+template <typename E>
+struct ItemLoop {
+  using R = uint16_t;
   using M = SharedMfma<E>;
   using vec8 = typename M::vec8;
-  using R = uint16_t;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
-  const int tid = threadIdx.x;
-  const int lane = tid % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int G = a.group;
-  const int rows = it.seqs * G;
-  const int col = lane % 16;   // MFMA column: query row of a 16-row tile
-  const int quad = lane / 16;  // MFMA row group: positions 4 quad .. + 3
-  const int lb = a.lb;
+  const SharedArgs& a;
+  const SharedItem& it;
+  const int kv_head, lane, wave, col, quad, rows;
+  const ConstI32* table;
+  const R* kc;
+  const R* vc;
+
+  __device__ __forceinline__ ItemLoop(const SharedArgs& args, const SharedItem& item, int head)
+      : a(args), it(item), kv_head(head), lane(threadIdx.x % kWave),
+        wave(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave)), col(lane % 16),
+        quad(lane / 16), rows(item.seqs * args.group),
+        table((const ConstI32*)(args.tables + item.seq * args.t_stride)),
+        kc(static_cast<const R*>(args.kc) + head * args.c_hs),
+        vc(static_cast<const R*>(args.vc) + head * args.c_hs) {}
+
+  // Byte offset of load u of a half-tile, swizzled as K (or V) rows are.
+  __device__ __forceinline__ uint32_t load_offset(int u, bool v) const {
+    const int row = 4 * u + lane / 16;
+    const int swz = v ? swz_v(row) : swz_k(row);
+    return static_cast<uint32_t>((row * static_cast<int>(a.c_ts) + ((lane % 16) ^ swz) * 8) * 2);
+  }
+  // Element offset of the tile at position p in the caches; an invalid block
+  // id reads block 0 (and is masked).
+  __device__ __forceinline__ int64_t tile_base(int p, bool* ok) const {
+    const int blk = table[p >> a.lb];
+    *ok = blk >= 0 && blk < a.num_blocks;
+    return *ok ? static_cast<int64_t>(blk) * a.c_bs +
+                     static_cast<int64_t>(p & (a.block_size - 1)) * a.c_ts
+               : 0;
+  }
+  // Query row r (clamped to the item's) of this KV head.
+  __device__ __forceinline__ const R* query_row(int r) const {
+    r = min(r, rows - 1);
+    const int i = r / a.group;
+    return static_cast<const R*>(a.q) + (it.seq + i) * a.q_ts +
+           (kv_head * a.group + (r - i * a.group)) * a.q_hs;
+  }
+  // Query fragments (B operand): dims 32 ks + 8 quad .. + 7 of row `col` of a
+  // 16-row LDS tile laid out as K rows are; K fragments (A operand) alike.
+  __device__ __forceinline__ void row_fragments(const char* tile, vec8 (&f)[kD / 32]) const {
+#pragma unroll
+    for (int ks = 0; ks < kD / 32; ++ks) {
+      const int chunk = (4 * ks + quad) ^ swz_k(col);
+      f[ks] = __builtin_bit_cast(
+          vec8, *reinterpret_cast<const Pack<R, 8>*>(tile + col * kRowBytes + chunk * 16));
+    }
+  }
+  // V^T fragments: dim 16 db + col of positions 4 quad .. + 3.
+  __device__ __forceinline__ void v_fragments(const char* tile, short4_t (&f)[kD / 16]) const {
+    const int row = 4 * quad + col / 4;
+    const char* base = tile + row * kRowBytes + 8 * (col & 1);
+#pragma unroll
+    for (int db = 0; db < kD / 16; ++db) {
+      const int chunk = (2 * db + ((col % 4) >> 1)) ^ swz_v(row);
+      f[db] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) short4_t*)(base + chunk * 16));
+    }
+  }
+};
+
+// The running softmax of one query row per lane (shared by the lanes of equal
+// `col`), with the row's sums over 128 dims in o.
+struct RowState {
+  f32x4_t o[kD / 16];
+  float m = -INFINITY, l = 0.f;
+  __device__ __forceinline__ RowState() {
+#pragma unroll
+    for (int db = 0; db < kD / 16; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // Moves the maximum when some row's new scores exceed its by 2^15.
+  __device__ __forceinline__ void see(float tmax, int lane) {
+    tmax = fmaxf(tmax, lane_xor16(tmax, lane));
+    tmax = fmaxf(tmax, lane_xor32(tmax, lane));
+    if (__ballot(tmax > m + kRescaleSlack) == 0) return;
+    const float mnew = fmaxf(m, tmax);
+    const float alpha = mnew == -INFINITY ? 1.f : fast_exp2(m - mnew);
+    l *= alpha;
+#pragma unroll
+    for (int db = 0; db < kD / 16; ++db) o[db] *= alpha;
+    m = mnew;
+  }
+  // The weight of a score, rounded to the cache's type for the product with
+  // V; the sum adds the rounded weight.
+  template <typename E>
+  __device__ __forceinline__ uint16_t weigh(float score) {
+    const uint16_t p = SharedMfma<E>::round(fast_exp2(score - (m == -INFINITY ? 0.f : m)));
+    l += E::load(p);
+    return p;
+  }
+  __device__ __forceinline__ void close(int lane) {
+    l += lane_xor16(l, lane);
+    l += lane_xor32(l, lane);
+  }
+};
+
+// Up to 16 query rows: wave w takes tiles w, w + kWaves, ... of the positions,
+// staged in two slots of its own, and the waves' sums are joined through LDS.
+template <typename E>
+__device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedItem& it,
+                                             int kv_head, Lds& s) {
+  using Loop = ItemLoop<E>;
+  using M = SharedMfma<E>;
+  using R = uint16_t;
+  const Loop x(a, it, kv_head);
+  const int lane = x.lane, wave = x.wave, col = x.col, quad = x.quad;
   const int ntiles = (it.end - it.begin + kTile - 1) / kTile;
-  const ConstI32* table = (const ConstI32*)(a.tables + it.seq * a.t_stride);
-  const R* kc = static_cast<const R*>(a.kc) + kv_head * a.c_hs;
-  const R* vc = static_cast<const R*>(a.vc) + kv_head * a.c_hs;
-  const int c_ts = static_cast<int>(a.c_ts);
   uint32_t off_k[kLoadsPerHalf], off_v[kLoadsPerHalf];
 #pragma unroll
   for (int u = 0; u < kLoadsPerHalf; ++u) {
-    const int row = 4 * u + lane / 16;
-    off_k[u] = static_cast<uint32_t>((row * c_ts + ((lane % 16) ^ swz_k(row)) * 8) * 2);
-    off_v[u] = static_cast<uint32_t>((row * c_ts + ((lane % 16) ^ swz_v(row)) * 8) * 2);
+    off_k[u] = x.load_offset(u, false);
+    off_v[u] = x.load_offset(u, true);
   }
-  char* ring = s_ring + wave * kRegionBytes;
-
-  // Issues tile k's loads into ring slot `slot`; false for an invalid block id
-  // (block 0 is read and masked).
+  char* ring = s.ring + wave * kSlots * kTileBytes;
   auto issue = [&](int slot, int k) -> bool {
-    const int p0 = it.begin + k * kTile;
-    const int blk = table[p0 >> lb];
-    const bool ok = blk >= 0 && blk < a.num_blocks;
-    const int64_t base = ok ? static_cast<int64_t>(blk) * a.c_bs +
-                                  static_cast<int64_t>(p0 & (a.block_size - 1)) * a.c_ts
-                            : 0;
-    char* dst = ring + slot * kSlotBytes;
+    bool ok;
+    const int64_t base = x.tile_base(it.begin + k * kTile, &ok);
+    char* dst = ring + slot * kTileBytes;
 #pragma unroll
     for (int u = 0; u < kLoadsPerHalf; ++u) {
-      lds_load16_sbase(kc + base, off_k[u], dst + u * kLoadBytes);
-      lds_load16_sbase(vc + base, off_v[u], dst + kHalfBytes + u * kLoadBytes);
+      lds_load16_sbase(x.kc + base, off_k[u], dst + u * kLoadBytes);
+      lds_load16_sbase(x.vc + base, off_v[u], dst + kHalfBytes + u * kLoadBytes);
     }
     return ok;
   };
-
-  f32x4_t o[MT][kD / 16];
-  float m[MT], l[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-#pragma unroll
-    for (int db = 0; db < kD / 16; ++db) o[t][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    m[t] = -INFINITY;
-    l[t] = 0.f;
+  {
+    // A quarter of the query rows each.
+    const int r = 4 * wave + lane / 16;
+    lds_load16(x.query_row(r) + ((lane % 16) ^ swz_k(r)) * 8, s.q + wave * kLoadBytes);
   }
-  bool ok_slot[kSlots];
-#pragma unroll
-  for (int j = 0; j < kSlots; ++j) ok_slot[j] = false;
+  bool ok0 = false, ok1 = false;  // of the slots
+  int issued = 0;
   if (wave < ntiles) {
-    ok_slot[0] = issue(0, wave);
-    // Query fragments (B operand): dims 32 ks + 8 quad .. + 7 of row 16 t + col.
-    vec8 qf[MT][kD / 32];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const int r = 16 * t + col;
-      const int i = r / G;
-      const R* qrow = static_cast<const R*>(a.q) + (it.seq + i) * a.q_ts +
-                      (kv_head * G + (r - i * G)) * a.q_hs;
-#pragma unroll
-      for (int ks = 0; ks < kD / 32; ++ks) {
-        Pack<R, 8> p = zero_pack<R, 8>();
-        if (r < rows) p = load_pack<R, 8>(qrow + ks * 32 + quad * 8);
-        qf[t][ks] = __builtin_bit_cast(vec8, p);
-      }
-    }
-    // All in flight is waited for once, so that the loop's waits are its own.
+    ok0 = issue(0, wave);
+    ++issued;
+  }
+  if (wave + kWaves < ntiles) {
+    ok1 = issue(1, wave + kWaves);
+    ++issued;
+  }
+  if (issued == 2)
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerTile));
+  else if (issued == 1)
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerTile));
+  else
     __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-#pragma unroll
-    for (int j = 1; j < kSlots; ++j)
-      if (wave + j * kWaves < ntiles) ok_slot[j] = issue(j, wave + j * kWaves);
-    int k = wave, slot = 0;
-    while (true) {
-      const int younger = min(kSlots - 1, (ntiles - 1 - k) / kWaves);
-      if (younger == 0)
-        __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-      else if (younger == 1)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  RowState row;
+  if (wave < ntiles) {
+    typename M::vec8 qf[kD / 32];
+    x.row_fragments(s.q, qf);
+    int slot = 0;
+    for (int k = wave;; k += kWaves) {
+      if (k + kWaves < ntiles)
         __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerTile));
-      else if (younger == 2)
-        __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerTile));
       else
-        __builtin_amdgcn_s_waitcnt(vmcnt_only(3 * kLoadsPerTile));
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      char* cur = ring + slot * kSlotBytes;
-      bool ok = ok_slot[0];
-#pragma unroll
-      for (int j = 1; j < kSlots; ++j)
-        if (slot == j) ok = ok_slot[j];
+        __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      asm volatile("" ::: "memory");
+      char* cur = ring + slot * kTileBytes;
+      const bool ok = slot ? ok1 : ok0;
       const int p0 = it.begin + k * kTile;
       if (!ok || p0 + kTile > it.end) {
         // Masked rows may hold anything, and 0 * NaN is NaN: zero their V.
         const int r = lane / 4;
         if (!ok || p0 + r >= it.end) {
-          char* row = cur + kHalfBytes + r * kRowBytes + (lane % 4) * 64;
+          char* v = cur + kHalfBytes + r * kRowBytes + (lane % 4) * 64;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<Pack<uint32_t, 4>*>(row + c * 16) = zero_pack<uint32_t, 4>();
+            *reinterpret_cast<Pack<uint32_t, 4>*>(v + c * 16) = zero_pack<uint32_t, 4>();
         }
       }
-      vec8 kf[kD / 32];
-#pragma unroll
-      for (int ks = 0; ks < kD / 32; ++ks) {
-        const int chunk = (4 * ks + quad) ^ swz_k(col);
-        kf[ks] = __builtin_bit_cast(
-            vec8, *reinterpret_cast<const Pack<R, 8>*>(cur + col * kRowBytes + chunk * 16));
-      }
+      typename M::vec8 kf[kD / 32];
+      x.row_fragments(cur, kf);
       short4_t vf[kD / 16];
-      {
-        const int vrow = 4 * quad + col / 4;
-        const char* vbase = cur + kHalfBytes + vrow * kRowBytes + 8 * (col & 1);
+      x.v_fragments(cur + kHalfBytes, vf);
+      f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int db = 0; db < kD / 16; ++db) {
-          const int chunk = (2 * db + ((col % 4) >> 1)) ^ swz_v(vrow);
-          vf[db] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) short4_t*)(vbase + chunk * 16));
-        }
+      for (int ks = 0; ks < kD / 32; ++ks) sc = M::qk(kf[ks], qf[ks], sc);
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[i] = ok && p0 + 4 * quad + i < it.end ? sc[i] * a.scale_log2 : -INFINITY;
+        tmax = fmaxf(tmax, sc[i]);
       }
+      row.see(tmax, lane);
+      Pack<R, 4> pk;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 4; ++i) pk.v[i] = row.template weigh<E>(sc[i]);
+      const short4_t pf = __builtin_bit_cast(short4_t, pk);
 #pragma unroll
-        for (int ks = 0; ks < kD / 32; ++ks) s = M::qk(kf[ks], qf[t][ks], s);
-        float sc[4];
-        float tmax = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[i] = ok && p0 + 4 * quad + i < it.end ? s[i] * a.scale_log2 : -INFINITY;
-          tmax = fmaxf(tmax, sc[i]);
-        }
-        tmax = fmaxf(tmax, lane_xor16(tmax, lane));
-        tmax = fmaxf(tmax, lane_xor32(tmax, lane));
-        if (__ballot(tmax > m[t] + kRescaleSlack) != 0) {
-          const float mnew = fmaxf(m[t], tmax);
-          const float alpha = mnew == -INFINITY ? 1.f : fast_exp2(m[t] - mnew);
-          l[t] *= alpha;
-#pragma unroll
-          for (int db = 0; db < kD / 16; ++db) o[t][db] *= alpha;
-          m[t] = mnew;
-        }
-        const float neg_m = m[t] == -INFINITY ? 0.f : -m[t];
-        // The weights round to the cache's type for the product; their sum
-        // adds the rounded values.
-        Pack<R, 4> pk;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pk.v[i] = M::round(fast_exp2(sc[i] + neg_m));
-          l[t] += E::load(pk.v[i]);
-        }
-        const short4_t pf = __builtin_bit_cast(short4_t, pk);
-#pragma unroll
-        for (int db = 0; db < kD / 16; ++db) o[t][db] = M::pv(vf[db], pf, o[t][db]);
-      }
+      for (int db = 0; db < kD / 16; ++db) row.o[db] = M::pv(vf[db], pf, row.o[db]);
       if (k + kWaves >= ntiles) break;
       if (k + kSlots * kWaves < ntiles) {
         // This slot's fragment reads have returned; refill it.
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        asm volatile("" ::: "memory");
         const bool next = issue(slot, k + kSlots * kWaves);
-#pragma unroll
-        for (int j = 0; j < kSlots; ++j)
-          if (slot == j) ok_slot[j] = next;
+        if (slot) ok1 = next; else ok0 = next;
       }
-      k += kWaves;
-      slot = slot + 1 == kSlots ? 0 : slot + 1;
+      slot ^= 1;
     }
   }
-  // No load is in flight and this wave's fragments are read: its region takes
-  // its sums.
+  // No load of this wave is in flight and its fragments are read: its slots
+  // take its sums.
   __builtin_amdgcn_s_waitcnt(0x0070);
-  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  asm volatile("" ::: "memory");
+  row.close(lane);
   float* acc = reinterpret_cast<float*>(ring);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    l[t] += lane_xor16(l[t], lane);
-    l[t] += lane_xor32(l[t], lane);
-    const int r = 16 * t + col;
-#pragma unroll
-    for (int db = 0; db < kD / 16; ++db)
-      *reinterpret_cast<f32x4_t*>(acc + r * kAccStride + db * 16 + 4 * quad) = o[t][db];
-    if (quad == 0) {
-      s_m[wave][r] = m[t];
-      s_l[wave][r] = l[t];
-    }
+  for (int db = 0; db < kD / 16; ++db)
+    *reinterpret_cast<f32x4_t*>(acc + col * kAccStride + db * 16 + 4 * quad) = row.o[db];
+  if (quad == 0) {
+    s.m[wave][col] = row.m;
+    s.l[wave][col] = row.l;
   }
   __syncthreads();
-  const int d = tid % kD;
-  for (int r = tid / kD; r < rows; r += kThreads / kD) {
+  const int d = threadIdx.x % kD;
+  for (int r = threadIdx.x / kD; r < x.rows; r += kThreads / kD) {
     float mx = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s_m[w][r]);
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s.m[w][r]);
     float ls = 0.f, os = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float mw = s_m[w][r];
+      const float mw = s.m[w][r];
       const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
-      ls = fmaf(f, s_l[w][r], ls);
+      ls = fmaf(f, s.l[w][r], ls);
       os = fmaf(f,
-                reinterpret_cast<const float*>(s_ring + w * kRegionBytes)[r * kAccStride + d], os);
+                reinterpret_cast<const float*>(s.ring + w * kSlots * kTileBytes)
+                    [r * kAccStride + d], os);
     }
     const int64_t at = static_cast<int64_t>(it.first_row + r) * a.num_kv_heads + kv_head;
     a.ws_acc[at * kD + d] = os;
@@ -521,11 +562,154 @@ __device__ __forceinline__ void run_item(const SharedArgs& a, const SharedItem& 
   }
 }
 
+// More query rows: the workgroup walks the positions in stages of 32 that all
+// its waves load and read, and wave w has rows 16 w .. 16 w + 15 of each.
 template <typename E>
-__global__ __launch_bounds__(kThreads) void shared_decode_kernel(const SharedArgs a) {
-  __shared__ __attribute__((aligned(16))) char s_ring[kWaves * kRegionBytes];
-  __shared__ float s_m[kWaves][kMaxRows];
-  __shared__ float s_l[kWaves][kMaxRows];
+__device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedItem& it,
+                                              int kv_head, Lds& s) {
+  using Loop = ItemLoop<E>;
+  using M = SharedMfma<E>;
+  using vec8 = typename M::vec8;
+  using R = uint16_t;
+  const Loop x(a, it, kv_head);
+  const int lane = x.lane, wave = x.wave, quad = x.quad;
+  const int nstages = (it.end - it.begin + kStageTiles * kTile - 1) / (kStageTiles * kTile);
+  const int last = it.end - 1;
+  // Wave w loads K (even w) or V (odd) of tile w / 2.
+  const bool loads_v = wave & 1;
+  const R* half = loads_v ? x.vc : x.kc;
+  uint32_t off[kLoadsPerHalf];
+#pragma unroll
+  for (int u = 0; u < kLoadsPerHalf; ++u) off[u] = x.load_offset(u, loads_v);
+  // Issues this wave's part of stage k; which of its tiles are valid.
+  auto issue = [&](int k) -> int {
+    const int p = it.begin + k * kStageTiles * kTile;
+    bool ok[kStageTiles];
+    int64_t base[kStageTiles];
+#pragma unroll
+    for (int j = 0; j < kStageTiles; ++j)  // a tile past the end: any valid position
+      base[j] = x.tile_base(min(p + j * kTile, last & ~(kTile - 1)), &ok[j]);
+    const int64_t mine = wave / 2 ? base[1] : base[0];
+    char* dst = s.ring + (k % kStages) * kStageBytes + wave * kHalfBytes;
+#pragma unroll
+    for (int u = 0; u < kLoadsPerHalf; ++u)
+      lds_load16_sbase(half + mine, off[u], dst + u * kLoadBytes);
+    return (ok[0] ? 1 : 0) | (ok[1] ? 2 : 0);
+  };
+  // The wave's own query rows wait in the last stage's buffer, which is filled
+  // when the first stage is read.
+  char* q_tile = s.ring + (kStages - 1) * kStageBytes + wave * kHalfBytes;
+#pragma unroll
+  for (int u = 0; u < kLoadsPerHalf; ++u) {
+    const int r = 4 * u + lane / 16;
+    lds_load16(x.query_row(16 * wave + r) + ((lane % 16) ^ swz_k(r)) * 8,
+               q_tile + u * kLoadBytes);
+  }
+  int ok[kStages] = {0, 0, 0, 0};
+  ok[0] = issue(0);
+  if (nstages > 1) ok[1] = issue(1);
+  if (nstages > 2) ok[2] = issue(2);
+  if (nstages > 2)
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(3 * kLoadsPerHalf));
+  else if (nstages > 1)
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerHalf));
+  else
+    __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerHalf));
+  asm volatile("" ::: "memory");
+  vec8 qf[kD / 32];
+  x.row_fragments(q_tile, qf);
+  const bool active = 16 * wave < x.rows;
+  RowState row;
+  for (int k = 0; k < nstages; ++k) {
+    // Stage k's loads of this wave are done, its earlier reads too; behind the
+    // barrier those of every wave are.
+    const int younger = min(2, nstages - 1 - k);
+    if (younger == 0)
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+    else if (younger == 1)
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerHalf));
+    else
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerHalf));
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int now = ok[0];
+    ok[0] = ok[1];
+    ok[1] = ok[2];
+    if (k + 3 < nstages) ok[2] = issue(k + 3);
+    if (!active) continue;
+    const char* stage = s.ring + (k % kStages) * kStageBytes;
+    const int p0 = it.begin + k * kStageTiles * kTile;
+    f32x4_t sc[kStageTiles];
+    short4_t vf[kStageTiles][kD / 16];
+#pragma unroll
+    for (int j = 0; j < kStageTiles; ++j) {
+      vec8 kf[kD / 32];
+      x.row_fragments(stage + j * kTileBytes, kf);
+      x.v_fragments(stage + j * kTileBytes + kHalfBytes, vf[j]);
+      sc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < kD / 32; ++ks) sc[j] = M::qk(kf[ks], qf[ks], sc[j]);
+    }
+    float tmax = -INFINITY;
+    if (now == 3 && p0 + kStageTiles * kTile <= it.end) {
+#pragma unroll
+      for (int j = 0; j < kStageTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[j][i] *= a.scale_log2;
+          tmax = fmaxf(tmax, sc[j][i]);
+        }
+    } else {
+      // Masked positions: no score, and zeros for whatever their V rows hold
+      // (0 * NaN is NaN).
+#pragma unroll
+      for (int j = 0; j < kStageTiles; ++j) {
+        short4_t keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = (now >> j & 1) && p0 + j * kTile + 4 * quad + i < it.end;
+          sc[j][i] = in ? sc[j][i] * a.scale_log2 : -INFINITY;
+          tmax = fmaxf(tmax, sc[j][i]);
+          keep[i] = in ? -1 : 0;
+        }
+#pragma unroll
+        for (int db = 0; db < kD / 16; ++db) vf[j][db] &= keep;
+      }
+    }
+    row.see(tmax, lane);
+    // The contraction runs over k = 8 quad + 4 j + i: position 4 quad + i of
+    // tile j, for the weights as for V.
+    Pack<R, 8> pk;
+#pragma unroll
+    for (int j = 0; j < kStageTiles; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pk.v[4 * j + i] = row.template weigh<E>(sc[j][i]);
+    const vec8 pf = __builtin_bit_cast(vec8, pk);
+#pragma unroll
+    for (int db = 0; db < kD / 16; ++db) {
+      const vec8 v8 = __builtin_bit_cast(
+          vec8, __builtin_shufflevector(vf[0][db], vf[1][db], 0, 1, 2, 3, 4, 5, 6, 7));
+      row.o[db] = M::qk(v8, pf, row.o[db]);
+    }
+  }
+  row.close(lane);
+  const int r = 16 * wave + x.col;
+  if (r >= x.rows) return;
+  const int64_t at = static_cast<int64_t>(it.first_row + r) * a.num_kv_heads + kv_head;
+#pragma unroll
+  for (int db = 0; db < kD / 16; ++db)
+    *reinterpret_cast<f32x4_t*>(a.ws_acc + at * kD + db * 16 + 4 * quad) = row.o[db];
+  if (quad == 0) {
+    a.ws_ml[at * 2] = row.m;
+    a.ws_ml[at * 2 + 1] = row.l;
+  }
+}
+
+template <typename E>
+__global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(const SharedArgs a) {
+  __shared__ Lds s;
   typedef int32_t int8v __attribute__((ext_vector_type(8)));
   using ConstItem = __attribute__((address_space(4))) const int8v;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
@@ -539,63 +723,79 @@ __global__ __launch_bounds__(kThreads) void shared_decode_kernel(const SharedArg
       it.end <= it.begin || it.end > a.t_width << a.lb || it.first_row < 0 ||
       it.first_row > a.max_rows - it.seqs * a.group)
     return;
-  const int rows = it.seqs * a.group;
-  if (rows <= 16)
-    run_item<E, 1>(a, it, kv_head, s_ring, s_m, s_l);
-  else if (rows <= 32)
-    run_item<E, 2>(a, it, kv_head, s_ring, s_m, s_l);
+  if (it.seqs * a.group <= kFewRows)
+    run_few_rows<E>(a, it, kv_head, s);
   else
-    run_item<E, 4>(a, it, kv_head, s_ring, s_m, s_l);
+    run_many_rows<E>(a, it, kv_head, s);
 }
 
 constexpr int kJoinThreads = 256;
+constexpr int kJoinLanes = kD / 4;  // a float4 each
+constexpr int kJoinWays = kJoinThreads / kJoinLanes;
 
-// out of one sequence and KV head from its pieces, in their order.
+// (m, l, o) += 2^(..) of another piece; pieces of no position weigh nothing.
+__device__ __forceinline__ void join_piece(float& m, float& l, f32x4_t& o, float mb, float lb,
+                                           f32x4_t ob) {
+  if (mb == -INFINITY) return;
+  const float mnew = fmaxf(m, mb);
+  const float fo = m == -INFINITY ? 0.f : fast_exp2(m - mnew);
+  const float fb = fast_exp2(mb - mnew);
+  l = fmaf(l, fo, lb * fb);
+  o = o * fo + ob * fb;
+  m = mnew;
+}
+
+// One query row of one sequence from its pieces: way w of 8 joins pieces w, w
+// + 8, ... (two at a time), then the ways are joined in order.
 template <typename E>
 __global__ __launch_bounds__(kJoinThreads) void shared_join_kernel(const SharedArgs a) {
-  const int kv_head = blockIdx.x % a.num_kv_heads;
-  const int seq = blockIdx.x / a.num_kv_heads;
+  __shared__ f32x4_t s_o[kJoinWays][kJoinLanes];
+  __shared__ float s_m[kJoinWays], s_l[kJoinWays];
+  const int hq = a.num_kv_heads * a.group;
+  const int head = blockIdx.x % hq;
+  const int seq = blockIdx.x / hq;
+  const int kv_head = head / a.group;
+  const int g = head - kv_head * a.group;
   const SharedSeq q = a.seqs[seq];
-  const int G = a.group;
+  const int lane = threadIdx.x % kJoinLanes;
+  const int way = threadIdx.x / kJoinLanes;
   // As above: a foreign plan's pieces stay inside the workspace, and are no
   // more than a plan can have.
   const int prefix_parts = min(max(q.prefix_parts, 0), a.max_items);
   const int parts = prefix_parts + min(max(q.own_parts, 0), a.max_items);
-  auto row_of = [&](int p) {
-    const int64_t row = p < prefix_parts
-                            ? q.prefix_row + static_cast<int64_t>(p) * q.prefix_step
-                            : q.own_row + static_cast<int64_t>(p - prefix_parts) * G;
-    return min(max(row, int64_t(0)), static_cast<int64_t>(a.max_rows - G));
-  };
-  constexpr int kBatch = 8;
-  for (int e = threadIdx.x; e < G * kD; e += kJoinThreads) {
-    const int h = e / kD, d = e % kD;
-    float mx = -INFINITY, ls = 0.f, os = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += kBatch) {
-      float mb[kBatch], lb[kBatch], ob[kBatch];
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int p0 = way; p0 < parts; p0 += 2 * kJoinWays) {
+    float mb[2], lb[2];
+    f32x4_t ob[2];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int64_t at =
-            (row_of(min(p0 + b, parts - 1)) + h) * a.num_kv_heads + kv_head;
-        mb[b] = a.ws_ml[at * 2];
-        lb[b] = a.ws_ml[at * 2 + 1];
-        ob[b] = a.ws_acc[at * kD + d];
-      }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        if (p0 + b >= parts || mb[b] == -INFINITY) continue;
-        const float mnew = fmaxf(mx, mb[b]);
-        const float fo = mx == -INFINITY ? 0.f : fast_exp2(mx - mnew);
-        const float fb = fast_exp2(mb[b] - mnew);
-        ls = fmaf(ls, fo, lb[b] * fb);
-        os = fmaf(os, fo, ob[b] * fb);
-        mx = mnew;
-      }
+    for (int b = 0; b < 2; ++b) {
+      const int p = min(p0 + b * kJoinWays, parts - 1);
+      int64_t row = p < prefix_parts
+                        ? q.prefix_row + static_cast<int64_t>(p) * q.prefix_step
+                        : q.own_row + static_cast<int64_t>(p - prefix_parts) * a.group;
+      row = min(max(row + g, int64_t(0)), static_cast<int64_t>(a.max_rows - 1));
+      const int64_t at = row * a.num_kv_heads + kv_head;
+      mb[b] = a.ws_ml[at * 2];
+      lb[b] = a.ws_ml[at * 2 + 1];
+      ob[b] = *reinterpret_cast<const f32x4_t*>(a.ws_acc + at * kD + lane * 4);
     }
-    const float inv = ls > 0.f ? 1.f / ls : 0.f;  // no position: zeros
-    static_cast<uint16_t*>(a.out)[seq * a.o_ts + (kv_head * G + h) * a.o_hs + d] =
-        E::store(os * inv);
+    join_piece(m, l, o, mb[0], lb[0], ob[0]);
+    if (p0 + kJoinWays < parts) join_piece(m, l, o, mb[1], lb[1], ob[1]);
   }
+  s_o[way][lane] = o;
+  if (lane == 0) {
+    s_m[way] = m;
+    s_l[way] = l;
+  }
+  __syncthreads();
+  if (way != 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWays; ++w) join_piece(m, l, o, s_m[w], s_l[w], s_o[w][lane]);
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // no position: zeros
+  uint16_t* out = static_cast<uint16_t*>(a.out) + seq * a.o_ts + head * a.o_hs + lane * 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = E::store(o[i] * inv);
 }
 
 // Arguments that plan, sizes and call share; MI_OK if there is a kernel.
@@ -621,8 +821,8 @@ int32_t check_shape(const char* what, int32_t num_seqs, int32_t num_q_heads,
   if (static_cast<int64_t>(width) * block_size > kMaxPositions)
     return fail(MI_ERR_UNSUPPORTED, name + ": block tables of more than 2^30 positions");
   // The launch's threads are counted in 32 bits.
-  if ((num_seqs + num_seqs / 2 + kTargetGroups + 1ll) * num_kv_heads > (1 << 23))
-    return fail(MI_ERR_UNSUPPORTED, name + ": too many sequences times KV heads");
+  if ((num_seqs + num_seqs / 2 + kTargetGroups + 1ll) * num_q_heads > (1 << 23))
+    return fail(MI_ERR_UNSUPPORTED, name + ": too many sequences times query heads");
   return MI_OK;
 }
 
@@ -753,7 +953,7 @@ extern "C" int32_t mi_shared_decode(
   a.scale_log2 = scale * 1.4426950408889634f;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t blocks = static_cast<uint32_t>(z.max_items) * num_kv_heads;
-  const uint32_t joins = static_cast<uint32_t>(num_seqs) * num_kv_heads;
+  const uint32_t joins = static_cast<uint32_t>(num_seqs) * num_q_heads;
   if (dtype == MI_DTYPE_BF16) {
     shared_decode_kernel<BF16><<<blocks, kThreads, 0, s>>>(a);
     shared_join_kernel<BF16><<<joins, kJoinThreads, 0, s>>>(a);

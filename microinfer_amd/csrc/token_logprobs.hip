@@ -11,13 +11,17 @@
 // whose maximum is the type's lowest value stay right.
 //
 // The alternatives come out of the same registers. A row's values order as
-// 64-bit words (order key of the value, then the lower index). After its first
-// tile a wave knows the num_top-th largest of its 64 lanes' maxima: at least
-// num_top values are no smaller than that threshold, so only values above it
-// can matter and go to a small list in LDS, and values equal to it fill up
-// from the lowest index if the list is short. That fill-up is what rows of
-// equal or masked values run on; NaN, infinities and lists that overflow take
-// num_top rounds of a maximum over the tile instead.
+// 64-bit words (order key of the value, then the lower index). Each wave keeps
+// a list of candidates of its own in LDS: after the first tile each finds the
+// key that a quarter of num_top of its lanes' maxima reach, and as at least
+// num_top values are no smaller than the least of these four, only values from
+// that floor on can matter (about num_top / 4 of a wave's 2048 ordinary
+// values). From then on, without barriers, the floor follows the lanes' maxima.
+// At the end the highest of the waves' floors holds for the workgroup; what
+// lies above it, some tens of words, is ranked. A tile with too many values at
+// its floor (equal or masked ones) leaves those out, and if they are needed
+// they are taken in order of their index by a scan at the end. Tiles with a
+// NaN compare order keys instead of values.
 //
 // Few rows are split over many workgroups: each publishes (maximum, S, E) and
 // its own best words, and the last to arrive at the row's counter joins them.
@@ -63,10 +67,14 @@ struct LogprobArgs {
   int32_t* counters;
 };
 
+constexpr uint32_t kNanKey = 0xffffffffu;
+constexpr uint32_t kInfKey = 0xff800000u;      // of +inf
+constexpr uint32_t kMinusInfKey = 0x007fffffu;  // of -inf, the least
+
 // Unsigned order of float values: NaN above everything, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float v) {
   uint32_t b = __float_as_uint(v);
-  if (v != v) return 0xffffffffu;
+  if (v != v) return kNanKey;
   if ((b << 1) == 0) b = 0;
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
@@ -79,12 +87,6 @@ __device__ __forceinline__ uint64_t make_word(float v, uint32_t index) {
 }
 __device__ __forceinline__ uint32_t word_index(uint64_t w) {
   return 0x7fffffffu - static_cast<uint32_t>(w);
-}
-
-__device__ __forceinline__ uint64_t shfl_xor_word(uint64_t v, int mask) {
-  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), mask, kWave);
-  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(v >> 32), mask, kWave);
-  return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
 // The largest t with at least n lanes' keys >= t, in the upper BITS bits: the
@@ -100,7 +102,8 @@ __device__ __forceinline__ uint32_t nth_key(uint32_t key, int n) {
   return t;
 }
 
-// Bits of a float32 that can differ between values of the type.
+// Bits of an order key that can differ between values of the type; the lower
+// ones are all zeros, or all ones for negative values.
 template <typename E>
 struct KeyBits;
 template <>
@@ -116,59 +119,91 @@ struct KeyBits<BF16> {
   static constexpr int value = 16;
 };
 
+// nth_key of values of the type, at least -inf's.
+template <typename E>
+__device__ __forceinline__ uint32_t nth_value_key(uint32_t key, int n) {
+  constexpr int kBits = KeyBits<E>::value;
+  uint32_t t = nth_key<kBits>(key, n);
+  if (kBits < 32 && !(t & 0x80000000u)) t |= 0xffffffffu >> (kBits & 31);
+  return t > kInfKey ? kNanKey : max(t, kMinusInfKey);
+}
+
+// The n-th largest word of the wave, or a word below it and above the next
+// smaller value's words.
+template <typename E>
+__device__ __forceinline__ uint64_t nth_word(uint64_t word, int n) {
+  const uint32_t key = static_cast<uint32_t>(word >> 32);
+  const uint32_t hi = nth_key<KeyBits<E>::value>(key, n);
+  const int equal = __popcll(__ballot(key >> (32 - KeyBits<E>::value) ==
+                                      hi >> (32 - KeyBits<E>::value)));
+  uint32_t lo = 0;
+  if (equal > 4) {
+    // Ties: the lower indices among them.
+    const int above = __popcll(__ballot(key > (hi | (0xffffffffu >> (KeyBits<E>::value - 1) >> 1))));
+    const uint32_t full = hi & 0x80000000u ? hi : hi | (0xffffffffu >> (KeyBits<E>::value - 1) >> 1);
+    lo = nth_key<32>(key == full ? static_cast<uint32_t>(word) : 0u, n - above);
+    return (static_cast<uint64_t>(full) << 32) | lo;
+  }
+  return static_cast<uint64_t>(hi) << 32;
+}
+
+constexpr int kWaveCap = kListCap / kWaves;
+constexpr int kTilePasses = 4;  // packs per thread and tile
+constexpr int kScanLanes = 32;
+
+// LDS of a launch: with the lists of the alternatives, or without.
+template <bool TOP>
 struct Shared {
-  uint64_t list[kListCap];
-  uint64_t kept[kMaxTop];  // select()'s result, largest first
-  uint64_t wave_word[kWaves];
-  uint32_t wave_key[kWaves];
   float wave_ref[kWaves], wave_sum[kWaves], wave_ent[kWaves];
-  int32_t count;  // words in the list
-  int32_t bad;    // a sum is NaN
-  int32_t fill[kWaves];
   int32_t arrived;
 };
+template <>
+struct Shared<true> : Shared<false> {
+  // The waves' lists, then the workgroup's (zeros behind its last word).
+  uint64_t list[kListCap + 8];
+  uint64_t kept[kMaxTop];  // the best words, largest first
+  // Packs of lanes whose values are looked through, and whose they are.
+  __attribute__((aligned(16))) char scan[kWaves][kScanLanes * kTilePasses * 16];
+  uint8_t scan_lane[kWaves][kScanLanes];
+  uint32_t wave_key[kWaves];    // what each wave contributes to the shared floor
+  uint32_t wave_first[kWaves];  // the num_top-th key of each wave's first tile
+  uint32_t wave_floor[kWaves];
+  int32_t wave_open[kWaves];  // values equal to the wave's floor are left out
+  int32_t count;              // words in the workgroup's list
+  int32_t fill[kWaves];
+};
+using Lists = Shared<true>;
+
+// Each wave shares the key that top / kWaves of its lanes reach; the least of
+// these is reached by top values of the workgroup. Waves read it as it comes:
+// the keys only rise, so an old one is a floor too.
+__device__ __forceinline__ void share(Lists& s, int wave, uint32_t key) {
+  __hip_atomic_store(&s.wave_key[wave], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+__device__ __forceinline__ uint32_t shared_floor(Lists& s) {
+  uint32_t key = kNanKey;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    key = min(key, __hip_atomic_load(&s.wave_key[w], __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_WORKGROUP));
+  return __builtin_amdgcn_readfirstlane(key);
+}
 
 // The `top` largest of list[0, n) into kept[0, top), largest first, zeros
-// behind them. All threads; the list is spoilt.
-__device__ void select_words(Shared& s, int n, int top) {
+// behind them: each word's rank is the number of larger ones. All threads,
+// after a barrier.
+__device__ void rank_words(Lists& s, int n, int top) {
   const int t = threadIdx.x;
-  const int lane = t % kWave, wave = t / kWave;
-  __syncthreads();
-  uint64_t mine[kListCap / kThreads];
-  uint64_t best = 0;
-#pragma unroll
-  for (int i = 0; i < kListCap / kThreads; ++i) {
-    const int at = i * kThreads + t;
-    mine[i] = at < n ? s.list[at] : 0;
-    best = mine[i] > best ? mine[i] : best;
-  }
+  if (t < 8) s.list[n + t] = 0;
   if (t < top) s.kept[t] = 0;
-  uint32_t hi = 0, lo = 0;
-  if (n > kWave) {
-    // A word that at least `top` words are no smaller than: the top-th largest
-    // of a wave's lanes' maxima, the best wave's.
-    hi = nth_key<32>(static_cast<uint32_t>(best >> 32), top);
-    const uint32_t above = static_cast<uint32_t>(best >> 32);
-    const int more = __popcll(__ballot(above > hi));
-    lo = nth_key<32>(above == hi ? static_cast<uint32_t>(best) : 0, top - more);
-  }
-  const uint64_t floor_word = (static_cast<uint64_t>(hi) << 32) | lo;
-  if (lane == 0) s.wave_word[wave] = floor_word;
-  if (t == 0) s.count = 0;
   __syncthreads();
-  uint64_t least = 1;  // zeros are no words
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) least = s.wave_word[w] > least ? s.wave_word[w] : least;
-#pragma unroll
-  for (int i = 0; i < kListCap / kThreads; ++i)
-    if (mine[i] >= least) s.list[atomicAdd(&s.count, 1)] = mine[i];
-  __syncthreads();
-  // Each word's rank is the number of larger ones; words are distinct.
-  const int m = s.count;
-  for (int at = t; at < m; at += kThreads) {
+  for (int at = t; at < n; at += kThreads) {
     const uint64_t w = s.list[at];
     int rank = 0;
-    for (int j = 0; j < m && rank < top; ++j) rank += s.list[j] > w;
+    for (int j = 0; j < n; j += 8) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) rank += s.list[j + k] > w;
+    }
     if (rank < top) s.kept[rank] = w;
   }
   __syncthreads();
@@ -177,12 +212,13 @@ __device__ void select_words(Shared& s, int n, int top) {
 // Appends the first `want` indices of [lo, hi) whose value has key `key` to the
 // list. All threads.
 template <typename E>
-__device__ void fill_equal(Shared& s, const typename E::raw* row, int lo, int hi, uint32_t key,
+__device__ void fill_equal(Lists& s, const typename E::raw* row, int lo, int hi, uint32_t key,
                            int want) {
   const int t = threadIdx.x;
   const int lane = t % kWave, wave = t / kWave;
   int found = 0;
   const int start = s.count;
+  __syncthreads();
   for (int at = lo; at < hi && found < want; at += kThreads) {
     const int v = at + t;
     const bool hit = v < hi && order_key(E::load(row[v])) == key;
@@ -204,6 +240,68 @@ __device__ void fill_equal(Shared& s, const typename E::raw* row, int lo, int hi
   __syncthreads();
 }
 
+// A wave's candidates.
+struct Candidates {
+  uint64_t* list;      // kWaveCap words
+  int count = 0;       // wave-uniform, as all of this
+  int raised_at = 0;   // the count when the floor was last looked at
+  bool first = true;   // no floor yet
+  bool open = false;   // values equal to the floor are not in the list
+  uint32_t floor = 0;  // key
+
+  // Keeps about the `top` largest words (at most `top` words a lane's slice
+  // holds), and raises the floor to the least of `top` of them.
+  __device__ void compress(int top) {
+    const int lane = threadIdx.x % kWave;
+    uint64_t mine[kWaveCap / kWave];
+    uint64_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kWaveCap / kWave; ++i) {
+      const int at = i * kWave + lane;
+      mine[i] = at < count ? list[at] : 0;
+      best = mine[i] > best ? mine[i] : best;
+    }
+    const uint32_t hi = nth_key<32>(static_cast<uint32_t>(best >> 32), top);
+    const uint32_t key = static_cast<uint32_t>(best >> 32);
+    const uint32_t lo = nth_key<32>(key == hi ? static_cast<uint32_t>(best) : 0u,
+                                    top - __popcll(__ballot(key > hi)));
+    const uint64_t least = (static_cast<uint64_t>(hi) << 32) | lo;
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < kWaveCap / kWave; ++i) {
+      const bool keep = mine[i] != 0 && mine[i] >= least;
+      const uint64_t hits = __ballot(keep);
+      if (keep) list[count + __popcll(hits & ((1ull << lane) - 1))] = mine[i];
+      count += __popcll(hits);
+    }
+    raise(hi);
+    raised_at = count;
+  }
+
+  // A floor that `top` values of the list reach.
+  __device__ void raise(uint32_t key) {
+    if (key <= floor) return;
+    floor = key;
+    open = false;
+  }
+
+  // Leaves out of the list what is not above `key`, the new floor.
+  __device__ void reopen(uint32_t key) {
+    const int lane = threadIdx.x % kWave;
+    int kept = 0;
+    for (int i = 0; i < count; i += kWave) {
+      const uint64_t w = i + lane < count ? list[i + lane] : 0;
+      const bool keep = static_cast<uint32_t>(w >> 32) > key;
+      const uint64_t hits = __ballot(keep);
+      if (keep) list[kept + __popcll(hits & ((1ull << lane) - 1))] = w;
+      kept += __popcll(hits);
+    }
+    raised_at = count = kept;
+    floor = key;
+    open = true;
+  }
+};
+
 __device__ __forceinline__ void store_agent(uint64_t* p, uint64_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -222,8 +320,8 @@ __device__ __forceinline__ void add_sums(float r, float sum, float ent, float to
 
 // What a row's outputs need once its sums and best words are known. All
 // threads.
-template <typename E>
-__device__ void write_row(const LogprobArgs& a, const Shared& s, int row,
+template <typename E, bool TOP>
+__device__ void write_row(const LogprobArgs& a, const Shared<TOP>& s, int row,
                           const typename E::raw* logits, float r, float temperature, float S,
                           float ent) {
   const float log_sum = log2f(S);
@@ -236,21 +334,24 @@ __device__ void write_row(const LogprobArgs& a, const Shared& s, int row,
     a.logprobs[static_cast<int64_t>(row) * a.given + i] = lp;
   }
   if (a.entropy != nullptr && threadIdx.x == 0) a.entropy[row] = kLn2 * (log_sum - ent / S);
-  if (threadIdx.x < a.top) {
-    const uint64_t w = s.kept[threadIdx.x];
-    const int64_t at = static_cast<int64_t>(row) * a.top + threadIdx.x;
-    a.top_tokens[at] = word_index(w);
-    a.top_logprobs[at] = logprob(key_value(static_cast<uint32_t>(w >> 32)));
+  if constexpr (TOP) {
+    if (threadIdx.x < a.top) {
+      const uint64_t w = s.kept[threadIdx.x];
+      const int64_t at = static_cast<int64_t>(row) * a.top + threadIdx.x;
+      a.top_tokens[at] = word_index(w);
+      a.top_logprobs[at] = logprob(key_value(static_cast<uint32_t>(w >> 32)));
+    }
   }
 }
 
 // NP packs of VEC elements per thread make a tile.
-template <typename E, int NP, bool TOP, bool ENT>
-__global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) {
+template <typename E, bool TOP, bool ENT>
+__global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs a) {
   using R = typename E::raw;
   constexpr int VEC = 16 / sizeof(R);
+  constexpr int NP = kTilePasses;
   constexpr int kTilePacks = kThreads * NP;
-  __shared__ Shared s;
+  __shared__ Shared<TOP> s;
   const int row = blockIdx.x / a.parts;
   const int part = blockIdx.x - row * a.parts;
   const int t = threadIdx.x;
@@ -267,41 +368,40 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
   const int pack_end = min((lead + a.vocab + VEC - 1) / VEC, pack_begin + a.part_packs);
   const int v_begin = max(0, pack_begin * VEC - lead);
 
-  if (TOP && t == 0) {
-    s.count = 0;
-    s.bad = 0;
-  }
   float ref = -INFINITY;   // wave-uniform reference of the sums; -inf: none yet
   float sum = 0.f, ent = 0.f, top_value = -INFINITY;
-  bool first = true;       // no threshold yet
-  bool complete = false;   // the list holds every value seen
-  uint32_t floor_key = 0;  // values of larger keys are in the list
-  float floor_value = -INFINITY;
+  Candidates cand;
+  if constexpr (TOP) cand.list = s.list + wave * kWaveCap;
+  uint32_t lane_key = 0;  // of the lane's largest value
+  const int quarter = (a.top + kWaves - 1) / kWaves;
+
+  // Pack u of this thread in the tile that begins at pack p0, -inf outside the
+  // row.
+  auto load_tile = [&](int p0, int u) {
+    const int p = p0 + u * kThreads + t;
+    const int v0 = p * VEC - lead;
+    Pack<R, VEC> x;
+    if (p < pack_end && v0 >= 0 && v0 + VEC <= a.vocab) {
+      x = load_pack<R, VEC>(grid + static_cast<int64_t>(p) * VEC);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        x.v[j] = E::store(-INFINITY);
+        if (p < pack_end && v0 + j >= 0 && v0 + j < a.vocab) x.v[j] = logits[v0 + j];
+      }
+    }
+    return x;
+  };
 
   for (int p0 = pack_begin; p0 < pack_end; p0 += kTilePacks) {
     Pack<R, VEC> x[NP];
 #pragma unroll
-    for (int u = 0; u < NP; ++u) {
-      const int p = p0 + u * kThreads + t;
-      const int v0 = p * VEC - lead;
-      if (p < pack_end && v0 >= 0 && v0 + VEC <= a.vocab) {
-        x[u] = load_pack<R, VEC>(grid + static_cast<int64_t>(p) * VEC);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          x[u].v[j] = E::store(-INFINITY);
-          if (p < pack_end && v0 + j >= 0 && v0 + j < a.vocab) x[u].v[j] = logits[v0 + j];
-        }
-      }
-    }
-    float pack_max[NP];
+    for (int u = 0; u < NP; ++u) x[u] = load_tile(p0, u);
     float tile_max = -INFINITY;
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
-      pack_max[u] = E::load(x[u].v[0]);
 #pragma unroll
-      for (int j = 1; j < VEC; ++j) pack_max[u] = fmaxf(pack_max[u], E::load(x[u].v[j]));
-      tile_max = fmaxf(tile_max, pack_max[u]);
+      for (int j = 0; j < VEC; ++j) tile_max = fmaxf(tile_max, E::load(x[u].v[j]));
     }
     top_value = fmaxf(top_value, tile_max);
     // The reference: the first tile's maximum, moved when it lies too low.
@@ -317,6 +417,12 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
     }
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
+      // A pack at a time, unpacked again: what the registers of the list's code
+      // leave room for.
+      if constexpr (TOP) {
+        __builtin_amdgcn_sched_barrier(0);
+        pin(x[u]);
+      }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float d = (E::load(x[u].v[j]) - ref) * c;
@@ -326,106 +432,107 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
       }
     }
     if constexpr (TOP) {
-      const int before = first ? 0 : s.count;
-      if (first) {
-        constexpr int kBits = KeyBits<E>::value;
-        uint32_t key = nth_key<kBits>(order_key(tile_max), a.top);
-        if (!(key & 0x80000000u)) key |= (kBits == 32 ? 0u : 0xffffffffu >> kBits);
-        if (lane == 0) s.wave_key[wave] = key;
-      }
-      if (sum != sum) s.bad = 1;
-      __syncthreads();
-      if (first) {
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) floor_key = max(floor_key, s.wave_key[w]);
-        floor_key = max(floor_key, order_key(-INFINITY));
-        floor_value = key_value(floor_key);
-      }
-      const bool was_first = first;
-      first = false;
-      const bool bad = s.bad != 0;
-      if (!bad) {
-#pragma unroll
+      // Both sums are done here: else the entropy's is put off past the branches
+      // below, with every weight kept for it (76 registers, 128 and spills).
+      asm volatile("" : "+v"(sum), "+v"(ent));
+      // The tile's keys again, for the paths that hardly a tile takes.
+      auto each_key = [&](auto&& f) {
+#pragma unroll 1
         for (int u = 0; u < NP; ++u) {
-          if (pack_max[u] > floor_value) {
-            const int v0 = (p0 + u * kThreads + t) * VEC - lead;
+          const Pack<R, VEC> y = load_tile(p0, u);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const float v = E::load(x[u].v[j]);
-              if (v > floor_value) {
-                const int at = atomicAdd(&s.count, 1);
-                if (at < kListCap) s.list[at] = make_word(v, v0 + j);
-              }
-            }
-          }
+          for (int j = 0; j < VEC; ++j) f(order_key(E::load(y.v[j])));
         }
+      };
+      // The key of the lane's largest value in this tile, and so far.
+      uint32_t tile_key = order_key(tile_max);
+      if (__ballot(sum != sum) != 0) each_key([&](uint32_t k) { tile_key = max(tile_key, k); });
+      lane_key = max(lane_key, tile_key);
+      const bool was_first = cand.first;
+      if (was_first) {
+        cand.first = false;
+        const uint32_t part_key = nth_value_key<E>(lane_key, quarter);
+        const uint32_t all_key = nth_value_key<E>(lane_key, a.top);
+        if (lane == 0) {
+          share(s, wave, part_key);
+          s.wave_first[wave] = all_key;  // a wave may be alone in a short tile
+        }
+        __syncthreads();  // every part has a tile, so every wave is here
+        cand.floor = shared_floor(s);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) cand.floor = max(cand.floor, s.wave_first[w]);
+        cand.floor = __builtin_amdgcn_readfirstlane(cand.floor);
       }
-      __syncthreads();
-      const int n = s.count;
-      __syncthreads();
-      if (bad || n > kListCap) {
-        // Rounds: the tile's best words one after the other.
-        if (t == 0) s.count = before;
-        __syncthreads();
-        // First what the tiles before hold of values equal to the threshold.
-        if (!was_first && !complete && before < a.top)
-          fill_equal<E>(s, logits, v_begin, max(v_begin, p0 * VEC - lead), floor_key,
-                        a.top - before);
-        select_words(s, s.count, a.top);
-        if (t < a.top) s.list[t] = s.kept[t];
-        uint64_t last = ~0ull;
-        for (int i = 0; i < a.top; ++i) {
-          uint64_t best = 0;
+      // Puts the tile's values of keys from `least` on behind the list; how many
+      // it then has, stored or not. The lanes that have such values put their
+      // packs into LDS, 32 at a time, where all lanes look through them.
+      auto gather = [&](uint32_t least) -> int {
+        int n = cand.count;
+        if (least == 0) return n;  // above NaN: nothing
+        uint64_t lanes = __ballot(tile_key >= least);
+        while (lanes != 0) {
+          const int rank = __popcll(lanes & ((1ull << lane) - 1));
+          const bool puts = (lanes >> lane & 1) && rank < kScanLanes;
+          const uint64_t put = __ballot(puts);
+          if (puts) {
 #pragma unroll
-          for (int u = 0; u < NP; ++u) {
-            const int p = p0 + u * kThreads + t;
-            const int v0 = p * VEC - lead;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const int v = v0 + j;
-              if (p < pack_end && v >= 0 && v < a.vocab) {
-                const uint64_t w = make_word(E::load(x[u].v[j]), v);
-                if (w < last && w > best) best = w;
-              }
+            for (int u = 0; u < NP; ++u)
+              store_pack<R, VEC>(reinterpret_cast<R*>(s.scan[wave]) + (rank * NP + u) * VEC, x[u]);
+            s.scan_lane[wave][rank] = static_cast<uint8_t>(lane);
+          }
+          __builtin_amdgcn_wave_barrier();
+          const int values = __popcll(put) * NP * VEC;
+          for (int e0 = 0; e0 < values; e0 += kWave) {
+            const int e = e0 + lane;  // NP VEC is a multiple of 16, so is `values`
+            bool hit = e < values;
+            float v = 0.f;
+            int at_v = 0;
+            if (hit) {
+              v = E::load(reinterpret_cast<const R*>(s.scan[wave])[e]);
+              const int u = e / VEC % NP;
+              const int p = p0 + u * kThreads + wave * kWave + s.scan_lane[wave][e / (NP * VEC)];
+              at_v = p * VEC - lead + e % VEC;
+              hit = order_key(v) >= least && p < pack_end && at_v >= 0 && at_v < a.vocab;
             }
+            const uint64_t hits = __ballot(hit);
+            const int at = n + __popcll(hits & ((1ull << lane) - 1));
+            if (hit && at < kWaveCap) cand.list[at] = make_word(v, at_v);
+            n += __popcll(hits);
           }
-#pragma unroll
-          for (int o = 1; o < kWave; o <<= 1) {
-            const uint64_t other = shfl_xor_word(best, o);
-            best = other > best ? other : best;
-          }
-          __syncthreads();
-          if (lane == 0) s.wave_word[wave] = best;
-          __syncthreads();
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) best = s.wave_word[w] > best ? s.wave_word[w] : best;
-          if (t == 0) s.list[a.top + i] = best;
-          if (best == 0) {
-            for (int k = i + t; k < a.top; k += kThreads) s.list[a.top + k] = 0;
-            break;
-          }
-          last = best;
+          __builtin_amdgcn_wave_barrier();
+          lanes &= ~put;
         }
-        select_words(s, 2 * a.top, a.top);
-        if (t < a.top) s.list[t] = s.kept[t];
-        complete = s.kept[a.top - 1] == 0;  // fewer values than alternatives so far
-        __syncthreads();
-        if (t == 0) s.count = complete ? 0 : a.top;
-        if (complete) {
-          // Only the row's last tile can leave it so.
-          if (t < a.top && s.kept[t] != 0) atomicAdd(&s.count, 1);
+        return n;
+      };
+      const int before = cand.count;
+      int n = gather(cand.floor + (was_first ? 0 : 1));
+      for (int attempt = 1; n > kWaveCap; ++attempt) {
+        if (attempt == 1 && was_first) {
+          cand.open = true;  // too many values equal to the floor: leave them out
+        } else if (attempt == 1) {
+          cand.compress(a.top);
         } else {
-          floor_key = static_cast<uint32_t>(s.kept[a.top - 1] >> 32);
-          floor_value = key_value(floor_key);
+          // Many large values in few lanes: the tile's own top-th largest key.
+          uint32_t key = 0;
+          for (int b = 31; b >= 0; --b) {
+            const uint32_t trial = key | (1u << b);
+            int mine = 0;
+            each_key([&](uint32_t k) { mine += k >= trial; });
+            if (wave_sum_int(mine) >= a.top) key = trial;
+          }
+          cand.reopen(key);
         }
-        __syncthreads();
-      } else if (n > kListCap / 2) {
-        select_words(s, n, a.top);
-        if (t < a.top) s.list[t] = s.kept[t];
-        if (t == 0) s.count = a.top;
-        floor_key = static_cast<uint32_t>(s.kept[a.top - 1] >> 32);
-        floor_value = key_value(floor_key);
-        __syncthreads();
+        n = gather(cand.floor + 1);
+      }
+      cand.count = n;
+      if (was_first) {
+        cand.raised_at = n;
+      } else if (n != before && n > cand.raised_at + a.top / 2) {
+        if (lane == 0) share(s, wave, nth_value_key<E>(lane_key, quarter));
+        // Another wave may be ahead, so its values equal to the floor may come
+        // later in the row: only what is below it cannot matter.
+        cand.raise(max(nth_value_key<E>(lane_key, a.top), shared_floor(s) - 1));
+        cand.raised_at = n;
       }
     }
   }
@@ -437,6 +544,13 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
     float S = 0.f, N = 0.f;
     add_sums(ref == -INFINITY ? kLowest : ref, group_sum<kWave>(sum), group_sum<kWave>(ent),
              wave_max, c, S, N);
+    if constexpr (TOP) {
+      if (t == 0) s.count = 0;
+      if (lane == 0) {
+        s.wave_floor[wave] = cand.floor;
+        s.wave_open[wave] = cand.open;
+      }
+    }
     if (lane == 0) {
       s.wave_ref[wave] = wave_max;
       s.wave_sum[wave] = S;
@@ -451,14 +565,37 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
   for (int w = 0; w < kWaves; ++w)
     add_sums(s.wave_ref[w], s.wave_sum[w], s.wave_ent[w], r, c, S, N);
   if constexpr (TOP) {
-    if (!complete && s.count < a.top) {
-      const int v_end = min(a.vocab, pack_end * VEC - lead);
-      fill_equal<E>(s, logits, v_begin, v_end, floor_key, a.top - s.count);
+    // What lies above the highest floor, or at it.
+    uint32_t floor = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) floor = max(floor, s.wave_floor[w]);
+    bool open = false;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) open = open || (s.wave_open[w] && s.wave_floor[w] == floor);
+    uint64_t mine[kWaveCap / kWave];
+#pragma unroll
+    for (int i = 0; i < kWaveCap / kWave; ++i) {
+      const int at = i * kWave + lane;
+      mine[i] = at < cand.count ? cand.list[at] : 0;
     }
-    select_words(s, s.count, a.top);
+    __syncthreads();
+    if (cand.count > 0) {
+#pragma unroll
+      for (int i = 0; i < kWaveCap / kWave; ++i) {
+        const uint32_t key = static_cast<uint32_t>(mine[i] >> 32);
+        if (key > floor || (key == floor && !open && key != 0))
+          s.list[atomicAdd(&s.count, 1)] = mine[i];
+      }
+    }
+    __syncthreads();
+    if (open && s.count < a.top)
+      fill_equal<E>(s, logits, v_begin, min(a.vocab, pack_end * VEC - lead), floor,
+                    a.top - s.count);
+    const int n = s.count;
+    rank_words(s, n, a.top);
   }
   if (a.parts == 1) {
-    write_row<E>(a, s, row, logits, r, temperature, S, N);
+    write_row<E, TOP>(a, s, row, logits, r, temperature, S, N);
     return;
   }
 
@@ -469,7 +606,9 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
     store_agent(mine, __builtin_bit_cast(uint64_t, Float2{r, S}));
     store_agent(mine + 1, __builtin_bit_cast(uint64_t, Float2{N, 0.f}));
   }
-  if (TOP && t < a.top) store_agent(mine + 2 + t, s.kept[t]);
+  if constexpr (TOP) {
+    if (t < a.top) store_agent(mine + 2 + t, s.kept[t]);
+  }
   wait_stores();
   __syncthreads();
   if (t == 0)
@@ -487,30 +626,57 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobArgs a) 
     nn = __builtin_bit_cast(Float2, load_agent(rec + 1));
   }
   if constexpr (TOP) {
-    for (int i = t; i < a.parts * a.top; i += kThreads) {
-      const int q = i / a.top;
-      s.list[i] = load_agent(
-          reinterpret_cast<const uint64_t*>(records + q * a.part_bytes) + 2 + (i - q * a.top));
+    // Every part's words are sorted, so the best 64 / parts of each are a good
+    // sample: the top-th largest of those is a floor.
+    auto word_of = [&](int q, int i) {
+      return load_agent(reinterpret_cast<const uint64_t*>(records + q * a.part_bytes) + 2 + i);
+    };
+    const int deep = lane / a.parts;
+    uint64_t probe = 0;
+    if (deep < a.top) probe = word_of(lane - deep * a.parts, deep);
+    const int words = a.parts * a.top;
+    uint64_t mine[kListCap / kThreads];
+#pragma unroll
+    for (int i = 0; i < kListCap / kThreads; ++i) {
+      const int at = i * kThreads + t;
+      mine[i] = 0;
+      if (at < words) mine[i] = word_of(at / a.top, at % a.top);
     }
-    select_words(s, a.parts * a.top, a.top);
+    // Fewer words than that in the sample: no floor.
+    const uint64_t floor = __popcll(__ballot(probe != 0)) >= a.top ? nth_word<E>(probe, a.top) : 0;
+    if (t == 0) s.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kListCap / kThreads; ++i)
+      if (mine[i] != 0 && mine[i] >= floor) s.list[atomicAdd(&s.count, 1)] = mine[i];
+    __syncthreads();
+    const int n = s.count;
+    rank_words(s, n, a.top);
   }
   const float all = xor_max<1, kWave>(rs.x);
   S = N = 0.f;
   add_sums(rs.x, rs.y, nn.x, all, c, S, N);
-  write_row<E>(a, s, row, logits, all, temperature, group_sum<kWave>(S),
+  write_row<E, TOP>(a, s, row, logits, all, temperature, group_sum<kWave>(S),
                group_sum<kWave>(N));
 }
 static_assert(kMaxParts <= kWave, "a lane per part");
 
-// Parts of a row: enough workgroups to fill the chip twice, each of at least
-// kMinPartPacks packs. From the sizes alone, so a workspace fits every call.
-constexpr int kMinPartPacks = 512;
-int32_t row_parts(int32_t rows, int32_t vocab, int32_t dtype) {
+constexpr int kWantParts = 1024;
+
+// Packs of a part of a row, a whole number of tiles: about kWantParts
+// workgroups in all, at most kMaxParts in a row. From the sizes alone, so a
+// workspace fits every call; every alignment of a row fits.
+struct RowSplit {
+  int32_t parts, part_packs;
+};
+RowSplit split_row(int32_t rows, int32_t vocab, int32_t dtype) {
   const int vec = dtype == MI_DTYPE_F32 ? 4 : 8;
   const int64_t packs = (static_cast<int64_t>(vocab) + 2 * vec - 2) / vec;
-  const int64_t want = (512 + rows - 1) / rows;
-  const int64_t most = std::max<int64_t>(1, packs / kMinPartPacks);
-  return static_cast<int32_t>(std::min<int64_t>(std::min<int64_t>(want, most), kMaxParts));
+  const int64_t tile = kThreads * kTilePasses;
+  const int64_t tiles = (packs + tile - 1) / tile;
+  const int64_t want = std::min<int64_t>((kWantParts + rows - 1) / rows, kMaxParts);
+  const int64_t each = (tiles + want - 1) / want;
+  return {static_cast<int32_t>((tiles + each - 1) / each), static_cast<int32_t>(each * tile)};
 }
 
 constexpr int kPartBytes = 16;  // (maximum, S), (E, -); then the words
@@ -518,7 +684,7 @@ constexpr int kPartBytes = 16;  // (maximum, S), (E, -); then the words
 template <typename E, bool TOP, bool ENT>
 int32_t launch_logprobs(const LogprobArgs& a, int32_t rows, hipStream_t stream) {
   const uint32_t blocks = static_cast<uint32_t>(rows) * static_cast<uint32_t>(a.parts);
-  logprob_kernel<E, 4, TOP, ENT><<<blocks, kThreads, 0, stream>>>(a);
+  logprob_kernel<E, TOP, ENT><<<blocks, kThreads, 0, stream>>>(a);
   return check_launch("mi_token_logprobs");
 }
 
@@ -538,7 +704,7 @@ extern "C" int64_t mi_token_logprobs_workspace_bytes(int32_t num_rows, int32_t v
                                                      int32_t num_top, int32_t dtype) {
   using namespace mi;
   if (num_rows <= 0 || vocab_size <= 0 || num_top < 0 || !valid_dtype(dtype)) return 0;
-  const int32_t parts = row_parts(num_rows, vocab_size, dtype);
+  const int32_t parts = split_row(num_rows, vocab_size, dtype).parts;
   return parts == 1 ? 0
                     : static_cast<int64_t>(num_rows) * parts * (kPartBytes + 8 * int64_t(num_top));
 }
@@ -581,18 +747,16 @@ extern "C" int32_t mi_token_logprobs(const void* logits, int64_t row_stride, int
                 "mi_token_logprobs_workspace_bytes() long");
   if (need > 0 && (!counters || off(counters, 4)))
     return fail(MI_ERR_WORKSPACE, "mi_token_logprobs: counters (num_rows zeros) are missing");
-  if (static_cast<int64_t>(num_rows) * row_parts(num_rows, vocab_size, dtype) >
+  if (static_cast<int64_t>(num_rows) * split_row(num_rows, vocab_size, dtype).parts >
       0xffffffffll / kThreads)
     return fail(MI_ERR_UNSUPPORTED, "mi_token_logprobs: too many rows for one launch");
   LogprobArgs a;
   a.logits = logits;
   a.row_stride = num_rows > 1 ? row_stride : 0;
   a.vocab = vocab_size;
-  a.parts = row_parts(num_rows, vocab_size, dtype);
-  const int vec = dtype == MI_DTYPE_F32 ? 4 : 8;
-  // Every alignment of a row fits: the most packs that it can touch.
-  const int packs = (vocab_size + 2 * vec - 2) / vec;
-  a.part_packs = (packs + a.parts - 1) / a.parts;
+  const RowSplit split = split_row(num_rows, vocab_size, dtype);
+  a.parts = split.parts;
+  a.part_packs = split.part_packs;
   a.temperatures = temperatures;
   a.tokens = tokens;
   a.token_stride = token_stride;

@@ -9,6 +9,7 @@ thread (AsyncEngine's worker) launch on that thread's current stream.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -176,8 +177,25 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def stream_handle(device: torch.device) -> int:
-    """Raw hipStream_t of torch's current stream on ``device``."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """Raw hipStream_t of torch's current stream on ``device``.
+
+    The handle alone (0.1 us a call), without the ``torch.cuda.Stream`` object
+    of ``torch.cuda.current_stream`` (1.9 us)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if index is None else index)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one, as launches on its
+    streams need; nothing to enter where it already is."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(index)
 
 
 def require_device(*tensors: torch.Tensor, what: str) -> None:

@@ -65,7 +65,7 @@ constexpr int kTile = 16;       // positions per tile
 constexpr int kMaxRows = 64;    // query rows of an item
 constexpr int kFewRows = 16;    // up to here the waves split the positions, not the rows
 constexpr int kMaxGroup = 16;   // query heads per KV head
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kRowBytes = kD * 2;
 constexpr int kHalfBytes = kTile * kRowBytes;  // K (or V) of a tile
@@ -73,17 +73,21 @@ constexpr int kTileBytes = 2 * kHalfBytes;     // K then V
 constexpr int kLoadBytes = kWave * 16;
 constexpr int kLoadsPerHalf = kHalfBytes / kLoadBytes;
 constexpr int kLoadsPerTile = 2 * kLoadsPerHalf;
-// 64 KiB of tiles in flight per workgroup, two workgroups per CU.
-constexpr int kRingBytes = 64 * 1024;
-constexpr int kSlots = kRingBytes / (kWaves * kTileBytes);  // few rows: slots per wave
-constexpr int kStageTiles = 2;                              // many rows: tiles per stage
+// 64 KiB of tiles per workgroup, two workgroups per CU: a tile per wave (few
+// rows), or two stages of four tiles (many).
+constexpr int kRingBytes = kWaves * kTileBytes;
+constexpr int kStageTiles = 4;
 constexpr int kStageBytes = kStageTiles * kTileBytes;
-constexpr int kStages = kRingBytes / kStageBytes;
+constexpr int kRowWaves = kMaxRows / kTile;       // waves that split the rows
+constexpr int kKeyWaves = kWaves / kRowWaves;     // and the tiles of a stage
+constexpr int kWaveTiles = kStageTiles / kKeyWaves;
 constexpr int kAccStride = kD + 4;  // floats: rows of a wave's sums, 4 banks apart
 constexpr int kRescaleSlack = 15;
-static_assert(kSlots == 2 && kStages == 4, "the waits count these");
-static_assert(kFewRows * kAccStride * 4 <= kSlots * kTileBytes, "a wave's sums fit its slots");
+static_assert(2 * kStageBytes == kRingBytes, "two stages");
 static_assert(kStageTiles * 2 == kWaves, "a stage is one half-tile per wave");
+static_assert(kKeyWaves == 2 && kWaveTiles == 2, "two key waves, 32 positions each");
+static_assert(kFewRows * kD * 4 <= kTileBytes, "a wave's sums fit its tile");
+static_assert(kRowWaves * kTile * kAccStride * 4 <= kRingBytes, "half the waves' sums fit");
 
 // A piece of work, for every KV head: the rows of sequences [seq, seq + seqs)
 // over positions [begin, end) of sequence seq's table. Its row r is partial
@@ -101,10 +105,13 @@ struct alignas(32) SharedHead {
 };
 
 constexpr int kPlanThreads = 256;
+constexpr int kMaxGroups = 4096;
 // About this many workgroups a launch.
 constexpr int kTargetGroups = 512;
-constexpr int kPartUnit = 64;  // a tile for every wave
+constexpr int kPartUnit = 64;
 constexpr int kMinPart = 128;
+constexpr int kMaxMinPart = 512;
+constexpr int kMostParts = 16;
 constexpr int kMaxPositions = 1 << 30;  // of a block table: sums of two stay int32
 
 struct SharedSizes {
@@ -134,63 +141,90 @@ struct PlanArgs {
   int32_t max_items, max_rows;
 };
 
+// Own items in the order of their length, longest first, in this many classes:
+// a long one that starts last would end long after the others.
+constexpr int kClasses = 16;
+
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArgs a) {
+  __shared__ int s_starts[kMaxGroups + 1];
+  __shared__ int s_shared[kMaxGroups];
   __shared__ int s_ctx[kMaxPlanSeqs];
   __shared__ int s_group[kMaxPlanSeqs];
-  __shared__ int s_least[kMaxPlanSeqs];  // of a group's first sequence: shared whole pages
+  // Of a group's first sequence: the whole pages that all its contexts have.
+  __shared__ int s_least[kMaxPlanSeqs];
   __shared__ unsigned long long s_work;
+  __shared__ int s_longest;
   __shared__ int s_scan[kPlanThreads / kWave][4];
+  __shared__ int s_class[kClasses];  // items of a class, then where its next one goes
   const int t = threadIdx.x;
   const int per_tile = kMaxRows / a.group;  // sequences
-  if (t == 0) s_work = 0;
+  if (t == 0) {
+    s_work = 0;
+    s_longest = 0;
+  }
+  if (t < kClasses) s_class[t] = 0;
   for (int s = t; s < a.num_seqs; s += kPlanThreads) {
     s_ctx[s] = min(max(a.ctx[s], 0), a.width << a.lb);
+    s_least[s] = a.width;
+  }
+  for (int g = t; g < a.num_groups; g += kPlanThreads) s_shared[g] = a.shared[g];
+  if (a.num_groups > 0)
+    for (int g = t; g <= a.num_groups; g += kPlanThreads) s_starts[g] = a.starts[g];
+  __syncthreads();
+  for (int s = t; s < a.num_seqs; s += kPlanThreads) {
     // The last group that starts at or before s, if s lies in it.
     int lo = -1, hi = a.num_groups - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (a.starts[mid] <= s) lo = mid; else hi = mid - 1;
+      if (s_starts[mid] <= s) lo = mid; else hi = mid - 1;
     }
-    s_group[s] = lo >= 0 && a.starts[lo] <= s && s < a.starts[lo + 1] ? lo : -1;
-    s_least[s] = a.width;
+    const bool in = lo >= 0 && s_starts[lo] <= s && s < s_starts[lo + 1];
+    s_group[s] = in ? lo : -1;
+    if (in) atomicMin(&s_least[max(s_starts[lo], 0)], s_ctx[s] >> a.lb);
   }
   __syncthreads();
-  for (int s = t; s < a.num_seqs; s += kPlanThreads)
-    if (s_group[s] >= 0)
-      atomicMin(&s_least[max(a.starts[s_group[s]], 0)], s_ctx[s] >> a.lb);
-  __syncthreads();
 
-  // Positions of s's group that all its sequences share, s's first in the
+  // Positions of s's group that all its sequences share; s's first in the
   // group and the group's end.
   auto shared_of = [&](int s, int* first, int* last) {
     const int g = s_group[s];
     *first = s;
     *last = s + 1;
     if (g < 0) return 0;
-    *first = max(a.starts[g], 0);
-    *last = min(a.starts[g + 1], a.num_seqs);
+    *first = max(s_starts[g], 0);
+    *last = min(s_starts[g + 1], a.num_seqs);
     if (*last - *first < 2) return 0;
-    return min(max(a.shared[g], 0), s_least[*first]) << a.lb;
+    return min(max(s_shared[g], 0), s_least[*first]) << a.lb;
   };
+  // Sequences of the row tile that begins with s (0: none does).
   auto tile_seqs = [&](int s, int first, int last, int shared) {
     return shared > 0 && (s - first) % per_tile == 0 ? min(per_tile, last - s) : 0;
   };
 
   unsigned long long work = 0;
+  int longest = 0;
   for (int s = t; s < a.num_seqs; s += kPlanThreads) {
     int first, last;
     const int shared = shared_of(s, &first, &last);
     work += max(s_ctx[s] - shared, 0);
+    longest = max(longest, max(s_ctx[s] - shared, shared));
     if (tile_seqs(s, first, last, shared) > 0) work += shared;
   }
-  atomicAdd(&s_work, work);
+  if (work != 0) atomicAdd(&s_work, work);
+  if (longest != 0) atomicMax(&s_longest, longest);
   __syncthreads();
   const int target = (kTargetGroups + a.num_kv_heads - 1) / a.num_kv_heads;
   const int unit = max(kPartUnit, 1 << a.lb);
   const unsigned long long want = (s_work + target - 1) / target;
+  const int least = min(max(s_longest / kMostParts, kMinPart), kMaxMinPart);
   const int part = static_cast<int>(
-      min((max(want, static_cast<unsigned long long>(kMinPart)) + unit - 1) / unit * unit,
+      min((max(want, static_cast<unsigned long long>(least)) + unit - 1) / unit * unit,
           static_cast<unsigned long long>(kMaxPositions)));
+  // 0 for the longest items.
+  auto class_of = [&](int positions) {
+    return kClasses - 1 -
+           static_cast<int>((positions - 1) * static_cast<int64_t>(kClasses) / part);
+  };
 
   // Each thread's run of sequences: prefix items and rows, own items and rows
   // before it.
@@ -206,9 +240,12 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArg
       mine[0] += parts;
       mine[1] += parts * tile * a.group;
     }
-    const int own = (max(s_ctx[s] - shared, 0) + part - 1) / part;
-    mine[2] += own;
-    mine[3] += own * a.group;
+    const int own = max(s_ctx[s] - shared, 0);
+    const int full = own / part, rest = own - full * part;
+    if (full > 0) atomicAdd(&s_class[0], full);
+    if (rest > 0) atomicAdd(&s_class[class_of(rest)], 1);
+    mine[2] += full + (rest > 0);
+    mine[3] += (full + (rest > 0)) * a.group;
   }
   const int lane = t % kWave, wave = t / kWave;
   int before[4], total[4];
@@ -228,10 +265,15 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArg
       total[i] += s_scan[w][i];
     }
   }
+  int class_begin = total[0];
+  if (t < kClasses)
+    for (int i = 0; i < t; ++i) class_begin += s_class[i];
+  __syncthreads();
+  if (t < kClasses) s_class[t] = class_begin;
   if (t == 0) a.head->items = min(total[0] + total[2], a.max_items);
+  __syncthreads();
+
   // Prefix items first (they have more rows); own rows behind prefix rows.
-  int item = before[0], row = before[1], own_item = total[0] + before[2],
-      own_row = total[1] + before[3];
   auto put = [&](int at, int seq, int seqs, int begin, int end, int first_row) {
     if (at >= a.max_items || first_row + seqs * a.group > a.max_rows) return;
     SharedItem it{};
@@ -242,10 +284,17 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArg
     it.first_row = first_row;
     a.items[at] = it;
   };
+  int item = before[0], row = before[1], own_row = total[1] + before[3];
   for (int s = s0; s < s1; ++s) {
     int first, last;
     const int shared = shared_of(s, &first, &last);
     const int tile = tile_seqs(s, first, last, shared);
+    // The prefix pieces of every sequence of a tile, by the thread that has it.
+    for (int i = 0; i < tile; ++i) {
+      a.seqs[s + i].prefix_row = row + i * a.group;
+      a.seqs[s + i].prefix_step = tile * a.group;
+      a.seqs[s + i].prefix_parts = (shared + part - 1) / part;
+    }
     if (tile > 0) {
       for (int p = 0; p < shared; p += part) {
         put(item++, s, tile, p, min(p + part, shared), row);
@@ -256,27 +305,13 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(const PlanArg
     const int ctx = s_ctx[s];
     int own = 0;
     for (int p = shared; p < ctx; p += part) {
-      put(own_item++, s, 1, p, min(p + part, ctx), own_row);
+      const int end = min(p + part, ctx);
+      put(atomicAdd(&s_class[class_of(end - p)], 1), s, 1, p, end, own_row);
       own_row += a.group;
       ++own;
     }
     a.seqs[s].own_parts = own;
     if (shared == 0) a.seqs[s].prefix_parts = 0;
-  }
-  // The prefix pieces of every sequence of a tile, by the thread that has it.
-  item = before[0];
-  row = before[1];
-  for (int s = s0; s < s1; ++s) {
-    int first, last;
-    const int shared = shared_of(s, &first, &last);
-    const int tile = tile_seqs(s, first, last, shared);
-    const int parts = (shared + part - 1) / part;
-    for (int i = 0; i < tile; ++i) {
-      a.seqs[s + i].prefix_row = row + i * a.group;
-      a.seqs[s + i].prefix_step = tile * a.group;
-      a.seqs[s + i].prefix_parts = parts;
-    }
-    if (tile > 0) row += parts * tile * a.group;
   }
 }
 
@@ -342,10 +377,14 @@ struct ItemLoop {
     const int swz = v ? swz_v(row) : swz_k(row);
     return static_cast<uint32_t>((row * static_cast<int>(a.c_ts) + ((lane % 16) ^ swz) * 8) * 2);
   }
-  // Element offset of the tile at position p in the caches; an invalid block
-  // id reads block 0 (and is masked).
-  __device__ __forceinline__ int64_t tile_base(int p, bool* ok) const {
-    const int blk = table[p >> a.lb];
+  // Block id of position p, clamped to the item's last position. The loops load
+  // it (a scalar load) a turn before they need it.
+  __device__ __forceinline__ int block_at(int p) const {
+    return table[min(p, it.end - 1) >> a.lb];
+  }
+  // Element offset of the tile at position p, in block blk; an invalid id reads
+  // block 0 (and is masked).
+  __device__ __forceinline__ int64_t tile_base(int p, int blk, bool* ok) const {
     *ok = blk >= 0 && blk < a.num_blocks;
     return *ok ? static_cast<int64_t>(blk) * a.c_bs +
                      static_cast<int64_t>(p & (a.block_size - 1)) * a.c_ts
@@ -416,8 +455,12 @@ struct RowState {
   }
 };
 
+// Where a few-rows wave keeps float c of row r of its sums: 16-byte chunks
+// permuted within the row, or all rows' chunks would share banks.
+__device__ __forceinline__ int sum_at(int r, int c) { return r * kD + (c ^ ((r & 7) * 4)); }
+
 // Up to 16 query rows: wave w takes tiles w, w + kWaves, ... of the positions,
-// staged in two slots of its own, and the waves' sums are joined through LDS.
+// and the waves' sums are joined through LDS.
 template <typename E>
 __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedItem& it,
                                              int kv_head, Lds& s) {
@@ -433,39 +476,32 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
     off_k[u] = x.load_offset(u, false);
     off_v[u] = x.load_offset(u, true);
   }
-  char* ring = s.ring + wave * kSlots * kTileBytes;
-  auto issue = [&](int slot, int k) -> bool {
+  char* tile = s.ring + wave * kTileBytes;
+  auto block_of = [&](int k) { return x.block_at(it.begin + k * kTile); };
+  auto issue = [&](int k, int blk) -> bool {
     bool ok;
-    const int64_t base = x.tile_base(it.begin + k * kTile, &ok);
-    char* dst = ring + slot * kTileBytes;
+    const int64_t base = x.tile_base(it.begin + k * kTile, blk, &ok);
 #pragma unroll
     for (int u = 0; u < kLoadsPerHalf; ++u) {
-      lds_load16_sbase(x.kc + base, off_k[u], dst + u * kLoadBytes);
-      lds_load16_sbase(x.vc + base, off_v[u], dst + kHalfBytes + u * kLoadBytes);
+      lds_load16_sbase(x.kc + base, off_k[u], tile + u * kLoadBytes);
+      lds_load16_sbase(x.vc + base, off_v[u], tile + kHalfBytes + u * kLoadBytes);
     }
     return ok;
   };
-  {
+  const int blk0 = block_of(wave);
+  int blk_next = block_of(wave + kWaves);
+  if (wave < kLoadsPerHalf) {
     // A quarter of the query rows each.
     const int r = 4 * wave + lane / 16;
     lds_load16(x.query_row(r) + ((lane % 16) ^ swz_k(r)) * 8, s.q + wave * kLoadBytes);
   }
-  bool ok0 = false, ok1 = false;  // of the slots
-  int issued = 0;
+  bool ok = false;
   if (wave < ntiles) {
-    ok0 = issue(0, wave);
-    ++issued;
-  }
-  if (wave + kWaves < ntiles) {
-    ok1 = issue(1, wave + kWaves);
-    ++issued;
-  }
-  if (issued == 2)
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerTile));
-  else if (issued == 1)
+    ok = issue(wave, blk0);
     __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerTile));
-  else
+  } else {
     __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+  }
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -473,37 +509,39 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
   if (wave < ntiles) {
     typename M::vec8 qf[kD / 32];
     x.row_fragments(s.q, qf);
-    int slot = 0;
     for (int k = wave;; k += kWaves) {
-      if (k + kWaves < ntiles)
-        __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerTile));
-      else
-        __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
       asm volatile("" ::: "memory");
-      char* cur = ring + slot * kTileBytes;
-      const bool ok = slot ? ok1 : ok0;
       const int p0 = it.begin + k * kTile;
       if (!ok || p0 + kTile > it.end) {
         // Masked rows may hold anything, and 0 * NaN is NaN: zero their V.
         const int r = lane / 4;
         if (!ok || p0 + r >= it.end) {
-          char* v = cur + kHalfBytes + r * kRowBytes + (lane % 4) * 64;
+          char* v = tile + kHalfBytes + r * kRowBytes + (lane % 4) * 64;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<Pack<uint32_t, 4>*>(v + c * 16) = zero_pack<uint32_t, 4>();
         }
       }
       typename M::vec8 kf[kD / 32];
-      x.row_fragments(cur, kf);
+      x.row_fragments(tile, kf);
       short4_t vf[kD / 16];
-      x.v_fragments(cur + kHalfBytes, vf);
+      x.v_fragments(tile + kHalfBytes, vf);
       f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < kD / 32; ++ks) sc = M::qk(kf[ks], qf[ks], sc);
+      const bool cur_ok = ok;
+      if (k + kWaves < ntiles) {
+        // The tile's fragments are in registers: refill it.
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        ok = issue(k + kWaves, blk_next);
+        blk_next = block_of(k + 2 * kWaves);
+      }
       float tmax = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sc[i] = ok && p0 + 4 * quad + i < it.end ? sc[i] * a.scale_log2 : -INFINITY;
+        sc[i] = cur_ok && p0 + 4 * quad + i < it.end ? sc[i] * a.scale_log2 : -INFINITY;
         tmax = fmaxf(tmax, sc[i]);
       }
       row.see(tmax, lane);
@@ -514,25 +552,17 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
 #pragma unroll
       for (int db = 0; db < kD / 16; ++db) row.o[db] = M::pv(vf[db], pf, row.o[db]);
       if (k + kWaves >= ntiles) break;
-      if (k + kSlots * kWaves < ntiles) {
-        // This slot's fragment reads have returned; refill it.
-        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-        asm volatile("" ::: "memory");
-        const bool next = issue(slot, k + kSlots * kWaves);
-        if (slot) ok1 = next; else ok0 = next;
-      }
-      slot ^= 1;
     }
   }
-  // No load of this wave is in flight and its fragments are read: its slots
-  // take its sums.
+  // No load of this wave is in flight and its fragments are read: its tile
+  // takes its sums.
   __builtin_amdgcn_s_waitcnt(0x0070);
   asm volatile("" ::: "memory");
   row.close(lane);
-  float* acc = reinterpret_cast<float*>(ring);
+  float* acc = reinterpret_cast<float*>(tile);
 #pragma unroll
   for (int db = 0; db < kD / 16; ++db)
-    *reinterpret_cast<f32x4_t*>(acc + col * kAccStride + db * 16 + 4 * quad) = row.o[db];
+    *reinterpret_cast<f32x4_t*>(acc + sum_at(col, db * 16 + 4 * quad)) = row.o[db];
   if (quad == 0) {
     s.m[wave][col] = row.m;
     s.l[wave][col] = row.l;
@@ -549,9 +579,7 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
       const float mw = s.m[w][r];
       const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
       ls = fmaf(f, s.l[w][r], ls);
-      os = fmaf(f,
-                reinterpret_cast<const float*>(s.ring + w * kSlots * kTileBytes)
-                    [r * kAccStride + d], os);
+      os = fmaf(f, reinterpret_cast<const float*>(s.ring + w * kTileBytes)[sum_at(r, d)], os);
     }
     const int64_t at = static_cast<int64_t>(it.first_row + r) * a.num_kv_heads + kv_head;
     a.ws_acc[at * kD + d] = os;
@@ -562,8 +590,10 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
   }
 }
 
-// More query rows: the workgroup walks the positions in stages of 32 that all
-// its waves load and read, and wave w has rows 16 w .. 16 w + 15 of each.
+// More query rows: the workgroup walks the positions in stages of 64 that all
+// its waves load; wave w has rows 16 (w % 4) .. + 15 and 32 of the positions
+// of each stage, the first for waves 0-3, the second for waves 4-7, whose sums
+// are joined at the end.
 template <typename E>
 __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedItem& it,
                                               int kv_head, Lds& s) {
@@ -572,79 +602,79 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
   using vec8 = typename M::vec8;
   using R = uint16_t;
   const Loop x(a, it, kv_head);
-  const int lane = x.lane, wave = x.wave, quad = x.quad;
-  const int nstages = (it.end - it.begin + kStageTiles * kTile - 1) / (kStageTiles * kTile);
-  const int last = it.end - 1;
-  // Wave w loads K (even w) or V (odd) of tile w / 2.
+  const int lane = x.lane, wave = x.wave, col = x.col, quad = x.quad;
+  const int row_wave = wave % kRowWaves, key_wave = wave / kRowWaves;
+  constexpr int kStage = kStageTiles * kTile;
+  const int nstages = (it.end - it.begin + kStage - 1) / kStage;
+  // Wave w loads K (even w) or V (odd) of tile w / 2, one of the two that it
+  // computes with.
   const bool loads_v = wave & 1;
   const R* half = loads_v ? x.vc : x.kc;
   uint32_t off[kLoadsPerHalf];
 #pragma unroll
   for (int u = 0; u < kLoadsPerHalf; ++u) off[u] = x.load_offset(u, loads_v);
-  // Issues this wave's part of stage k; which of its tiles are valid.
-  auto issue = [&](int k) -> int {
-    const int p = it.begin + k * kStageTiles * kTile;
-    bool ok[kStageTiles];
-    int64_t base[kStageTiles];
+  // First position of this wave's two tiles in stage k.
+  auto begin_of = [&](int k) { return it.begin + k * kStage + key_wave * kWaveTiles * kTile; };
+  struct Blocks {
+    int id[kWaveTiles];
+  };
+  auto blocks_of = [&](int k) {
+    Blocks b;
 #pragma unroll
-    for (int j = 0; j < kStageTiles; ++j)  // a tile past the end: any valid position
-      base[j] = x.tile_base(min(p + j * kTile, last & ~(kTile - 1)), &ok[j]);
-    const int64_t mine = wave / 2 ? base[1] : base[0];
-    char* dst = s.ring + (k % kStages) * kStageBytes + wave * kHalfBytes;
+    for (int j = 0; j < kWaveTiles; ++j) b.id[j] = x.block_at(begin_of(k) + j * kTile);
+    return b;
+  };
+  // Issues this wave's part of stage k; which of its two tiles are valid. A
+  // tile past the end reads the last one.
+  const int last_tile = (it.end - 1) & ~(kTile - 1);
+  auto issue = [&](int k, const Blocks& blocks) -> int {
+    bool ok[kWaveTiles];
+    int64_t base[kWaveTiles];
+#pragma unroll
+    for (int j = 0; j < kWaveTiles; ++j)
+      base[j] = x.tile_base(min(begin_of(k) + j * kTile, last_tile), blocks.id[j], &ok[j]);
+    const int64_t mine = wave / 2 % kWaveTiles ? base[1] : base[0];
+    char* dst = s.ring + (k & 1) * kStageBytes + wave * kHalfBytes;
 #pragma unroll
     for (int u = 0; u < kLoadsPerHalf; ++u)
       lds_load16_sbase(half + mine, off[u], dst + u * kLoadBytes);
     return (ok[0] ? 1 : 0) | (ok[1] ? 2 : 0);
   };
-  // The wave's own query rows wait in the last stage's buffer, which is filled
+  // The wave's query rows wait in the second stage's buffer, which is filled
   // when the first stage is read.
-  char* q_tile = s.ring + (kStages - 1) * kStageBytes + wave * kHalfBytes;
+  char* q_tile = s.ring + kStageBytes + wave * kHalfBytes;
 #pragma unroll
   for (int u = 0; u < kLoadsPerHalf; ++u) {
     const int r = 4 * u + lane / 16;
-    lds_load16(x.query_row(16 * wave + r) + ((lane % 16) ^ swz_k(r)) * 8,
+    lds_load16(x.query_row(kTile * row_wave + r) + ((lane % 16) ^ swz_k(r)) * 8,
                q_tile + u * kLoadBytes);
   }
-  int ok[kStages] = {0, 0, 0, 0};
-  ok[0] = issue(0);
-  if (nstages > 1) ok[1] = issue(1);
-  if (nstages > 2) ok[2] = issue(2);
-  if (nstages > 2)
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(3 * kLoadsPerHalf));
-  else if (nstages > 1)
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerHalf));
-  else
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerHalf));
+  const Blocks first = blocks_of(0);
+  Blocks next = blocks_of(1);
+  int ok = issue(0, first);
+  __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerHalf));
   asm volatile("" ::: "memory");
   vec8 qf[kD / 32];
   x.row_fragments(q_tile, qf);
-  const bool active = 16 * wave < x.rows;
+  const bool active = kTile * row_wave < x.rows;
   RowState row;
   for (int k = 0; k < nstages; ++k) {
     // Stage k's loads of this wave are done, its earlier reads too; behind the
     // barrier those of every wave are.
-    const int younger = min(2, nstages - 1 - k);
-    if (younger == 0)
-      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-    else if (younger == 1)
-      __builtin_amdgcn_s_waitcnt(vmcnt_only(kLoadsPerHalf));
-    else
-      __builtin_amdgcn_s_waitcnt(vmcnt_only(2 * kLoadsPerHalf));
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int now = ok[0];
-    ok[0] = ok[1];
-    ok[1] = ok[2];
-    if (k + 3 < nstages) ok[2] = issue(k + 3);
-    if (!active) continue;
-    const char* stage = s.ring + (k % kStages) * kStageBytes;
-    const int p0 = it.begin + k * kStageTiles * kTile;
-    f32x4_t sc[kStageTiles];
-    short4_t vf[kStageTiles][kD / 16];
+    const int now = ok;
+    if (k + 1 < nstages) ok = issue(k + 1, next);
+    next = blocks_of(k + 2);
+    const int p0 = begin_of(k);
+    if (!active || p0 >= it.end) continue;
+    const char* stage = s.ring + (k & 1) * kStageBytes + key_wave * kWaveTiles * kTileBytes;
+    f32x4_t sc[kWaveTiles];
+    short4_t vf[kWaveTiles][kD / 16];
 #pragma unroll
-    for (int j = 0; j < kStageTiles; ++j) {
+    for (int j = 0; j < kWaveTiles; ++j) {
       vec8 kf[kD / 32];
       x.row_fragments(stage + j * kTileBytes, kf);
       x.v_fragments(stage + j * kTileBytes + kHalfBytes, vf[j]);
@@ -653,9 +683,9 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
       for (int ks = 0; ks < kD / 32; ++ks) sc[j] = M::qk(kf[ks], qf[ks], sc[j]);
     }
     float tmax = -INFINITY;
-    if (now == 3 && p0 + kStageTiles * kTile <= it.end) {
+    if (now == 3 && p0 + kWaveTiles * kTile <= it.end) {
 #pragma unroll
-      for (int j = 0; j < kStageTiles; ++j)
+      for (int j = 0; j < kWaveTiles; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sc[j][i] *= a.scale_log2;
@@ -665,7 +695,7 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
       // Masked positions: no score, and zeros for whatever their V rows hold
       // (0 * NaN is NaN).
 #pragma unroll
-      for (int j = 0; j < kStageTiles; ++j) {
+      for (int j = 0; j < kWaveTiles; ++j) {
         short4_t keep;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -683,7 +713,7 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
     // tile j, for the weights as for V.
     Pack<R, 8> pk;
 #pragma unroll
-    for (int j = 0; j < kStageTiles; ++j)
+    for (int j = 0; j < kWaveTiles; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) pk.v[4 * j + i] = row.template weigh<E>(sc[j][i]);
     const vec8 pf = __builtin_bit_cast(vec8, pk);
@@ -695,28 +725,50 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
     }
   }
   row.close(lane);
-  const int r = 16 * wave + x.col;
-  if (r >= x.rows) return;
+  // Every wave has read its last stage, no load is in flight: the second key
+  // waves' sums go through the ring.
+  __syncthreads();
+  float* acc = reinterpret_cast<float*>(s.ring) + (row_wave * kTile + col) * kAccStride + 4 * quad;
+  if (key_wave == 1 && active) {
+#pragma unroll
+    for (int db = 0; db < kD / 16; ++db) *reinterpret_cast<f32x4_t*>(acc + db * 16) = row.o[db];
+    if (quad == 0) {
+      s.m[row_wave][col] = row.m;
+      s.l[row_wave][col] = row.l;
+    }
+  }
+  __syncthreads();
+  const int r = kTile * row_wave + col;
+  if (key_wave == 1 || r >= x.rows) return;
+  const float m1 = s.m[row_wave][col];
+  const float m = fmaxf(row.m, m1);
+  const float f0 = row.m == -INFINITY ? 0.f : fast_exp2(row.m - m);
+  const float f1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m);
   const int64_t at = static_cast<int64_t>(it.first_row + r) * a.num_kv_heads + kv_head;
 #pragma unroll
-  for (int db = 0; db < kD / 16; ++db)
-    *reinterpret_cast<f32x4_t*>(a.ws_acc + at * kD + db * 16 + 4 * quad) = row.o[db];
+  for (int db = 0; db < kD / 16; ++db) {
+    const f32x4_t other = *reinterpret_cast<const f32x4_t*>(acc + db * 16);
+    f32x4_t sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = fmaf(row.o[db][i], f0, other[i] * f1);
+    *reinterpret_cast<f32x4_t*>(a.ws_acc + at * kD + db * 16 + 4 * quad) = sum;
+  }
   if (quad == 0) {
-    a.ws_ml[at * 2] = row.m;
-    a.ws_ml[at * 2 + 1] = row.l;
+    a.ws_ml[at * 2] = m;
+    a.ws_ml[at * 2 + 1] = fmaf(row.l, f0, s.l[row_wave][col] * f1);
   }
 }
 
 template <typename E>
-__global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(const SharedArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void shared_decode_kernel(const SharedArgs a) {
   __shared__ Lds s;
   typedef int32_t int8v __attribute__((ext_vector_type(8)));
   using ConstItem = __attribute__((address_space(4))) const int8v;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
   const int kv_head = blockIdx.x % a.num_kv_heads;
   const int w = blockIdx.x / a.num_kv_heads;
-  if (w >= ((const ConstI32*)(a.head))[0]) return;
   const SharedItem it = __builtin_bit_cast(SharedItem, ((ConstItem*)(a.items))[w]);
+  if (w >= ((const ConstI32*)(a.head))[0]) return;
   // A foreign plan can give wrong attention, never an access out of bounds.
   if (it.seq < 0 || it.seqs < 1 || it.seqs > kMaxRows / a.group ||
       it.seq > a.num_seqs - it.seqs || it.begin < 0 || it.begin % kTile != 0 ||
@@ -729,9 +781,10 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(const Shared
     run_many_rows<E>(a, it, kv_head, s);
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 128;
 constexpr int kJoinLanes = kD / 4;  // a float4 each
 constexpr int kJoinWays = kJoinThreads / kJoinLanes;
+constexpr int kJoinBatch = 4;
 
 // (m, l, o) += 2^(..) of another piece; pieces of no position weigh nothing.
 __device__ __forceinline__ void join_piece(float& m, float& l, f32x4_t& o, float mb, float lb,
@@ -745,8 +798,8 @@ __device__ __forceinline__ void join_piece(float& m, float& l, f32x4_t& o, float
   m = mnew;
 }
 
-// One query row of one sequence from its pieces: way w of 8 joins pieces w, w
-// + 8, ... (two at a time), then the ways are joined in order.
+// One query row of one sequence from its pieces: way w of 4 joins pieces w, w
+// + 4, ... (four at a time), then the ways are joined in order.
 template <typename E>
 __global__ __launch_bounds__(kJoinThreads) void shared_join_kernel(const SharedArgs a) {
   __shared__ f32x4_t s_o[kJoinWays][kJoinLanes];
@@ -765,23 +818,25 @@ __global__ __launch_bounds__(kJoinThreads) void shared_join_kernel(const SharedA
   const int parts = prefix_parts + min(max(q.own_parts, 0), a.max_items);
   float m = -INFINITY, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int p0 = way; p0 < parts; p0 += 2 * kJoinWays) {
-    float mb[2], lb[2];
-    f32x4_t ob[2];
+  for (int p0 = way; p0 < parts; p0 += kJoinBatch * kJoinWays) {
+    float mb[kJoinBatch], lb[kJoinBatch];
+    f32x4_t ob[kJoinBatch];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kJoinBatch; ++b) {
       const int p = min(p0 + b * kJoinWays, parts - 1);
       int64_t row = p < prefix_parts
                         ? q.prefix_row + static_cast<int64_t>(p) * q.prefix_step
                         : q.own_row + static_cast<int64_t>(p - prefix_parts) * a.group;
       row = min(max(row + g, int64_t(0)), static_cast<int64_t>(a.max_rows - 1));
       const int64_t at = row * a.num_kv_heads + kv_head;
-      mb[b] = a.ws_ml[at * 2];
-      lb[b] = a.ws_ml[at * 2 + 1];
+      const Float2 ml = *reinterpret_cast<const Float2*>(a.ws_ml + at * 2);
+      mb[b] = ml.x;
+      lb[b] = ml.y;
       ob[b] = *reinterpret_cast<const f32x4_t*>(a.ws_acc + at * kD + lane * 4);
     }
-    join_piece(m, l, o, mb[0], lb[0], ob[0]);
-    if (p0 + kJoinWays < parts) join_piece(m, l, o, mb[1], lb[1], ob[1]);
+#pragma unroll
+    for (int b = 0; b < kJoinBatch; ++b)
+      if (p0 + b * kJoinWays < parts) join_piece(m, l, o, mb[b], lb[b], ob[b]);
   }
   s_o[way][lane] = o;
   if (lane == 0) {
@@ -793,9 +848,11 @@ __global__ __launch_bounds__(kJoinThreads) void shared_join_kernel(const SharedA
 #pragma unroll
   for (int w = 1; w < kJoinWays; ++w) join_piece(m, l, o, s_m[w], s_l[w], s_o[w][lane]);
   const float inv = l > 0.f ? 1.f / l : 0.f;  // no position: zeros
-  uint16_t* out = static_cast<uint16_t*>(a.out) + seq * a.o_ts + head * a.o_hs + lane * 4;
+  Pack<uint16_t, 4> out;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[i] = E::store(o[i] * inv);
+  for (int i = 0; i < 4; ++i) out.v[i] = E::store(o[i] * inv);
+  store_pack<uint16_t, 4>(
+      static_cast<uint16_t*>(a.out) + seq * a.o_ts + head * a.o_hs + lane * 4, out);
 }
 
 // Arguments that plan, sizes and call share; MI_OK if there is a kernel.
@@ -860,6 +917,8 @@ extern "C" int32_t mi_shared_decode_plan(const int32_t* context_lens, int32_t nu
   if (st != MI_OK) return st;
   if (num_groups < 0)
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode_plan: negative num_groups");
+  if (num_groups > kMaxGroups)
+    return fail(MI_ERR_UNSUPPORTED, "mi_shared_decode_plan: more than 4096 groups");
   if (num_seqs == 0) return MI_OK;
   if (!context_lens || (num_groups > 0 && (!group_starts || !shared_blocks)))
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode_plan: null pointer");
@@ -909,8 +968,8 @@ extern "C" int32_t mi_shared_decode(
   if (!query || !key_cache || !value_cache || !block_tables || !out)
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode: null pointer");
   if (off_grid(query, 16) || off_grid(key_cache, 16) || off_grid(value_cache, 16) ||
-      off_grid(out, 2) || off_grid(block_tables, 4) || q_token_stride % 8 || q_head_stride % 8 ||
-      cache_block_stride % 8 || cache_token_stride % 8 || cache_head_stride % 8)
+      off_grid(out, 16) || off_grid(block_tables, 4) || q_token_stride % 8 || q_head_stride % 8 ||
+      out_token_stride % 8 || out_head_stride % 8 || cache_block_stride % 8 || cache_token_stride % 8 || cache_head_stride % 8)
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode: misaligned pointers or strides");
   if (cache_token_stride < 0 || cache_token_stride * kTile >= (int64_t(1) << 30))
     return fail(MI_ERR_UNSUPPORTED, "mi_shared_decode: token stride outside 2^26 elements");

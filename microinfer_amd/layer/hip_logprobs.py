@@ -18,11 +18,11 @@ from microinfer_amd import _lib
 _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 MAX_TOP = 32
 
-# Arrival counters: one zero-filled array per (device, stream), left zero by
-# every launch. Captured launches get their own (_zero_counters). An array
-# outgrown by a larger batch stays alive: launches may still be using it.
-_counters: dict[tuple[int, int], torch.Tensor] = {}
-_retired: list[torch.Tensor] = []
+# Scratch of a stream's launches: arrival counters (zero-filled once, left zero
+# by every launch) and the parts' results. Captured launches get their own
+# (_scratch). Memory outgrown by a larger call goes back to torch's allocator,
+# which reuses it on that stream behind the launches that still use it.
+_scratches: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor]] = {}
 
 
 class TokenLogprobs(NamedTuple):
@@ -32,18 +32,21 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor | None  # float32 [rows, top]
 
 
-def _zero_counters(device: torch.device, stream: int, rows: int) -> torch.Tensor:
+def _scratch(device: torch.device, stream: int, rows: int, nbytes: int):
+    """Counters for ``rows`` rows and ``nbytes`` of workspace."""
     if torch.cuda.is_current_stream_capturing():
         # Part of the graph, so graphs replayed side by side do not share them.
-        return torch.zeros(rows, dtype=torch.int32, device=device)
+        return (torch.zeros(rows, dtype=torch.int32, device=device),
+                torch.empty(nbytes, dtype=torch.uint8, device=device))
     key = (device.index, stream)
-    counters = _counters.get(key)
-    if counters is None or counters.numel() < rows:
-        if counters is not None:
-            _retired.append(counters)
-        counters = torch.zeros(max(rows, 1024), dtype=torch.int32, device=device)
-        _counters[key] = counters
-    return counters
+    have = _scratches.get(key)
+    if have is None or have[0].numel() < rows or have[1].numel() < nbytes:
+        if have is not None:
+            rows, nbytes = max(rows, have[0].numel()), max(nbytes, have[1].numel())
+        have = (torch.zeros(max(rows, 1024), dtype=torch.int32, device=device),
+                torch.empty(max(nbytes, 1 << 18), dtype=torch.uint8, device=device))
+        _scratches[key] = have
+    return have
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0,
@@ -89,36 +92,29 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
 
-    def empty(dtype, *shape):
-        return torch.empty(shape, dtype=dtype, device=device)
-
     result = TokenLogprobs(
-        None if tokens is None else empty(torch.float32, *tokens.shape),
-        empty(torch.float32, rows) if entropy else None,
-        empty(torch.int64, rows, top) if top else None,
-        empty(torch.float32, rows, top) if top else None)
+        None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=device),
+        torch.empty(rows, dtype=torch.float32, device=device) if entropy else None,
+        torch.empty((rows, top), dtype=torch.int64, device=device) if top else None,
+        torch.empty((rows, top), dtype=torch.float32, device=device) if top else None)
     if rows == 0 or not (given or top or entropy):
         return result
-    if tokens is not None:
+    if tokens is not None and (tokens.dtype != torch.int64 or not tokens.is_contiguous()):
         tokens = tokens.to(torch.int64).contiguous()
     if temperatures is not None:
         temperatures = temperatures.contiguous()
-    lib, code = _lib.load(), _lib.dtype_code(logits.dtype)
+    lib, code = _lib.load(), _lib.DTYPE_CODES[logits.dtype]
     need = lib.mi_token_logprobs_workspace_bytes(rows, vocab, top, code)
-
-    def pointer(t):
-        return None if t is None else t.data_ptr()
-
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         stream = _lib.stream_handle(device)
-        workspace = counters = None
+        counters = workspace = None
         if need:
-            workspace = empty(torch.uint8, need)
-            counters = _zero_counters(device, stream, rows)
+            counters, workspace = _scratch(device, stream, rows, need)
         status = lib.mi_token_logprobs(
-            logits.data_ptr(), logits.stride(0), rows, vocab, code, pointer(temperatures),
-            pointer(tokens), given, given, pointer(result.logprobs), pointer(result.entropy),
-            pointer(result.top_tokens), pointer(result.top_logprobs), top, pointer(workspace),
-            need, pointer(counters), stream)
+            logits.data_ptr(), logits.stride(0), rows, vocab, code,
+            *[None if t is None else t.data_ptr() for t in (temperatures, tokens)], given, given,
+            *[None if t is None else t.data_ptr() for t in result], top,
+            None if workspace is None else workspace.data_ptr(), need,
+            None if counters is None else counters.data_ptr(), stream)
     _lib.check(status, "mi_token_logprobs")
     return result

@@ -27,6 +27,23 @@ from microinfer_amd.layer.hip_paged_attention import (_check_caches, _index32,
 MAX_SEQS = 4096
 
 
+# Workspaces by (device, stream): the calls on a stream run one after the other.
+# Captured calls get their own. One outgrown by a larger call goes back to
+# torch's allocator, which reuses it on that stream behind the calls before.
+_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, stream)
+    have = _workspaces.get(key)
+    if have is None or have.numel() < nbytes:
+        have = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _workspaces[key] = have
+    return have
+
+
 @dataclass(frozen=True)
 class SharedDecodePlan:
     """One step's work (``shared_decode_plan``), for calls of its sizes."""
@@ -66,6 +83,8 @@ def shared_decode_plan(context_lens: torch.Tensor, group_starts: torch.Tensor,
     groups = shared_blocks.numel()
     if group_starts.numel() != groups + 1 and (groups or group_starts.numel()):
         raise ValueError("group_starts must have one entry more than shared_blocks")
+    if groups > MAX_SEQS:
+        raise ValueError(f"at most {MAX_SEQS} groups")
     if any(t.device != context_lens.device for t in (group_starts, shared_blocks)):
         raise ValueError("context_lens, group_starts and shared_blocks must share a device")
     num_seqs = context_lens.numel()
@@ -83,7 +102,7 @@ def shared_decode_plan(context_lens: torch.Tensor, group_starts: torch.Tensor,
     context_lens, group_starts, shared_blocks = (
         _index32(t) for t in (context_lens, group_starts, shared_blocks))
     lib = _lib.load()
-    with torch.cuda.device(context_lens.device):
+    with _lib.on_device(context_lens.device):
         nbytes = lib.mi_shared_decode_plan_bytes(num_seqs, num_q_heads, num_kv_heads)
         buffer = torch.empty(nbytes, dtype=torch.uint8, device=context_lens.device)
         status = lib.mi_shared_decode_plan(
@@ -135,16 +154,16 @@ def hip_shared_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
         scale = 1.0 / math.sqrt(head_dim)
     lib = _lib.load()
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    with torch.cuda.device(query.device):
+    with _lib.on_device(query.device):
         ws_bytes = lib.mi_shared_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads)
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device)
+        stream = _lib.stream_handle(query.device)
+        workspace = _workspace(query.device, stream, ws_bytes)
         status = lib.mi_shared_decode(
             query.data_ptr(), query.stride(0), query.stride(1), key_cache.data_ptr(),
             value_cache.data_ptr(), *key_cache.stride()[:3], block_tables.data_ptr(),
             block_tables.stride(0), block_tables.shape[1], plan.buffer.data_ptr(),
             plan.buffer.numel(), out.data_ptr(), out.stride(0), out.stride(1),
             workspace.data_ptr(), ws_bytes, num_seqs, num_q_heads, num_kv_heads, head_dim,
-            block_size, num_blocks, float(scale), _lib.dtype_code(query.dtype),
-            _lib.stream_handle(query.device))
+            block_size, num_blocks, float(scale), _lib.DTYPE_CODES[query.dtype], stream)
     _lib.check(status, "mi_shared_decode")
     return out

@@ -67,7 +67,7 @@ def copy_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor, src, dst, *,
     if pairs == 0 or layers == 0:
         return
     layer_stride = key_cache.stride(0) if key_cache.ndim == 5 else 0
-    with torch.cuda.device(key_cache.device):
+    with _lib.on_device(key_cache.device):
         status = _lib.load().mi_kv_copy_blocks(
             key_cache.data_ptr(), value_cache.data_ptr(), layer_stride, *key_cache.stride()[-4:-1],
             sources.buffer_info()[0], targets.buffer_info()[0],

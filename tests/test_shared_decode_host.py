@@ -68,6 +68,7 @@ def test_shapes_are_checked_before_launch(call):
 def test_plan_pointers_are_checked():
     lib = _lib.load()
     assert _plan_call(lib, groups=-1) == 1 and "num_groups" in _lib.last_error()
+    assert _plan_call(lib, groups=4097) == 2 and "groups" in _lib.last_error()
     for name in ("lens", "starts", "shared"):
         assert _plan_call(lib, **{name: None}) == 1 and "null" in _lib.last_error()
         assert _plan_call(lib, **{name: 4098}) == 1 and "misaligned" in _lib.last_error()
@@ -82,7 +83,7 @@ def test_call_pointers_are_checked():
     for name in ("q", "kc", "vc", "tables", "out"):
         assert _call(lib, **{name: None}) == 1 and "null" in _lib.last_error()
         assert _call(lib, **{name: 4097}) == 1 and "misaligned" in _lib.last_error()
-    for name in ("q_ts", "q_hs", "bs", "ts", "hs"):
+    for name in ("q_ts", "q_hs", "bs", "ts", "hs", "o_ts", "o_hs"):
         assert _call(lib, **{name: 100}) == 1 and "misaligned" in _lib.last_error()
     assert _call(lib, blocks=0) == 1
     assert _call(lib, ts=1 << 27) == 2 and "stride" in _lib.last_error()

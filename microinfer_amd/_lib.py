@@ -19,6 +19,7 @@ import torch
 LIBRARY_PATH = Path(__file__).resolve().parent / "libmi_attn.so"
 
 MI_OK = 0
+MI_ERR_INVALID_ARGUMENT = 1
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 _P = ctypes.c_void_p

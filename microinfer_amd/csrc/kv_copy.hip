@@ -31,7 +31,7 @@ struct PageShape {
   uint32_t size[3];
   int32_t token_dim;  // which of the three counts tokens
   uint32_t words_per_row;
-  uint32_t words;  // words of a page, K and V
+  uint32_t words_per_token;  // all heads, K and V
   int64_t layer_stride, block_stride;  // bytes
 };
 
@@ -51,47 +51,63 @@ struct GroupList {
   uint16_t start[kMaxOps + 1];
 };
 
-constexpr int kCopyThreads = 256;
-constexpr int kCopyUnroll = 4;
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
 
-// Byte offset of word w inside a page, and its token row.
-__device__ __forceinline__ int64_t word_offset(const PageShape& p, uint32_t w, int word_bytes,
-                                               int* token) {
+constexpr int kCopyThreads = 256;
+// Words in flight per thread: 1, 8 and 64 forked pages of 28 layers 2.5, 3.4 and
+// 15.3 us with two, 2.7, 3.5 and 16.0 with four, 3.2, 4.2 and 16.3 with eight.
+constexpr int kCopyUnroll = 2;
+// More bytes than the last-level cache holds: nothing read stays in it, so
+// reading past it costs nothing and leaves it to others (1000 pages of 28
+// layers 706 us, 721 without). Fewer may lie in it, as forked pages do, which
+// were just written (64 of them 16 us, 30 past it).
+constexpr int64_t kStreamBytes = int64_t(1) << 28;
+
+// Byte offset of word w among the words of a page's first `tokens` rows, and
+// its token row.
+__device__ __forceinline__ int64_t word_offset(const PageShape& p, uint32_t tokens, uint32_t w,
+                                               int word_bytes, uint32_t* token) {
+  const uint32_t size0 = p.token_dim == 0 ? tokens : p.size[0];
+  const uint32_t size1 = p.token_dim == 1 ? tokens : p.size[1];
   const uint32_t row = w / p.words_per_row;
   const uint32_t col = w - row * p.words_per_row;
-  const uint32_t r1 = row / p.size[0];
-  const uint32_t i0 = row - r1 * p.size[0];
-  const uint32_t i2 = r1 / p.size[1];
-  const uint32_t i1 = r1 - i2 * p.size[1];
+  const uint32_t r1 = row / size0;
+  const uint32_t i0 = row - r1 * size0;
+  const uint32_t i2 = r1 / size1;
+  const uint32_t i1 = r1 - i2 * size1;
   *token = p.token_dim == 0 ? i0 : p.token_dim == 1 ? i1 : i2;
   return i0 * p.stride[0] + i1 * p.stride[1] + i2 * p.stride[2] +
          static_cast<int64_t>(col) * word_bytes;
 }
 
-// One slice of one pair's page in one layer: a workgroup.
-template <typename W>
+// One slice of one pair's rows in one layer: a workgroup. All of a thread's
+// loads are issued before its first store (words past the end load the page's
+// first), and the stores are not kept in the caches, where nobody reads them
+// before the next step: they would push out what is read.
+template <typename W, bool STREAM>
 __global__ __launch_bounds__(kCopyThreads) void kv_copy_kernel(char* base, const PageShape p,
-                                                              const CopyList list, int slices) {
-  const int pair = blockIdx.x / slices;
-  const int slice = blockIdx.x - pair * slices;
-  const CopyOp op = list.op[pair];
-  char* layer = base + blockIdx.y * p.layer_stride;
+                                                              const CopyList list) {
+  const CopyOp op = list.op[blockIdx.y];
+  const uint32_t words = p.words_per_token * op.tokens;
+  const uint32_t first = blockIdx.x * (kCopyThreads * kCopyUnroll);
+  if (first >= words) return;
+  char* layer = base + blockIdx.z * p.layer_stride;
   const char* from = layer + op.src * p.block_stride;
   char* to = layer + op.dst * p.block_stride;
   W v[kCopyUnroll];
   int64_t off[kCopyUnroll];
-  bool there[kCopyUnroll];
 #pragma unroll
   for (int u = 0; u < kCopyUnroll; ++u) {
-    const uint32_t w = (slice * kCopyUnroll + u) * kCopyThreads + threadIdx.x;
-    int token;
-    off[u] = word_offset(p, w, sizeof(W), &token);
-    there[u] = w < p.words && token < op.tokens;
-    if (there[u]) v[u] = *reinterpret_cast<const W*>(from + off[u]);
+    const uint32_t w = first + u * kCopyThreads + threadIdx.x;
+    uint32_t token;
+    off[u] = word_offset(p, op.tokens, w < words ? w : 0, sizeof(W), &token);
+    const W* at = reinterpret_cast<const W*>(from + off[u]);
+    v[u] = STREAM ? __builtin_nontemporal_load(at) : *at;
   }
 #pragma unroll
   for (int u = 0; u < kCopyUnroll; ++u)
-    if (there[u]) *reinterpret_cast<W*>(to + off[u]) = v[u];
+    if (first + u * kCopyThreads + threadIdx.x < words)
+      __builtin_nontemporal_store(v[u], reinterpret_cast<W*>(to + off[u]));
 }
 
 // Dependent copies: a thread per word of the page walks its group's ops.
@@ -102,13 +118,14 @@ __global__ __launch_bounds__(kCopyThreads) void kv_copy_group_kernel(char* base,
                                                                     int slices) {
   const int group = blockIdx.x / slices;
   const uint32_t w = (blockIdx.x - group * slices) * kCopyThreads + threadIdx.x;
-  if (w >= p.words) return;
-  int token;
-  char* at = base + blockIdx.y * p.layer_stride + word_offset(p, w, sizeof(W), &token);
+  if (w >= p.words_per_token * p.size[p.token_dim]) return;
+  uint32_t token;
+  char* at = base + blockIdx.y * p.layer_stride +
+             word_offset(p, p.size[p.token_dim], w, sizeof(W), &token);
   W kept{};
   for (int i = list.start[group]; i < list.start[group + 1]; ++i) {
     const CopyOp op = list.op[i];
-    if (token >= op.tokens) continue;
+    if (token >= static_cast<uint32_t>(op.tokens)) continue;
     W v = kept;
     if (op.src >= 0) v = *reinterpret_cast<const W*>(at + op.src * p.block_stride);
     if (op.dst >= 0)
@@ -183,24 +200,34 @@ void order_pairs(const std::vector<CopyOp>& ops, const std::vector<int32_t>& int
 }
 
 template <typename W>
-int32_t launch_copies(char* base, const PageShape& shape, int32_t layers, const Order& order,
-                      hipStream_t stream) {
+int32_t launch_copies(char* base, const PageShape& shape, int32_t row_bytes, int32_t layers,
+                      const Order& order, hipStream_t stream) {
   PageShape p = shape;
-  const uint32_t row_words = p.words_per_row / sizeof(W);  // words_per_row holds bytes here
-  p.words_per_row = row_words;
-  p.words = row_words * p.size[0] * p.size[1] * p.size[2];
-  const int per = kCopyThreads * kCopyUnroll;
-  const int slices = static_cast<int>((p.words + per - 1) / per);
+  p.words_per_row = row_bytes / sizeof(W);
+  p.words_per_token = p.words_per_row;
+  for (int i = 0; i < 3; ++i)
+    if (i != p.token_dim) p.words_per_token *= p.size[i];
+  const uint32_t page_words = p.words_per_token * p.size[p.token_dim];
+  const uint32_t per = kCopyThreads * kCopyUnroll;
+  int64_t tokens = 0;
+  for (const CopyOp& op : order.single) tokens += op.tokens;
+  const bool stream_reads = tokens * p.words_per_token * layers > kStreamBytes / int64_t(sizeof(W));
   for (size_t i = 0; i < order.single.size(); i += kMaxOps) {
     const int n = static_cast<int>(std::min<size_t>(kMaxOps, order.single.size() - i));
     CopyList list;
     std::copy_n(order.single.begin() + i, n, list.op);
-    kv_copy_kernel<W><<<dim3(n * slices, layers), kCopyThreads, 0, stream>>>(base, p, list,
-                                                                           slices);
+    int32_t most = 0;
+    for (int k = 0; k < n; ++k) most = std::max(most, list.op[k].tokens);
+    const uint32_t slices = (p.words_per_token * most + per - 1) / per;
+    const dim3 grid(slices, n, layers);
+    if (stream_reads)
+      kv_copy_kernel<W, true><<<grid, kCopyThreads, 0, stream>>>(base, p, list);
+    else
+      kv_copy_kernel<W, false><<<grid, kCopyThreads, 0, stream>>>(base, p, list);
     const int32_t status = check_launch("mi_kv_copy_blocks");
     if (status != MI_OK) return status;
   }
-  const int thin = static_cast<int>((p.words + kCopyThreads - 1) / kCopyThreads);
+  const uint32_t thin = (page_words + kCopyThreads - 1) / kCopyThreads;
   GroupList list;
   int ops = 0, groups = 0;
   auto flush = [&]() {
@@ -281,15 +308,14 @@ int32_t copy_blocks(char* keys, char* values, int64_t layer_stride, int64_t bloc
     p.size[i] = dims[i].size;
     if (dims[i].token) p.token_dim = i;
   }
-  p.words_per_row = row_bytes;
   p.layer_stride = layer_stride;
   p.block_stride = block_stride;
   const uint64_t bits = static_cast<uint64_t>(row_bytes) | layer_stride | block_stride |
                         token_stride | head_stride | reinterpret_cast<uintptr_t>(keys) |
                         reinterpret_cast<uintptr_t>(values);
-  if ((bits & 15u) == 0) return launch_copies<uint4>(keys, p, num_layers, order, stream);
-  if ((bits & 3u) == 0) return launch_copies<uint32_t>(keys, p, num_layers, order, stream);
-  return launch_copies<uint16_t>(keys, p, num_layers, order, stream);
+  if ((bits & 15u) == 0) return launch_copies<Words4>(keys, p, row_bytes, num_layers, order, stream);
+  if ((bits & 3u) == 0) return launch_copies<uint32_t>(keys, p, row_bytes, num_layers, order, stream);
+  return launch_copies<uint16_t>(keys, p, row_bytes, num_layers, order, stream);
 }
 
 }  // namespace

@@ -36,7 +36,8 @@ def copy_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor, src, dst, *,
     ``key_cache``/``value_cache`` are one layer's ``[blocks, B, Hkv, D]`` views
     or all layers' ``[L, blocks, B, Hkv, D]``, of equal strides. ``src``, ``dst``
     and ``tokens`` (default: whole blocks) are host lists of equal length; no
-    block is written twice. A block may be read by several pairs and be written
+    block is written twice (ValueError, like an id outside the cache, before
+    anything is copied). A block may be read by several pairs and be written
     by another one (chains, swaps and cycles of up to 255 blocks). Runs on the
     current stream; a captured call replays the pairs of its capture.
     """
@@ -56,13 +57,6 @@ def copy_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor, src, dst, *,
     if len(targets) != pairs or (rows is not None and len(rows) != pairs):
         raise ValueError("src, dst and tokens must have one entry per pair")
     num_blocks, block_size = key_cache.shape[-4], key_cache.shape[-3]
-    if pairs and not (0 <= min(sources) and max(sources) < num_blocks
-                      and 0 <= min(targets) and max(targets) < num_blocks):
-        raise ValueError("block id outside the cache")
-    if len(set(targets)) != pairs:
-        raise ValueError("a block is written twice")
-    if rows is not None and pairs and not (0 <= min(rows) and max(rows) <= block_size):
-        raise ValueError("tokens must lie between 0 and the block size")
     layers = key_cache.shape[0] if key_cache.ndim == 5 else 1
     if pairs == 0 or layers == 0:
         return
@@ -74,4 +68,6 @@ def copy_blocks(key_cache: torch.Tensor, value_cache: torch.Tensor, src, dst, *,
             None if rows is None else rows.buffer_info()[0], pairs, layers,
             key_cache.shape[-2], key_cache.shape[-1], block_size, num_blocks,
             _lib.dtype_code(key_cache.dtype), _lib.stream_handle(key_cache.device))
+    if status == _lib.MI_ERR_INVALID_ARGUMENT:  # the lists, before anything is copied
+        raise ValueError(_lib.last_error())
     _lib.check(status, "mi_kv_copy_blocks")

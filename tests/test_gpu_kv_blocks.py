@@ -104,9 +104,38 @@ def test_lists_longer_than_a_launch():
         copy_blocks(k, v, ids[:256], ids[1:256] + ids[:1])
 
 
+def test_refusals_leave_the_pool_alone():
+    cache = _cache(2, 8, 16, 2, 64)
+    k, v = cache.keys, cache.values
+    before = k.clone(), v.clone()
+    for src, dst, tokens, what in [([0, 1], [2, 2], None, "twice"), ([0, 8], [2, 3], None, "id"),
+                                   ([0, -1], [2, 3], None, "id"), ([0, 1], [2, 8], None, "id"),
+                                   ([0, 1], [2, 3], [3, 17], "tokens"),
+                                   ([0, 1], [2, 3], [3, -1], "tokens"), ([0], [2, 3], None, "one"),
+                                   ([0, 1], [2, 3], [3], "one"), ([0.5], [1], None, "src")]:
+        with pytest.raises(ValueError, match=what):
+            copy_blocks(k, v, src, dst, tokens=tokens)
+    with pytest.raises(ValueError, match="host"):
+        copy_blocks(k, v, torch.tensor([0], device=DEV), [1])
+    with pytest.raises(ValueError, match="shapes"):
+        copy_blocks(k, v[:1], [0], [1])
+    with pytest.raises(ValueError, match="layout"):
+        copy_blocks(k, v.clone(memory_format=torch.contiguous_format), [0], [1])
+    with pytest.raises(ValueError, match="dtype"):
+        copy_blocks(k[0], v[0].view(torch.float16), [0], [1])
+    copy_blocks(k, v, [], [])
+    assert torch.equal(k, before[0]) and torch.equal(v, before[1])
+
+
 def test_fork_of_a_model_sized_pool_leaves_the_rest():
     cache = _cache(28, 64, 16, 8, 128)
     _check(cache.keys, cache.values, [5] * 16, list(range(20, 36)), [11] * 16)
+
+
+def test_more_than_the_last_level_cache():
+    cache = _cache(6, 900, 16, 8, 128)
+    ids = random.Random(5).sample(range(900), 900)
+    _check(cache.keys, cache.values, ids[:440], ids[440:880])
 
 
 def test_offsets_past_32_bits():

@@ -150,6 +150,7 @@ __device__ __forceinline__ uint64_t nth_word(uint64_t word, int n) {
 constexpr int kWaveCap = kListCap / kWaves;
 constexpr int kTilePasses = 4;  // packs per thread and tile
 constexpr int kScanLanes = 32;
+constexpr int kKeptWords = 256;  // what compress() leaves at most: kMaxTop per list slice
 
 // LDS of a launch: with the lists of the alternatives, or without.
 template <bool TOP>
@@ -159,11 +160,15 @@ struct Shared {
 };
 template <>
 struct Shared<true> : Shared<false> {
-  // The waves' lists, then the workgroup's (zeros behind its last word).
+  // The waves' lists; joining parts, the row's.
   uint64_t list[kListCap + 8];
   uint64_t kept[kMaxTop];  // the best words, largest first
-  // Packs of lanes whose values are looked through, and whose they are.
-  __attribute__((aligned(16))) char scan[kWaves][kScanLanes * kTilePasses * 16];
+  // Packs of lanes whose values are looked through, and whose they are; once the
+  // tiles are done, the workgroup's list.
+  union {
+    __attribute__((aligned(16))) char scan[kWaves][kScanLanes * kTilePasses * 16];
+    uint64_t best[kWaves * kKeptWords + 8];
+  };
   uint8_t scan_lane[kWaves][kScanLanes];
   uint32_t wave_key[kWaves];    // what each wave contributes to the shared floor
   uint32_t wave_first[kWaves];  // the num_top-th key of each wave's first tile
@@ -191,26 +196,26 @@ __device__ __forceinline__ uint32_t shared_floor(Lists& s) {
 
 // The `top` largest of list[0, n) into kept[0, top), largest first, zeros
 // behind them: each word's rank is the number of larger ones. All threads,
-// after a barrier.
-__device__ void rank_words(Lists& s, int n, int top) {
+// after a barrier; eight words behind the last are overwritten.
+__device__ void rank_words(Lists& s, uint64_t* list, int n, int top) {
   const int t = threadIdx.x;
-  if (t < 8) s.list[n + t] = 0;
+  if (t < 8) list[n + t] = 0;
   if (t < top) s.kept[t] = 0;
   __syncthreads();
   for (int at = t; at < n; at += kThreads) {
-    const uint64_t w = s.list[at];
+    const uint64_t w = list[at];
     int rank = 0;
     for (int j = 0; j < n; j += 8) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) rank += s.list[j + k] > w;
+      for (int k = 0; k < 8; ++k) rank += list[j + k] > w;
     }
     if (rank < top) s.kept[rank] = w;
   }
   __syncthreads();
 }
 
-// Appends the first `want` indices of [lo, hi) whose value has key `key` to the
-// list. All threads.
+// Appends the first `want` indices of [lo, hi) whose value has key `key` to
+// best. All threads.
 template <typename E>
 __device__ void fill_equal(Lists& s, const typename E::raw* row, int lo, int hi, uint32_t key,
                            int want) {
@@ -232,7 +237,7 @@ __device__ void fill_equal(Lists& s, const typename E::raw* row, int lo, int hi,
       all += s.fill[w];
     }
     before += __popcll(hits & ((1ull << lane) - 1));
-    if (hit && before < want) s.list[start + before] = make_word(key_value(key), v);
+    if (hit && before < want) s.best[start + before] = make_word(key_value(key), v);
     found = all;
     __syncthreads();
   }
@@ -395,8 +400,17 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
 
   for (int p0 = pack_begin; p0 < pack_end; p0 += kTilePacks) {
     Pack<R, VEC> x[NP];
+    const int wave_begin = p0 + wave * kWave;
+    const int wave_end = wave_begin + (NP - 1) * kThreads + kWave;
+    if (wave_begin * VEC >= lead && wave_end <= pack_end && wave_end * VEC - lead <= a.vocab) {
+      // All of the wave's packs are whole: its loads go out together.
 #pragma unroll
-    for (int u = 0; u < NP; ++u) x[u] = load_tile(p0, u);
+      for (int u = 0; u < NP; ++u)
+        x[u] = load_pack<R, VEC>(grid + static_cast<int64_t>(wave_begin + u * kThreads + lane) * VEC);
+    } else {
+#pragma unroll
+      for (int u = 0; u < NP; ++u) x[u] = load_tile(p0, u);
+    }
     float tile_max = -INFINITY;
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
@@ -452,16 +466,20 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
       if (was_first) {
         cand.first = false;
         const uint32_t part_key = nth_value_key<E>(lane_key, quarter);
-        const uint32_t all_key = nth_value_key<E>(lane_key, a.top);
+        // A wave may be alone in a short tile.
+        const bool is_short = p0 + kTilePacks > pack_end;
+        const uint32_t all_key = is_short ? nth_value_key<E>(lane_key, a.top) : 0;
         if (lane == 0) {
           share(s, wave, part_key);
-          s.wave_first[wave] = all_key;  // a wave may be alone in a short tile
+          s.wave_first[wave] = all_key;
         }
         __syncthreads();  // every part has a tile, so every wave is here
         cand.floor = shared_floor(s);
+        if (is_short) {
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) cand.floor = max(cand.floor, s.wave_first[w]);
-        cand.floor = __builtin_amdgcn_readfirstlane(cand.floor);
+          for (int w = 0; w < kWaves; ++w) cand.floor = max(cand.floor, s.wave_first[w]);
+          cand.floor = __builtin_amdgcn_readfirstlane(cand.floor);
+        }
       }
       // Puts the tile's values of keys from `least` on behind the list; how many
       // it then has, stored or not. The lanes that have such values put their
@@ -537,6 +555,9 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
     }
   }
 
+  if constexpr (TOP) {
+    if (cand.count > kKeptWords) cand.compress(a.top);
+  }
   // The workgroup's sums, relative to its maximum (of the wave's reference
   // where every value is below it).
   const float wave_max = fmaxf(xor_max<1, kWave>(top_value), kLowest);
@@ -572,27 +593,17 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
     bool open = false;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) open = open || (s.wave_open[w] && s.wave_floor[w] == floor);
-    uint64_t mine[kWaveCap / kWave];
-#pragma unroll
-    for (int i = 0; i < kWaveCap / kWave; ++i) {
-      const int at = i * kWave + lane;
-      mine[i] = at < cand.count ? cand.list[at] : 0;
-    }
-    __syncthreads();
-    if (cand.count > 0) {
-#pragma unroll
-      for (int i = 0; i < kWaveCap / kWave; ++i) {
-        const uint32_t key = static_cast<uint32_t>(mine[i] >> 32);
-        if (key > floor || (key == floor && !open && key != 0))
-          s.list[atomicAdd(&s.count, 1)] = mine[i];
-      }
+    for (int i = lane; i < cand.count; i += kWave) {
+      const uint64_t w = cand.list[i];
+      const uint32_t key = static_cast<uint32_t>(w >> 32);
+      if (key > floor || (key == floor && !open)) s.best[atomicAdd(&s.count, 1)] = w;
     }
     __syncthreads();
     if (open && s.count < a.top)
       fill_equal<E>(s, logits, v_begin, min(a.vocab, pack_end * VEC - lead), floor,
                     a.top - s.count);
     const int n = s.count;
-    rank_words(s, n, a.top);
+    rank_words(s, s.best, n, a.top);
   }
   if (a.parts == 1) {
     write_row<E, TOP>(a, s, row, logits, r, temperature, S, N);
@@ -634,24 +645,20 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
     const int deep = lane / a.parts;
     uint64_t probe = 0;
     if (deep < a.top) probe = word_of(lane - deep * a.parts, deep);
-    const int words = a.parts * a.top;
-    uint64_t mine[kListCap / kThreads];
-#pragma unroll
-    for (int i = 0; i < kListCap / kThreads; ++i) {
-      const int at = i * kThreads + t;
-      mine[i] = 0;
-      if (at < words) mine[i] = word_of(at / a.top, at % a.top);
-    }
-    // Fewer words than that in the sample: no floor.
-    const uint64_t floor = __popcll(__ballot(probe != 0)) >= a.top ? nth_word<E>(probe, a.top) : 0;
+    // Fewer words than that in the sample: no floor but zero's, of no word.
+    uint64_t floor = 1;
+    if (__popcll(__ballot(probe != 0)) >= a.top) floor = nth_word<E>(probe, a.top);
     if (t == 0) s.count = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kListCap / kThreads; ++i)
-      if (mine[i] != 0 && mine[i] >= floor) s.list[atomicAdd(&s.count, 1)] = mine[i];
+    const int words = a.parts * a.top;
+#pragma unroll 2
+    for (int at = t; at < words; at += kThreads) {
+      const uint64_t w = word_of(at / a.top, at % a.top);
+      if (w >= floor) s.list[atomicAdd(&s.count, 1)] = w;
+    }
     __syncthreads();
     const int n = s.count;
-    rank_words(s, n, a.top);
+    rank_words(s, s.list, n, a.top);
   }
   const float all = xor_max<1, kWave>(rs.x);
   S = N = 0.f;
@@ -660,6 +667,8 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
                group_sum<kWave>(N));
 }
 static_assert(kMaxParts <= kWave, "a lane per part");
+static_assert(kMaxTop * (kWaveCap / kWave) <= kKeptWords, "compressed lists fit");
+static_assert(kMaxTop <= kKeptWords, "and a scan's words");
 
 constexpr int kWantParts = 1024;
 

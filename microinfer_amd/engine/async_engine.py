@@ -167,10 +167,20 @@ class _EngineThread(threading.Thread):
                 self.engine.add_request(arg)
                 self.live.add(arg.seq_id)
                 result = arg.seq_id
+            elif kind == "fork":
+                children = self.engine.fork(*arg)
+                self.live.update(seq.seq_id for seq in children)
+                # Their channels exist before the next step's updates arrive.
+                return self.report(self.frontend._settle_fork, future, arg[1],
+                                   [(seq.seq_id, seq.num_prompt_tokens) for seq in children],
+                                   None, self.engine.stats())
             else:  # "abort"
                 result = self.engine.abort(arg)
                 self.live.discard(arg)
-        except Exception as exc:  # a refused admission is raised to its caller
+        except Exception as exc:  # a refused admission or fork is raised to its caller
+            if kind == "fork":
+                return self.report(self.frontend._settle_fork, future, arg[1], [], exc,
+                                   self.engine.stats())
             return self.report(self.frontend._settle, future, None, exc, self.engine.stats())
         return self.report(self.frontend._settle, future, result, None, self.engine.stats())
 
@@ -211,6 +221,7 @@ class AsyncEngine:
         self._thread: _EngineThread | None = None
         self._channels: dict[int, RequestChannel] = {}
         self._engine_stats = engine.stats()
+        self._reserved = 0  # room for forks under way
         self._stopping = False
         self._error: BaseException | None = None
 
@@ -239,6 +250,19 @@ class AsyncEngine:
         else:
             future.set_result(result)
 
+    def _settle_fork(self, future: asyncio.Future, n: int, children, exc, stats) -> None:
+        """A fork's requests, from the engine thread: their channels, to its
+        caller, for whom the room of ``n`` was reserved."""
+        self._reserved -= n
+        if future.cancelled():  # nobody will read them
+            loop = asyncio.get_running_loop()
+            for seq_id, _ in children:
+                self._thread.post("abort", seq_id, loop.create_future())
+            children = []
+        channels = [RequestChannel(*child) for child in children]
+        self._channels.update((channel.seq_id, channel) for channel in channels)
+        self._settle(future, channels, exc, stats)
+
     def _deliver(self, updates, stats) -> None:
         """A step's updates: publish them, then grant the next step."""
         self._engine_stats = stats
@@ -265,8 +289,9 @@ class AsyncEngine:
             raise TypeError("sampling_params must be a SampleParameter")
         if self._stopping:
             raise RuntimeError("AsyncEngine is stopping")
-        if len(self._channels) >= self.max_waiting:
-            raise BackpressureError(f"{len(self._channels)} requests already tracked "
+        tracked = len(self._channels) + self._reserved
+        if tracked >= self.max_waiting:
+            raise BackpressureError(f"{tracked} requests already tracked "
                                     f"(max_waiting={self.max_waiting})")
         seq = Sequence(list(prompt), sampling_params)
         channel = RequestChannel(seq.seq_id, seq.num_prompt_tokens)
@@ -277,6 +302,26 @@ class AsyncEngine:
             del self._channels[seq.seq_id]
             raise
         return channel
+
+    async def fork(self, request: RequestChannel, n: int = 1,
+                   sampling_params: SampleParameter | None = None) -> list[RequestChannel]:
+        """``n`` requests that continue a running one from its tokens so far
+        (``LLMEngine.fork``); their streams begin with those tokens."""
+        if sampling_params is not None and not isinstance(sampling_params, SampleParameter):
+            raise TypeError("sampling_params must be a SampleParameter")
+        if type(n) is not int or n < 1:
+            raise ValueError("the number of forks must be a positive integer")
+        if self._stopping:
+            raise RuntimeError("AsyncEngine is stopping")
+        tracked = len(self._channels) + self._reserved
+        if tracked + n > self.max_waiting:
+            raise BackpressureError(f"{tracked} requests already tracked "
+                                    f"(max_waiting={self.max_waiting})")
+        loop = asyncio.get_running_loop()
+        future = loop.create_future()
+        self._thread_for(loop).post("fork", (request.seq_id, n, sampling_params), future)
+        self._reserved += n
+        return await future
 
     async def abort(self, seq_id: int) -> bool:
         removed = await self._command("abort", seq_id)

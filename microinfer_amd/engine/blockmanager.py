@@ -178,6 +178,64 @@ class BlockManager:
                 self.blocks[block_id].update(h, tokens)
             seq.block_table.append(block_id)
 
+    # -- forks and compaction ------------------------------------------------
+    def can_fork(self, parent: Sequence, children: int) -> bool:
+        """Whether ``children`` forks of ``parent`` fit: each needs a block of
+        its own for a cached last block that is not full."""
+        partial = parent.num_cached_tokens % self.block_size > 0
+        return not partial or len(self._free) >= children
+
+    def fork(self, parent: Sequence, child: Sequence) -> tuple[int, int, int] | None:
+        """Give ``child`` the cached tokens of ``parent``: its full blocks are
+        shared, a last one that is not full becomes a block of the child's own.
+        Returns ``(source, destination, rows)`` of the copy that this needs."""
+        if child.block_table:
+            raise ValueError(f"request {child.seq_id} already owns cache blocks")
+        if not self.can_fork(parent, 1):
+            raise RuntimeError("KV cache has no free blocks")
+        full, rows = divmod(parent.num_cached_tokens, self.block_size)
+        for block_id in parent.block_table[:full]:
+            self.blocks[block_id].ref_count += 1
+            child.block_table.append(block_id)
+        child.num_cached_tokens = parent.num_cached_tokens
+        if rows == 0:
+            return None
+        own = self._allocate_block()
+        child.block_table.append(own)
+        return parent.block_table[full], own, rows
+
+    def compact(self, seqs) -> list[tuple[int, int]]:
+        """Move the blocks in use to the lowest ids and rewrite the tables of
+        ``seqs`` (every sequence that holds blocks). Returns the ``(source,
+        destination)`` moves whose contents the caller copies, all at once.
+        Cached prefixes in the free blocks that are moved into are forgotten."""
+        in_use = len(self.used_block_ids)
+        holes = iter(sorted(b for b in self._free if b < in_use))
+        moves = [(b, next(holes)) for b in sorted(self.used_block_ids) if b >= in_use]
+        for source, target in moves:
+            old, new = self.blocks[source], self.blocks[target]
+            if new.token_ids:
+                self.prefix_cache_evictions += 1
+            self._forget(target)
+            del self._free[target]
+            new.ref_count, new.hash, new.token_ids = old.ref_count, old.hash, old.token_ids
+            hashes = self._published.pop(source, set())
+            if hashes:
+                self._published[target] = hashes
+            for h in hashes:
+                if self.hash_to_block_id.get(h) == source:
+                    self.hash_to_block_id[h] = target
+            old.ref_count, old.hash, old.token_ids = 0, -1, []
+            self.used_block_ids.remove(source)
+            self.used_block_ids.add(target)
+        if moves:
+            # The blocks moved out of hold nothing: first in line for reuse.
+            self._free = dict.fromkeys([s for s, _ in moves] + list(self._free))
+            new_id = dict(moves)
+            for seq in seqs:
+                seq.block_table[:] = [new_id.get(b, b) for b in seq.block_table]
+        return moves
+
     def deallocate(self, seq: Sequence) -> None:
         seq.num_cached_tokens = 0
         for block_id in seq.block_table:

@@ -5,7 +5,8 @@ fields of ``EngineConfig`` (microinfer/config/engine.py:6-68) that this
 engine acts on, with the same validation errors. The reference's switches
 for torch.compile and n-gram speculative decoding have no counterpart here:
 decode runs from hipGraphs of the HIP kernels, and speculation is not part
-of the attention path.
+of the attention path. ``SampleParameter.logprobs`` and
+``EngineConfig.shared_prefix_decode`` have no counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -14,12 +15,18 @@ import math
 from dataclasses import dataclass
 
 
+MAX_LOGPROBS = 32  # alternatives that mi_token_logprobs gives
+
+
 @dataclass(slots=True)
 class SampleParameter:
     temperature: float = 1.0
     max_tokens: int = 64
     ignore_eos: bool = False
     greedy: bool = False
+    # Record each sampled token's log probability with this many alternatives
+    # (0: the token alone; None: nothing), of the model's own distribution.
+    logprobs: int | None = None
 
     def __post_init__(self):
         # A temperature near zero is rejected: greedy decoding is asked for
@@ -29,6 +36,9 @@ class SampleParameter:
         )
         if type(self.max_tokens) is not int or self.max_tokens <= 0:
             raise ValueError("max_tokens must be a positive integer")
+        if self.logprobs is not None and (
+                type(self.logprobs) is not int or not 0 <= self.logprobs <= MAX_LOGPROBS):
+            raise ValueError(f"logprobs must be None or an integer between 0 and {MAX_LOGPROBS}")
 
 
 @dataclass(frozen=True)
@@ -41,6 +51,9 @@ class EngineConfig:
     debug_mode: bool = False
     use_cuda_graph: bool = False  # decode buckets replayed from hipGraphs
     mixed_batch: bool = True  # fill the budget with prefill after running decode
+    # Decode batches whose sequences share enough cache blocks (forks, common
+    # prompts) read them once; captures a second graph per bucket.
+    shared_prefix_decode: bool = False
 
     def __post_init__(self):
         for name in ("max_num_seqs", "max_num_batched_tokens", "max_num_prefill_tokens",
@@ -51,6 +64,6 @@ class EngineConfig:
         if self.eos_token_id is not None and (
                 type(self.eos_token_id) is not int or self.eos_token_id < 0):
             raise ValueError("eos_token_id must be a nonnegative integer or None")
-        for name in ("debug_mode", "use_cuda_graph", "mixed_batch"):
+        for name in ("debug_mode", "use_cuda_graph", "mixed_batch", "shared_prefix_decode"):
             if type(getattr(self, name)) is not bool:
                 raise ValueError(f"{name} must be a boolean")

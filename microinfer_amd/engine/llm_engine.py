@@ -4,7 +4,8 @@ Mirrors ``LLMEngine`` (microinfer/engine/llm_engine.py:5-94, :226-238)
 without speculative decoding: a mixed step runs its decode rows (graph path)
 and its prefill rows as two model calls and merges the tokens in schedule
 order; a failing model call aborts every scheduled request before any block
-hash is published, then re-raises.
+hash is published, then re-raises. Without counterpart there: forks of running
+requests, compaction of the cache, and log probabilities of the kept tokens.
 """
 
 from __future__ import annotations
@@ -47,7 +48,14 @@ class LLMEngine:
             for seq in seqs:  # KV may be partly written: publish nothing
                 self.scheduler.abort(seq.seq_id)
             raise
+        lengths = [len(s) for s in seqs]
         self.scheduler.postprocess(seqs, tokens, prefill)
+        if any(s.sampling.logprobs is not None for s in seqs):
+            # Of the tokens that were kept: a prompt chunk's sample is not.
+            logprobs = self.model_runner.take_logprobs()
+            for seq, length in zip(seqs, lengths):
+                if len(seq) > length and seq.seq_id in logprobs:
+                    seq.logprobs.append(logprobs[seq.seq_id])
         done = [s.status == SequenceStatus.FINISHED for s in seqs]
         finished = [(s.seq_id, s.completion_token_ids) for s, d in zip(seqs, done) if d]
         updates = [(s.seq_id, tuple(s.completion_token_ids), d, s.finish_reason)
@@ -61,6 +69,29 @@ class LLMEngine:
 
     def abort(self, seq_id: int) -> bool:
         return self.scheduler.abort(seq_id)
+
+    def fork(self, seq_id: int, n: int = 1, sampling_params=None) -> list[Sequence]:
+        """``n`` requests that continue running request ``seq_id`` from its
+        tokens so far, each sampling on its own (``sampling_params``, or the
+        request's). Its full cache blocks are shared; the last one, if it is
+        not full, is copied. Call it between steps."""
+        children, copies = self.scheduler.fork(seq_id, n, sampling_params)
+        try:
+            if copies:
+                self.model_runner.copy_blocks(*map(list, zip(*copies)))
+        except Exception:
+            for child in children:
+                self.scheduler.abort(child.seq_id)
+            raise
+        return children
+
+    def compact(self) -> int:
+        """Move the cache blocks in use to the lowest ids, between steps; the
+        number of blocks moved. Cached prefixes in their way are forgotten."""
+        moves = self.scheduler.compact()
+        if moves:
+            self.model_runner.copy_blocks(*map(list, zip(*moves)))
+        return len(moves)
 
     def generate(self, prompts, sampling_params) -> list[list[int]]:
         """Run requests to completion; completions in prompt order."""

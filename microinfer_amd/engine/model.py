@@ -161,7 +161,7 @@ class Qwen3Model:
         """Attention output ``[T, Hq D]`` of one layer's fused QKV rows."""
         c = self.config
         tokens = qkv.shape[0]
-        if (metadata.is_decode and metadata.slots_at_end
+        if (metadata.is_decode and metadata.slots_at_end and metadata.group_starts is None
                 and supported_qkv_decode(qkv, cache.keys, cache.values, c.num_q_head)
                 and prefer_qkv_decode(qkv, cache.keys, metadata.block_tables)):
             attn = hip_qkv_decode(

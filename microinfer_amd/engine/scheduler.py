@@ -112,6 +112,41 @@ class Scheduler:
         if seq.block_table:
             raise ValueError(f"request {seq.seq_id} already owns cache blocks")
 
+    def fork(self, seq_id: int, n: int = 1, sampling=None):
+        """``n`` new running requests that continue running request ``seq_id``
+        between two steps, and the block copies ``(source, destination, rows)``
+        that must be done before the next step. ValueError if it is not
+        running, RuntimeError if the cache cannot hold the forks; nothing is
+        changed then."""
+        if self._inflight is not None:
+            raise RuntimeError("requests are forked between steps")
+        if type(n) is not int or n < 1:
+            raise ValueError("the number of forks must be a positive integer")
+        parent = next((s for s in self.running if s.seq_id == seq_id), None)
+        if parent is None:
+            raise ValueError(f"request {seq_id} is not running")
+        if sampling is not None and sampling.max_tokens <= parent.num_completion_tokens:
+            raise ValueError(f"request {seq_id} already has the forks' max_tokens")
+        if not self.block_manager.can_fork(parent, n):
+            raise RuntimeError("KV cache has no free blocks")
+        children, copies = [], []
+        for _ in range(n):
+            child = parent.fork(sampling)
+            copy = self.block_manager.fork(parent, child)
+            if copy is not None:
+                copies.append(copy)
+            child.is_prefill = False
+            child.start_running()
+            self.running.append(child)
+            children.append(child)
+        return children, copies
+
+    def compact(self) -> list[tuple[int, int]]:
+        """``BlockManager.compact`` over every queued request, between steps."""
+        if self._inflight is not None:
+            raise RuntimeError("the cache is compacted between steps")
+        return self.block_manager.compact([*self.waiting, *self.running])
+
     # -- one step -----------------------------------------------------------
     def schedule(self) -> tuple[list[Sequence], bool]:
         """The requests of the next step and whether any of them prefills."""

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 from enum import Enum, auto
 from itertools import count
+from typing import NamedTuple
 
 from microinfer_amd.engine.config import SampleParameter
 
@@ -37,6 +38,15 @@ def _checked_tokens(token_ids) -> list[int]:
         if type(t) is not int or t < 0:
             raise ValueError(f"prompt token {t!r} is not a nonnegative int")
     return tokens
+
+
+class TokenLogprob(NamedTuple):
+    """A sampled token's log probability and the step's best alternatives,
+    ``(token id, log probability)`` best first."""
+
+    token_id: int
+    logprob: float
+    alternatives: tuple[tuple[int, float], ...]
 
 
 class Sequence:
@@ -58,6 +68,8 @@ class Sequence:
         self.num_cached_tokens = 0
         self.num_scheduled_tokens = 0
         self.is_prefill = True
+        # One TokenLogprob per token that was sampled while they were asked for.
+        self.logprobs: list[TokenLogprob] = []
 
     # -- tokens -------------------------------------------------------------
     @property
@@ -161,6 +173,15 @@ class Sequence:
         self.status = SequenceStatus.WAITING
         self.is_prefill = True
         self.num_scheduled_tokens = 0
+
+    def fork(self, sampling: SampleParameter | None = None) -> Sequence:
+        """A new request with this one's tokens so far, prompt split and log
+        probabilities, sampling on its own from here. It has no blocks yet."""
+        child = Sequence(self._tokens, sampling if sampling is not None else self.sampling)
+        child._prompt_len = self._prompt_len
+        child.block_size = self.block_size
+        child.logprobs = list(self.logprobs)
+        return child
 
     def finish(self, reason: str) -> None:
         self.status = SequenceStatus.FINISHED

@@ -53,6 +53,48 @@ class SharedDecodePlan:
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
 
 
+def shared_groups(tables, contexts, block_size: int) -> tuple[list[int], list[int], int]:
+    """Groups of neighbours in ``tables`` (host lists of block ids) that share
+    their first whole blocks, for ``shared_decode_plan``: group starts (one
+    more than groups), the shared blocks of each, and the positions that the
+    groups' sequences need not read again. Put tables with a common beginning
+    next to each other (``sorted``): a sequence joins the group before it
+    unless that would halve what the group shares, or what the sequence shares
+    with its other neighbour."""
+    n = len(tables)
+    whole = [min(context // block_size, len(table)) for table, context in zip(tables, contexts)]
+    common = [0] * (n + 1)  # of each sequence and the one before it
+    for i in range(1, n):
+        common[i] = _common_blocks(tables[i - 1], tables[i], min(whole[i - 1], whole[i]))
+    starts, shared = [], []
+    for i in range(n):
+        if starts:
+            alone = shared[-1] is None
+            both = common[i] if alone else min(common[i], shared[-1])
+            if both and 2 * both >= max(common[i + 1], 0 if alone else shared[-1]):
+                shared[-1] = both
+                continue
+        starts.append(i)
+        shared.append(None)
+    bounds = starts + [n]
+    shared = [n or 0 for n in shared]
+    saved = sum((bounds[g + 1] - bounds[g] - 1) * s for g, s in enumerate(shared))
+    return bounds, shared, saved * block_size
+
+
+def _common_blocks(a: list[int], b: list[int], most: int) -> int:
+    """Length of the common beginning of two tables, at most ``most``."""
+    if a[:most] == b[:most]:
+        return most
+    return next(i for i in range(most) if a[i] != b[i])
+
+
+def prefer_shared_decode(saved_positions: int, num_kv_heads: int) -> bool:
+    """Whether a decode step with these groups (``shared_groups``) is better
+    done with them."""
+    return saved_positions * num_kv_heads >= 1 << 17
+
+
 def supported_shared_decode(num_q_heads: int, num_kv_heads: int, head_dim: int,
                             dtype: torch.dtype, block_size: int, num_seqs: int) -> bool:
     """Whether sequences of this shape read shared pages once."""

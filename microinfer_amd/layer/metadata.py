@@ -34,6 +34,11 @@ class AttentionMetadata:
     # slot of the pad block). Then norm, RoPE, append and attention may share a
     # launch; other slots need the append to finish first.
     slots_at_end: bool = False
+    # Decode: groups of consecutive sequences whose tables share their first
+    # blocks (shared_decode_plan's group_starts and shared_blocks). None: every
+    # sequence reads its own context.
+    group_starts: torch.Tensor | None = None
+    shared_blocks: torch.Tensor | None = None
     _cu_q_cpu: tuple[int, ...] | None = field(default=None, repr=False)
     _context_lens_cpu: tuple[int, ...] | None = field(default=None, repr=False)
     _q_lens_cpu: tuple[int, ...] | None = field(default=None, repr=False)
@@ -43,6 +48,7 @@ class AttentionMetadata:
     _slot_offsets: torch.Tensor | None = field(default=None, repr=False)
     _decode_plans: dict = field(default_factory=dict, repr=False)
     _prefill_plans: dict = field(default_factory=dict, repr=False)
+    _shared_plans: dict = field(default_factory=dict, repr=False)
 
     @classmethod
     def build(
@@ -111,6 +117,26 @@ class AttentionMetadata:
                                block_size=block_size, block_table_width=key[2], heads=heads)
             self._decode_plans[key] = plan
         return plan
+
+    def shared_plan(self, query: torch.Tensor, key_cache: torch.Tensor):
+        """Device plan of this decode step's shared blocks, built once and
+        reused by every layer."""
+        if self.group_starts is None or self.shared_blocks is None:
+            raise ValueError("shared decode needs group_starts and shared_blocks")
+        if self.context_lens is None or self.block_tables is None:
+            raise ValueError("decode plan needs context_lens and block_tables")
+        from microinfer_amd.layer.hip_shared_decode import shared_decode_plan
+
+        _, block_size, num_kv_heads, _ = key_cache.shape
+        _, num_q_heads, head_dim = query.shape
+        key = (num_q_heads, num_kv_heads, head_dim, query.dtype, block_size,
+               self.block_tables.shape[1])
+        if key not in self._shared_plans:
+            self._shared_plans[key] = shared_decode_plan(
+                self.context_lens, self.group_starts, self.shared_blocks,
+                num_q_heads=num_q_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
+                dtype=query.dtype, block_size=block_size, block_table_width=key[-1])
+        return self._shared_plans[key]
 
     def prefill_plan(self, query: torch.Tensor, key_cache: torch.Tensor, *, paged: bool = True):
         """Device launch plan for this step's prefill calls, built once and

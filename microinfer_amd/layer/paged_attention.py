@@ -5,7 +5,8 @@ Mirrors ``paged_attention_meta`` and ``_gather_paged_kv``
 between FlashAttention, Triton, gather + FA varlen and its PyTorch reference;
 here every route is a gfx950 kernel and nothing falls back to the CPU:
 
-* decode metadata        -> ``hip_paged_decode`` (split-K planned on device)
+* decode metadata        -> ``hip_paged_decode`` (split-K planned on device), or
+  ``hip_shared_decode`` where it names groups of sequences that share blocks
 * prefill / mixed chunks -> ``hip_paged_prefill`` (reads the pages in place,
   so the reference's ``Σctx >= 4 Σq`` choice between in-place and gathered
   prefill, :104-139, disappears)
@@ -29,6 +30,7 @@ from microinfer_amd.layer.hip_paged_attention import (
     hip_paged_prefill,
     vector_heads,
 )
+from microinfer_amd.layer.hip_shared_decode import hip_shared_decode
 from microinfer_amd.layer.metadata import AttentionMetadata
 
 
@@ -92,6 +94,10 @@ def paged_attention_meta(
     if metadata.is_decode:
         if metadata.context_lens is None:
             raise RuntimeError("decode metadata requires context_lens")
+        if metadata.group_starts is not None:
+            return hip_shared_decode(query, key_cache, value_cache, metadata.block_tables,
+                                     metadata.context_lens, scale=scale,
+                                     plan=metadata.shared_plan(query, key_cache))
         plan = None
         if metadata.context_lens.is_cuda:
             block_size, num_kv_heads = key_cache.shape[1:3]

@@ -215,10 +215,18 @@ class DecodeBuffers:
         self.slot_mapping = torch.empty(capacity, dtype=torch.int32, device=dev)
         self.context_lens = torch.empty(capacity, dtype=torch.int32, device=dev)
         self.block_tables = torch.empty((capacity, width), dtype=torch.int32, device=dev)
+        # Groups that share blocks: capacity + 1 starts, then capacity counts.
+        self.groups = torch.zeros(capacity + 1, dtype=torch.int64, device=dev)
         self.capacity, self.width = capacity, width
         # Columns at or past this index are -1 in every row (a new table holds
         # garbage everywhere).
         self.table_written = width
+
+    def set_groups(self, metadata: AttentionMetadata, batch: int) -> None:
+        """Name the buffers' groups in ``metadata``."""
+        words = self.groups.view(torch.int32)
+        metadata.group_starts = words[:batch + 1]
+        metadata.shared_blocks = words[self.capacity + 1:self.capacity + 1 + batch]
 
     def metadata(self, batch: int) -> AttentionMetadata:
         """Decode metadata over the first ``batch`` rows (``_make_decode_metadata``,
@@ -304,6 +312,7 @@ class StepMetadataBuilder:
         self._upload = _Upload(self.device)
         self._decode_buffers: DecodeBuffers | None = None
         self._decode_upload: torch.Tensor | None = None
+        self._group_upload: _Upload | None = None
 
     def _check_blocks(self, last_positions: np.ndarray, counts: np.ndarray,
                       blocks: np.ndarray) -> None:
@@ -449,11 +458,27 @@ class StepMetadataBuilder:
                      buffers.positions.data_ptr(), buffers.input_ids.data_ptr())
         buffers.table_written = needed if rows == buffers.capacity else cols
 
-    def prepare_decode(self, seqs):
+    def fill_groups(self, buffers: DecodeBuffers, starts: list[int], shared: list[int]) -> None:
+        """Write the groups (``shared_groups`` of the batch) into ``buffers``.
+        Rows past the last group, a graph's pad rows, are in none."""
+        capacity, groups = buffers.capacity, len(shared)
+        if len(starts) != groups + 1 or groups > capacity:
+            raise ValueError("groups do not fit the buffers")
+        if self._group_upload is None:
+            self._group_upload = _Upload(self.device)
+        _, h32 = self._group_upload.stage(capacity + 1)
+        h32[:groups + 1] = starts
+        h32[groups + 1:capacity + 1] = starts[-1]
+        h32[capacity + 1:capacity + 1 + groups] = shared
+        h32[capacity + 1 + groups:2 * capacity + 2] = 0
+        self._group_upload.commit(buffers.groups, capacity + 1)
+
+    def prepare_decode(self, seqs, groups=None):
         """``ModelRunner.prepare_decode`` (microinfer/runner.py:348-385) on the device.
 
         The returned tensors are views of buffers reused by the next call,
-        as in the reference.
+        as in the reference. ``groups``: ``(starts, shared)`` of
+        ``shared_groups`` for sequences that read shared blocks once.
         """
         n = len(seqs)
         width = max((len(s.block_table) for s in seqs), default=0)
@@ -471,6 +496,9 @@ class StepMetadataBuilder:
             validate_cache_write=self.debug_mode,
         )
         metadata.slots_at_end = True
+        if groups is not None and n:
+            self.fill_groups(buffers, *groups)
+            buffers.set_groups(metadata, n)
         if self.debug_mode:
             self.validate(seqs, buffers.input_ids[:n], buffers.positions[:n], metadata, False)
         return buffers.input_ids[:n], buffers.positions[:n], metadata
@@ -503,11 +531,13 @@ class DecodeGraphRunner:
     capture-safe. With ``greedy`` its output is ``[batch, vocab]`` logits and
     the graph also selects each row's greedy token with the HIP argmax
     (runner.py:236-240); ``run`` then returns ``(logits, tokens)`` like
-    ``_run_decode`` (runner.py:603).
+    ``_run_decode`` (runner.py:603). With ``shared`` the captured step reads
+    the blocks that groups of sequences share once; the groups are given
+    to ``run`` and may change from step to step.
     """
 
     def __init__(self, builder: StepMetadataBuilder, forward, *, max_num_seqs: int,
-                 table_width: int, greedy: bool = False):
+                 table_width: int, greedy: bool = False, shared: bool = False):
         if builder.pad_block_id is None:
             raise ValueError("graph buckets need the builder's pad block")
         if builder.device.type != "cuda":
@@ -515,6 +545,7 @@ class DecodeGraphRunner:
         self.builder = builder
         self.forward = forward
         self.greedy = greedy
+        self.shared = shared
         self.table_width = table_width
         self.buckets = []
         self.pool = None
@@ -524,13 +555,15 @@ class DecodeGraphRunner:
     def _capture(self, batch: int) -> None:
         device = self.builder.device
         buffers = self.builder.pad_buffers(batch, self.table_width)
+        if self.shared:
+            self.builder.fill_groups(buffers, [0], [])
         ids, positions = buffers.input_ids[:batch], buffers.positions[:batch]
         torch.cuda.synchronize(device)
         side = torch.cuda.Stream(device=device)
         side.wait_stream(torch.cuda.current_stream(device))
         with torch.cuda.stream(side), torch.inference_mode():
             for _ in range(2):
-                self._step(ids, positions, buffers.metadata(batch))
+                self._step(ids, positions, self._metadata(buffers, batch))
         torch.cuda.current_stream(device).wait_stream(side)
         torch.cuda.synchronize(device)
         graph = torch.cuda.CUDAGraph()
@@ -539,11 +572,17 @@ class DecodeGraphRunner:
         # row slots) is reused rather than allocated and zero-filled inside
         # the graph.
         with capture_graph(graph, self.pool, stream=side), torch.inference_mode():
-            out = self._step(ids, positions, buffers.metadata(batch))
+            out = self._step(ids, positions, self._metadata(buffers, batch))
         if self.pool is None:
             self.pool = graph.pool()
         torch.cuda.synchronize(device)
         self.buckets.append((batch, buffers, graph, out))
+
+    def _metadata(self, buffers: DecodeBuffers, batch: int) -> AttentionMetadata:
+        metadata = buffers.metadata(batch)
+        if self.shared:
+            buffers.set_groups(metadata, batch)
+        return metadata
 
     def _step(self, ids, positions, metadata):
         out = self.forward(ids, positions, metadata)
@@ -555,14 +594,18 @@ class DecodeGraphRunner:
                 return bucket
         return None
 
-    def run(self, seqs):
+    def run(self, seqs, groups=None):
         """Replay the bucket that holds ``seqs``; None if the batch is larger
-        than every bucket (the caller then runs eagerly, as the reference does)."""
+        than every bucket (the caller then runs eagerly, as the reference does).
+        ``groups``: the batch's ``(starts, shared)`` where the graphs are for
+        shared blocks."""
         bucket = self.select(len(seqs))
         if bucket is None:
             return None
         batch, buffers, graph, out = bucket
         self.builder.fill_decode(buffers, seqs, rows=batch)
+        if self.shared:
+            self.builder.fill_groups(buffers, *(groups or ([0], [])))
         n = len(seqs)
         if self.builder.debug_mode:
             # The batch's rows as the graph will read them (microinfer/

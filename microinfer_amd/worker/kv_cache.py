@@ -25,6 +25,7 @@ from dataclasses import dataclass
 
 import torch
 
+from microinfer_amd.worker.hip_kv_blocks import copy_blocks
 from microinfer_amd.worker.hip_kv_store import launch_append
 
 LAYOUTS = ("paired", "head_major", "token_major")
@@ -138,6 +139,11 @@ class KVCache:
             self.keys.numel() * self.keys.element_size()
             + self.values.numel() * self.values.element_size()
         )
+
+    def copy_blocks(self, src, dst, tokens=None) -> None:
+        """Copy blocks (or their first ``tokens[i]`` rows) to other blocks in
+        every layer: ``hip_kv_blocks.copy_blocks`` over the whole pool."""
+        copy_blocks(self.keys, self.values, src, dst, tokens=tokens)
 
     def layer(self, index: int) -> LayerKVCache:
         """Basic indexing shares storage; binding does not copy the cache."""

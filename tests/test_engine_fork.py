@@ -1,0 +1,319 @@
+"""Forks, compaction and log probabilities in the engine's host logic, with
+stand-in runners (CPU, no kernels): block ownership and copies of a fork, the
+moves of a compaction with its prefix cache, what the step loop records, and
+the asyncio frontend's forks.
+"""
+
+import asyncio
+import random
+
+import pytest
+
+from microinfer_amd.engine.async_engine import AsyncEngine, BackpressureError
+from microinfer_amd.engine.config import SampleParameter
+from microinfer_amd.engine.llm_engine import LLMEngine
+from microinfer_amd.engine.sequence import SequenceStatus, TokenLogprob
+from microinfer_amd.layer.hip_shared_decode import prefer_shared_decode, shared_groups
+
+
+class PoolRunner:
+    """Samples a function of the tokens and keeps a pool of them: row ``p`` of a
+    sequence's table holds ``(tokens up to p)``, checked for every cached row."""
+
+    def __init__(self, block_size, width=97):
+        self.block_size, self.width = block_size, width
+        self.pool = {}
+        self.copies = []
+        self.asked = {}
+        self.fail_copy = False
+
+    def run(self, seqs, is_prefill):
+        out = []
+        for s in seqs:
+            start = s.num_cached_tokens if is_prefill else len(s) - 1
+            for p in range(start):
+                assert self.pool[self._slot(s, p)] == tuple(s[:p + 1]), "a cached row is wrong"
+            for p in range(start, start + s.num_scheduled_tokens):
+                self.pool[self._slot(s, p)] = tuple(s[:p + 1])
+            token = 100 + (sum(s.token_ids) * 7 + s.seq_id) % self.width
+            out.append(token)
+            if s.sampling.logprobs is not None:
+                self.asked[s.seq_id] = TokenLogprob(token, -float(len(s)), ())
+        return out
+
+    def _slot(self, s, p):
+        return s.block_table[p // self.block_size], p % self.block_size
+
+    def copy_blocks(self, src, dst, tokens=None):
+        if self.fail_copy:
+            raise RuntimeError("copy failed")
+        tokens = tokens or [self.block_size] * len(src)
+        self.copies.append((src, dst, tokens))
+        before = dict(self.pool)
+        for s, d, n in zip(src, dst, tokens):
+            for r in range(n):
+                self.pool[d, r] = before.get((s, r))
+
+    def take_logprobs(self):
+        taken, self.asked = self.asked, {}
+        return taken
+
+
+def make(scheduler_factory, **limits):
+    values = dict(num_blocks=16, max_num_seqs=8, max_num_batched_tokens=16, max_model_len=60)
+    values.update(limits)
+    scheduler, manager = scheduler_factory(**values)
+    runner = PoolRunner(manager.block_size)
+    return LLMEngine(scheduler, runner), runner, manager
+
+
+def params(n, **values):
+    return SampleParameter(max_tokens=n, ignore_eos=True, **values)
+
+
+def run_out(engine):
+    while not engine.is_finished():
+        engine.step()
+
+
+def refs(manager):
+    return {b.block_id: b.ref_count for b in manager.blocks if b.ref_count}
+
+
+@pytest.mark.parametrize("prompt,steps", [(6, 1), (8, 1), (9, 1), (3, 5), (4, 1), (4, 2), (1, 1)])
+def test_fork_shares_full_blocks_and_copies_the_last(scheduler_factory, sequence_cls, prompt,
+                                                     steps):
+    engine, runner, manager = make(scheduler_factory)
+    seq = sequence_cls(list(range(1, prompt + 1)), params(20))
+    engine.add_request(seq)
+    for _ in range(steps):
+        engine.step()
+    cached = seq.num_cached_tokens
+    assert cached == len(seq) - 1
+    full, rest = divmod(cached, 4)
+    children = engine.fork(seq.seq_id, 3)
+    assert len({c.seq_id for c in children} | {seq.seq_id}) == 4
+    for c in children:
+        assert c.token_ids == seq.token_ids and c.token_ids is not seq.token_ids
+        assert c.num_prompt_tokens == prompt and c.num_cached_tokens == cached
+        assert c.status is SequenceStatus.RUNNING and not c.is_prefill and c.block_size == 4
+        assert c.block_table[:full] == seq.block_table[:full]
+        assert len(c.block_table) == full + (rest > 0)
+    last = [s.block_table[full] for s in [seq, *children] if rest]
+    assert len(set(last)) == len(last)
+    if rest:
+        assert runner.copies == [([seq.block_table[full]] * 3, last[1:], [rest] * 3)]
+    else:
+        assert runner.copies == []
+    for b in seq.block_table[:full]:
+        assert manager.blocks[b].ref_count == 4
+    run_out(engine)  # the runner checks every cached row of every step
+    outs = [s.completion_token_ids for s in [seq, *children]]
+    assert all(len(o) == 20 and o[:steps] == outs[0][:steps] for o in outs)
+    assert len({tuple(o) for o in outs}) > 1
+    assert not manager.used_block_ids and refs(manager) == {}
+
+
+def test_fork_refusals_change_nothing(scheduler_factory, sequence_cls):
+    engine, runner, manager = make(scheduler_factory, num_blocks=3)
+    seq = sequence_cls([1, 2, 3, 4, 5], params(6))
+    engine.add_request(seq)
+    with pytest.raises(ValueError, match="not running"):
+        engine.fork(seq.seq_id)
+    engine.step()
+    before = refs(manager), set(manager.free_block_ids)
+    with pytest.raises(RuntimeError, match="no free blocks"):
+        engine.fork(seq.seq_id, 2)  # one block is free, two would be needed
+    for n in (0, -1, 1.5, True and 0):
+        with pytest.raises(ValueError):
+            engine.fork(seq.seq_id, n)
+    with pytest.raises(ValueError, match="not running"):
+        engine.fork(seq.seq_id + 1000)
+    with pytest.raises(ValueError, match="max_tokens"):
+        engine.fork(seq.seq_id, 1, params(1))  # it has one token already
+    runner.fail_copy = True
+    with pytest.raises(RuntimeError, match="copy failed"):
+        engine.fork(seq.seq_id)
+    runner.fail_copy = False
+    assert (refs(manager), set(manager.free_block_ids)) == before
+    assert list(engine.scheduler.running) == [seq] and runner.copies == []
+    engine.scheduler.schedule()
+    with pytest.raises(RuntimeError, match="between steps"):
+        engine.fork(seq.seq_id)
+    with pytest.raises(RuntimeError, match="between steps"):
+        engine.compact()
+
+
+def test_forks_survive_preemption_and_abort(scheduler_factory, sequence_cls):
+    engine, runner, manager = make(scheduler_factory, num_blocks=7, max_num_batched_tokens=30)
+    seq = sequence_cls([1, 2, 3, 4, 5, 6], params(12))
+    engine.add_request(seq)
+    engine.step()
+    children = engine.fork(seq.seq_id, 2) + engine.fork(seq.seq_id, 1, params(5))
+    assert engine.abort(seq.seq_id)
+    run_out(engine)
+    assert engine.stats()["num_preemptions"] > 0
+    assert [len(c.completion_token_ids) for c in children] == [12, 12, 5]
+    assert not manager.used_block_ids
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_forks_aborts_and_compactions(scheduler_factory, sequence_cls, seed):
+    rng = random.Random(seed)
+    # Either preemptions or prompts in chunks: with both, a preempted request can
+    # wait for ever behind the blocks of a chunked prompt, with or without forks.
+    blocks, budget = rng.choice([(12, 400), (24, 400), (160, 5), (160, 16)])
+    engine, runner, manager = make(scheduler_factory, num_blocks=blocks,
+                                   max_num_batched_tokens=budget,
+                                   mixed_batch=rng.random() < 0.7)
+    shared = [rng.randrange(1, 9) for _ in range(9)]
+    made = []
+    for step in range(120):
+        if len(made) < 14 and rng.random() < 0.3:
+            prompt = shared[:rng.randrange(9)] + [rng.randrange(1, 9)
+                                                  for _ in range(rng.randrange(1, 8))]
+            made.append(sequence_cls(prompt, params(rng.randrange(1, 14))))
+            engine.add_request(made[-1])
+        running = [s.seq_id for s in engine.scheduler.running]
+        if running and len(made) < 14 and rng.random() < 0.3:
+            n = rng.randrange(1, 4)
+            try:
+                made += engine.fork(rng.choice(running), n, params(rng.randrange(14, 20)))
+            except RuntimeError:
+                pass
+        if running and rng.random() < 0.05:
+            engine.abort(rng.choice(running))
+        if rng.random() < 0.3:
+            moved = engine.compact()
+            used = sorted(manager.used_block_ids)
+            assert used == list(range(len(used))) and moved >= 0
+        if not engine.is_finished():
+            engine.step()
+        tables = [s.block_table for s in [*engine.scheduler.waiting, *engine.scheduler.running]]
+        counted = {}
+        for b in (b for t in tables for b in t):
+            counted[b] = counted.get(b, 0) + 1
+        assert counted == refs(manager) and set(counted) == manager.used_block_ids
+        assert set(manager.free_block_ids) | set(counted) == set(range(len(manager.blocks)))
+        assert not set(manager.free_block_ids) & set(counted)
+        for h, b in manager.hash_to_block_id.items():  # what is cached is findable and right
+            assert h in manager._published[b]
+    run_out(engine)
+    assert not manager.used_block_ids and refs(manager) == {}
+
+
+def test_compaction_keeps_published_prefixes(scheduler_factory, sequence_cls):
+    engine, runner, manager = make(scheduler_factory, num_blocks=12)
+    low = sequence_cls([9, 9, 9, 9, 9], params(1))
+    keep = sequence_cls(list(range(1, 10)), params(8))
+    engine.add_request(low)
+    engine.add_request(keep)
+    engine.step()  # `low` is done; its blocks 0 and 1 are free, and cached
+    assert low.is_finished and min(keep.block_table) >= 2
+    cached = len(manager.hash_to_block_id)
+    table = list(keep.block_table)
+    assert engine.compact() == 2
+    assert sorted(keep.block_table) == list(range(len(keep.block_table)))
+    assert runner.copies[-1] == (table[-2:], [0, 1], [4, 4]) or \
+        sorted(runner.copies[-1][1]) == [0, 1]
+    assert len(manager.hash_to_block_id) == cached - 1  # low's prefix went, keep's stays
+    assert engine.compact() == 0
+    follow = sequence_cls(list(range(1, 10)) + [5], params(2))
+    engine.add_request(follow)
+    engine.step()
+    assert manager.prefix_cache_hit_blocks == 2
+    run_out(engine)
+
+
+def test_logprobs_follow_the_kept_tokens(scheduler_factory, sequence_cls):
+    engine, runner, _ = make(scheduler_factory, max_num_batched_tokens=4)
+    a = sequence_cls([1, 2, 3, 4, 5, 6, 7], params(3, logprobs=2))  # two prompt chunks
+    b = sequence_cls([1], params(3))
+    engine.add_request(a)
+    engine.add_request(b)
+    engine.step()
+    assert a.logprobs == []  # the first chunk's sample is dropped
+    for _ in range(2):
+        engine.step()
+    child, = engine.fork(a.seq_id)
+    assert child.logprobs == a.logprobs and child.logprobs is not a.logprobs
+    run_out(engine)
+    for s in (a, child):
+        assert [x.token_id for x in s.logprobs] == s.completion_token_ids
+        assert [x.logprob for x in s.logprobs] == [-7.0, -8.0, -9.0]
+    assert b.logprobs == []
+
+
+def test_sampling_values_are_checked():
+    for bad in (-1, 33, 1.0, True, "3"):
+        with pytest.raises(ValueError, match="logprobs"):
+            SampleParameter(logprobs=bad)
+    assert SampleParameter(logprobs=0).logprobs == 0
+    assert SampleParameter().logprobs is None
+
+
+def test_async_forks_stream_from_the_tokens_so_far(scheduler_factory, sequence_cls):
+    engine, runner, manager = make(scheduler_factory)
+
+    async def scenario():
+        frontend = AsyncEngine(engine, max_waiting=3)
+        request = await frontend.add_request([1, 2, 3], params(12))
+        stream = frontend.stream(request)
+        first = await anext(stream)
+        with pytest.raises(BackpressureError):
+            await frontend.fork(request, 3)
+        forks = await frontend.fork(request, 2, params(15))
+        with pytest.raises(BackpressureError):
+            await frontend.add_request([4], params(1))
+        with pytest.raises(TypeError):
+            await frontend.fork(request, 1, {"max_tokens": 1})
+        with pytest.raises(ValueError):
+            await frontend.fork(request, 0)
+        outs = [await frontend.collect(f) for f in forks]
+        async for event in stream:
+            last = event
+        assert len(last.token_ids) == 12 and all(len(o.token_ids) == 15 for o in outs)
+        assert all(o.token_ids[:1] == first.token_ids[:1] for o in outs)
+        with pytest.raises(ValueError, match="not running"):
+            await frontend.fork(request)  # it has finished
+        assert frontend.stats()["active_requests"] == 0
+        again = await frontend.generate([1, 2], params(2))  # the room came back
+        request = await frontend.add_request([1, 2, 3], params(30))
+        stream = frontend.stream(request)
+        await anext(stream)
+        task = asyncio.ensure_future(frontend.fork(request, 2))
+        await asyncio.sleep(0)
+        task.cancel()
+        with pytest.raises(asyncio.CancelledError):
+            await task
+        async for event in stream:
+            pass
+        assert len(event.token_ids) == 30
+        assert frontend._reserved == 0 and not frontend._channels
+        assert len(again.token_ids) == 2
+        await frontend.stop()
+        assert not manager.used_block_ids
+
+    asyncio.run(scenario())
+
+
+def test_shared_groups_of_neighbours():
+    a = list(range(10))
+    tables = [a + [20], a + [21, 22], a[:8] + [23, 24], [50, 51], [50, 52], [60]]
+    lens = [4 * len(t) for t in tables]
+    # Ten blocks shared by two, eight by three (saves more than it costs);
+    # a single block by the next two; nothing by the last.
+    assert shared_groups(tables, lens, 4) == ([0, 3, 5, 6], [8, 1, 0], 4 * (2 * 8 + 1))
+    # Blocks must be whole in every context.
+    assert shared_groups(tables[:2], [40, 39], 4) == ([0, 2], [9], 36)
+    assert shared_groups(tables[:2], [3, 44], 4) == ([0, 1, 2], [0, 0], 0)
+    # A sequence that shares little does not take it from the others.
+    assert shared_groups([a, a, a[:3] + [9]], [40, 40, 16], 4) == ([0, 2, 3], [10, 0], 40)
+    # Long contexts behind a short common beginning.
+    b, c = [1, 2] + list(range(100, 140)), [1, 2] + list(range(200, 230))
+    assert shared_groups([b, c], [168, 128], 4) == ([0, 2], [2], 8)
+    # The next neighbour shares more.
+    assert shared_groups([b, c, c + [7]], [168, 128, 132], 4) == ([0, 1, 3], [0, 32], 128)
+    assert shared_groups([], [], 4) == ([0], [], 0)
+    assert shared_groups([a], [40], 4) == ([0, 1], [0], 0)
+    assert not prefer_shared_decode(0, 8) and prefer_shared_decode(1 << 20, 8)

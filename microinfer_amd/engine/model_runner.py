@@ -26,8 +26,9 @@ from microinfer_amd.engine.config import EngineConfig
 from microinfer_amd.engine.sequence import TokenLogprob
 from microinfer_amd.layer.hip_logprobs import token_logprobs
 from microinfer_amd.layer.hip_sampler import Sampler, greedy_argmax
-from microinfer_amd.layer.hip_shared_decode import (prefer_shared_decode, shared_groups,
-                                                    supported_shared_decode)
+from microinfer_amd.layer.hip_shared_decode import (least_shared_positions,
+                                                    prefer_shared_decode, shared_groups,
+                                                    shared_order, supported_shared_decode)
 from microinfer_amd.runner import DecodeGraphRunner, StepMetadataBuilder
 from microinfer_amd.worker.kv_cache import KVCache
 
@@ -77,12 +78,17 @@ class ModelRunner:
     def _shared_groups(self, seqs):
         """The decode batch ordered so that sequences with a common beginning
         are neighbours, and its groups; None where they are not worth it."""
-        ordered = sorted(seqs, key=lambda s: s.block_table)
-        starts, shared, saved = shared_groups([s.block_table for s in ordered],
-                                              [len(s) for s in ordered], self.block_size)
-        if not prefer_shared_decode(saved, self.kv_cache.num_kv_heads):
+        contexts = [len(s) for s in seqs]
+        heads = self.kv_cache.num_kv_heads
+        if sum(contexts) < least_shared_positions(len(seqs), heads):
             return seqs, None
-        return ordered, (starts, shared)
+        tables = [s.block_table for s in seqs]
+        order = shared_order(tables)
+        starts, shared = shared_groups([tables[i] for i in order], [contexts[i] for i in order],
+                                       self.block_size)
+        if not prefer_shared_decode(starts, shared, self.block_size, heads):
+            return seqs, None
+        return [seqs[i] for i in order], (starts, shared)
 
     @torch.inference_mode()
     def run(self, seqs, is_prefill: bool) -> list[int]:

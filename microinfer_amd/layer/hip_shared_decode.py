@@ -53,20 +53,39 @@ class SharedDecodePlan:
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
 
 
-def shared_groups(tables, contexts, block_size: int) -> tuple[list[int], list[int], int]:
-    """Groups of neighbours in ``tables`` (host lists of block ids) that share
-    their first whole blocks, for ``shared_decode_plan``: group starts (one
-    more than groups), the shared blocks of each, and the positions that the
-    groups' sequences need not read again. Put tables with a common beginning
-    next to each other (``sorted``): a sequence joins the group before it
-    unless that would halve what the group shares, or what the sequence shares
-    with its other neighbour."""
+def shared_order(tables) -> list[int]:
+    """An order of ``tables`` (host lists of block ids) that puts those with a
+    common beginning next to each other, in the order of their first."""
+    firsts: dict = {}
+    for i, table in enumerate(tables):
+        firsts.setdefault(table[0] if table else None, []).append(i)
+    order = []
+    for same in firsts.values():
+        if len(same) > 2:
+            first = tables[same[0]]
+            rank = {}
+            for i in same:  # by what they share with the first, then by what follows
+                table = tables[i]
+                n = _common_blocks(first, table, min(len(first), len(table)))
+                rank[i] = (-n, table[n] if n < len(table) else -1)
+            same.sort(key=rank.__getitem__)
+        order += same
+    return order
+
+
+def shared_groups(tables, contexts, block_size: int) -> tuple[list[int], list[int]]:
+    """Groups of neighbours in ``tables`` that share their first whole blocks,
+    for ``shared_decode_plan``: group starts (one more than groups) and the
+    shared blocks of each. A sequence joins the group before it unless that
+    would halve what the group shares, or what the sequence shares with its
+    other neighbour, so order the tables first (``shared_order``)."""
     n = len(tables)
     whole = [min(context // block_size, len(table)) for table, context in zip(tables, contexts)]
     common = [0] * (n + 1)  # of each sequence and the one before it
     for i in range(1, n):
         common[i] = _common_blocks(tables[i - 1], tables[i], min(whole[i - 1], whole[i]))
-    starts, shared = [], []
+    starts: list[int] = []
+    shared: list = []
     for i in range(n):
         if starts:
             alone = shared[-1] is None
@@ -76,23 +95,53 @@ def shared_groups(tables, contexts, block_size: int) -> tuple[list[int], list[in
                 continue
         starts.append(i)
         shared.append(None)
-    bounds = starts + [n]
-    shared = [n or 0 for n in shared]
-    saved = sum((bounds[g + 1] - bounds[g] - 1) * s for g, s in enumerate(shared))
-    return bounds, shared, saved * block_size
+    return starts + [n], [blocks or 0 for blocks in shared]
 
 
 def _common_blocks(a: list[int], b: list[int], most: int) -> int:
     """Length of the common beginning of two tables, at most ``most``."""
-    if a[:most] == b[:most]:
-        return most
-    return next(i for i in range(most) if a[i] != b[i])
+    low, high = 0, most
+    if most and a[0] != b[0]:
+        return 0
+    while low < high:  # the slices halve, so at most 2 * most entries are compared
+        mid = (low + high + 1) // 2
+        if a[low:mid] == b[low:mid]:
+            low = mid
+        else:
+            high = mid - 1
+    return low
 
 
-def prefer_shared_decode(saved_positions: int, num_kv_heads: int) -> bool:
-    """Whether a decode step with these groups (``shared_groups``) is better
+def least_shared_positions(num_seqs: int, num_kv_heads: int) -> int:
+    """Positions that the groups of a decode step must share, counted once for
+    each of their sequences but two, to be better read once.
+
+    Whole steps of a 28-layer model (16 query, 8 KV heads, head_dim 128, bf16,
+    block 16, 100 tokens of each sequence's own, from graphs), µs without and
+    with the groups, and what finding them takes the host. The second sequence
+    of a group finds its pages in the caches: 16 pairs with 8192 shared tokens
+    take 3606 and 3760, so pairs do not count. What has to be gained is the
+    launch that the fused QKV decode saves, the plan, each sequence's join
+    and the host's time:
+
+        sequences  shared tokens on both sides of the rule
+        1 x 4      8192: 1260, 1251 + 22    32000: 2135, 1777 + 42
+        1 x 8      2048: 1137, 1187 + 23     4096: 1269, 1229 + 30
+        1 x 16     2048: 1265, 1247 + 42     4096: 1555, 1334 + 54
+        1 x 64     1024: 1539, 1471 + 125    2048: 1841, 1563 + 156
+        4 x 4      2048: 1301, 1327 + 40     4096: 1618, 1489 + 53
+        8 x 8      1024: 1618, 1636 + 124    2048: 1996, 1783 + 147
+    """
+    return ((1 << 17) + 8192 * num_seqs) // num_kv_heads
+
+
+def prefer_shared_decode(starts, shared, block_size: int, num_kv_heads: int) -> bool:
+    """Whether a decode step with the groups of ``shared_groups`` is better
     done with them."""
-    return saved_positions * num_kv_heads >= 1 << 17
+    counted = sum((starts[g + 1] - starts[g] - 2) * blocks for g, blocks in enumerate(shared)
+                  if blocks)
+    return counted > 0 and \
+        counted * block_size >= least_shared_positions(starts[-1], num_kv_heads)
 
 
 def supported_shared_decode(num_q_heads: int, num_kv_heads: int, head_dim: int,

@@ -54,7 +54,9 @@ def shared_calls(monkeypatch):
         return launch(query, *args, **kwargs)
 
     monkeypatch.setattr(paged_attention, "hip_shared_decode", counted)
-    monkeypatch.setattr(runner_module, "prefer_shared_decode", lambda saved, heads: saved > 0)
+    monkeypatch.setattr(runner_module, "least_shared_positions", lambda *sizes: 0)
+    monkeypatch.setattr(runner_module, "prefer_shared_decode",
+                        lambda starts, shared, *sizes: any(shared))
     return calls
 
 

@@ -313,8 +313,10 @@ int32_t copy_blocks(char* keys, char* values, int64_t layer_stride, int64_t bloc
   const uint64_t bits = static_cast<uint64_t>(row_bytes) | layer_stride | block_stride |
                         token_stride | head_stride | reinterpret_cast<uintptr_t>(keys) |
                         reinterpret_cast<uintptr_t>(values);
-  if ((bits & 15u) == 0) return launch_copies<Words4>(keys, p, row_bytes, num_layers, order, stream);
-  if ((bits & 3u) == 0) return launch_copies<uint32_t>(keys, p, row_bytes, num_layers, order, stream);
+  if ((bits & 15u) == 0)
+    return launch_copies<Words4>(keys, p, row_bytes, num_layers, order, stream);
+  if ((bits & 3u) == 0)
+    return launch_copies<uint32_t>(keys, p, row_bytes, num_layers, order, stream);
   return launch_copies<uint16_t>(keys, p, row_bytes, num_layers, order, stream);
 }
 

@@ -442,7 +442,9 @@ struct RowState {
     m = mnew;
   }
   // The weight of a score, rounded to the cache's type for the product with
-  // V; the sum adds the rounded weight.
+  // V; the sum adds the rounded weight, so what rounding moves cancels in
+  // part. In fp16 a weight below 2^-25 of a wave's largest is lost: of a
+  // wave's positions in an item, a few thousand at most, 2^-13 altogether.
   template <typename E>
   __device__ __forceinline__ uint16_t weigh(float score) {
     const uint16_t p = SharedMfma<E>::round(fast_exp2(score - (m == -INFINITY ? 0.f : m)));
@@ -965,11 +967,13 @@ extern "C" int32_t mi_shared_decode(
   if (num_blocks <= 0)
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode: invalid sizes");
   if (num_seqs == 0) return MI_OK;
-  if (!query || !key_cache || !value_cache || !block_tables || !out)
+  // Tables of no columns (no sequence has a context) are never read.
+  if (!query || !key_cache || !value_cache || !out || (!block_tables && block_table_width > 0))
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode: null pointer");
   if (off_grid(query, 16) || off_grid(key_cache, 16) || off_grid(value_cache, 16) ||
       off_grid(out, 16) || off_grid(block_tables, 4) || q_token_stride % 8 || q_head_stride % 8 ||
-      out_token_stride % 8 || out_head_stride % 8 || cache_block_stride % 8 || cache_token_stride % 8 || cache_head_stride % 8)
+      out_token_stride % 8 || out_head_stride % 8 || cache_block_stride % 8 ||
+      cache_token_stride % 8 || cache_head_stride % 8)
     return fail(MI_ERR_INVALID_ARGUMENT, "mi_shared_decode: misaligned pointers or strides");
   if (cache_token_stride < 0 || cache_token_stride * kTile >= (int64_t(1) << 30))
     return fail(MI_ERR_UNSUPPORTED, "mi_shared_decode: token stride outside 2^26 elements");

@@ -139,8 +139,9 @@ __device__ __forceinline__ uint64_t nth_word(uint64_t word, int n) {
   uint32_t lo = 0;
   if (equal > 4) {
     // Ties: the lower indices among them.
-    const int above = __popcll(__ballot(key > (hi | (0xffffffffu >> (KeyBits<E>::value - 1) >> 1))));
-    const uint32_t full = hi & 0x80000000u ? hi : hi | (0xffffffffu >> (KeyBits<E>::value - 1) >> 1);
+    constexpr uint32_t kLow = 0xffffffffu >> (KeyBits<E>::value - 1) >> 1;
+    const int above = __popcll(__ballot(key > (hi | kLow)));
+    const uint32_t full = hi & 0x80000000u ? hi : hi | kLow;
     lo = nth_key<32>(key == full ? static_cast<uint32_t>(word) : 0u, n - above);
     return (static_cast<uint64_t>(full) << 32) | lo;
   }
@@ -405,8 +406,10 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
     if (wave_begin * VEC >= lead && wave_end <= pack_end && wave_end * VEC - lead <= a.vocab) {
       // All of the wave's packs are whole: its loads go out together.
 #pragma unroll
-      for (int u = 0; u < NP; ++u)
-        x[u] = load_pack<R, VEC>(grid + static_cast<int64_t>(wave_begin + u * kThreads + lane) * VEC);
+      for (int u = 0; u < NP; ++u) {
+        const int64_t pack = wave_begin + u * kThreads + lane;
+        x[u] = load_pack<R, VEC>(grid + pack * VEC);
+      }
     } else {
 #pragma unroll
       for (int u = 0; u < NP; ++u) x[u] = load_tile(p0, u);

@@ -87,10 +87,16 @@ class LLMEngine:
 
     def compact(self) -> int:
         """Move the cache blocks in use to the lowest ids, between steps; the
-        number of blocks moved. Cached prefixes in their way are forgotten."""
+        number of blocks moved. Cached prefixes in their way are forgotten. A
+        failing copy aborts every request that holds blocks and forgets all
+        cached prefixes, then re-raises."""
         moves = self.scheduler.compact()
         if moves:
-            self.model_runner.copy_blocks(*map(list, zip(*moves)))
+            try:
+                self.model_runner.copy_blocks(*map(list, zip(*moves)))
+            except Exception:
+                self.scheduler.abort_all()
+                raise
         return len(moves)
 
     def generate(self, prompts, sampling_params) -> list[list[int]]:

@@ -289,3 +289,11 @@ class Scheduler:
                 self._inflight = (kept, self._inflight[1]) if kept else None
             return True
         return False
+
+    def abort_all(self) -> None:
+        """Finish every request that holds cache blocks and forget the cached
+        prefixes: for when the blocks' contents are no longer known."""
+        for seq in [*self.waiting, *self.running]:
+            if seq.block_table:
+                self.abort(seq.seq_id)
+        self.block_manager.reset_prefix_cache()

@@ -226,6 +226,24 @@ def test_compaction_keeps_published_prefixes(scheduler_factory, sequence_cls):
     run_out(engine)
 
 
+def test_a_failing_compaction_leaves_nothing_behind(scheduler_factory, sequence_cls):
+    engine, runner, manager = make(scheduler_factory, num_blocks=12)
+    low = sequence_cls([9, 9, 9, 9, 9], params(1))
+    keep = sequence_cls(list(range(1, 10)), params(8))
+    for seq in (low, keep):
+        engine.add_request(seq)
+    engine.step()
+    late = sequence_cls(list(range(1, 10)), params(2))
+    engine.add_request(late)  # holds no blocks
+    runner.fail_copy = True
+    with pytest.raises(RuntimeError, match="copy failed"):
+        engine.compact()
+    assert keep.is_finished and keep.finish_reason == "abort" and not manager.used_block_ids
+    assert not manager.hash_to_block_id
+    run_out(engine)  # the runner would see a wrong block
+    assert len(late.completion_token_ids) == 2 and manager.prefix_cache_hit_blocks == 0
+
+
 def test_logprobs_follow_the_kept_tokens(scheduler_factory, sequence_cls):
     engine, runner, _ = make(scheduler_factory, max_num_batched_tokens=4)
     a = sequence_cls([1, 2, 3, 4, 5, 6, 7], params(3, logprobs=2))  # two prompt chunks

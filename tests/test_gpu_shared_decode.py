@@ -281,3 +281,37 @@ def test_refusals():
         batch.plan(starts=[0, 1, 2])
     with pytest.raises(ValueError, match="entry per request"):
         hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables, _ints([1]), plan=plan)
+
+
+def test_tables_without_columns():
+    # No sequence has a position: zeros, whatever the groups say.
+    batch = Batch([(1, [16, 20])])
+    contexts, tables = _ints([0, 0]), batch.tables[:, :0]
+    plan = shared_decode_plan(contexts, _ints([0, 2]), _ints([1]), num_q_heads=16, num_kv_heads=8,
+                              head_dim=128, dtype=torch.bfloat16, block_size=16,
+                              block_table_width=0)
+    for tab in (tables, tables.clone()):
+        out = hip_shared_decode(batch.q, batch.keys, batch.values, tab, contexts, plan=plan)
+        assert out.shape == batch.q.shape and not out.any()
+
+
+def test_the_most_sequences():
+    # 4096 sequences: pairs, one group, and groups of one.
+    batch = Batch([(1, [17 + i % 5, 18]) for i in range(2048)], hkv=1, hq=2)
+    batch.check()
+    one = Batch([(1, [16 + i % 7 for i in range(4096)])], hkv=1, hq=2)
+    one.check()
+    alone = one.plan(starts=list(range(4097)), shared=[1] * 4096)
+    one.check(alone)
+    with pytest.raises(ValueError, match="at most 4096 groups"):
+        one.plan(starts=list(range(4098)), shared=[0] * 4097)
+
+
+def test_lengths_of_other_types_and_strides():
+    batch = Batch([(6, _tails(96, 5, 40, 1))])
+    want = batch.check()
+    wide = torch.stack([_ints(batch.contexts), _ints([0] * 5)], 1).long()[:, 0]
+    tables = batch.tables.t().contiguous().t()  # columns outermost
+    got = hip_shared_decode(batch.q, batch.keys, batch.values, tables, wide,
+                            plan=batch.plan(contexts=wide))
+    assert torch.equal(got, want)

@@ -27,7 +27,12 @@
 // its own best words, and the last to arrive at the row's counter joins them.
 //
 // Bound by memory for many rows (about ten operations an element, one of them
-// an exp2 at a quarter of the rate), by latency for few.
+// an exp2 at a quarter of the rate): 3000 rows of 151936 in bf16 with entropy
+// 164-172 us, 5.3-5.5 TB/s, a large read's rate; with 20 alternatives 195. By
+// latency for few: 64 rows 11.6 us with entropy, 19.2 with 20 alternatives as
+// well (3.5 at the rate of a read); one row 5.3, and 9.3 with 5 alternatives.
+// 333 float32 rows of 32003 values in unaligned rows, 8 alternatives: 18.5-20.4
+// (7.6).
 #include <algorithm>
 
 #include "mi_common.h"
@@ -673,6 +678,8 @@ static_assert(kMaxParts <= kWave, "a lane per part");
 static_assert(kMaxTop * (kWaveCap / kWave) <= kKeptWords, "compressed lists fit");
 static_assert(kMaxTop <= kKeptWords, "and a scan's words");
 
+// Four workgroups a CU: 64 rows with 20 alternatives take 30.6 us with 512,
+// 19.1 with 700, 19.2 with 1024, 19.5 with 2048.
 constexpr int kWantParts = 1024;
 
 // Packs of a part of a row, a whole number of tiles: about kWantParts

@@ -681,6 +681,11 @@ static_assert(kMaxTop <= kKeptWords, "and a scan's words");
 // Four workgroups a CU: 64 rows with 20 alternatives take 30.6 us with 512,
 // 19.1 with 700, 19.2 with 1024, 19.5 with 2048.
 constexpr int kWantParts = 1024;
+// A part less where rounding up ends past five a CU, some of which would start
+// when others end: 1000 rows with 20 alternatives 91.6 us with two parts, 81.3
+// with one; 900 of 65536 values with 5 43.1, 33.5; 700 rows 68.1, 69.2. 300
+// rows keep four parts, 1200 workgroups: 38.7, 40.9 with three.
+constexpr int kMostGroups = 1280;
 
 // Packs of a part of a row, a whole number of tiles: about kWantParts
 // workgroups in all, at most kMaxParts in a row. From the sizes alone, so a
@@ -693,7 +698,9 @@ RowSplit split_row(int32_t rows, int32_t vocab, int32_t dtype) {
   const int64_t packs = (static_cast<int64_t>(vocab) + 2 * vec - 2) / vec;
   const int64_t tile = kThreads * kTilePasses;
   const int64_t tiles = (packs + tile - 1) / tile;
-  const int64_t want = std::min<int64_t>((kWantParts + rows - 1) / rows, kMaxParts);
+  int64_t want = (kWantParts + rows - 1) / rows;
+  if (want > 1 && want * rows > kMostGroups) --want;
+  want = std::min<int64_t>(want, kMaxParts);
   const int64_t each = (tiles + want - 1) / want;
   return {static_cast<int32_t>((tiles + each - 1) / each), static_cast<int32_t>(each * tile)};
 }

@@ -698,7 +698,7 @@ RowSplit split_row(int32_t rows, int32_t vocab, int32_t dtype) {
   const int64_t packs = (static_cast<int64_t>(vocab) + 2 * vec - 2) / vec;
   const int64_t tile = kThreads * kTilePasses;
   const int64_t tiles = (packs + tile - 1) / tile;
-  int64_t want = (kWantParts + rows - 1) / rows;
+  int64_t want = (kWantParts + int64_t(rows) - 1) / rows;
   if (want > 1 && want * rows > kMostGroups) --want;
   want = std::min<int64_t>(want, kMaxParts);
   const int64_t each = (tiles + want - 1) / want;

@@ -57,3 +57,17 @@ def test_workspace_is_checked():
     assert _call(lib, **big, workspace_bytes=need - 1) == 3
     assert _call(lib, **big, workspace=4104) == 3
     assert _call(lib, **big, counters=None) == 3 and "counters" in _lib.last_error()
+
+
+def test_parts_of_any_number_of_rows():
+    # A whole number of records per row, none where the rows fill the chip, up
+    # to the last int32.
+    size = _lib.load().mi_token_logprobs_workspace_bytes
+    for rows in (1, 2, 19, 64, 100, 333, 700, 1000, 1024, 1025, 1281, (1 << 31) - 1024,
+                 (1 << 31) - 1):
+        for vocab, dtype in ((4096, 2), (32003, 0), (151936, 1), (1 << 30, 2)):
+            need = size(rows, vocab, 8, dtype)
+            assert need >= 0 and need % (rows * (16 + 64)) == 0
+            parts = need // (rows * (16 + 64))
+            assert parts != 1 and parts <= 64 and (rows <= 1024 or parts == 0)
+            assert rows * parts <= 1280 or parts == 0

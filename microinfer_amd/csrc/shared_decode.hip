@@ -18,7 +18,7 @@
 // groups and their shared pages, once for all layers of a step.
 //
 // Bound by latency below some 50 MB of K/V, by memory above. Measured per layer
-// (block 16, 8 KV heads, bf16, captured; the plan's eighth of 8-12 us and the
+// (block 16, 8 KV heads, bf16, captured; the plan's eighth of 6-10 us and the
 // join's 2.5-4 us included), us here / each sequence reading its own context:
 //   4 sequences, 500 shared tokens, 16 query heads         9.3 /  8.8
 //   16 with 12000 shared, up to 500 own, 32 query heads   26.5 / 66.8

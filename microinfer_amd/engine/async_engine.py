@@ -38,7 +38,7 @@ import threading
 from dataclasses import dataclass
 
 from microinfer_amd.engine.config import SampleParameter
-from microinfer_amd.engine.sequence import Sequence
+from microinfer_amd.engine.sequence import Sequence, TokenLogprob
 
 logger = logging.getLogger(__name__)
 
@@ -62,6 +62,8 @@ class RequestOutput:
     token_ids: tuple[int, ...]
     finished: bool
     finish_reason: str | None
+    # As ``Sequence.logprobs``, where they were asked for.
+    logprobs: tuple[TokenLogprob, ...] = ()
 
 
 class RequestChannel:
@@ -70,9 +72,12 @@ class RequestChannel:
     Only the event loop's thread writes to it.
     """
 
-    def __init__(self, seq_id: int, prompt_tokens: int):
+    def __init__(self, seq_id: int, prompt_tokens: int, logprobs: list | None = None):
         self.seq_id = seq_id
         self.prompt_tokens = prompt_tokens
+        # The sequence's own list, which the engine thread appends to: it may be
+        # a token ahead of the events.
+        self.logprobs = logprobs if logprobs is not None else []
         self.token_ids: tuple[int, ...] = ()
         self.text = ""
         self.finished = False
@@ -172,8 +177,8 @@ class _EngineThread(threading.Thread):
                 self.live.update(seq.seq_id for seq in children)
                 # Their channels exist before the next step's updates arrive.
                 return self.report(self.frontend._settle_fork, future, arg[1],
-                                   [(seq.seq_id, seq.num_prompt_tokens) for seq in children],
-                                   None, self.engine.stats())
+                                   [(seq.seq_id, seq.num_prompt_tokens, seq.logprobs)
+                                    for seq in children], None, self.engine.stats())
             else:  # "abort"
                 result = self.engine.abort(arg)
                 self.live.discard(arg)
@@ -256,7 +261,7 @@ class AsyncEngine:
         self._reserved -= n
         if future.cancelled():  # nobody will read them
             loop = asyncio.get_running_loop()
-            for seq_id, _ in children:
+            for seq_id, *_ in children:
                 self._thread.post("abort", seq_id, loop.create_future())
             children = []
         channels = [RequestChannel(*child) for child in children]
@@ -294,7 +299,7 @@ class AsyncEngine:
             raise BackpressureError(f"{tracked} requests already tracked "
                                     f"(max_waiting={self.max_waiting})")
         seq = Sequence(list(prompt), sampling_params)
-        channel = RequestChannel(seq.seq_id, seq.num_prompt_tokens)
+        channel = RequestChannel(seq.seq_id, seq.num_prompt_tokens, seq.logprobs)
         self._channels[seq.seq_id] = channel  # counts against max_waiting at once
         try:
             await self._command("admit", seq)
@@ -347,7 +352,8 @@ class AsyncEngine:
             last = event
         if last is None:
             raise RuntimeError("request stream ended without an event")
-        return RequestOutput(request.seq_id, last.token_ids, last.finished, last.finish_reason)
+        return RequestOutput(request.seq_id, last.token_ids, last.finished, last.finish_reason,
+                             tuple(request.logprobs))
 
     async def generate(self, prompt, sampling_params: SampleParameter) -> RequestOutput:
         return await self.collect(await self.add_request(prompt, sampling_params))

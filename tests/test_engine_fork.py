@@ -316,6 +316,28 @@ def test_async_forks_stream_from_the_tokens_so_far(scheduler_factory, sequence_c
     asyncio.run(scenario())
 
 
+def test_async_requests_carry_their_logprobs(scheduler_factory):
+    engine, _, _ = make(scheduler_factory)
+
+    async def scenario():
+        frontend = AsyncEngine(engine)
+        plain = await frontend.generate([1, 2], params(3))
+        assert plain.logprobs == ()
+        request = await frontend.add_request([1, 2, 3], params(6, logprobs=0))
+        stream = frontend.stream(request)
+        event = await anext(stream)
+        assert len(request.logprobs) >= len(event.token_ids)
+        fork, = await frontend.fork(request)
+        for out in (await frontend.collect(fork), request):
+            async for event in stream:
+                pass
+            assert [e.token_id for e in out.logprobs] == list(out.token_ids)
+            assert [e.logprob for e in out.logprobs] == [-3.0, -4.0, -5.0, -6.0, -7.0, -8.0]
+        await frontend.stop()
+
+    asyncio.run(scenario())
+
+
 def test_shared_groups_of_neighbours():
     a = list(range(10))
     tables = [a + [20], a + [21, 22], a[:8] + [23, 24], [50, 51], [50, 52], [60]]

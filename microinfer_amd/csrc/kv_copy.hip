@@ -49,6 +49,7 @@ constexpr int kMaxOps = 256;
 struct CopyList {
   CopyOp op[kMaxOps];
 };
+constexpr int64_t kMaxGroupBlocks = 1 << 23;
 // Groups of dependent copies: group g is ops [start[g], start[g + 1]). dst = -1
 // keeps the source's word, src = -1 writes the kept word.
 struct GroupList {
@@ -147,9 +148,41 @@ struct Order {
   std::vector<size_t> whole_from;           // per group: ops from here on share a launch
 };
 
-// Orders `ops` (distinct destinations, src != dst); into[b] is 1 + the index of
-// the op that writes block b, 0 if none does.
-void order_pairs(const std::vector<CopyOp>& ops, const std::vector<int32_t>& into, Order* out) {
+// Which op writes a block: a table of the pool's blocks, or for few pairs the
+// sorted destinations. A table takes 24 ns per 1000 blocks to clear, sorting
+// and finding 35 ns a pair: calls of 1 and 500 pairs in a pool of 150000 blocks
+// 11.0 and 21.6 us with a table, 7.5 and 34.4 without.
+class Writers {
+ public:
+  Writers(const int32_t* dst, int32_t num_pairs, int32_t num_blocks) {
+    if (num_pairs < num_blocks / 1024) {
+      sorted_.reserve(num_pairs);
+      for (int32_t i = 0; i < num_pairs; ++i) sorted_.push_back({dst[i], 0});
+      std::sort(sorted_.begin(), sorted_.end());
+    } else {
+      table_.assign(num_blocks, 0);
+    }
+  }
+  // Of block b: 1 + the index of the op that writes it, -1 if its pair needs no
+  // op, 0 if no pair writes it.
+  int32_t operator[](int32_t b) {
+    const int32_t* at = find(b);
+    return at == nullptr ? 0 : *at;
+  }
+  void set(int32_t b, int32_t value) { *find(b) = value; }
+
+ private:
+  int32_t* find(int32_t b) {
+    if (!table_.empty()) return &table_[b];
+    const auto it = std::lower_bound(sorted_.begin(), sorted_.end(), std::make_pair(b, INT32_MIN));
+    return it != sorted_.end() && it->first == b ? &it->second : nullptr;
+  }
+  std::vector<int32_t> table_;
+  std::vector<std::pair<int32_t, int32_t>> sorted_;
+};
+
+// Orders `ops` (distinct destinations, src != dst).
+void order_pairs(const std::vector<CopyOp>& ops, Writers& into, Order* out) {
   const int n = static_cast<int>(ops.size());
   // readers[i]: how many ops still to run read the block that op i writes.
   std::vector<int32_t> readers(n, 0), group(n);
@@ -249,7 +282,9 @@ int32_t launch_copies(char* base, const PageShape& shape, int32_t row_bytes, int
     for (size_t i = 0; i < all.size();) {
       // A cycle goes whole; other ops one by one, in order over the launches.
       const size_t take = i == order.whole_from[g] ? all.size() - i : 1;
-      if (ops + take > static_cast<size_t>(kMaxOps)) {
+      // A launch's threads are counted in 32 bits.
+      if (ops + take > static_cast<size_t>(kMaxOps) ||
+          (groups + 1) * static_cast<int64_t>(thin) > kMaxGroupBlocks) {
         const int32_t status = flush();
         if (status != MI_OK) return status;
       }
@@ -267,25 +302,24 @@ int32_t copy_blocks(char* keys, char* values, int64_t layer_stride, int64_t bloc
                     int32_t block_size, int32_t num_blocks, hipStream_t stream) {
   std::vector<CopyOp> ops;
   ops.reserve(num_pairs);
-  std::vector<int32_t> into(num_blocks, 0);
-  std::vector<char> written(num_blocks, 0);
-  for (int32_t i = 0; i < num_pairs; ++i) {
-    const int32_t n = tokens == nullptr ? block_size : tokens[i];
+  for (int32_t i = 0; i < num_pairs; ++i)
     if (src[i] < 0 || src[i] >= num_blocks || dst[i] < 0 || dst[i] >= num_blocks)
       return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: block id outside the pool");
+  Writers into(dst, num_pairs, num_blocks);
+  for (int32_t i = 0; i < num_pairs; ++i) {
+    const int32_t n = tokens == nullptr ? block_size : tokens[i];
     if (n < 0 || n > block_size)
       return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: tokens outside the block");
-    if (written[dst[i]])
+    if (into[dst[i]] != 0)
       return fail(MI_ERR_INVALID_ARGUMENT, "mi_kv_copy_blocks: a block is written twice");
-    written[dst[i]] = 1;
-    if (n == 0 || src[i] == dst[i]) continue;
-    ops.push_back(CopyOp{src[i], dst[i], n});
-    into[dst[i]] = static_cast<int32_t>(ops.size());
+    const bool copies = n > 0 && src[i] != dst[i];
+    if (copies) ops.push_back(CopyOp{src[i], dst[i], n});
+    into.set(dst[i], copies ? static_cast<int32_t>(ops.size()) : -1);
   }
   if (ops.empty()) return MI_OK;
   Order order;
   bool free_order = true;
-  for (const CopyOp& op : ops) free_order = free_order && into[op.src] == 0;
+  for (const CopyOp& op : ops) free_order = free_order && into[op.src] <= 0;
   if (free_order)
     order.single.swap(ops);
   else

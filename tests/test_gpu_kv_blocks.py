@@ -184,3 +184,18 @@ def test_another_stream_and_a_captured_call():
         torch.cuda.synchronize()
         for s, d in ((1, 8), (1, 9), (2, 10)):
             assert torch.equal(k[:, d], k[:, s]) and torch.equal(v[:, d], v[:, s])
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_few_pairs_of_many_blocks(seed):
+    rng = random.Random(seed)
+    cache = _cache(2, 40000, 4, 2, 8, torch.bfloat16, LAYOUTS[seed % 3], seed)
+    k, v = cache.keys, cache.values
+    a, b, c, d, e, f, g = rng.sample(range(40000), 7)
+    _check(k, v, [a], [b])
+    _check(k, v, [a, b], [b, a])
+    _check(k, v, [a, b, c, b, d, e, a], [b, c, a, d, e, f, g])
+    for n in (2, 17, 38, 124):
+        dst = rng.sample(range(40000), n)
+        src = [rng.choice(dst) if rng.random() < 0.7 else rng.randrange(40000) for _ in range(n)]
+        _check(k, v, src, dst, [rng.randint(0, 4) for _ in range(n)])

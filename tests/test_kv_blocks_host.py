@@ -30,8 +30,8 @@ def _call(lib, src=(0, 1), dst=(2, 3), tokens=None, **over):
         return None if values is None else (ctypes.c_int32 * max(len(values), 1))(*values)
 
     args = dict(keys=4096, values=8192, ls=1 << 16, bs=4096, ts=128, hs=2048, src=ints(src),
-                dst=ints(dst), tokens=ints(tokens), pairs=len(src or dst), layers=2, heads=2, dim=128,
-                block=16, blocks=8, dtype=2)
+                dst=ints(dst), tokens=ints(tokens), pairs=len(src or dst), layers=2, heads=2,
+                dim=128, block=16, blocks=8, dtype=2)
     args.update(over)
     return lib.mi_kv_copy_blocks(*args.values(), None)
 
@@ -57,7 +57,14 @@ def test_c_entry_validates_before_launch():
     assert _call(lib, tokens=(-1, 3)) == 1
     assert _call(lib, dst=(2, 2)) == 1 and "twice" in _lib.last_error()
     assert _call(lib, dst=(2, 2), tokens=(0, 16)) == 1
+    # The same in a pool of many more blocks than pairs.
+    big = dict(blocks=1 << 20)
+    assert _call(lib, src=(0, 1 << 20), **big) == 1 and "block id" in _lib.last_error()
+    assert _call(lib, dst=(9, 9), **big) == 1 and "twice" in _lib.last_error()
+    assert _call(lib, dst=(9, 9), tokens=(0, 16), **big) == 1
+    assert _call(lib, tokens=(0, 17), **big) == 1 and "tokens" in _lib.last_error()
     ring = tuple(range(300))
+    assert _call(lib, src=ring, dst=ring[1:] + ring[:1], **big) == 2
     assert _call(lib, src=ring, dst=ring[1:] + ring[:1], blocks=300) == 2
     assert "cycle" in _lib.last_error()
 
@@ -67,4 +74,6 @@ def test_nothing_to_copy_is_no_launch():
     assert _call(lib, src=(), dst=()) == 0
     assert _call(lib, tokens=(0, 0)) == 0
     assert _call(lib, src=(4, 5), dst=(4, 5)) == 0
+    assert _call(lib, src=(4, 5), dst=(4, 5), blocks=5000) == 0
+    assert _call(lib, src=(4, 5), dst=(5, 6), tokens=(0, 0), blocks=5000) == 0
     assert _lib.last_error() == ""

@@ -14,7 +14,6 @@ of at least 16 have a kernel of their own; every other shape that
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -51,6 +50,7 @@ class SharedDecodePlan:
     buffer: torch.Tensor
     shared: bool  # False: a ``decode_plan`` for ``hip_paged_decode``
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
+    workspace_bytes: int = 0  # of a call with it
 
 
 def shared_order(tables) -> list[int]:
@@ -202,7 +202,9 @@ def shared_decode_plan(context_lens: torch.Tensor, group_starts: torch.Tensor,
             _lib.dtype_code(dtype), buffer.data_ptr(), nbytes,
             _lib.stream_handle(context_lens.device))
     _lib.check(status, "mi_shared_decode_plan")
-    return SharedDecodePlan(buffer, True, sizes)
+    return SharedDecodePlan(
+        buffer, True, sizes,
+        lib.mi_shared_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads))
 
 
 def hip_shared_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -214,47 +216,53 @@ def hip_shared_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
     The caches hold the step's K/V rows already. Without a plan there are no
     groups to share pages in: call ``hip_paged_decode``.
     """
-    if query.ndim != 3:
+    shape, dtype, device = query.shape, query.dtype, query.device
+    if len(shape) != 3:
         raise ValueError("query must have shape [requests, Hq, D]")
     if key_cache.ndim != 4:
         raise ValueError("key_cache must have shape [blocks, B, Hkv, D]")
-    num_seqs, num_q_heads, head_dim = query.shape
+    num_seqs, num_q_heads, head_dim = shape
     num_blocks, block_size, num_kv_heads, kv_dim = key_cache.shape
     if kv_dim != head_dim:
         raise ValueError("query and cache head dimensions differ")
-    if query.device != key_cache.device or query.dtype != key_cache.dtype:
+    if device != key_cache.device or dtype != key_cache.dtype:
         raise ValueError("query and cache must share device/dtype")
     if block_tables.ndim != 2 or block_tables.shape[0] != num_seqs:
         raise ValueError("block_tables must have one row per request")
     if context_lens.numel() != num_seqs:
         raise ValueError("context_lens must have one entry per request")
-    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, query.dtype, block_size,
-             block_tables.shape[1])
+    width = block_tables.shape[1]
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size, width)
     if not isinstance(plan, SharedDecodePlan) or plan.sizes != sizes:
         raise ValueError("plan must come from shared_decode_plan() for this call's sizes")
     _lib.require_device(query, block_tables, context_lens, what="hip_shared_decode")
-    if plan.buffer.device != query.device or block_tables.device != query.device:
+    buffer = plan.buffer
+    if buffer.device != device or block_tables.device != device:
         raise ValueError("plan and block_tables must be on the query's device")
     key_cache, value_cache = _check_caches(key_cache, value_cache)
     query = _inner_contiguous(query)
     if not plan.shared:
         return hip_paged_decode(query, key_cache, value_cache, block_tables, context_lens,
-                                scale=scale, plan=plan.buffer if num_seqs else None)
+                                scale=scale, plan=buffer if num_seqs else None)
     block_tables = _index32(block_tables)
     if scale is None:
-        scale = 1.0 / math.sqrt(head_dim)
+        scale = head_dim ** -0.5
+    q_token_stride, q_head_stride, _ = query.stride()
+    if (query.data_ptr() | 2 * q_token_stride | 2 * q_head_stride) & 15:
+        query = query.clone(memory_format=torch.contiguous_format)  # rows of whole vectors
+        q_token_stride, q_head_stride, _ = query.stride()
     lib = _lib.load()
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    with _lib.on_device(query.device):
-        ws_bytes = lib.mi_shared_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads)
-        stream = _lib.stream_handle(query.device)
-        workspace = _workspace(query.device, stream, ws_bytes)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    with _lib.on_device(device):
+        stream = _lib.stream_handle(device)
+        workspace = _workspace(device, stream, plan.workspace_bytes)
+        block_stride, token_stride, head_stride, _ = key_cache.stride()
         status = lib.mi_shared_decode(
-            query.data_ptr(), query.stride(0), query.stride(1), key_cache.data_ptr(),
-            value_cache.data_ptr(), *key_cache.stride()[:3], block_tables.data_ptr(),
-            block_tables.stride(0), block_tables.shape[1], plan.buffer.data_ptr(),
-            plan.buffer.numel(), out.data_ptr(), out.stride(0), out.stride(1),
-            workspace.data_ptr(), ws_bytes, num_seqs, num_q_heads, num_kv_heads, head_dim,
-            block_size, num_blocks, float(scale), _lib.DTYPE_CODES[query.dtype], stream)
+            query.data_ptr(), q_token_stride, q_head_stride, key_cache.data_ptr(),
+            value_cache.data_ptr(), block_stride, token_stride, head_stride,
+            block_tables.data_ptr(), width, width, buffer.data_ptr(), buffer.numel(),
+            out.data_ptr(), num_q_heads * head_dim, head_dim, workspace.data_ptr(),
+            plan.workspace_bytes, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+            num_blocks, float(scale), _lib.DTYPE_CODES[dtype], stream)
     _lib.check(status, "mi_shared_decode")
     return out

@@ -315,3 +315,16 @@ def test_lengths_of_other_types_and_strides():
     got = hip_shared_decode(batch.q, batch.keys, batch.values, tables, wide,
                             plan=batch.plan(contexts=wide))
     assert torch.equal(got, want)
+
+
+def test_unaligned_queries():
+    batch = Batch([(6, _tails(96, 5, 40, 1))])
+    want = batch.check()
+    wide = torch.zeros(5, 16, 131, device=DEV, dtype=torch.bfloat16)
+    wide[:, :, 3:] = batch.q
+    flat = torch.zeros(batch.q.numel() + 1, device=DEV, dtype=torch.bfloat16)
+    flat[1:] = batch.q.flatten()
+    for q in (wide[:, :, 3:], flat[1:].view_as(batch.q)):
+        got = hip_shared_decode(q, batch.keys, batch.values, batch.tables, _ints(batch.contexts),
+                                plan=batch.plan())
+        assert torch.equal(got, want) and got.is_contiguous()

@@ -15,7 +15,6 @@ import torch
 
 from microinfer_amd import _lib
 
-_FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 MAX_TOP = 32
 
 # Scratch of a stream's launches: arrival counters (zero-filled once, left zero
@@ -66,7 +65,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     still in order. Results that were not asked for are ``None``.
     """
     _lib.require_device(logits, tokens, temperatures, what="token log probabilities")
-    if logits.dtype not in _FLOAT_DTYPES:
+    code = _lib.DTYPE_CODES.get(logits.dtype)
+    if code is None:
         raise ValueError("logits must be float16, bfloat16 or float32")
     if logits.ndim != 2 or logits.shape[1] == 0:
         raise ValueError("logits must be [rows, vocab] with vocab > 0")
@@ -76,9 +76,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         raise ValueError("vocab must be at most 2^30")
     if type(top) is not int or not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be an integer between 0 and {MAX_TOP}, at most vocab")
-    if any(t is not None and t.device != device for t in (tokens, temperatures)):
+    if (tokens is not None and tokens.device != device) or \
+            (temperatures is not None and temperatures.device != device):
         raise ValueError("tokens and temperatures must be on the logits' device")
     given = 0
+    logprobs = ent = top_tokens = top_logprobs = None
+    logprobs_at = ent_at = top_tokens_at = top_logprobs_at = temperatures_at = None
     if tokens is not None:
         if tokens.dtype not in (torch.int64, torch.int32) or tokens.ndim not in (1, 2) \
                 or tokens.shape[0] != rows:
@@ -92,29 +95,37 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
 
-    result = TokenLogprobs(
-        None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=device),
-        torch.empty(rows, dtype=torch.float32, device=device) if entropy else None,
-        torch.empty((rows, top), dtype=torch.int64, device=device) if top else None,
-        torch.empty((rows, top), dtype=torch.float32, device=device) if top else None)
+    if tokens is not None:
+        logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=device)
+        logprobs_at = logprobs.data_ptr()
+    if entropy:
+        ent = torch.empty(rows, dtype=torch.float32, device=device)
+        ent_at = ent.data_ptr()
+    if top:
+        top_tokens = torch.empty((rows, top), dtype=torch.int64, device=device)
+        top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+        top_tokens_at, top_logprobs_at = top_tokens.data_ptr(), top_logprobs.data_ptr()
+    result = TokenLogprobs(logprobs, ent, top_tokens, top_logprobs)
     if rows == 0 or not (given or top or entropy):
         return result
-    if tokens is not None and (tokens.dtype != torch.int64 or not tokens.is_contiguous()):
-        tokens = tokens.to(torch.int64).contiguous()
+    tokens_at = counters_at = workspace_at = None
+    if tokens is not None:
+        if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+            tokens = tokens.to(torch.int64).contiguous()
+        tokens_at = tokens.data_ptr()
     if temperatures is not None:
         temperatures = temperatures.contiguous()
-    lib, code = _lib.load(), _lib.DTYPE_CODES[logits.dtype]
+        temperatures_at = temperatures.data_ptr()
+    lib = _lib.load()
     need = lib.mi_token_logprobs_workspace_bytes(rows, vocab, top, code)
     with _lib.on_device(device):
         stream = _lib.stream_handle(device)
-        counters = workspace = None
         if need:
             counters, workspace = _scratch(device, stream, rows, need)
+            counters_at, workspace_at = counters.data_ptr(), workspace.data_ptr()
         status = lib.mi_token_logprobs(
-            logits.data_ptr(), logits.stride(0), rows, vocab, code,
-            *[None if t is None else t.data_ptr() for t in (temperatures, tokens)], given, given,
-            *[None if t is None else t.data_ptr() for t in result], top,
-            None if workspace is None else workspace.data_ptr(), need,
-            None if counters is None else counters.data_ptr(), stream)
+            logits.data_ptr(), logits.stride(0), rows, vocab, code, temperatures_at, tokens_at,
+            given, given, logprobs_at, ent_at, top_tokens_at, top_logprobs_at, top, workspace_at,
+            need, counters_at, stream)
     _lib.check(status, "mi_token_logprobs")
     return result

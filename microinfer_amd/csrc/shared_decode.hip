@@ -29,10 +29,12 @@
 // The long prefixes reach 3.4 TB/s of distinct rows: of the 16 sequences'
 // launch (20 us, 11.6 at the rate of a large read) 4 us pass before the first
 // tiles are there and 1.5 at the end; between, a workgroup takes 1.2 us for
-// a stage of 64 positions, of which its waves' reads of LDS are 0.4 (each of
-// the four row waves reads every tile). Stages begun one earlier (two in
-// flight, a barrier more) moved these by 3 % either way, and so 16 waves on
-// 128 KiB, one workgroup per CU (10.1, 26.5, 25.5, 36.5).
+// a stage of 64 positions, and two on a CU take turns: each of the four row
+// waves reads every tile, 160 KB of LDS traffic a stage. Moved by 3 % at most,
+// either way: stages begun one earlier (two in flight, a barrier more), half
+// the vector instructions (row sums by dot products, a maximum joined only
+// when it moves, block ids from registers), 16 waves on 128 KiB, one workgroup
+// per CU (10.1, 26.5, 25.5, 36.5).
 #include <algorithm>
 
 #include "paged_attention.h"

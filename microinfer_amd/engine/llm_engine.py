@@ -48,12 +48,12 @@ class LLMEngine:
             for seq in seqs:  # KV may be partly written: publish nothing
                 self.scheduler.abort(seq.seq_id)
             raise
-        lengths = [len(s) for s in seqs]
+        scored = [(s, len(s)) for s in seqs if s.sampling.logprobs is not None]
         self.scheduler.postprocess(seqs, tokens, prefill)
-        if any(s.sampling.logprobs is not None for s in seqs):
+        if scored:
             # Of the tokens that were kept: a prompt chunk's sample is not.
             logprobs = self.model_runner.take_logprobs()
-            for seq, length in zip(seqs, lengths):
+            for seq, length in scored:
                 if len(seq) > length and seq.seq_id in logprobs:
                     seq.logprobs.append(logprobs[seq.seq_id])
         done = [s.status == SequenceStatus.FINISHED for s in seqs]

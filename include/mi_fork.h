@@ -68,9 +68,9 @@ int32_t mi_kv_copy_blocks(void* key_cache, void* value_cache, int64_t layer_stri
  * initialisation, its own for calls that may run concurrently. Both sizes
  * depend on their arguments only. bf16/f16, head_dim 128, at most 16 query
  * heads per KV head, block_size >= 16 and a power of two, at most 4096
- * sequences and groups (MI_ERR_UNSUPPORTED otherwise: mi_paged_decode takes those).
- * query, the caches and out 16-byte aligned, with strides of whole 16-byte
- * vectors.
+ * sequences and groups (MI_ERR_UNSUPPORTED otherwise: mi_paged_decode takes
+ * those). query, the caches and out 16-byte aligned, with strides of whole
+ * 16-byte vectors; block_tables may be NULL where it has no columns.
  */
 int64_t mi_shared_decode_plan_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads);
 int64_t mi_shared_decode_workspace_bytes(int32_t num_seqs, int32_t num_q_heads,

@@ -328,3 +328,42 @@ def test_unaligned_queries():
         got = hip_shared_decode(q, batch.keys, batch.values, batch.tables, _ints(batch.contexts),
                                 plan=batch.plan())
         assert torch.equal(got, want) and got.is_contiguous()
+
+
+def test_two_graphs_and_eager_calls_share_nothing():
+    batches = [Batch([(60, _tails(960, 12, 200, s))], hq=32, seed=s) for s in (1, 2, 3)]
+    want = [batch.check() for batch in batches]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs, outs, kept = [], [], []
+    for batch, stream in zip(batches, streams):
+        args = [_ints(x) for x in (batch.contexts, batch.starts, batch.shared)]
+        kept.append(args)  # the graph reads them
+        sizes = dict(num_q_heads=32, num_kv_heads=8, head_dim=128, dtype=torch.bfloat16,
+                     block_size=16, block_table_width=batch.tables.shape[1])
+
+        def step(batch=batch, args=args, sizes=sizes):
+            return hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables, args[0],
+                                     plan=shared_decode_plan(*args, **sizes))
+
+        if len(graphs) == 2:
+            break
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with capture_graph(graph, stream=stream):
+            outs.append(step())
+        graphs.append(graph)
+    for _ in range(10):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = [step() for _ in range(3)]
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        assert all(torch.equal(x, want[2]) for x in eager)

@@ -36,6 +36,7 @@
 // when it moves, block ids from registers), 16 waves on 128 KiB, one workgroup
 // per CU (10.1, 26.5, 25.5, 36.5).
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attention.h"
 #include "mi_fork.h"
@@ -101,7 +102,9 @@ constexpr int kRowWaves = kMaxRows / kTile;       // waves that split the rows
 constexpr int kKeyWaves = kWaves / kRowWaves;     // and the tiles of a stage
 constexpr int kWaveTiles = kStageTiles / kKeyWaves;
 constexpr int kAccStride = kD + 4;  // floats: rows of a wave's sums, 4 banks apart
-constexpr int kRescaleSlack = 15;
+// Weights go up to 2^kMostWeight (fp16 ends at 2^16) before a row's reference
+// moves.
+constexpr int kMostWeight = 15;
 static_assert(2 * kStageBytes == kRingBytes, "two stages");
 static_assert(kStageTiles * 2 == kWaves, "a stage is one half-tile per wave");
 static_assert(kKeyWaves == 2 && kWaveTiles == 2, "two key waves, 32 positions each");
@@ -456,36 +459,49 @@ struct ItemLoop {
   }
 };
 
+// A weight in the cache's type: what it rounds to, and what that leaves out,
+// rounded again.
+struct Weight {
+  uint16_t high, low;
+};
+
 // The running softmax of one query row per lane (shared by the lanes of equal
-// `col`), with the row's sums over 128 dims in o.
+// `col`), with the row's sums over 128 dims in o. The reference m is near the
+// maximum; fp16 keeps it 2^10 below, so that only weights under 2^-35 of a
+// wave's largest vanish (bf16 has float32's range).
+template <typename E>
 struct RowState {
+  static constexpr float kBelow = std::is_same<E, F16>::value ? 10.f : 0.f;
   f32x4_t o[kD / 16];
   float m = -INFINITY, l = 0.f;
   __device__ __forceinline__ RowState() {
 #pragma unroll
     for (int db = 0; db < kD / 16; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  // Moves the maximum when some row's new scores exceed its by 2^15.
+  // Moves the references when some row's new scores lie too far above.
   __device__ __forceinline__ void see(float tmax, int lane) {
     tmax = fmaxf(tmax, lane_xor16(tmax, lane));
     tmax = fmaxf(tmax, lane_xor32(tmax, lane));
-    if (__ballot(tmax > m + kRescaleSlack) == 0) return;
-    const float mnew = fmaxf(m, tmax);
+    if (__ballot(tmax > m + kMostWeight) == 0) return;
+    const float mnew = fmaxf(m, tmax - kBelow);
     const float alpha = mnew == -INFINITY ? 1.f : fast_exp2(m - mnew);
     l *= alpha;
 #pragma unroll
     for (int db = 0; db < kD / 16; ++db) o[db] *= alpha;
     m = mnew;
   }
-  // The weight of a score, rounded to the cache's type for the product with
-  // V; the sum adds the rounded weight, so what rounding moves cancels in
-  // part. In fp16 a weight below 2^-25 of a wave's largest is lost: of a
-  // wave's positions in an item, a few thousand at most, 2^-13 altogether.
-  template <typename E>
-  __device__ __forceinline__ uint16_t weigh(float score) {
-    const uint16_t p = SharedMfma<E>::round(fast_exp2(score - (m == -INFINITY ? 0.f : m)));
-    l += E::load(p);
-    return p;
+  // The weight of a score in two halves, which meet V one after the other: to
+  // 2^-16 of it in bf16, 2^-22 in fp16. One half alone leaves an output 2^-8 or
+  // 2^-11 of the values off, as much again as its own rounding (16 sequences
+  // behind 12000 tokens in bf16: 0.00231 of the outputs' size from 64 bits, 0.00166
+  // with both, which is their rounding alone; 26.5 us either way).
+  __device__ __forceinline__ Weight weigh(float score) {
+    const float p = fast_exp2(score - (m == -INFINITY ? 0.f : m));
+    l += p;
+    Weight w;
+    w.high = SharedMfma<E>::round(p);
+    w.low = SharedMfma<E>::round(p - E::load(w.high));
+    return w;
   }
   __device__ __forceinline__ void close(int lane) {
     l += lane_xor16(l, lane);
@@ -543,7 +559,7 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  RowState row;
+  RowState<E> row;
   if (wave < ntiles) {
     typename M::vec8 qf[kD / 32];
     x.row_fragments(s.q, qf);
@@ -583,12 +599,19 @@ __device__ __forceinline__ void run_few_rows(const SharedArgs& a, const SharedIt
         tmax = fmaxf(tmax, sc[i]);
       }
       row.see(tmax, lane);
-      Pack<R, 4> pk;
+      Pack<R, 4> high, low;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pk.v[i] = row.template weigh<E>(sc[i]);
-      const short4_t pf = __builtin_bit_cast(short4_t, pk);
+      for (int i = 0; i < 4; ++i) {
+        const Weight w = row.weigh(sc[i]);
+        high.v[i] = w.high;
+        low.v[i] = w.low;
+      }
+      const short4_t pf = __builtin_bit_cast(short4_t, high);
+      const short4_t pl = __builtin_bit_cast(short4_t, low);
 #pragma unroll
       for (int db = 0; db < kD / 16; ++db) row.o[db] = M::pv(vf[db], pf, row.o[db]);
+#pragma unroll
+      for (int db = 0; db < kD / 16; ++db) row.o[db] = M::pv(vf[db], pl, row.o[db]);
       if (k + kWaves >= ntiles) break;
     }
   }
@@ -695,7 +718,7 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
   vec8 qf[kD / 32];
   x.row_fragments(q_tile, qf);
   const bool active = kTile * row_wave < x.rows;
-  RowState row;
+  RowState<E> row;
   for (int k = 0; k < nstages; ++k) {
     // Stage k's loads of this wave are done, its earlier reads too; behind the
     // barrier those of every wave are.
@@ -749,17 +772,23 @@ __device__ __forceinline__ void run_many_rows(const SharedArgs& a, const SharedI
     row.see(tmax, lane);
     // The contraction runs over k = 8 quad + 4 j + i: position 4 quad + i of
     // tile j, for the weights as for V.
-    Pack<R, 8> pk;
+    Pack<R, 8> high, low;
 #pragma unroll
     for (int j = 0; j < kWaveTiles; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pk.v[4 * j + i] = row.template weigh<E>(sc[j][i]);
-    const vec8 pf = __builtin_bit_cast(vec8, pk);
+      for (int i = 0; i < 4; ++i) {
+        const Weight w = row.weigh(sc[j][i]);
+        high.v[4 * j + i] = w.high;
+        low.v[4 * j + i] = w.low;
+      }
+    const vec8 pf = __builtin_bit_cast(vec8, high);
+    const vec8 pl = __builtin_bit_cast(vec8, low);
 #pragma unroll
     for (int db = 0; db < kD / 16; ++db) {
       const vec8 v8 = __builtin_bit_cast(
           vec8, __builtin_shufflevector(vf[0][db], vf[1][db], 0, 1, 2, 3, 4, 5, 6, 7));
       row.o[db] = M::qk(v8, pf, row.o[db]);
+      row.o[db] = M::qk(v8, pl, row.o[db]);
     }
   }
   row.close(lane);

@@ -367,3 +367,54 @@ def test_two_graphs_and_eager_calls_share_nothing():
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
         assert all(torch.equal(x, want[2]) for x in eager)
+
+
+def _exact(batch, s, scale):
+    """Sequence s in float64: its output and the same of |v|."""
+    c, (_, _, hkv, dim) = batch.contexts[s], batch.keys.shape
+    ids = batch.tables[s, : -(-c // batch.block)].long()
+    k, v = (x[ids].flatten(0, 1)[:c].double().transpose(0, 1).contiguous()
+            for x in (batch.keys, batch.values))
+    q = batch.q[s].double().view(hkv, -1, dim)
+    p = torch.softmax(torch.matmul(q, k.transpose(1, 2).contiguous()) * scale, -1)
+    return torch.matmul(p, v).view(-1, dim), torch.matmul(p, v.abs()).view(-1, dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("groups", [
+    [(2, _tails(32, 12, 30, 1)), (1, _tails(16, 7, 9, 2))], [(0, _tails(0, 5, 70, 3))],
+    [(30, _tails(480, 16, 90, 4))],
+])
+def test_an_output_is_off_by_its_own_rounding(dtype, groups):
+    # A weight is held to 2^-16 of itself in bf16 and 2^-22 in fp16 (two
+    # roundings of half a step each), scores and exponentials to less than 2^-16
+    # of a weight (float32 sums of values up to some tens): beyond the output's
+    # rounding nothing but that remains.
+    batch = Batch(groups, hq=32, dtype=dtype, seed=5)
+    out = batch.run().double()
+    half = torch.finfo(dtype).eps / 2
+    rest = 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -16 + 2.0 ** -22
+    for s in range(len(batch.contexts)):
+        want, size = _exact(batch, s, 128 ** -0.5)
+        over = (out[s] - want).abs() - (half * want.abs() + rest * (1 + half) * size)
+        assert (over <= 0).all(), f"sequence {s}: {over.max()} over"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_small_weights_add_up(dtype):
+    # One position of value 0 outweighs each of the others 2^26 times: what they
+    # leave is the output, within the bounds above.
+    batch = Batch([(3, [64, 49, 50])], hq=32, dtype=dtype, seed=6)
+    for pool, fill in ((batch.keys, 0.0), (batch.values, 1024.0)):  # outputs stay normal numbers
+        pool.fill_(fill)
+    batch.q.fill_(1.0)
+    scale = 26 * math.log(2) / 128
+    at = batch.tables[:, 0].long()  # the first position, shared or not
+    batch.keys[at, 0] = 1.0
+    batch.values[at, 0] = 0.0
+    out = batch.run(scale=scale).double()
+    half = torch.finfo(dtype).eps / 2
+    for s, c in enumerate(batch.contexts):
+        want, size = _exact(batch, s, scale)
+        assert (want > 0).all()
+        assert ((out[s] - want).abs() <= half * want + 2.0 ** -15 * (1 + half) * size).all()

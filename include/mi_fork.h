@@ -61,7 +61,8 @@ int32_t mi_kv_copy_blocks(void* key_cache, void* value_cache, int64_t layer_stri
  * arrays (context_lens [num_seqs], group_starts [num_groups + 1],
  * shared_blocks [num_groups]); mi_shared_decode runs a layer with it, so one
  * plan serves all layers of a step. A negative or too large block id is
- * masked; sequences of context 0 give zeros. Both are capture-safe.
+ * masked; sequences of context 0 give zeros; a NaN score makes its row NaN
+ * wherever the context is split. Both are capture-safe.
  *
  * plan: mi_shared_decode_plan_bytes() bytes, 32-byte aligned; workspace:
  * mi_shared_decode_workspace_bytes() bytes, 16-byte aligned, no

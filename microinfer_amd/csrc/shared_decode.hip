@@ -855,10 +855,12 @@ constexpr int kJoinLanes = kD / 4;  // a float4 each
 constexpr int kJoinWays = kJoinThreads / kJoinLanes;
 constexpr int kJoinBatch = 4;
 
-// (m, l, o) += 2^(..) of another piece; pieces of no position weigh nothing.
+// (m, l, o) += 2^(..) of another piece; pieces of no weight add nothing. The
+// maximum passes over NaN scores, so a piece of them alone has none, and NaN for
+// its sums, which have to reach the output.
 __device__ __forceinline__ void join_piece(float& m, float& l, f32x4_t& o, float mb, float lb,
                                            f32x4_t ob) {
-  if (mb == -INFINITY) return;
+  if (mb == -INFINITY && lb == 0.f) return;
   const float mnew = fmaxf(m, mb);
   const float fo = m == -INFINITY ? 0.f : fast_exp2(m - mnew);
   const float fb = fast_exp2(mb - mnew);
@@ -916,7 +918,7 @@ __global__ __launch_bounds__(kJoinThreads) void shared_join_kernel(const SharedA
   if (way != 0) return;
 #pragma unroll
   for (int w = 1; w < kJoinWays; ++w) join_piece(m, l, o, s_m[w], s_l[w], s_o[w][lane]);
-  const float inv = l > 0.f ? 1.f / l : 0.f;  // no position: zeros
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no position: zeros
   Pack<uint16_t, 4> out;
 #pragma unroll
   for (int i = 0; i < 4; ++i) out.v[i] = E::store(o[i] * inv);

@@ -418,3 +418,51 @@ def test_many_small_weights_add_up(dtype):
         want, size = _exact(batch, s, scale)
         assert (want > 0).all()
         assert ((out[s] - want).abs() <= half * want + 2.0 ** -15 * (1 + half) * size).all()
+
+
+def _nan_rows(batch, plan=None):
+    """Which outputs are NaN, by the kernel and by float64 attention."""
+    out = batch.run(plan)
+    want = torch.stack([_exact(batch, s, 128 ** -0.5)[0] for s in range(len(batch.contexts))])
+    assert bool((out.isnan() == want.isnan()).all())
+    fine = want.isfinite()
+    half = torch.finfo(out.dtype).eps / 2
+    size = want[fine].abs().max()
+    assert ((out.double() - want)[fine].abs() <= half * want[fine].abs() + 2 ** -13 * size).all()
+    return out.isnan()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("members,hq", [(3, 8), (3, 32), (20, 16), (20, 32)])
+def test_nan_reaches_the_output(dtype, members, hq):
+    # Groups of few and of many query rows; one sequence has a single position
+    # behind the shared pages, one none.
+    prefix = 20 * 16
+    ctx = [prefix + 1, prefix] + _tails(prefix, members - 2, 40, 3)
+
+    def batch(seed):
+        return Batch([(20, ctx), (0, [1, 40])], hq=hq, dtype=dtype, seed=seed)
+
+    one = batch(1)
+    one.q[2, 3, 7] = math.nan                        # one head of one sequence
+    one.q[members, 1, 0] = math.nan                  # and of one that has a single position
+    nan = _nan_rows(one)
+    assert nan[2, 3].all() and nan[members, 1].all() and nan.sum() == 2 * 128
+
+    one = batch(2)
+    own = int(one.tables[0, 20])                     # a page whose only position is NaN
+    one.keys[own, 0] = math.nan
+    nan = _nan_rows(one)
+    assert nan[0].all() and not nan[1:].any()
+
+    one = batch(3)
+    one.keys[int(one.tables[0, 9]), 5, 1] = math.nan  # one KV head of a shared position
+    share = hq // 8
+    nan = _nan_rows(one)
+    assert nan[:members, share:2 * share].all() and nan.sum() == members * share * 128
+
+    one = batch(4)
+    one.keys[one.tables[0, :20].long()] = math.nan   # every shared position
+    one.values[int(one.tables[members + 1, 1]), 3, 2, 9] = math.nan  # one value elsewhere
+    nan = _nan_rows(one)
+    assert nan[:members].all() and nan[members:].sum() == share

@@ -259,14 +259,19 @@ class AsyncEngine:
         """A fork's requests, from the engine thread: their channels, to its
         caller, for whom the room of ``n`` was reserved."""
         self._reserved -= n
-        if future.cancelled():  # nobody will read them
-            loop = asyncio.get_running_loop()
-            for seq_id, *_ in children:
-                self._thread.post("abort", seq_id, loop.create_future())
+        if future.cancelled():
+            self._drop([seq_id for seq_id, *_ in children])
             children = []
         channels = [RequestChannel(*child) for child in children]
         self._channels.update((channel.seq_id, channel) for channel in channels)
         self._settle(future, channels, exc, stats)
+
+    def _drop(self, seq_ids) -> None:
+        """Abort and forget requests that nobody will read."""
+        loop = asyncio.get_running_loop()
+        for seq_id in seq_ids:
+            self._channels.pop(seq_id, None)
+            self._thread.post("abort", seq_id, loop.create_future())
 
     def _deliver(self, updates, stats) -> None:
         """A step's updates: publish them, then grant the next step."""
@@ -326,7 +331,13 @@ class AsyncEngine:
         future = loop.create_future()
         self._thread_for(loop).post("fork", (request.seq_id, n, sampling_params), future)
         self._reserved += n
-        return await future
+        try:
+            return await future
+        except asyncio.CancelledError:
+            # Cancelled once the answer was there: its requests are this call's alone.
+            if future.done() and not future.cancelled() and future.exception() is None:
+                self._drop([channel.seq_id for channel in future.result()])
+            raise
 
     async def abort(self, seq_id: int) -> bool:
         removed = await self._command("abort", seq_id)

@@ -398,3 +398,60 @@ def test_groups_are_used_where_they_pay():
     least = -(-((1 << 17) + 8192 * 6) // (8 * 16 * 2))  # blocks, two sequences counted
     assert prefer_shared_decode([0, 4, 6], [least, 0], 16, 8)
     assert not prefer_shared_decode([0, 4, 6], [least - 1, 9999], 16, 8)
+
+
+def test_a_fork_cancelled_when_its_requests_exist_drops_them(scheduler_factory):
+    engine, runner, manager = make(scheduler_factory, num_blocks=24)
+
+    async def scenario():
+        frontend = AsyncEngine(engine, max_waiting=3)
+        request = await frontend.add_request([1, 2, 3], params(40))
+        stream = frontend.stream(request)
+        await anext(stream)
+        settle, tasks = frontend._settle_fork, []
+
+        def settle_and_cancel(*args):
+            settle(*args)
+            tasks[0].cancel()  # the answer is there, its caller has not run yet
+
+        frontend._settle_fork = settle_and_cancel
+        tasks.append(asyncio.ensure_future(frontend.fork(request, 2)))
+        with pytest.raises(asyncio.CancelledError):
+            await tasks[0]
+        frontend._settle_fork = settle
+        assert list(frontend._channels) == [request.seq_id] and frontend._reserved == 0
+        forks = await frontend.fork(request, 2)  # the room is there at once
+        assert len(engine.scheduler.running) == 3  # the dropped ones run no more
+        tokens = [len((await frontend.collect(f)).token_ids) for f in forks]
+        async for event in stream:
+            pass
+        assert tokens == [40, 40] and len(event.token_ids) == 40
+        assert not frontend._channels
+        await frontend.stop()
+        assert not manager.used_block_ids
+
+    asyncio.run(scenario())
+
+
+def test_a_failed_fork_cancelled_by_then_leaves_nothing(scheduler_factory):
+    engine, runner, manager = make(scheduler_factory)
+
+    async def scenario():
+        frontend = AsyncEngine(engine, max_waiting=3)
+        request = await frontend.add_request([1, 2, 3], params(20))
+        stream = frontend.stream(request)
+        await anext(stream)
+        settle, tasks = frontend._settle_fork, []
+
+        def settle_and_cancel(*args):
+            settle(*args)
+            tasks[0].cancel()
+
+        frontend._settle_fork = settle_and_cancel
+        tasks.append(asyncio.ensure_future(frontend.fork(request, 1, params(1))))  # refused
+        with pytest.raises(asyncio.CancelledError):
+            await tasks[0]
+        assert list(frontend._channels) == [request.seq_id] and frontend._reserved == 0
+        await frontend.stop()
+
+    asyncio.run(scenario())

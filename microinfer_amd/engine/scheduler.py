@@ -20,7 +20,9 @@ tests pin (tests/components/test_scheduler.py), restated as rules:
 4. A running request that needs a fresh block when none is free evicts the
    newest running request (which goes back to the front of the waiting queue
    with all its tokens, to be prefilled again); with nobody else left it
-   evicts itself.
+   evicts itself. Where nothing can run because prompts taken in part hold the
+   blocks that the head of the waiting queue needs, the last of them gives
+   its blocks back and waits to be prefilled again.
 5. After the step, ``postprocess`` publishes the hashes of completed blocks,
    advances each request's cached count, drops the sample of a prompt chunk
    that did not reach the end of its prompt, and finishes requests on EOS or
@@ -166,8 +168,10 @@ class Scheduler:
             if step.entries:
                 break
             # Decode pressure can have evicted requests into the waiting
-            # queue; if its head fits now, build the step again.
-            if not self.waiting or self.block_manager.can_allocate(self.waiting[0]) < 0:
+            # queue; if its head fits now, or blocks behind it can be had,
+            # build the step again.
+            if not self.waiting or (self.block_manager.can_allocate(self.waiting[0]) < 0
+                                    and not self._reclaim()):
                 raise RuntimeError("KV cache cannot make progress")
         seqs = step.entries
         n_prefill = sum(1 for s in seqs if s.is_prefill)
@@ -246,6 +250,16 @@ class Scheduler:
         seq.requeue()
         self.block_manager.deallocate(seq)
         self.waiting.appendleft(seq)
+
+    def _reclaim(self) -> bool:
+        """Free the blocks of the last waiting request that holds any behind
+        the queue's head; False if there is none."""
+        for seq in reversed(self.waiting):
+            if seq.block_table and seq is not self.waiting[0]:
+                self._counts["num_preemptions"] += 1
+                self.block_manager.deallocate(seq)
+                return True
+        return False
 
     def postprocess(self, seqs: list[Sequence], token_ids: list[int], is_prefill: bool) -> None:
         if self.config.debug_mode:

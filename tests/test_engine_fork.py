@@ -455,3 +455,46 @@ def test_a_failed_fork_cancelled_by_then_leaves_nothing(scheduler_factory):
         await frontend.stop()
 
     asyncio.run(scenario())
+
+
+def test_preempted_forks_pass_a_chunked_prompt_that_holds_blocks(scheduler_factory, sequence_cls):
+    engine, runner, manager = make(scheduler_factory, num_blocks=9, max_num_prefill_tokens=4)
+    seq = sequence_cls(list(range(1, 11)), params(24))
+    engine.add_request(seq)
+    while not seq.num_completion_tokens:
+        engine.step()
+    forks = engine.fork(seq.seq_id, 4)
+    run_out(engine)  # the runner checks every cached row of every step
+    assert [len(s.completion_token_ids) for s in [seq, *forks]] == [24] * 5
+    assert engine.stats()["num_preemptions"] > 0
+    assert not manager.used_block_ids and refs(manager) == {}
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_preemptions_and_chunked_prompts_together(scheduler_factory, sequence_cls, seed):
+    rng = random.Random(seed)
+    engine, runner, manager = make(scheduler_factory, num_blocks=rng.choice([9, 12]),
+                                   max_num_batched_tokens=rng.choice([5, 16]), max_model_len=36,
+                                   max_num_prefill_tokens=rng.choice([3, 400]),
+                                   mixed_batch=rng.random() < 0.7)
+    made = []
+    for _ in range(14):
+        prompt = [rng.randrange(1, 9) for _ in range(rng.randrange(1, 15))]
+        made.append(sequence_cls(prompt, params(rng.randrange(1, 20))))
+        engine.add_request(made[-1])
+    for step in range(4000):
+        if engine.is_finished():
+            break
+        engine.step()
+        running = [s.seq_id for s in engine.scheduler.running]
+        if running and len(made) < 20 and rng.random() < 0.2:
+            try:
+                made += engine.fork(rng.choice(running), rng.randrange(1, 3), params(20))
+            except RuntimeError:
+                pass
+        held = {b for s in [*engine.scheduler.waiting, *engine.scheduler.running]
+                for b in s.block_table}
+        assert held == manager.used_block_ids
+    assert engine.is_finished()
+    assert all(len(s.completion_token_ids) == s.max_tokens or len(s) >= 36 for s in made)
+    assert not manager.used_block_ids and refs(manager) == {}

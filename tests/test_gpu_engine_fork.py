@@ -243,3 +243,17 @@ def test_scores_of_requests_that_do_not_ask_cost_nothing(tiny_model, monkeypatch
     engine = make_engine(tiny_model)
     out = engine.generate([prompt(11, 20, TINY)], params(4))
     assert len(out[0]) == 4
+
+
+def test_preempted_forks_with_prompts_in_chunks(tiny_model):
+    # A preempted fork waits in front of another's prompt, of which a chunk is done.
+    engine = make_engine(tiny_model, num_blocks=9, max_num_prefill_tokens=16)
+    seq = Sequence(prompt(10, 60, TINY), params(40, logprobs=2))
+    engine.add_request(seq)
+    while not seq.num_completion_tokens:
+        engine.step()
+    forks = engine.fork(seq.seq_id, 4)
+    while not engine.is_finished():
+        engine.step()
+    assert engine.stats()["num_preemptions"] > 0
+    check(tiny_model, [seq, *forks], 1e-4)

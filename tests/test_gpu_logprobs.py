@@ -12,6 +12,7 @@ The order of the alternatives is exact.
 """
 
 import math
+import sys
 
 import pytest
 import torch
@@ -263,3 +264,59 @@ def test_two_graphs_and_eager_calls_share_nothing():
         torch.cuda.synchronize()
         for out, expect in zip(outs + [beside], want + want[:1]):
             assert all(torch.equal(a, b) for a, b in zip(out, expect)), f"replay {replay}"
+
+
+def _rows_that_turn_late(vocab, dtype):
+    """Rows whose later tiles overthrow what the first showed (a tile is 8192
+    values in 16 bits, 4096 in 32)."""
+    at = torch.arange(vocab, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    noise = 2.5 * torch.randn(vocab, generator=gen, device=DEV)
+    few = at % 64 < 8
+    rows = [
+        torch.where(at < 8192, -math.inf, noise),           # the first tile masked
+        torch.where(at < 8192, torch.finfo(dtype).min, noise),
+        torch.where(at < vocab - 20, -math.inf, noise),     # all but the last values masked
+        noise + at // 4096 * 14.0,                          # the reference moves every tile
+        noise + at // 2000 * 3.0,
+        at / vocab * 60 - 30,                               # rising, falling
+        30 - at / vocab * 60,
+        torch.where(at < 8192, noise - 20, 5.0),            # thousands of equal best ones, late
+        torch.where(at >= vocab // 2, 3.0, noise.clamp(max=3.0)),
+        torch.where(few & (at > 9000), 20.0 + at % 7, noise),   # many large ones in few lanes
+        torch.where(few & (at > 9000), 20.0 + at / vocab, noise),
+        torch.where(at % 4096 < 5, 10.0, -10.0),            # ties over all tiles
+        torch.where(at < 9000, -0.0, 0.0),
+        torch.where(at == 3, 60.0, noise - 40),             # everything vanishes behind it
+        torch.where(at == vocab - 2, 60.0, noise),
+        torch.where(at > vocab - 3000, math.nan, noise),    # more NaN than a list holds
+        torch.where(at == vocab - 9, math.nan, noise + at // 4096 * 14.0),
+        torch.where(at == vocab - 9, math.inf, noise),
+        torch.where(at % 3 == 0, -math.inf, noise),
+        noise,
+    ]
+    return torch.stack([r.float() for r in rows]).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(1040, 50021), (300, 151936), (1040, 151936)])
+def test_rows_that_turn_late(dtype, rows, vocab, monkeypatch):
+    # 1040 rows are one part each, of 7 to 38 tiles; 300 are a few parts of
+    # several tiles. The type's lowest value at a temperature of 0.3 has a log
+    # probability of -1.1e39, which is -inf in float32.
+    def expected(logits, temperatures, exact=_expected):
+        want = exact(logits, temperatures)
+        return want.masked_fill(want < torch.finfo(torch.float32).min, -math.inf)
+
+    monkeypatch.setattr(sys.modules[__name__], "_expected", expected)
+    kinds = _rows_that_turn_late(vocab, dtype)
+    n = len(kinds)
+    logits = kinds.repeat(rows // n, 1)
+    assert len(logits) == rows
+    tokens = torch.tensor([[0, 3, vocab - 1, vocab // 2]], device=DEV).expand(rows, 4)
+    hot = (torch.arange(rows, device=DEV) // n % 3 == 2).float() * 1.7 + 0.3
+    for top in (1, 5, 32):
+        got = check(logits, tokens, top=top, temperatures=hot if top == 5 else None)
+        again = got.top_tokens.view(rows // n, n, top)
+        assert bool((again == again[:1]).all())
+    check(logits, tokens)

@@ -104,8 +104,8 @@ int32_t mi_shared_decode(const void* query, int64_t q_token_stride, int64_t q_he
  * first among equals. A masked logit (-inf) has probability 0 and log
  * probability -inf. A token outside [0, vocab_size) gives NaN, and so do all
  * of a row's log probabilities and its entropy where the row has a NaN, +inf
- * or nothing above -inf, or a temperature that is not finite and positive;
- * its top_tokens are still in order.
+ * or nothing above -inf, or a temperature that is not finite or below the
+ * smallest normal float32 (2^-126); its top_tokens are still in order.
  *
  * tokens (int64, row stride token_stride) and logprobs ([num_rows, num_given],
  * contiguous) may be NULL with num_given 0, top_tokens (int64) and

@@ -51,6 +51,8 @@ constexpr int kMaxParts = kListCap / kMaxTop;
 // and (x - r) c of at most 10 rounds to 2^-21 when it is scaled.
 constexpr float kSlack = 10.f;
 constexpr float kLowest = -3.4028234663852886e38f;
+// log2(e) / temperature is finite from here on: the smallest normal number.
+constexpr float kLeastTemperature = 1.1754943508222875e-38f;
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
   const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const R* logits = static_cast<const R*>(a.logits) + row * a.row_stride;
   float temperature = a.temperatures == nullptr ? 1.f : a.temperatures[row];
-  if (!(temperature > 0.f && temperature < INFINITY)) temperature = NAN;
+  if (!(temperature >= kLeastTemperature && temperature < INFINITY)) temperature = NAN;
   const float c = kLog2E / temperature;
   // Packs lie on the 16-byte grid; the row's first and last may be partial.
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(R));
@@ -484,7 +486,9 @@ __global__ __launch_bounds__(kThreads, 4) void logprob_kernel(const LogprobArgs 
           share(s, wave, part_key);
           s.wave_first[wave] = all_key;
         }
-        __syncthreads();  // every part has a tile, so every wave is here
+        // Every wave of the workgroup is here, or none: an aligned row's last part
+        // can be empty.
+        __syncthreads();
         cand.floor = shared_floor(s);
         if (is_short) {
 #pragma unroll

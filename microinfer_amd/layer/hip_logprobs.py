@@ -61,8 +61,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     among equals. ``temperatures`` is float32 ``[rows]``. A masked logit
     (``-inf``) has probability 0 and log probability ``-inf``; a row that holds
     NaN, ``+inf`` or nothing above ``-inf``, or whose temperature is not finite
-    and positive, has NaN log probabilities and entropy, its ``top_tokens``
-    still in order. Results that were not asked for are ``None``.
+    or below the smallest normal float32 (2^-126), has NaN log probabilities and
+    entropy, its ``top_tokens`` still in order. Results that were not asked for are ``None``.
     """
     _lib.require_device(logits, tokens, temperatures, what="token log probabilities")
     code = _lib.DTYPE_CODES.get(logits.dtype)

@@ -320,3 +320,38 @@ def test_rows_that_turn_late(dtype, rows, vocab, monkeypatch):
         again = got.top_tokens.view(rows // n, n, top)
         assert bool((again == again[:1]).all())
     check(logits, tokens)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_least_temperature(dtype):
+    # The smallest normal float32 and from there on; below it, NaN.
+    least = torch.finfo(torch.float32).tiny
+    logits = _logits(7, 9001, dtype, 13)
+    logits[:, 77] = 31.0
+    logits[1:, 5000] = 31.0
+    values = [least, least, 2 * least, 1e-30, least / 2, 4.3e-39, 1e-45]
+    temperatures = torch.tensor(values, device=DEV)
+    got = token_logprobs(logits, torch.full((7,), 77, device=DEV), top=4, entropy=True,
+                         temperatures=temperatures)
+    fine = [0.0] + [-math.log(2)] * 3  # the best alone, or both of them
+    want = torch.tensor(fine + [math.nan] * 3, device=DEV, dtype=torch.float64)
+    assert torch.allclose(got.logprobs.double(), want, rtol=2 ** -22, atol=0, equal_nan=True)
+    assert torch.allclose(got.entropy.double(), -want, rtol=2 ** -22, atol=0, equal_nan=True)
+    # Differences of 10 and more: past float32's range below 1e-37, not at 1e-30.
+    assert bool((got.top_logprobs[:3, 2:] == -math.inf).all())
+    assert bool((got.top_logprobs[3, 2:] < -1e30).all())
+    assert bool(got.top_logprobs[4:].isnan().all())
+    order = torch.sort(logits.float(), dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(got.top_tokens, order)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_part_without_values(dtype):
+    # Parts leave room for rows that start off the 16-byte grid: aligned rows of
+    # whole tiles leave the last one empty.
+    for rows, vocab in ((4, 32768), (3, 8192), (1, 262144)):
+        logits = _logits(rows, vocab, dtype, vocab)
+        check(logits, _tokens(rows, vocab, 1, 2), top=32)
+        check(logits, top=0)
+        logits[0] = -math.inf
+        check(logits, _tokens(rows, vocab, 1, 2), top=3)

@@ -14,7 +14,7 @@ of at least 16 have a kernel of their own; every other shape that
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -26,23 +26,6 @@ from microinfer_amd.layer.hip_paged_attention import (_check_caches, _index32,
 MAX_SEQS = 4096
 
 
-# Workspaces by (device, stream): the calls on a stream run one after the other.
-# Captured calls get their own. One outgrown by a larger call goes back to
-# torch's allocator, which reuses it on that stream behind the calls before.
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
-
-
-def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream)
-    have = _workspaces.get(key)
-    if have is None or have.numel() < nbytes:
-        have = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _workspaces[key] = have
-    return have
-
-
 @dataclass(frozen=True)
 class SharedDecodePlan:
     """One step's work (``shared_decode_plan``), for calls of its sizes."""
@@ -51,6 +34,21 @@ class SharedDecodePlan:
     shared: bool  # False: a ``decode_plan`` for ``hip_paged_decode``
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
     workspace_bytes: int = 0  # of a call with it
+    # By stream: the calls on a stream run one after the other.
+    _workspaces: dict[int, torch.Tensor] = field(default_factory=dict, repr=False, compare=False)
+
+    def workspace(self, device: torch.device, stream: int) -> torch.Tensor:
+        """Memory of a call on ``stream``, the current one; a captured call's own,
+        as its graph keeps it."""
+        have = None
+        capturing = torch.cuda.is_current_stream_capturing()
+        if not capturing:
+            have = self._workspaces.get(stream)
+        if have is None:
+            have = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+            if not capturing:
+                self._workspaces[stream] = have
+        return have
 
 
 def shared_order(tables) -> list[int]:
@@ -255,7 +253,7 @@ def hip_shared_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache:
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
     with _lib.on_device(device):
         stream = _lib.stream_handle(device)
-        workspace = _workspace(device, stream, plan.workspace_bytes)
+        workspace = plan.workspace(device, stream)
         block_stride, token_stride, head_stride, _ = key_cache.stride()
         status = lib.mi_shared_decode(
             query.data_ptr(), q_token_stride, q_head_stride, key_cache.data_ptr(),

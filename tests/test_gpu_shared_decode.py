@@ -466,3 +466,23 @@ def test_nan_reaches_the_output(dtype, members, hq):
     one.values[int(one.tables[members + 1, 1]), 3, 2, 9] = math.nan  # one value elsewhere
     nan = _nan_rows(one)
     assert nan[:members].all() and nan[members:].sum() == share
+
+
+def test_workspaces_end_with_their_plan():
+    # One plan's calls on several streams; nothing stays allocated behind it.
+    batch = Batch([(60, _tails(960, 12, 200, 1))], hq=32)
+    want = batch.check()
+    plan = batch.plan()
+    contexts = _ints(batch.contexts)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    streams, outs = [torch.cuda.Stream() for _ in range(6)], []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            for _ in range(2):
+                outs.append(hip_shared_decode(batch.q, batch.keys, batch.values, batch.tables,
+                                              contexts, plan=plan))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+    del plan, outs
+    assert torch.cuda.memory_allocated() <= before

@@ -257,3 +257,57 @@ def test_preempted_forks_with_prompts_in_chunks(tiny_model):
         engine.step()
     assert engine.stats()["num_preemptions"] > 0
     check(tiny_model, [seq, *forks], 1e-4)
+
+
+@pytest.mark.parametrize("graph", [True, False])
+def test_shared_and_plain_steps_give_the_same_logits(wide_model, shared_calls, graph):
+    # The same tokens in both, those of the plain run. Each run's logits are within
+    # half the oracle's bound on deficits (0.1) of the oracle's, as `check` shows for
+    # the tokens it sees, so their difference is within that bound.
+    forced, logits = {}, []
+    for share in (False, True):
+        engine = make_engine(wide_model, shared_prefix_decode=share, use_cuda_graph=graph)
+        runner, seen, index = engine.model_runner, {}, {}
+        plain_run, record = runner.run, runner._record_logprobs
+
+        def run(seqs, is_prefill):
+            tokens = plain_run(seqs, is_prefill)
+            for i, seq in enumerate(seqs):
+                if seq.num_cached_tokens + seq.num_scheduled_tokens < len(seq):
+                    continue  # a prompt's chunk: its sample is dropped
+                key = index[seq.seq_id], len(seq)
+                tokens[i] = forced.setdefault(key, tokens[i])
+            return tokens
+
+        def recorded(seqs, rows, tokens):
+            for seq, row in zip(seqs, rows):
+                seen[index[seq.seq_id], len(seq)] = row.float().cpu()
+            record(seqs, rows, tokens)
+
+        runner.run, runner._record_logprobs = run, recorded
+        calls = len(shared_calls)
+        base = prompt(5, 100, WIDE)
+        seqs = [Sequence(base, params(14))]
+        seqs += [Sequence(base + prompt(6 + i, 3 + 5 * i, WIDE), params(14)) for i in range(5)]
+        for i, seq in enumerate(seqs):
+            index[seq.seq_id] = i
+            engine.add_request(seq)
+            while not seq.num_completion_tokens:
+                engine.step()
+        replays = count_replays(runner) if share and graph else None
+        while not engine.is_finished():
+            engine.step()
+        steps = len(replays) if replays is not None else \
+            (len(shared_calls) - calls) // WIDE.num_hidden_layer
+        assert steps >= 8 if share else steps == 0
+        logits.append(seen)
+        outs = [seq.completion_token_ids for seq in seqs]
+        if not share:
+            check(wide_model, seqs, 0.1)
+    plain, shared = logits
+    assert plain.keys() == shared.keys() and len(plain) >= 6 * 14
+    for key, row in plain.items():
+        off = (shared[key] - row).abs().max()
+        assert off <= 0.1, f"sequence {key[0]}, {key[1]} tokens: {off}"
+    assert outs == [[forced[i, len(s.token_ids) - 14 + k] for k in range(14)]
+                    for i, s in enumerate(seqs)]

@@ -79,14 +79,14 @@ class ModelRunner:
         """The decode batch ordered so that sequences with a common beginning
         are neighbours, and its groups; None where they are not worth it."""
         contexts = [len(s) for s in seqs]
-        heads = self.kv_cache.num_kv_heads
-        if sum(contexts) < least_shared_positions(len(seqs), heads):
+        heads = self.kv_cache.num_kv_heads, self.model.config.num_q_head
+        if sum(contexts) < least_shared_positions(len(seqs), *heads):
             return seqs, None
         tables = [s.block_table for s in seqs]
         order = shared_order(tables)
         starts, shared = shared_groups([tables[i] for i in order], [contexts[i] for i in order],
                                        self.block_size)
-        if not prefer_shared_decode(starts, shared, self.block_size, heads):
+        if not prefer_shared_decode(starts, shared, self.block_size, *heads):
             return seqs, None
         return [seqs[i] for i in order], (starts, shared)
 

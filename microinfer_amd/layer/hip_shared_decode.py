@@ -24,6 +24,7 @@ from microinfer_amd.layer.hip_paged_attention import (_check_caches, _index32,
                                                       hip_paged_decode)
 
 MAX_SEQS = 4096
+MAX_ROWS = 64  # query rows of a KV head that meet a shared page at once
 
 
 @dataclass(frozen=True)
@@ -110,36 +111,54 @@ def _common_blocks(a: list[int], b: list[int], most: int) -> int:
     return low
 
 
-def least_shared_positions(num_seqs: int, num_kv_heads: int) -> int:
-    """Positions that the groups of a decode step must share, counted once for
-    each of their sequences but two, to be better read once.
+def least_shared_positions(num_seqs: int, num_kv_heads: int,
+                           num_q_heads: int | None = None) -> int:
+    """Positions that the groups of a decode step must share, counted as often
+    as their reads become fewer (``prefer_shared_decode``), to be better read
+    together. ``num_q_heads``: by default two for each KV head.
 
-    Whole steps of a 28-layer model (16 query, 8 KV heads, head_dim 128, bf16,
-    block 16, 100 tokens of each sequence's own, from graphs), µs without and
-    with the groups, and what finding them takes the host. The second sequence
-    of a group finds its pages in the caches: 16 pairs with 8192 shared tokens
-    take 3606 and 3760, so pairs do not count. What has to be gained is the
-    launch that the fused QKV decode saves, the plan, each sequence's join
-    and the host's time:
+    What has to be gained is the launch that the fused QKV decode saves, the
+    plan, the host's time and, with each sequence and query head, the join. Whole
+    steps of a 28-layer model (head_dim 128, bf16, block 16, one group with 100
+    tokens of each sequence's own, from graphs), us without and with the groups,
+    and what finding them takes the host:
 
-        sequences  shared tokens on both sides of the rule
-        1 x 4      8192: 1260, 1251 + 22    32000: 2135, 1777 + 42
-        1 x 8      2048: 1137, 1187 + 23     4096: 1269, 1229 + 30
-        1 x 16     2048: 1265, 1247 + 42     4096: 1555, 1334 + 54
-        1 x 64     1024: 1539, 1471 + 125    2048: 1841, 1563 + 156
-        4 x 4      2048: 1301, 1327 + 40     4096: 1618, 1489 + 53
-        8 x 8      1024: 1618, 1636 + 124    2048: 1996, 1783 + 147
+        heads  sequences  shared tokens on both sides of the rule
+        16/8    4          5136: 1114, 1152 + 18    20496: 1679, 1537 + 31
+        16/8    8          2064: 1087, 1134 + 22     8208: 1499, 1291 + 37
+        16/8   16          1184: 1134, 1165 + 38     4688: 1579, 1302 + 57
+        16/8   64           672: 1350, 1384 + 113    2656: 1962, 1547 + 166
+        32/8   16          2352: 1337, 1315 + 45     4688: 1663, 1407 + 59
+        32/8   64          1328: 1663, 1635 + 138    2656: 2082, 1714 + 173
+        64/8   64          1328: 1909, 1944 + 136    5296: 3102, 2297 + 232
+        64/4    4                                   20496: 1785, 1614 + 32
+        64/4   64          5296: 2502, 2283 + 233   10576: 3523, 2781 + 327
+        32/2   64          5296: 1971, 1775 + 236   10576: 2687, 2103 + 327
+        16/16  16           592: 1102, 1206 + 32     2352: 1445, 1272 + 45
     """
-    return ((1 << 17) + 8192 * num_seqs) // num_kv_heads
+    if num_q_heads is None:
+        num_q_heads = 2 * num_kv_heads
+    base = min(1 << 14, (1 << 17) // num_kv_heads)  # few KV heads leave a plain step less parallel
+    return base + (5120 + 192 * num_q_heads) * num_seqs // num_kv_heads
 
 
-def prefer_shared_decode(starts, shared, block_size: int, num_kv_heads: int) -> bool:
+def prefer_shared_decode(starts, shared, block_size: int, num_kv_heads: int,
+                         num_q_heads: int | None = None) -> bool:
     """Whether a decode step with the groups of ``shared_groups`` is better
-    done with them."""
-    counted = sum((starts[g + 1] - starts[g] - 2) * blocks for g, blocks in enumerate(shared)
-                  if blocks)
+    done with them. ``num_q_heads``: as for ``least_shared_positions``.
+
+    A group's shared blocks are read once for every 64 query rows of a KV head,
+    instead of by every sequence, of which the second finds them in the caches
+    (16 pairs with 8192 shared tokens: 3606 us a step without and 3760 with)."""
+    if num_q_heads is None:
+        num_q_heads = 2 * num_kv_heads
+    per_tile = max(MAX_ROWS // (num_q_heads // num_kv_heads), 1)
+    counted = 0
+    for g, blocks in enumerate(shared):
+        members = starts[g + 1] - starts[g]
+        counted += max(members - 1 - -(-members // per_tile), 0) * blocks
     return counted > 0 and \
-        counted * block_size >= least_shared_positions(starts[-1], num_kv_heads)
+        counted * block_size >= least_shared_positions(starts[-1], num_kv_heads, num_q_heads)
 
 
 def supported_shared_decode(num_q_heads: int, num_kv_heads: int, head_dim: int,

@@ -13,7 +13,8 @@ from microinfer_amd.engine.async_engine import AsyncEngine, BackpressureError
 from microinfer_amd.engine.config import SampleParameter
 from microinfer_amd.engine.llm_engine import LLMEngine
 from microinfer_amd.engine.sequence import SequenceStatus, TokenLogprob
-from microinfer_amd.layer.hip_shared_decode import (prefer_shared_decode, shared_groups,
+from microinfer_amd.layer.hip_shared_decode import (least_shared_positions,
+                                                    prefer_shared_decode, shared_groups,
                                                     shared_order)
 
 
@@ -498,3 +499,36 @@ def test_preemptions_and_chunked_prompts_together(scheduler_factory, sequence_cl
     assert engine.is_finished()
     assert all(len(s.completion_token_ids) == s.max_tokens or len(s) >= 36 for s in made)
     assert not manager.used_block_ids and refs(manager) == {}
+
+
+@pytest.mark.parametrize("sequences,hq,hkv,prefix,worth", [
+    # Whole steps that were measured (28 layers, block 16): those that gain more
+    # than a twentieth, and those that lose.
+    (4, 16, 8, 20496, True), (8, 16, 8, 8208, True), (16, 16, 8, 4688, True),
+    (64, 16, 8, 2656, True), (8, 16, 8, 2064, False), (64, 16, 8, 672, False),
+    (64, 32, 8, 1328, False), (64, 32, 8, 2656, True), (16, 32, 8, 4688, True),
+    (64, 64, 8, 1328, False), (64, 64, 8, 5296, True), (16, 64, 8, 1184, False),
+    (64, 64, 4, 2656, False), (64, 64, 4, 5296, False), (64, 64, 4, 10576, True),
+    (64, 32, 2, 5296, False), (64, 32, 2, 10576, True), (4, 32, 2, 81936, True),
+    (4, 64, 4, 20496, True), (4, 32, 2, 40976, True), (64, 16, 16, 1328, True),
+    (16, 16, 16, 592, False), (8, 16, 16, 1040, False),
+])
+def test_the_rule_follows_the_measured_steps(sequences, hq, hkv, prefix, worth):
+    assert prefer_shared_decode([0, sequences], [prefix // 16], 16, hkv, hq) is worth
+    # Sequences that share nothing beside them only raise what has to be gained.
+    if not worth:
+        assert not prefer_shared_decode([0, sequences, sequences + 9], [prefix // 16, 0], 16,
+                                        hkv, hq)
+
+
+def test_the_rule_counts_reads_of_row_tiles():
+    # 64 rows meet a page at once: 16 sequences of four query heads a KV head.
+    def least(sequences, counted):
+        return -(-least_shared_positions(sequences, 8, 32) // (16 * counted))
+
+    for sequences, counted in ((3, 1), (16, 14), (17, 14), (32, 29), (33, 29)):
+        blocks = least(sequences, counted)
+        assert prefer_shared_decode([0, sequences], [blocks], 16, 8, 32)
+        assert not prefer_shared_decode([0, sequences], [blocks - 1], 16, 8, 32)
+    assert not prefer_shared_decode([0, 2], [1 << 20], 16, 8, 32)
+    assert not prefer_shared_decode([0, 1], [1 << 20], 16, 8, 32)

@@ -48,7 +48,8 @@ int32_t mi_kv_copy_blocks(void* key_cache, void* value_cache, int64_t layer_stri
 /*
  * Decode attention of sequences that share their first blocks: the result of
  * mi_paged_decode with the same tables and lengths (up to rounding), with the
- * blocks that a group of sequences shares read once for all of it.
+ * blocks that a group of sequences shares read once for every 64 query rows of
+ * a KV head (64 / G sequences of G query heads per KV head).
  *
  * Group g is the sequences [group_starts[g], group_starts[g + 1]) (rising;
  * sequences outside every group are on their own), whose tables hold the same
@@ -69,9 +70,10 @@ int32_t mi_kv_copy_blocks(void* key_cache, void* value_cache, int64_t layer_stri
  * initialisation, its own for calls that may run concurrently. Both sizes
  * depend on their arguments only. bf16/f16, head_dim 128, at most 16 query
  * heads per KV head, block_size >= 16 and a power of two, at most 4096
- * sequences and groups (MI_ERR_UNSUPPORTED otherwise: mi_paged_decode takes
- * those). query, the caches and out 16-byte aligned, with strides of whole
- * 16-byte vectors; block_tables may be NULL where it has no columns.
+ * sequences and groups, block tables of at most 2^30 positions
+ * (MI_ERR_UNSUPPORTED otherwise: mi_paged_decode takes the other types, heads
+ * and block sizes). query, the caches and out 16-byte aligned, with strides of
+ * whole 16-byte vectors; block_tables may be NULL where it has no columns.
  */
 int64_t mi_shared_decode_plan_bytes(int32_t num_seqs, int32_t num_q_heads, int32_t num_kv_heads);
 int64_t mi_shared_decode_workspace_bytes(int32_t num_seqs, int32_t num_q_heads,

@@ -1,9 +1,12 @@
 // Decode attention of sequences that share their first pages (forks of one
 // prompt, a common system prompt), gfx950.
 //
-// A group's shared pages are read once for all of its sequences: the query
-// rows of up to 64 / G sequences (G query heads each) meet a K/V row together,
-// as MFMA columns that the decode of single sequences would leave empty. With
+// A group's shared pages are read once for the query rows of up to 64 / G of its
+// sequences (G query heads each), which meet a K/V row together, as MFMA columns
+// that the decode of single sequences would leave empty; further 64 rows find the
+// pages in the L2, where a KV head's workgroups lie on one XCD (64 sequences
+// behind 3500 tokens issue loads of 156 MB a layer and read 117, of 114
+// distinct). With
 // the rest of each context as a work item of its own, an item is
 //   (query rows of one KV head, contiguous positions of one block table)
 // whether it is a piece of a shared prefix (up to 64 rows) or of one
@@ -20,11 +23,11 @@
 // Bound by latency below some 50 MB of K/V, by memory above. Measured per layer
 // (block 16, 8 KV heads, bf16, captured; the plan's eighth of 6-10 us and the
 // join's 2.5-4 us included), us here / each sequence reading its own context:
-//   4 sequences, 500 shared tokens, 16 query heads         9.3 /  8.8
+//   4 sequences, 500 shared tokens, 16 query heads         9.5 /  8.8
 //   16 with 12000 shared, up to 500 own, 32 query heads   26.5 / 66.8
-//   6 groups of 7, 300-3000 shared, 5-300 own             23.5 / 38.6
-//   64 with 3500 shared, 20-700 own, 32 query heads       33.8 / 62.5
-//   8 with 32000 shared, 10-100 own, 32 query heads       38.7 / 84.0
+//   6 groups of 7, 300-3000 shared, 5-300 own             23.3 / 38.6
+//   64 with 3500 shared, 20-700 own, 32 query heads       33.5 / 62.5
+//   8 with 32000 shared, 10-100 own, 32 query heads       39.2 / 84.0
 //   2 with 8000 shared                                    15.6 / 16.0
 // The long prefixes reach 3.4 TB/s of distinct rows: of the 16 sequences'
 // launch (20 us, 11.6 at the rate of a large read) 4 us pass before the first

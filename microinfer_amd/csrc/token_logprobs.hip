@@ -32,7 +32,11 @@
 // latency for few: 64 rows 11.6 us with entropy, 19.2 with 20 alternatives as
 // well (3.5 at the rate of a read); one row 5.3, and 9.3 with 5 alternatives.
 // 333 float32 rows of 32003 values in unaligned rows, 8 alternatives: 18.5-20.4
-// (7.6).
+// (7.6); 3000 of 151936 in float32 302, 332 with 20 alternatives (323). The
+// lists suit rows whose first tile tells what is large: with 20 alternatives and
+// entropy 64 rows take 20 us, also with nine values in ten masked, but 91 with the
+// first 8192 masked and 142 rising; 3000 rows 194, 498 and 5919 (each tile of a
+// rising row overflows the lists).
 #include <algorithm>
 
 #include "mi_common.h"

@@ -52,7 +52,7 @@ class EngineConfig:
     use_cuda_graph: bool = False  # decode buckets replayed from hipGraphs
     mixed_batch: bool = True  # fill the budget with prefill after running decode
     # Decode batches whose sequences share enough cache blocks (forks, common
-    # prompts) read them once; captures a second graph per bucket.
+    # prompts) read them together; captures a second graph per bucket.
     shared_prefix_decode: bool = False
 
     def __post_init__(self):

@@ -12,7 +12,7 @@ rows of graph buckets write their K/V there. With ``EngineConfig.debug_mode``
 each step's metadata is validated before launch (``runner.validate_step``).
 
 With ``EngineConfig.shared_prefix_decode`` a decode batch whose sequences
-share enough blocks (forks of a request, common prompts) reads them once
+share enough blocks (forks of a request, common prompts) reads them together
 (``hip_shared_decode``), from a second set of graphs; sequences that ask for
 ``logprobs`` get those of each token they keep (``token_logprobs`` of the
 step's logits).

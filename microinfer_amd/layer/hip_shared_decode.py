@@ -2,14 +2,16 @@
 
 ``hip_shared_decode`` is ``hip_paged_decode`` for continuations of common
 prompts (forks of a request, a system prompt): the pages that a group of
-sequences shares are read once for the whole group instead of once for each
-of its sequences. Groups are consecutive sequences of the batch;
+sequences shares are read once for every 64 query rows of a KV head (64 / G
+sequences of G query heads per KV head) instead of once for each sequence.
+Groups are consecutive sequences of the batch;
 ``shared_decode_plan`` lays out a step's work on the device from the lengths
 and groups, and every layer of the step uses that plan.
 
 16-bit caches with head_dim 128, up to 16 query heads per KV head and blocks
-of at least 16 have a kernel of their own; every other shape that
-``hip_paged_decode`` takes runs on it, with the same result.
+of at least 16 have a kernel of their own; the other types, heads and block
+sizes that ``hip_paged_decode`` takes run on it, with the same result. Block
+tables of more than 2^30 positions are refused.
 """
 
 from __future__ import annotations
@@ -163,7 +165,7 @@ def prefer_shared_decode(starts, shared, block_size: int, num_kv_heads: int,
 
 def supported_shared_decode(num_q_heads: int, num_kv_heads: int, head_dim: int,
                             dtype: torch.dtype, block_size: int, num_seqs: int) -> bool:
-    """Whether sequences of this shape read shared pages once."""
+    """Whether sequences of this shape read shared pages together."""
     return (dtype in (torch.float16, torch.bfloat16) and head_dim == 128
             and num_q_heads <= 16 * num_kv_heads and block_size >= 16
             and 0 < num_seqs <= MAX_SEQS)

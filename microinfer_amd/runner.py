@@ -478,7 +478,7 @@ class StepMetadataBuilder:
 
         The returned tensors are views of buffers reused by the next call,
         as in the reference. ``groups``: ``(starts, shared)`` of
-        ``shared_groups`` for sequences that read shared blocks once.
+        ``shared_groups`` for sequences that read shared blocks together.
         """
         n = len(seqs)
         width = max((len(s.block_table) for s in seqs), default=0)
@@ -532,7 +532,7 @@ class DecodeGraphRunner:
     the graph also selects each row's greedy token with the HIP argmax
     (runner.py:236-240); ``run`` then returns ``(logits, tokens)`` like
     ``_run_decode`` (runner.py:603). With ``shared`` the captured step reads
-    the blocks that groups of sequences share once; the groups are given
+    the blocks that groups of sequences share together; the groups are given
     to ``run`` and may change from step to step.
     """
 

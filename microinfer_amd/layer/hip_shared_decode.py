@@ -16,6 +16,7 @@ tables of more than 2^30 positions are refused.
 
 from __future__ import annotations
 
+import threading
 from dataclasses import dataclass, field
 
 import torch
@@ -37,20 +38,21 @@ class SharedDecodePlan:
     shared: bool  # False: a ``decode_plan`` for ``hip_paged_decode``
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
     workspace_bytes: int = 0  # of a call with it
-    # By stream: the calls on a stream run one after the other.
-    _workspaces: dict[int, torch.Tensor] = field(default_factory=dict, repr=False, compare=False)
+    # By thread and stream: its calls run one after the other. A call is two
+    # launches, between which another thread's may come.
+    _workspaces: dict[tuple[int, int], torch.Tensor] = field(default_factory=dict, repr=False,
+                                                             compare=False)
 
     def workspace(self, device: torch.device, stream: int) -> torch.Tensor:
         """Memory of a call on ``stream``, the current one; a captured call's own,
         as its graph keeps it."""
-        have = None
-        capturing = torch.cuda.is_current_stream_capturing()
-        if not capturing:
-            have = self._workspaces.get(stream)
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+        key = threading.get_ident(), stream
+        have = self._workspaces.get(key)
         if have is None:
             have = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
-            if not capturing:
-                self._workspaces[stream] = have
+            self._workspaces[key] = have
         return have
 
 

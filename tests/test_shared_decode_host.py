@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from microinfer_amd import _lib
-from microinfer_amd.layer.hip_shared_decode import shared_decode_plan, supported_shared_decode
+from microinfer_amd.layer.hip_shared_decode import (SharedDecodePlan, shared_decode_plan,
+                                                    supported_shared_decode)
 
 
 def _plan(**over):
@@ -91,3 +92,27 @@ def test_call_pointers_are_checked():
     assert _call(lib, workspace=4104) == 3
     need = lib.mi_shared_decode_workspace_bytes(4, 16, 8)
     assert _call(lib, ws_bytes=need - 1) == 3
+
+
+def test_threads_have_workspaces_of_their_own(monkeypatch):
+    # A call is two launches: another thread's, on the same stream, may come between.
+    import threading
+
+    capturing = [False]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    plan = SharedDecodePlan(torch.empty(0), True, (), 64)
+
+    def take(stream):
+        return plan.workspace(torch.device("cpu"), stream)
+
+    mine, others = take(1), []
+    thread = threading.Thread(target=lambda: others.append((take(1), take(1))))
+    thread.start()
+    thread.join()
+    assert mine.numel() == 64 and take(1) is mine and take(2) is not mine
+    assert others[0][0] is others[0][1] is not mine
+    assert others[0][0].data_ptr() != mine.data_ptr()
+    capturing[0] = True  # a graph keeps its own
+    assert take(1) is not mine
+    capturing[0] = False
+    assert take(1) is mine

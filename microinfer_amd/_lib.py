@@ -27,8 +27,11 @@ _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
 
+# An 8-bit cache: K, V, their strides, the scales and theirs.
+_QUANT_CACHE = [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64]
+
 # (restype, argtypes) of every entry point declared in include/mi_attn.h,
-# include/mi_model.h and include/mi_fork.h.
+# include/mi_model.h, include/mi_fork.h and include/mi_quant.h.
 SIGNATURES = {
     "mi_last_error": (ctypes.c_char_p, []),
     "mi_abi_version": (_I32, []),
@@ -133,6 +136,31 @@ SIGNATURES = {
         _I32,
         [_P, _I64, _I32, _I32, _I32, _P, _P, _I64, _I32, _P, _P, _P, _P, _I32, _P, _I64, _P,
          _P],
+    ),
+    "mi_quant_append_plan": (_I32, [_P, _I32, _I32, _I32, _I32, _P, _P]),
+    "mi_quant_append": (
+        _I32,
+        [_P, _I64, _I64, _P, _I64, _I64, *_QUANT_CACHE, _P, _I32, _P, _I32, _I32, _I32, _I32,
+         _I32, _I32, _I32, _P],
+    ),
+    "mi_quant_gather": (
+        _I32,
+        [*_QUANT_CACHE, _P, _I64, _I32, _P, _I32, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32,
+         _I32, _P],
+    ),
+    "mi_quant_decode_plan_bytes": (_I64, [_I32, _I32]),
+    "mi_quant_decode_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
+    "mi_quant_decode_plan": (
+        _I32, [_P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P, _P]),
+    "mi_quant_decode": (
+        _I32,
+        [_P, _I64, _I64, *_QUANT_CACHE, _P, _I64, _I32, _P, _I64, _P, _I64, _I64, _P, _I64, _P,
+         _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+    ),
+    "mi_quant_prefill": (
+        _I32,
+        [_P, _I64, _I64, *_QUANT_CACHE, _P, _P, _P, _I64, _I32, _P, _I64, _I64, _I32, _I32, _I32,
+         _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
     ),
 }
 

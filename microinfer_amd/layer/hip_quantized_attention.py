@@ -1,0 +1,225 @@
+"""Paged attention over an 8-bit KV cache, on the HIP library.
+
+``hip_quantized_decode`` and ``hip_quantized_prefill`` are ``hip_paged_decode``
+and ``hip_paged_prefill`` for a cache that holds each value as ``code * scale``
+(``hip_quantized_kv``): the query keeps its own type, codes are widened as they
+are read, the scales of each block of tokens and KV head meet the scores (K)
+and the softmax weights (V) in float32.
+"""
+
+from __future__ import annotations
+
+import threading
+from dataclasses import dataclass, field
+
+import torch
+
+from microinfer_amd import _lib
+from microinfer_amd.layer.hip_paged_attention import _index32
+from microinfer_amd.worker.hip_quantized_kv import check_quantized_cache, whole_vectors
+
+MAX_SEQS = 4096
+_FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _call_place(device: torch.device) -> tuple:
+    """What calls that run one after the other have in common."""
+    return (threading.get_ident(), _lib.stream_handle(device),
+            torch.cuda.is_current_stream_capturing())
+
+
+@dataclass(frozen=True)
+class QuantizedDecodePlan:
+    """One step's work (``quantized_decode_plan``), for calls of its sizes."""
+
+    buffer: torch.Tensor
+    counters: torch.Tensor  # zero, for calls in the place that made the plan
+    sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
+    place: tuple
+    workspace_bytes: int
+    _workspaces: dict = field(default_factory=dict, repr=False, compare=False)
+
+    def workspace(self, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+        """Partials and counters of a call from here: its thread's and stream's
+        own, a call's own where a graph holds it but not the plan."""
+        place = _call_place(device)
+        have = self._workspaces.get(place)
+        if have is None:
+            partials = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+            if place == self.place:
+                have = partials, self.counters
+            else:
+                have = partials, torch.zeros_like(self.counters)
+                if place[2]:
+                    return have
+            self._workspaces[place] = have
+        return have
+
+
+def quantized_decode_plan(context_lens: torch.Tensor, *, num_q_heads: int, num_kv_heads: int,
+                          head_dim: int, dtype: torch.dtype, block_size: int,
+                          block_table_width: int) -> QuantizedDecodePlan:
+    """The plan of one decode step over an 8-bit cache (shared by its layers),
+    from the lengths on the device alone (capture-safe). ``dtype``: the
+    query's."""
+    _lib.require_device(context_lens, what="quantized_decode_plan")
+    if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
+        raise ValueError("Hq must be divisible by Hkv")
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError("unsupported query dtype")
+    if block_size <= 0 or block_size & (block_size - 1):
+        raise ValueError("paged kernels require a power-of-two block size")
+    if context_lens.ndim != 1:
+        raise ValueError("context_lens must be 1-D")
+    num_seqs, device = context_lens.numel(), context_lens.device
+    if num_seqs > MAX_SEQS:
+        raise ValueError(f"at most {MAX_SEQS} sequences")
+    context_lens = _index32(context_lens)
+    lib = _lib.load()
+    with _lib.on_device(device):
+        nbytes = lib.mi_quant_decode_plan_bytes(num_seqs, num_kv_heads)
+        buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        counters = torch.empty(num_seqs * num_kv_heads, dtype=torch.int32, device=device)
+        status = lib.mi_quant_decode_plan(
+            context_lens.data_ptr(), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+            block_table_width, _lib.DTYPE_CODES[dtype], buffer.data_ptr(), nbytes,
+            counters.data_ptr(), _lib.stream_handle(device))
+        _lib.check(status, "mi_quant_decode_plan")
+        place = _call_place(device)
+    return QuantizedDecodePlan(
+        buffer, counters, (num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size,
+                           block_table_width), place,
+        lib.mi_quant_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim))
+
+
+def _check_query(query: torch.Tensor, key_cache: torch.Tensor, what: str) -> None:
+    if query.ndim != 3:
+        raise ValueError(f"query must have shape [{what}, Hq, D]")
+    if query.dtype not in _FLOAT_DTYPES:
+        raise ValueError("unsupported query dtype")
+    _, num_q_heads, head_dim = query.shape
+    if query.device != key_cache.device:
+        raise ValueError("query and cache must share a device")
+    if key_cache.shape[3] != head_dim:
+        raise ValueError("query and cache head dimensions differ")
+    if num_q_heads == 0 or num_q_heads % key_cache.shape[2]:
+        raise ValueError("Hq must be divisible by Hkv")
+
+
+def hip_quantized_decode(query: torch.Tensor, key_cache: torch.Tensor,
+                         value_cache: torch.Tensor, key_scales: torch.Tensor,
+                         value_scales: torch.Tensor, block_tables: torch.Tensor,
+                         context_lens: torch.Tensor, *, scale: float | None = None,
+                         plan: QuantizedDecodePlan | None = None) -> torch.Tensor:
+    """Decode one query row per request over an 8-bit paged cache.
+
+    ``query [R, Hq, D]`` (float16, bfloat16 or float32), caches
+    ``[N, B, Hkv, D]``, scales ``[N, Hkv]``, ``block_tables [R, W]`` and
+    ``context_lens [R]`` on the device. Returns ``[R, Hq, D]`` in the query's
+    dtype. The caches hold the step's rows already. ``plan``: of
+    ``quantized_decode_plan`` for these lengths; without it the call makes its
+    own. Sequences of length 0 give zeros, block ids outside the pool are
+    masked.
+    """
+    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
+                                        "hip_quantized_decode")
+    _check_query(query, key_cache, "requests")
+    num_seqs, num_q_heads, head_dim = query.shape
+    num_blocks, block_size, num_kv_heads, _ = key_cache.shape
+    device = query.device
+    if block_tables.ndim != 2 or block_tables.shape[0] != num_seqs:
+        raise ValueError("block_tables must have one row per request")
+    if context_lens.numel() != num_seqs:
+        raise ValueError("context_lens must have one entry per request")
+    _lib.require_device(block_tables, context_lens, what="hip_quantized_decode")
+    if block_tables.device != device or context_lens.device != device:
+        raise ValueError("block_tables and context_lens must be on the query's device")
+    width = block_tables.shape[1]
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, query.dtype, block_size, width)
+    if plan is None:
+        plan = quantized_decode_plan(
+            context_lens.reshape(-1), num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
+            head_dim=head_dim, dtype=query.dtype, block_size=block_size,
+            block_table_width=width)
+    elif not isinstance(plan, QuantizedDecodePlan) or plan.sizes != sizes:
+        raise ValueError("plan must come from quantized_decode_plan() for this call's sizes")
+    elif plan.buffer.device != device:
+        raise ValueError("plan must be on the query's device")
+    query, tables = whole_vectors(query), _index32(block_tables)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    if num_seqs == 0:
+        return out
+    with _lib.on_device(device):
+        partials, counters = plan.workspace(device)
+        status = _lib.load().mi_quant_decode(
+            query.data_ptr(), *query.stride()[:2], *cache, tables.data_ptr(), tables.stride(0),
+            width, plan.buffer.data_ptr(), plan.buffer.numel(), out.data_ptr(),
+            num_q_heads * head_dim, head_dim, partials.data_ptr(), partials.numel(),
+            counters.data_ptr(), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
+            num_blocks, float(head_dim ** -0.5 if scale is None else scale),
+            _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(device))
+    _lib.check(status, "mi_quant_decode")
+    return out
+
+
+def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, *,
+                           num_tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                           dtype: torch.dtype, block_size: int, block_table_width: int):
+    """The plan of ``hip_quantized_prefill`` calls of these sizes (None: they
+    run without one)."""
+    _lib.require_device(cu_seqlens_q, cu_seqlens_k, what="quantized_prefill_plan")
+    if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
+        raise ValueError("Hq must be divisible by Hkv")
+    if cu_seqlens_q.numel() != cu_seqlens_k.numel() or cu_seqlens_q.numel() == 0:
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must have num_requests + 1 entries")
+    return None
+
+
+def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
+                          value_cache: torch.Tensor, key_scales: torch.Tensor,
+                          value_scales: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                          cu_seqlens_k: torch.Tensor, block_tables: torch.Tensor, *,
+                          max_seqlen_q: int, scale: float | None = None,
+                          plan=None) -> torch.Tensor:
+    """Causal varlen attention over an 8-bit paged cache (bottom-right mask).
+
+    ``query [T, Hq, D]``; request r owns query rows ``cu_seqlens_q[r]..`` and
+    context ``cu_seqlens_k[r+1] - cu_seqlens_k[r]`` (it includes the new rows,
+    which the caller appended first). ``plan``: of ``quantized_prefill_plan``
+    for these lengths and sizes. Rows that see nothing give zeros.
+    """
+    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
+                                        "hip_quantized_prefill")
+    _check_query(query, key_cache, "tokens")
+    num_tokens, num_q_heads, head_dim = query.shape
+    num_blocks, block_size, num_kv_heads, _ = key_cache.shape
+    device = query.device
+    if block_tables.ndim != 2:
+        raise ValueError("block_tables must have one row per request")
+    num_requests, width = block_tables.shape
+    for name, offsets in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k)):
+        if offsets.numel() != num_requests + 1:
+            raise ValueError(f"{name} must have num_requests + 1 entries")
+    if max_seqlen_q <= 0 and num_tokens:
+        raise ValueError("max_seqlen_q must be positive")
+    _lib.require_device(cu_seqlens_q, cu_seqlens_k, block_tables, what="hip_quantized_prefill")
+    if any(t.device != device for t in (cu_seqlens_q, cu_seqlens_k, block_tables)):
+        raise ValueError("cu_seqlens and block_tables must be on the query's device")
+    if plan is not None:
+        raise ValueError("plan must come from quantized_prefill_plan() for this call's sizes")
+    if num_tokens and not num_requests:
+        raise ValueError("tokens without requests")
+    query, tables = whole_vectors(query), _index32(block_tables)
+    cu_q, cu_k = _index32(cu_seqlens_q), _index32(cu_seqlens_k)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    if num_tokens == 0:
+        return out
+    with _lib.on_device(device):
+        status = _lib.load().mi_quant_prefill(
+            query.data_ptr(), *query.stride()[:2], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
+            tables.data_ptr(), tables.stride(0), width, out.data_ptr(), num_q_heads * head_dim,
+            head_dim, num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim, block_size,
+            num_blocks, float(head_dim ** -0.5 if scale is None else scale),
+            _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(device))
+    _lib.check(status, "mi_quant_prefill")
+    return out

@@ -1,0 +1,195 @@
+"""Writes into and reads out of an 8-bit KV cache through the HIP library.
+
+A pool of ``torch.float8_e4m3fn`` or ``torch.int8`` holds each value as
+``code * scale`` with one float32 scale for each block of tokens and KV head, K
+and V apart (``KVCache(dtype=...)`` makes one). ``quantized_append`` is
+``append_slots`` for such a pool, ``quantized_gather`` is ``hip_gather_kv``:
+rows go in and come out as float32, float16 or bfloat16.
+
+A block's scale is the least power of two that brings its rows into the type's
+range. A row at offset 0 begins its block anew; rows at later offsets leave the
+scale or raise it, and then the rows before them are rounded again (in e4m3
+without loss, until they leave its normal range). So the rows of a block are
+written in the order of their offsets, as an engine does. What is not finite is
+held as NaN; int8 has none, there the block's scale becomes NaN.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from microinfer_amd import _lib
+
+QUANTIZED_DTYPES = (torch.float8_e4m3fn, torch.int8)
+MAX_SCANNED_TOKENS = 1024  # a larger call needs a plan, and makes one itself
+
+_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+_FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_INDEX_DTYPES = (torch.int32, torch.int64)
+
+
+def check_quantized_cache(key_cache, value_cache, key_scales, value_scales, what: str):
+    """ValueError / RuntimeError unless the four are an 8-bit cache on the GPU;
+    the arguments that describe it to the library, and its code."""
+    _lib.require_device(key_cache, value_cache, key_scales, value_scales, what=what)
+    if key_cache.ndim != 4 or value_cache.shape != key_cache.shape:
+        raise ValueError("key/value caches must have matching [blocks, B, Hkv, D] shapes")
+    if key_cache.dtype not in _CODES or value_cache.dtype != key_cache.dtype:
+        raise ValueError("8-bit caches are float8_e4m3fn or int8, K and V alike")
+    num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
+    for scales in (key_scales, value_scales):
+        if scales.shape != (num_blocks, num_kv_heads) or scales.dtype != torch.float32:
+            raise ValueError("scales must be float32 [blocks, Hkv]")
+    if key_cache.stride() != value_cache.stride() or key_scales.stride() != value_scales.stride():
+        raise ValueError("K/V caches must share one layout")
+    if key_cache.stride(-1) != 1:
+        raise ValueError("cache head_dim must be contiguous")
+    device = key_cache.device
+    if any(t.device != device for t in (value_cache, key_scales, value_scales)):
+        raise ValueError("caches and scales must share a device")
+    if block_size <= 0 or block_size & (block_size - 1):
+        raise ValueError("paged kernels require a power-of-two block size")
+    if head_dim & (head_dim - 1) or not 16 <= head_dim <= 256:
+        raise ValueError("8-bit caches need a power-of-two head_dim from 16 to 256")
+    block_stride, token_stride, head_stride, _ = key_cache.stride()
+    pointers = key_cache.data_ptr(), value_cache.data_ptr()
+    if (pointers[0] | pointers[1] | block_stride | token_stride | head_stride) & 7:
+        raise ValueError("8-bit cache rows must be 8-byte aligned")
+    return (*pointers, block_stride, token_stride, head_stride, key_scales.data_ptr(),
+            value_scales.data_ptr(), *key_scales.stride()), _CODES[key_cache.dtype]
+
+
+def whole_vectors(rows: torch.Tensor) -> torch.Tensor:
+    """``rows [T, H, D]``, or a copy, with 16-byte aligned head rows."""
+    size = rows.element_size()
+    token_stride, head_stride, inner = rows.stride()
+    if inner != 1 or (rows.data_ptr() | size * token_stride | size * head_stride) & 15:
+        return rows.clone(memory_format=torch.contiguous_format)
+    return rows
+
+
+def _slots(slot_mapping: torch.Tensor) -> torch.Tensor:
+    if slot_mapping.ndim != 1 or slot_mapping.dtype not in _INDEX_DTYPES:
+        raise ValueError("slots must be a 1-D integer tensor")
+    return slot_mapping.contiguous()
+
+
+@dataclass(frozen=True)
+class QuantizedAppendPlan:
+    """Where a step's rows go (``quantized_append_plan``), for every layer."""
+
+    rows: torch.Tensor
+    sizes: tuple  # tokens, block size, blocks
+
+
+def quantized_append_plan(slot_mapping: torch.Tensor, *, block_size: int,
+                          num_blocks: int) -> QuantizedAppendPlan:
+    """The plan of ``quantized_append`` calls with these slots, made on the
+    device (capture-safe)."""
+    _lib.require_device(slot_mapping, what="quantized_append_plan")
+    slots = _slots(slot_mapping)
+    if block_size <= 0 or block_size & (block_size - 1):
+        raise ValueError("paged kernels require a power-of-two block size")
+    if num_blocks <= 0:
+        raise ValueError("num_blocks must be positive")
+    rows = torch.empty(num_blocks * block_size, dtype=torch.int32, device=slots.device)
+    with _lib.on_device(slots.device):
+        status = _lib.load().mi_quant_append_plan(
+            slots.data_ptr(), int(slots.dtype == torch.int64), slots.numel(), block_size,
+            num_blocks, rows.data_ptr(), _lib.stream_handle(slots.device))
+    _lib.check(status, "mi_quant_append_plan")
+    return QuantizedAppendPlan(rows, (slots.numel(), block_size, num_blocks))
+
+
+def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     key_scales: torch.Tensor, value_scales: torch.Tensor,
+                     slot_mapping: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, *,
+                     plan: QuantizedAppendPlan | None = None) -> None:
+    """Quantise ``keys``/``values [T, Hkv, D]`` into the cache at
+    ``slot_mapping [T]`` (int32/int64; negative or too large ones are skipped).
+
+    Caches ``[N, B, Hkv, D]``, scales ``[N, Hkv]``, all written in place. In a
+    block, rows below the lowest offset written stay (rounded again where the
+    scale rises); the others stand for something only once they are written.
+    Of rows with equal slots one is written, whichever. ``plan``: of
+    ``quantized_append_plan`` for these slots; without it a call of more than
+    1024 rows makes its own.
+    """
+    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
+                                        "quantized_append")
+    _lib.require_device(slot_mapping, keys, values, what="quantized_append")
+    num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
+    if keys.ndim != 3 or values.shape != keys.shape:
+        raise ValueError("K/V must have matching [tokens, Hkv, D] shapes")
+    if keys.shape[1:] != key_cache.shape[2:]:
+        raise ValueError("K/V heads must match the cache")
+    if keys.dtype not in _FLOAT_DTYPES or values.dtype != keys.dtype:
+        raise ValueError("K/V must be float16, bfloat16 or float32, both alike")
+    tokens, device = keys.shape[0], key_cache.device
+    slots = _slots(slot_mapping)
+    if slots.numel() != tokens:
+        raise ValueError("one slot per token is required")
+    if any(t.device != device for t in (slots, keys, values)):
+        raise ValueError("slots and K/V must be on the cache device")
+    if block_size > 1024:
+        raise ValueError("8-bit caches are written in blocks of at most 1024 tokens")
+    if tokens == 0:
+        return
+    if plan is None:
+        if tokens > MAX_SCANNED_TOKENS:
+            plan = quantized_append_plan(slots, block_size=block_size, num_blocks=num_blocks)
+    elif not isinstance(plan, QuantizedAppendPlan) or plan.sizes != (tokens, block_size,
+                                                                     num_blocks):
+        raise ValueError("plan must come from quantized_append_plan() for this call's sizes")
+    elif plan.rows.device != device:
+        raise ValueError("plan must be on the cache device")
+    keys, values = whole_vectors(keys), whole_vectors(values)
+    with _lib.on_device(device):
+        status = _lib.load().mi_quant_append(
+            keys.data_ptr(), *keys.stride()[:2], values.data_ptr(), *values.stride()[:2], *cache,
+            slots.data_ptr(), int(slots.dtype == torch.int64),
+            None if plan is None else plan.rows.data_ptr(), tokens, num_kv_heads, head_dim,
+            block_size, num_blocks, _lib.DTYPE_CODES[keys.dtype], code,
+            _lib.stream_handle(device))
+    _lib.check(status, "mi_quant_append")
+
+
+def quantized_gather(key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     key_scales: torch.Tensor, value_scales: torch.Tensor,
+                     block_tables: torch.Tensor, cu_seqlens_k: torch.Tensor, total_rows: int, *,
+                     dtype: torch.dtype = torch.bfloat16):
+    """Each request's first rows as contiguous K/V ``[total_rows, Hkv, D]`` of
+    ``dtype``: request r's are rows ``cu_seqlens_k[r] : cu_seqlens_k[r + 1]``.
+    Rows of blocks outside the pool or the table are zeros."""
+    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
+                                        "quantized_gather")
+    _lib.require_device(block_tables, cu_seqlens_k, what="quantized_gather")
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError("rows are read as float16, bfloat16 or float32")
+    if block_tables.ndim != 2 or cu_seqlens_k.numel() != block_tables.shape[0] + 1:
+        raise ValueError("cu_seqlens_k must have one entry more than block_tables has rows")
+    device = key_cache.device
+    if block_tables.device != device or cu_seqlens_k.device != device:
+        raise ValueError("block_tables and cu_seqlens_k must be on the cache device")
+    if type(total_rows) is not int or total_rows < 0:
+        raise ValueError("total_rows must be a nonnegative integer")
+    num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
+    shape = (total_rows, num_kv_heads, head_dim)
+    keys = torch.empty(shape, dtype=dtype, device=device)
+    values = torch.empty_like(keys)
+    if total_rows == 0:
+        return keys, values
+    if block_tables.shape[0] == 0:
+        raise ValueError("rows without requests")
+    tables = block_tables.to(torch.int32).contiguous()
+    offsets = cu_seqlens_k.to(torch.int32).contiguous()
+    with _lib.on_device(device):
+        status = _lib.load().mi_quant_gather(
+            *cache, tables.data_ptr(), tables.stride(0), tables.shape[1], offsets.data_ptr(),
+            tables.shape[0], total_rows, keys.data_ptr(), values.data_ptr(), num_kv_heads,
+            head_dim, block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
+            _lib.stream_handle(device))
+    _lib.check(status, "mi_quant_gather")
+    return keys, values

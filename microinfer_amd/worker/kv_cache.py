@@ -15,6 +15,10 @@ same constructor, ``layer(i)``, ``num_bytes``, ``keys``/``values`` and
   ``[L, N, B, Hkv, D]`` and equal strides, so indexing
   (``cache.keys[l, blk, off]``) reads exactly what the reference would; the
   kernels take the view's strides.
+* 8-bit pools. ``dtype=torch.float8_e4m3fn`` or ``torch.int8`` makes a pool of
+  codes with a float32 scale for each block and KV head (``key_scales`` /
+  ``value_scales``, logical shape ``[L, N, Hkv]``, K's beside V's); writes
+  quantise (``hip_quantized_kv``).
 * Writes run on the GPU only (no advanced-indexing CPU fallback,
   kv_cache.py:78-79); a CPU cache can be built and validated but not written.
 """
@@ -25,28 +29,57 @@ from dataclasses import dataclass
 
 import torch
 
+from microinfer_amd.worker.hip_kv_blocks import _host_ints as host_ints
 from microinfer_amd.worker.hip_kv_blocks import copy_blocks
 from microinfer_amd.worker.hip_kv_store import launch_append
+from microinfer_amd.worker.hip_quantized_kv import (QUANTIZED_DTYPES, QuantizedAppendPlan,
+                                                    quantized_append)
 
 LAYOUTS = ("paired", "head_major", "token_major")
 
 
 @dataclass(frozen=True)
 class LayerKVCache:
-    """One layer's logical ``[blocks, B, Hkv, D]`` K/V views; no pool or layer id."""
+    """One layer's logical ``[blocks, B, Hkv, D]`` K/V views; no pool or layer id.
+    8-bit ones have their scales ``[blocks, Hkv]`` beside them."""
 
     keys: torch.Tensor
     values: torch.Tensor
+    key_scales: torch.Tensor | None = None
+    value_scales: torch.Tensor | None = None
 
     def __post_init__(self):
         if self.keys.ndim != 4 or self.keys.shape != self.values.shape:
             raise ValueError("K/V must have matching [blocks, B, Hkv, D] shapes")
         if self.keys.dtype != self.values.dtype or self.keys.device != self.values.device:
             raise ValueError("K/V must have matching dtype and device")
+        if self.quantized:
+            for scales in (self.key_scales, self.value_scales):
+                if scales is None or scales.shape != (self.keys.shape[0], self.keys.shape[2]):
+                    raise ValueError("8-bit K/V need scales of shape [blocks, Hkv]")
+        elif self.key_scales is not None or self.value_scales is not None:
+            raise ValueError("only 8-bit K/V have scales")
 
     @property
     def block_size(self):
         return self.keys.shape[1]
+
+    @property
+    def quantized(self) -> bool:
+        return self.keys.dtype in QUANTIZED_DTYPES
+
+    def _write(self, index0, index1, keys, values, plan=None):
+        if not self.quantized:
+            launch_append(self.keys, self.values, index0, index1, keys, values)
+            return
+        slots = index0
+        if index1 is not None:
+            if index0.shape != index1.shape:
+                raise ValueError("one offset per block is required")
+            inside = (index0 >= 0) & (index1 >= 0) & (index1 < self.block_size)
+            slots = torch.where(inside, index0 * self.block_size + index1, -1)
+        quantized_append(self.keys, self.values, self.key_scales, self.value_scales, slots,
+                         keys, values, plan=plan)
 
     def write_checked(self, slots, keys, values):
         """Checked write (kv_cache.py:30-50): -1 skips padding; validates first.
@@ -69,21 +102,25 @@ class LayerKVCache:
             raise ValueError("duplicate slot")
         if slots.numel() == 0:
             return
-        keys = keys.to(self.keys.dtype)
-        values = values.to(self.values.dtype)
-        launch_append(self.keys, self.values, slots, None, keys, values)
+        if not self.quantized:
+            keys = keys.to(self.keys.dtype)
+            values = values.to(self.values.dtype)
+        self._write(slots, None, keys, values)
 
     def write_fast(self, blocks, offsets, keys, values):
         """Hot path (kv_cache.py:52-79): caller guarantees valid, unique slots."""
-        launch_append(self.keys, self.values, blocks, offsets, keys, values)
+        self._write(blocks, offsets, keys, values)
 
-    def write_slots(self, slot_mapping, keys, values):
+    def write_slots(self, slot_mapping, keys, values, plan: QuantizedAppendPlan | None = None):
         """Hot path with the step's int32 slot map; -1 entries are skipped.
 
         Duplicate slots are allowed (graph pad rows share the pad block);
-        which duplicate lands is unspecified.
+        which duplicate lands is unspecified. ``plan``: the step's
+        ``quantized_append_plan``, for 8-bit caches.
         """
-        launch_append(self.keys, self.values, slot_mapping, None, keys, values)
+        if plan is not None and not self.quantized:
+            raise ValueError("only 8-bit caches are written by a plan")
+        self._write(slot_mapping, None, keys, values, plan)
 
 
 class KVCache:
@@ -132,21 +169,50 @@ class KVCache:
             self._value_storage = torch.zeros_like(self._key_storage)
             self.keys = self._key_storage
             self.values = self._value_storage
+        self.key_scales = self.value_scales = None
+        if self.quantized:
+            self._scale_storage = torch.zeros(num_layers, num_blocks, num_kv_heads, 2,
+                                              device=device)
+            self.key_scales = self._scale_storage[..., 0]
+            self.value_scales = self._scale_storage[..., 1]
+
+    @property
+    def quantized(self) -> bool:
+        return self.dtype in QUANTIZED_DTYPES
 
     @property
     def num_bytes(self):
-        return (
-            self.keys.numel() * self.keys.element_size()
-            + self.values.numel() * self.values.element_size()
-        )
+        pools = [self.keys, self.values]
+        if self.quantized:
+            pools += [self.key_scales, self.value_scales]
+        return sum(p.numel() * p.element_size() for p in pools)
 
     def copy_blocks(self, src, dst, tokens=None) -> None:
         """Copy blocks (or their first ``tokens[i]`` rows) to other blocks in
-        every layer: ``hip_kv_blocks.copy_blocks`` over the whole pool."""
-        copy_blocks(self.keys, self.values, src, dst, tokens=tokens)
+        every layer: ``hip_kv_blocks.copy_blocks`` over the whole pool. In an
+        8-bit pool a destination takes its source's scales too, so that its
+        other rows no longer stand for what they did."""
+        if not self.quantized:
+            copy_blocks(self.keys, self.values, src, dst, tokens=tokens)
+            return
+        # The copies move bytes: pairs of codes as 16-bit words, a block's
+        # scales as one row of a head each.
+        src, dst = host_ints(src, "src"), host_ints(dst, "dst")
+        moved = range(len(src))
+        if tokens is not None:
+            # A pair that copies nothing leaves its destination's scales too.
+            tokens = host_ints(tokens, "tokens")
+            moved = [i for i, n in enumerate(tokens) if n != 0]
+        copy_blocks(self.keys.view(torch.float16), self.values.view(torch.float16), src, dst,
+                    tokens=tokens)
+        scales = [s[:, :, None, :, None] for s in (self.key_scales, self.value_scales)]
+        copy_blocks(*scales, [src[i] for i in moved], [dst[i] for i in moved])
 
     def layer(self, index: int) -> LayerKVCache:
         """Basic indexing shares storage; binding does not copy the cache."""
         if not 0 <= index < self.num_layers:
             raise ValueError("layer outside cache")
-        return LayerKVCache(self.keys[index], self.values[index])
+        if not self.quantized:
+            return LayerKVCache(self.keys[index], self.values[index])
+        return LayerKVCache(self.keys[index], self.values[index], self.key_scales[index],
+                            self.value_scales[index])

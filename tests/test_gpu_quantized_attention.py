@@ -1,0 +1,308 @@
+"""Decode and varlen attention over an 8-bit cache against float64."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from microinfer_amd.layer.hip_quantized_attention import (hip_quantized_decode,
+                                                          hip_quantized_prefill,
+                                                          quantized_decode_plan,
+                                                          quantized_prefill_plan)
+from tests.quantized_support import CODES, DTYPES, Twin, check_attention, ints, tables_of
+
+pytestmark = pytest.mark.gpu
+
+# Bits to which a softmax weight is held for its product with V: two bf16
+# halves for 16-bit queries, three for float32.
+WEIGHT_BITS = {"bf16": 16, "f16": 16, "f32": 24}
+
+SHAPES = [  # Hq, Hkv, D, block, layout
+    (16, 8, 128, 16, "paired"), (32, 8, 128, 32, "head_major"), (5, 5, 128, 64, "token_major"),
+    (15, 5, 64, 16, "paired"), (8, 1, 64, 32, "token_major"), (16, 1, 128, 16, "paired"),
+    (6, 2, 32, 16, "paired"), (34, 2, 128, 16, "paired"), (4, 2, 16, 4, "head_major"),
+    (3, 1, 256, 16, "paired"), (2, 2, 128, 8, "token_major")]
+
+
+def query_of(rng, rows, heads, dim, dtype):
+    return torch.from_numpy(rng.standard_normal((rows, heads, dim))).to(DTYPES[dtype]).cuda()
+
+
+def decode_case(rng, contexts, shape, kind, dtype, blocks=None):
+    hq, hkv, dim, block, layout = shape
+    blocks = blocks or sum(-(-c // block) for c in contexts) + 2
+    twin = Twin(blocks, block, hkv, dim, kind, layout)
+    twin.fill(rng)
+    return twin, tables_of(rng, contexts, block, blocks), query_of(rng, len(contexts), hq, dim,
+                                                                   dtype)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_decode(kind, dtype, shape):
+    rng = np.random.default_rng(shape[0] + shape[2])
+    contexts = [1, 0, 17, 33, 700, 2, 64, 257]
+    twin, tables, query = decode_case(rng, contexts, shape, kind, dtype)
+    scale = 1 / math.sqrt(shape[2])
+    got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+    assert got.dtype == query.dtype and not got[1].any()
+    check_attention(got, query, twin, tables, contexts, list(range(9)), scale,
+                    WEIGHT_BITS[dtype])
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("contexts", [[4000], [2500, 3, 1900], [300] * 40, [1] * 70,
+                                      [40 + 7 * i for i in range(90)]])
+def test_decode_splits_and_batches(kind, dtype, contexts):
+    rng = np.random.default_rng(len(contexts))
+    twin, tables, query = decode_case(rng, contexts, (4, 2, 128, 16, "paired"), kind, dtype)
+    plan = quantized_decode_plan(ints(contexts), num_q_heads=4, num_kv_heads=2, head_dim=128,
+                                 dtype=query.dtype, block_size=16,
+                                 block_table_width=len(tables[0]))
+    for q in (query, query.flip(0)):
+        got = hip_quantized_decode(q, *twin.tensors, ints(tables), ints(contexts), plan=plan,
+                                   scale=0.11)
+        check_attention(got, q, twin, tables, contexts, list(range(len(contexts) + 1)), 0.11,
+                        WEIGHT_BITS[dtype])
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+def test_what_the_context_ends_before_does_not_matter(kind):
+    """NaN codes and scales behind the context, in the pages behind it and in
+    blocks that the table does not name."""
+    rng = np.random.default_rng(2)
+    contexts = [19, 5, 160, 513]
+    for shape in ((4, 2, 128, 16, "paired"), (4, 2, 64, 32, "paired"), (4, 4, 32, 16, "paired")):
+        twin, tables, query = decode_case(rng, contexts, shape, kind, "bf16")
+        block = shape[3]
+        used = {tables[s][j] for s, c in enumerate(contexts) for j in range(-(-c // block))}
+        for pool, scales in ((twin.layer.keys, twin.layer.key_scales),
+                             (twin.layer.values, twin.layer.value_scales)):
+            for page in range(pool.shape[0]):
+                if page not in used:
+                    scales[page] = float("nan")
+                    pool[page].view(torch.uint8).fill_(0x7f)
+            if kind == "fp8":
+                for s, c in enumerate(contexts):
+                    if c % block:
+                        pool[tables[s][c // block], c % block:].view(torch.uint8).fill_(0xff)
+        wide = [row + [page] * 2 for row, page in zip(tables, (0, 1, 2, 3))]
+        got = hip_quantized_decode(query, *twin.tensors, ints(wide), ints(contexts))
+        check_attention(got, query, twin, tables, contexts, list(range(5)),
+                        1 / math.sqrt(shape[2]), 16)
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, 16, "paired"), (4, 2, 64, 16, "paired"),
+                                   (4, 2, 128, 64, "paired"), (3, 3, 32, 16, "paired")])
+def test_blocks_outside_the_pool_are_masked(shape):
+    rng = np.random.default_rng(3)
+    contexts = [100, 900, 40, 33]
+    twin, tables, query = decode_case(rng, contexts, shape, "fp8", "f16")
+    blocks = twin.k.shape[0]
+    tables[0][0] = -1
+    tables[1][1] = blocks
+    tables[1][-1] = 2 ** 31 - 1
+    tables[2] = [-5] * len(tables[2])
+    tables[3][-(-33 // shape[3]) - 1] = -2 ** 31
+    got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+    assert not got[2].any()
+    check_attention(got, query, twin, tables, contexts, list(range(5)), 1 / math.sqrt(shape[2]),
+                    16)
+
+
+@pytest.mark.parametrize("dim", [128, 64, 32])
+def test_nan_reaches_the_output(dim):
+    """A NaN code or scale inside a context makes its rows NaN, wherever the
+    context is split, and no other sequence's."""
+    rng = np.random.default_rng(4)
+    contexts = [1500, 60, 1500, 900, 20]
+    twin, tables, query = decode_case(rng, contexts, (4, 2, dim, 16, "paired"), "fp8", "bf16")
+    twin.layer.keys[tables[0][93], 7, 0, 3:4].view(torch.uint8).fill_(0x7f)
+    twin.layer.value_scales[tables[2][0], 1] = float("nan")
+    twin.layer.key_scales[tables[3][50], 0] = float("nan")
+    twin.layer.values[tables[4][0], 19 % 16, 0, 5:6].view(torch.uint8).fill_(0xff)
+    twin.layer.values[tables[4][1], 3, 1, 6:7].view(torch.uint8).fill_(0xff)
+    got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts)).float().cpu()
+    assert got[0, :2].isnan().all() and not got[0, 2:].isnan().any()
+    assert not got[1].isnan().any()
+    assert got[2, 2:].isnan().all() and not got[2, :2].isnan().any()
+    assert got[3, :2].isnan().all() and not got[3, 2:].isnan().any()
+    assert got[4, 2:, 6].isnan().all()
+    rows = hip_quantized_prefill(query[:1], *twin.tensors, ints([0, 1]), ints([0, 1500]),
+                                 ints(tables[:1]), max_seqlen_q=1).float().cpu()
+    assert rows[0, :2].isnan().all() and not rows[0, 2:].isnan().any()
+
+
+def test_scales_far_apart():
+    """Blocks whose values differ by 2^60 in size, and weights that differ as
+    much the other way."""
+    rng = np.random.default_rng(5)
+    for dtype in DTYPES:
+        for kind in CODES:
+            contexts = [400, 70]
+            hq, hkv, dim, block, layout = 4, 2, 128, 16, "paired"
+            twin = Twin(40, block, hkv, dim, kind, layout)
+            twin.fill(rng, sizes=(-3, 3))
+            twin.vs *= np.exp2(rng.integers(-30, 31, twin.vs.shape))
+            twin.layer.value_scales.copy_(torch.from_numpy(twin.vs).float())
+            if dtype == "f16":  # outputs within its range
+                twin.vs *= 2.0 ** -30
+                twin.layer.value_scales.copy_(torch.from_numpy(twin.vs).float())
+            tables = tables_of(rng, contexts, block, 40)
+            query = 3 * query_of(rng, 2, hq, dim, dtype)
+            got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+            check_attention(got, query, twin, tables, contexts, [0, 1, 2], dim ** -0.5,
+                            WEIGHT_BITS[dtype])
+            cu_q = [0, 40, 41]
+            query = 3 * query_of(rng, 41, hq, dim, dtype)
+            got = hip_quantized_prefill(query, *twin.tensors, ints(cu_q), ints([0, 400, 470]),
+                                        ints(tables), max_seqlen_q=40)
+            check_attention(got, query, twin, tables, contexts, cu_q, dim ** -0.5,
+                            WEIGHT_BITS[dtype])
+
+
+def prefill(query, twin, tables, contexts, lengths, planned=False, **kw):
+    cu_q = np.cumsum([0] + lengths).tolist()
+    cu_k = np.cumsum([0] + contexts).tolist()
+    plan = None
+    if planned:
+        plan = quantized_prefill_plan(
+            ints(cu_q), ints(cu_k), num_tokens=query.shape[0], num_q_heads=query.shape[1],
+            num_kv_heads=twin.k.shape[2], head_dim=query.shape[2], dtype=query.dtype,
+            block_size=twin.k.shape[1], block_table_width=len(tables[0]))
+    return hip_quantized_prefill(query, *twin.tensors, ints(cu_q), ints(cu_k), ints(tables),
+                                 max_seqlen_q=max(lengths), plan=plan, **kw), cu_q
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_prefill(kind, dtype, shape):
+    rng = np.random.default_rng(shape[0] + shape[2] + 1)
+    contexts, lengths = [70, 1, 45, 130, 33, 9], [33, 1, 1, 70, 0, 9]
+    hq, hkv, dim, block, layout = shape
+    twin, tables, _ = decode_case(rng, contexts, shape, kind, dtype)
+    query = query_of(rng, sum(lengths), hq, dim, dtype)
+    for planned in (False, True):
+        got, cu_q = prefill(query, twin, tables, contexts, lengths, planned)
+        assert got.dtype == query.dtype
+        check_attention(got, query, twin, tables, contexts, cu_q, 1 / math.sqrt(dim),
+                        WEIGHT_BITS[dtype])
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("contexts,lengths", [
+    ([1800], [40]), ([1800, 900], [1, 129]), ([300, 310, 320, 330], [5, 4, 3, 2]),
+    ([257], [257]), ([600, 1, 500], [64, 1, 65])])
+def test_prefill_lengths(kind, contexts, lengths):
+    rng = np.random.default_rng(len(contexts))
+    twin, tables, _ = decode_case(rng, contexts, (8, 2, 128, 16, "paired"), kind, "bf16")
+    query = query_of(rng, sum(lengths), 8, 128, "bf16")
+    for planned in (False, True):
+        got, cu_q = prefill(query, twin, tables, contexts, lengths, planned, scale=0.07)
+        check_attention(got, query, twin, tables, contexts, cu_q, 0.07, 16)
+
+
+def test_prefill_rows_that_see_nothing_are_zeros():
+    """More query rows than positions, contexts of nothing, invalid blocks."""
+    rng = np.random.default_rng(7)
+    for shape in ((4, 2, 128, 16, "paired"), (4, 2, 64, 16, "paired"), (2, 2, 32, 16, "paired")):
+        contexts, lengths = [5, 0, 40, 20], [9, 3, 2, 20]
+        twin, tables, _ = decode_case(rng, contexts, shape, "int8", "bf16")
+        tables[3] = [-1] * len(tables[3])
+        query = query_of(rng, sum(lengths), shape[0], shape[2], "bf16")
+        for planned in (False, True):
+            got, cu_q = prefill(query, twin, tables, contexts, lengths, planned)
+            assert not got[:4].any() and not got[9:12].any() and not got[14:].any()
+            check_attention(got, query, twin, tables, contexts, cu_q, 1 / math.sqrt(shape[2]),
+                            16)
+
+
+def test_strides_of_queries():
+    rng = np.random.default_rng(8)
+    contexts = [90, 31]
+    twin, tables, _ = decode_case(rng, contexts, (4, 2, 128, 16, "paired"), "fp8", "bf16")
+    fused = query_of(rng, 2, 8, 128, "bf16")
+    for query in (fused[:, 2:6], query_of(rng, 2, 4, 130, "bf16")[..., 1:129],
+                  query_of(rng, 4, 2, 128, "bf16").transpose(0, 1)):
+        got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+        check_attention(got, query, twin, tables, contexts, [0, 1, 2], 128 ** -0.5, 16)
+        got = hip_quantized_prefill(query, *twin.tensors, ints([0, 1, 2]), ints([0, 90, 121]),
+                                    ints(tables), max_seqlen_q=1)
+        check_attention(got, query, twin, tables, contexts, [0, 1, 2], 128 ** -0.5, 16)
+
+
+def test_decode_graphs_and_eager_calls_share_nothing():
+    """Two captured graphs, an eager plan and a plan captured with its calls,
+    replayed among eager calls on another stream."""
+    rng = np.random.default_rng(9)
+    contexts = [1700, 300, 900]
+    shape = (8, 2, 128, 16, "paired")
+    twin, tables, query = decode_case(rng, contexts, shape, "fp8", "bf16")
+    tables, lens = ints(tables), ints(contexts)
+    sizes = dict(num_q_heads=8, num_kv_heads=2, head_dim=128, dtype=torch.bfloat16,
+                 block_size=16, block_table_width=tables.shape[1])
+    eager = quantized_decode_plan(lens, **sizes)
+    queries = [query, query.flip(0).contiguous(), (query * 2).contiguous()]
+    want = [hip_quantized_decode(q, *twin.tensors, tables, lens, plan=eager) for q in queries]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan = eager if i else quantized_decode_plan(lens, **sizes)
+            outs.append([hip_quantized_decode(q, *twin.tensors, tables, lens, plan=plan)
+                         for q in queries])
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        for out in outs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        third = torch.cuda.Stream()
+        with torch.cuda.stream(third):
+            again = hip_quantized_decode(queries[1], *twin.tensors, tables, lens, plan=eager)
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert torch.equal(again, want[1])
+
+
+def test_decode_replays_with_other_lengths():
+    rng = np.random.default_rng(10)
+    shape = (4, 2, 128, 16, "paired")
+    most = [1200, 700, 64]
+    twin, tables, query = decode_case(rng, most, shape, "int8", "f16")
+    lens = ints(most)
+    where = ints(tables)
+
+    def call():
+        return hip_quantized_decode(query, *twin.tensors, where, lens)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for contexts in ([3, 700, 1], [1200, 0, 64], [640, 333, 17]):
+        lens.copy_(ints(contexts))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(out, query, twin, tables, contexts, [0, 1, 2, 3], 128 ** -0.5, 16)
+
+
+def test_results_repeat():
+    rng = np.random.default_rng(11)
+    contexts = [3000, 40, 1500]
+    twin, tables, query = decode_case(rng, contexts, (8, 2, 128, 16, "paired"), "fp8", "bf16")
+    first = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+    for _ in range(5):
+        assert torch.equal(first, hip_quantized_decode(query, *twin.tensors, ints(tables),
+                                                       ints(contexts)))

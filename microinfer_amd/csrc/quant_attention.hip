@@ -1,7 +1,7 @@
 // C entry points of attention over an 8-bit K/V cache.
 #include <cmath>
 
-#include "quant.h"
+#include "quant_mfma.h"
 
 namespace mi {
 namespace {
@@ -66,7 +66,10 @@ extern "C" int32_t mi_quant_decode_plan(const int32_t* context_lens, int32_t num
       reinterpret_cast<uintptr_t>(plan) % 32 != 0)
     return fail(MI_ERR_WORKSPACE, fn + ": plan buffer too small or misaligned");
   return launch_decode_plan(context_lens, num_seqs, num_kv_heads, block_size, block_table_width,
-                            0, true, static_cast<PlanItem*>(plan), counters,
+                            0,
+                            !quant_decode_mfma_takes(head_dim, num_q_heads / num_kv_heads,
+                                                     block_size),
+                            static_cast<PlanItem*>(plan), counters,
                             static_cast<hipStream_t>(stream));
 }
 
@@ -128,7 +131,9 @@ extern "C" int32_t mi_quant_decode(
   a.num_seqs = a.num_rows = num_seqs;
   a.group = num_q_heads / num_kv_heads;
   a.scale_log2 = scale * kLog2e;
-  return launch_quant_vector(a, dtype, code, static_cast<hipStream_t>(stream));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (quant_decode_mfma_supported(a)) return launch_quant_decode_mfma(a, dtype, code, s);
+  return launch_quant_vector(a, dtype, code, s);
 }
 
 extern "C" int32_t mi_quant_prefill(

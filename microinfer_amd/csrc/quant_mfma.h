@@ -1,0 +1,91 @@
+// Matrix-instruction pieces shared by the attention kernels over an 8-bit K/V
+// cache: codes widened to bf16 (exactly: both types have at most eight
+// significant bits), float32 values split into bf16 parts.
+#pragma once
+
+#include "quant.h"
+
+namespace mi {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int int2v_t __attribute__((ext_vector_type(2)));
+
+// bf16 parts of a query: all of its bits (8, 11 and 24 of them).
+template <typename E>
+constexpr int kQueryParts = std::is_same<E, BF16>::value ? 1 : std::is_same<E, F16>::value ? 2 : 3;
+
+struct Word4 {
+  uint32_t w[4];
+};
+
+// Two of a word's codes (the upper two: HIGH) as a pair of bf16.
+template <typename C, bool HIGH>
+__device__ __forceinline__ uint32_t widen_pair(uint32_t w) {
+  if constexpr (std::is_same<C, E4M3>::value) {
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HIGH));
+  } else {
+    constexpr int s = HIGH ? 16 : 0;
+    const float lo = static_cast<float>(static_cast<int8_t>(w >> s));
+    const float hi = static_cast<float>(static_cast<int8_t>(w >> (s + 8)));
+    // Eight significant bits: the upper halves of the float32 values.
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+  }
+}
+
+// Eight codes (two words) as a matrix operand.
+template <typename C>
+__device__ __forceinline__ bf16x8_t widen_operand(uint32_t lo, uint32_t hi) {
+  Word4 r;
+  r.w[0] = widen_pair<C, false>(lo);
+  r.w[1] = widen_pair<C, true>(lo);
+  r.w[2] = widen_pair<C, false>(hi);
+  r.w[3] = widen_pair<C, true>(hi);
+  return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// x = part[0] + part[1] + ... in bf16, each what the ones before leave, rounded.
+template <int N>
+__device__ __forceinline__ void split8(const float* x, bf16x8_t* part) {
+  float rest[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __bf16 r = static_cast<__bf16>(rest[i]);
+      part[n][i] = r;
+      if (n + 1 < N) rest[i] -= static_cast<float>(r);
+    }
+  }
+}
+
+// Direct global -> LDS load of 4 bytes per lane (lane i's at lds_dst + 4 i),
+// untracked by the compiler like lds_load16.
+__device__ __forceinline__ void lds_load4(const void* src, const void* lds_dst) {
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (const __attribute__((address_space(3))) void*)(lds_dst)));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+               :
+               : "v"(src), "s"(lds)
+               : "memory", "m0");
+}
+
+// Eight one-byte elements, transposed across each group of 16 lanes
+// (ds_read_b64_tr_b8): lane i of a group receives byte i % 8 of the eight
+// bytes read by lanes i / 8, i / 8 + 2, ..., i / 8 + 14.
+__device__ __forceinline__ int2v_t read_tr8(const void* lds) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      (__attribute__((address_space(3))) int2v_t*)(lds));
+}
+
+// Whether the MFMA decode kernel takes calls of this shape, and its launch.
+bool quant_decode_mfma_takes(int32_t head_dim, int32_t group, int32_t block_size);
+bool quant_decode_mfma_supported(const QuantAttnArgs& a);
+int32_t launch_quant_decode_mfma(const QuantAttnArgs& a, int32_t dtype, int32_t code,
+                                 hipStream_t stream);
+
+}  // namespace mi

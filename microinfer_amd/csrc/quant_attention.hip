@@ -23,7 +23,16 @@ int32_t check_table(const std::string& fn, const int32_t* tables, int32_t width,
   return MI_OK;
 }
 
-int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int32_t check_prefill_workspace(const std::string& fn, int32_t num_tokens, int32_t num_requests,
+                                int32_t group, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t block_size, const void* workspace, int64_t bytes) {
+  const int64_t need = quant_prefill_workspace(num_tokens, num_requests, group, num_kv_heads,
+                                               head_dim, block_size);
+  if (workspace == nullptr || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return fail(MI_ERR_WORKSPACE, fn + ": workspace needs " + std::to_string(need) +
+                                      " bytes, 256-byte aligned");
+  return MI_OK;
+}
 
 }  // namespace
 }  // namespace mi
@@ -136,6 +145,39 @@ extern "C" int32_t mi_quant_decode(
   return launch_quant_vector(a, dtype, code, s);
 }
 
+extern "C" int64_t mi_quant_prefill_workspace_bytes(int32_t num_tokens, int32_t num_requests,
+                                                    int32_t num_q_heads, int32_t num_kv_heads,
+                                                    int32_t head_dim, int32_t block_size) {
+  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return 0;
+  return mi::quant_prefill_workspace(num_tokens, num_requests, num_q_heads / num_kv_heads,
+                                     num_kv_heads, head_dim, block_size);
+}
+
+extern "C" int32_t mi_quant_prefill_plan(const int32_t* cu_seqlens_q,
+                                         const int32_t* cu_seqlens_k, int32_t num_tokens,
+                                         int32_t num_requests, int32_t num_q_heads,
+                                         int32_t num_kv_heads, int32_t head_dim,
+                                         int32_t block_size, void* workspace,
+                                         int64_t workspace_bytes, void* stream) {
+  using namespace mi;
+  clear_error();
+  const std::string fn = "mi_quant_prefill_plan";
+  int32_t st = check_heads(fn, num_q_heads, num_kv_heads);
+  if (st != MI_OK) return st;
+  const int32_t group = num_q_heads / num_kv_heads;
+  if (quant_prefill_workspace(num_tokens, num_requests, group, num_kv_heads, head_dim,
+                              block_size) == 0)
+    return fail(MI_ERR_UNSUPPORTED, fn + ": these sizes take no plan");
+  if (!cu_seqlens_q || !cu_seqlens_k)
+    return fail(MI_ERR_INVALID_ARGUMENT, fn + ": null pointer");
+  st = check_prefill_workspace(fn, num_tokens, num_requests, group, num_kv_heads, head_dim,
+                               block_size, workspace, workspace_bytes);
+  if (st != MI_OK) return st;
+  return launch_quant_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_tokens, num_requests, group,
+                                   num_kv_heads, head_dim, workspace,
+                                   static_cast<hipStream_t>(stream));
+}
+
 extern "C" int32_t mi_quant_prefill(
     const void* query, int64_t q_token_stride, int64_t q_head_stride, const void* key_cache,
     const void* value_cache, int64_t cache_block_stride, int64_t cache_token_stride,
@@ -143,9 +185,9 @@ extern "C" int32_t mi_quant_prefill(
     int64_t scale_block_stride, int64_t scale_head_stride, const int32_t* cu_seqlens_q,
     const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t block_table_stride,
     int32_t block_table_width, void* out, int64_t out_token_stride, int64_t out_head_stride,
-    int32_t num_tokens, int32_t num_requests, int32_t num_q_heads, int32_t num_kv_heads,
-    int32_t head_dim, int32_t block_size, int32_t num_blocks, float scale, int32_t dtype,
-    int32_t code, void* stream) {
+    void* workspace, int64_t workspace_bytes, int32_t num_tokens, int32_t num_requests,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int32_t num_blocks, float scale, int32_t dtype, int32_t code, void* stream) {
   using namespace mi;
   clear_error();
   const std::string fn = "mi_quant_prefill";
@@ -184,5 +226,10 @@ extern "C" int32_t mi_quant_prefill(
   a.num_rows = num_tokens;
   a.group = num_q_heads / num_kv_heads;
   a.scale_log2 = scale * kLog2e;
-  return launch_quant_vector(a, dtype, code, static_cast<hipStream_t>(stream));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!quant_prefill_mfma_supported(a)) return launch_quant_vector(a, dtype, code, s);
+  st = check_prefill_workspace(fn, num_tokens, num_requests, a.group, num_kv_heads, head_dim,
+                               block_size, workspace, workspace_bytes);
+  if (st != MI_OK) return st;
+  return launch_quant_prefill_mfma(a, dtype, code, workspace, s);
 }

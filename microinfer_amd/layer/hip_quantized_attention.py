@@ -162,17 +162,60 @@ def hip_quantized_decode(query: torch.Tensor, key_cache: torch.Tensor,
     return out
 
 
+@dataclass(frozen=True)
+class QuantizedPrefillPlan:
+    """One step's work (``quantized_prefill_plan``), for calls of its sizes."""
+
+    cu_seqlens_q: torch.Tensor
+    cu_seqlens_k: torch.Tensor
+    sizes: tuple  # tokens, requests, Hq, Hkv, head_dim, block size
+    workspace_bytes: int
+    _workspaces: dict = field(default_factory=dict, repr=False, compare=False)
+
+    def workspace(self, device: torch.device) -> torch.Tensor:
+        """The plan with room for the partials of a call from here: its
+        thread's and stream's own, a call's own where a graph holds it but not
+        the plan."""
+        place = _call_place(device)
+        have = self._workspaces.get(place)
+        if have is None:
+            have = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+            tokens, requests, num_q_heads, num_kv_heads, head_dim, block_size = self.sizes
+            status = _lib.load().mi_quant_prefill_plan(
+                self.cu_seqlens_q.data_ptr(), self.cu_seqlens_k.data_ptr(), tokens, requests,
+                num_q_heads, num_kv_heads, head_dim, block_size, have.data_ptr(),
+                self.workspace_bytes, place[1])
+            _lib.check(status, "mi_quant_prefill_plan")
+            if not place[2] or not self._workspaces:
+                self._workspaces[place] = have
+        return have
+
+
 def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, *,
                            num_tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
-                           dtype: torch.dtype, block_size: int, block_table_width: int):
-    """The plan of ``hip_quantized_prefill`` calls of these sizes (None: they
-    run without one)."""
+                           dtype: torch.dtype, block_size: int,
+                           block_table_width: int) -> QuantizedPrefillPlan | None:
+    """The plan of one step's ``hip_quantized_prefill`` calls (shared by its
+    layers), from the cu_seqlens on the device (capture-safe). None: calls of
+    these sizes run without one."""
     _lib.require_device(cu_seqlens_q, cu_seqlens_k, what="quantized_prefill_plan")
     if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
         raise ValueError("Hq must be divisible by Hkv")
-    if cu_seqlens_q.numel() != cu_seqlens_k.numel() or cu_seqlens_q.numel() == 0:
+    if dtype not in _FLOAT_DTYPES:
+        raise ValueError("unsupported query dtype")
+    requests, device = cu_seqlens_q.numel() - 1, cu_seqlens_q.device
+    if requests < 0 or cu_seqlens_k.numel() != requests + 1:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have num_requests + 1 entries")
-    return None
+    if cu_seqlens_k.device != device:
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must share a device")
+    sizes = num_tokens, requests, num_q_heads, num_kv_heads, head_dim, block_size
+    nbytes = _lib.load().mi_quant_prefill_workspace_bytes(*sizes)
+    if nbytes == 0:
+        return None
+    plan = QuantizedPrefillPlan(_index32(cu_seqlens_q), _index32(cu_seqlens_k), sizes, nbytes)
+    with _lib.on_device(device):
+        plan.workspace(device)
+    return plan
 
 
 def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
@@ -180,13 +223,14 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
                           value_scales: torch.Tensor, cu_seqlens_q: torch.Tensor,
                           cu_seqlens_k: torch.Tensor, block_tables: torch.Tensor, *,
                           max_seqlen_q: int, scale: float | None = None,
-                          plan=None) -> torch.Tensor:
+                          plan: QuantizedPrefillPlan | None = None) -> torch.Tensor:
     """Causal varlen attention over an 8-bit paged cache (bottom-right mask).
 
     ``query [T, Hq, D]``; request r owns query rows ``cu_seqlens_q[r]..`` and
     context ``cu_seqlens_k[r+1] - cu_seqlens_k[r]`` (it includes the new rows,
     which the caller appended first). ``plan``: of ``quantized_prefill_plan``
-    for these lengths and sizes. Rows that see nothing give zeros.
+    for these lengths and sizes; without it the call makes its own. Rows that
+    see nothing give zeros.
     """
     cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
                                         "hip_quantized_prefill")
@@ -205,8 +249,11 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
     _lib.require_device(cu_seqlens_q, cu_seqlens_k, block_tables, what="hip_quantized_prefill")
     if any(t.device != device for t in (cu_seqlens_q, cu_seqlens_k, block_tables)):
         raise ValueError("cu_seqlens and block_tables must be on the query's device")
-    if plan is not None:
+    sizes = num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim, block_size
+    if plan is not None and (not isinstance(plan, QuantizedPrefillPlan) or plan.sizes != sizes):
         raise ValueError("plan must come from quantized_prefill_plan() for this call's sizes")
+    if plan is not None and plan.cu_seqlens_q.device != device:
+        raise ValueError("plan must be on the query's device")
     if num_tokens and not num_requests:
         raise ValueError("tokens without requests")
     query, tables = whole_vectors(query), _index32(block_tables)
@@ -214,12 +261,20 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if num_tokens == 0:
         return out
+    if plan is None:
+        plan = quantized_prefill_plan(
+            cu_q, cu_k, num_tokens=num_tokens, num_q_heads=num_q_heads,
+            num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=query.dtype,
+            block_size=block_size, block_table_width=width)
     with _lib.on_device(device):
+        workspace, nbytes = None, 0
+        if plan is not None:
+            workspace, nbytes = plan.workspace(device).data_ptr(), plan.workspace_bytes
         status = _lib.load().mi_quant_prefill(
             query.data_ptr(), *query.stride()[:2], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
             tables.data_ptr(), tables.stride(0), width, out.data_ptr(), num_q_heads * head_dim,
-            head_dim, num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim, block_size,
-            num_blocks, float(head_dim ** -0.5 if scale is None else scale),
+            head_dim, workspace, nbytes, num_tokens, num_requests, num_q_heads, num_kv_heads,
+            head_dim, block_size, num_blocks, float(head_dim ** -0.5 if scale is None else scale),
             _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(device))
     _lib.check(status, "mi_quant_prefill")
     return out

@@ -16,6 +16,8 @@ typedef int int2v_t __attribute__((ext_vector_type(2)));
 template <typename E>
 constexpr int kQueryParts = std::is_same<E, BF16>::value ? 1 : std::is_same<E, F16>::value ? 2 : 3;
 
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
 struct Word4 {
   uint32_t w[4];
 };
@@ -35,6 +37,30 @@ __device__ __forceinline__ uint32_t widen_pair(uint32_t w) {
   }
 }
 
+// The same as a pair of f16, which hold the codes as exactly.
+template <typename C, bool HIGH>
+__device__ __forceinline__ uint32_t widen_pair_f16(uint32_t w) {
+  if constexpr (std::is_same<C, E4M3>::value) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HIGH));
+  } else {
+    // 0x6400 + u is 1024 + u, for u = code + 128.
+    const uint32_t u = w ^ 0x80808080u;
+    const uint32_t x = __builtin_amdgcn_perm(0x64646464u, u, HIGH ? 0x04030402u : 0x04010400u);
+    const f16x2_t bias = {static_cast<_Float16>(1152.f), static_cast<_Float16>(1152.f)};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, x) - bias);
+  }
+}
+
+template <typename C>
+__device__ __forceinline__ f16x8_t widen_operand_f16(uint32_t lo, uint32_t hi) {
+  Word4 r;
+  r.w[0] = widen_pair_f16<C, false>(lo);
+  r.w[1] = widen_pair_f16<C, true>(lo);
+  r.w[2] = widen_pair_f16<C, false>(hi);
+  r.w[3] = widen_pair_f16<C, true>(hi);
+  return __builtin_bit_cast(f16x8_t, r);
+}
+
 // Eight codes (two words) as a matrix operand.
 template <typename C>
 __device__ __forceinline__ bf16x8_t widen_operand(uint32_t lo, uint32_t hi) {
@@ -46,17 +72,24 @@ __device__ __forceinline__ bf16x8_t widen_operand(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(bf16x8_t, r);
 }
 
-// x = part[0] + part[1] + ... in bf16, each what the ones before leave, rounded.
-template <int N>
-__device__ __forceinline__ void split8(const float* x, bf16x8_t* part) {
+// x = part[0] + part[1] + ... in bf16 (or f16), each what the ones before
+// leave, rounded.
+template <int N, typename V>
+__device__ __forceinline__ void split8(const float* x, V* part) {
+  using T = typename std::conditional<std::is_same<V, bf16x8_t>::value, __bf16, _Float16>::type;
   float rest[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) rest[i] = x[i];
+  for (int i = 0; i < 8; ++i) {
+    rest[i] = x[i];
+    // The compiler may fuse a product with its conversion to f16, which rounds
+    // once instead of twice, in one of its uses: the parts would not fit.
+    if constexpr (N > 1 && std::is_same<T, _Float16>::value) asm("" : "+v"(rest[i]));
+  }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const __bf16 r = static_cast<__bf16>(rest[i]);
+      const T r = static_cast<T>(rest[i]);
       part[n][i] = r;
       if (n + 1 < N) rest[i] -= static_cast<float>(r);
     }

@@ -77,15 +77,15 @@ def gather(codes, scales, tables, contexts) -> np.ndarray:
 
 def attention(query, k_codes, v_codes, k_scales, v_scales, tables, contexts, cu_q, scale):
     """Causal attention (bottom-right) of the rows of each request over its
-    context. Returns the outputs ``[T, Hq, D]``, the same with |v| in place of
-    v, and per row and head the largest scale * sum |q k| of the positions it
-    sees: what error bounds are made of."""
+    context. Returns the outputs ``[T, Hq, D]`` and what error bounds are made of:
+    the same with |v| in place of v, and per row and head the largest scale *
+    sum |q k| and the largest weight times its V scale of the positions it sees."""
     query = np.asarray(query, dtype=np.float64)
     blocks, size, hkv, dim = k_codes.shape
     hq = query.shape[1]
     share = hq // hkv
     out, around = np.zeros_like(query), np.zeros_like(query)
-    reach = np.zeros(query.shape[:2])
+    reach, peak = np.zeros((2, *query.shape[:2]))
     for r, c in enumerate(contexts):
         c = min(c, len(tables[r]) * size)
         rows = range(cu_q[r], cu_q[r + 1])
@@ -108,4 +108,5 @@ def attention(query, k_codes, v_codes, k_scales, v_scales, tables, contexts, cu_
                 out[row, h] = p @ vv
                 around[row, h] = p @ np.abs(vv)
                 reach[row, h] = abs(scale) * (np.abs(kk) @ np.abs(query[row, h])).max()
-    return out, around, reach
+                peak[row, h] = (p * v_scales[page[seen], h // share]).max()
+    return out, around, reach, peak

@@ -70,7 +70,7 @@ def ints(values, device="cuda"):
     return torch.tensor(values, dtype=torch.int32, device=device)
 
 
-def check_attention(got, query, twin, tables, contexts, cu_q, scale, half_bits=24):
+def check_attention(got, query, twin, tables, contexts, cu_q, scale, weights):
     """``got`` against float64, with the bounds of the arithmetic.
 
     A score is a sum of D products in float32, then a few factors: off by at
@@ -78,15 +78,21 @@ def check_attention(got, query, twin, tables, contexts, cu_q, scale, half_bits=2
     it by that plus the rounding of its argument (2^-24 |s|) and of exp2 (2^-22).
     Weights and their sum both carry it: twice. A sum of n weighted values in
     float32 adds n 2^-24 of sum p |v| at most, partitions and waves merge in a
-    few more, the weight's own rounding for the product with V 2^-half_bits; the
-    result rounds to the output's type by half a step.
+    few more. ``weights``: (bits, lost): a weight times its V scale is rounded to
+    2^-bits of it for the product with V, and f16 rounds it to 2^-25 at most
+    where the row's largest is 2^10 or more, lost = 2^-35 of that (``peak``) for
+    each of n, times a code of up to MOST. The result rounds to the output's type
+    by half a step.
     """
-    out, around, reach = oracle.attention(query.double().cpu().numpy(), twin.k, twin.v, twin.ks,
-                                          twin.vs, tables, contexts, cu_q, scale)
+    out, around, reach, peak = oracle.attention(
+        query.double().cpu().numpy(), twin.k, twin.v, twin.ks, twin.vs, tables, contexts, cu_q,
+        scale)
+    bits, lost = weights
     dim = query.shape[-1]
     n = max([1] + [int(c) for c in contexts])
     weight = 2 * ((dim + 8) * 2.0 ** -24 + 2.0 ** -24) * reach + 2 * 2.0 ** -22
-    bound = (weight[..., None] + n * 2.0 ** -24 + 16 * 2.0 ** -24 + 2 * 2.0 ** -half_bits) * around
+    bound = (weight[..., None] + n * 2.0 ** -24 + 16 * 2.0 ** -24 + 2 * 2.0 ** -bits) * around
+    bound += n * lost * oracle.MOST[twin.kind] * peak[..., None]
     half = torch.finfo(got.dtype).eps / 2
     bound += half * (np.abs(out) + bound) + torch.finfo(got.dtype).smallest_normal * half * 2
     err = np.abs(got.double().cpu().numpy() - out)

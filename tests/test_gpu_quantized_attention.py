@@ -14,9 +14,12 @@ from tests.quantized_support import CODES, DTYPES, Twin, check_attention, ints, 
 
 pytestmark = pytest.mark.gpu
 
-# Bits to which a softmax weight is held for its product with V: two bf16
-# halves for 16-bit queries, three for float32.
-WEIGHT_BITS = {"bf16": 16, "f16": 16, "f32": 24}
+# How a softmax weight is held for its product with V (``check_attention``).
+# Decode: two bf16 parts for 16-bit queries (half a step of each: 2^-8 of 2^-8),
+# three for float32. Varlen: one f16 part for bf16 queries (half a step, 2^-11),
+# two for f16 ones, three bf16 parts for float32.
+DECODE = {"bf16": (16, 0), "f16": (16, 0), "f32": (24, 0)}
+VARLEN = {"bf16": (11, 2.0 ** -35), "f16": (22, 2.0 ** -35), "f32": (24, 0)}
 
 SHAPES = [  # Hq, Hkv, D, block, layout
     (16, 8, 128, 16, "paired"), (32, 8, 128, 32, "head_major"), (5, 5, 128, 64, "token_major"),
@@ -49,7 +52,7 @@ def test_decode(kind, dtype, shape):
     got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
     assert got.dtype == query.dtype and not got[1].any()
     check_attention(got, query, twin, tables, contexts, list(range(9)), scale,
-                    WEIGHT_BITS[dtype])
+                    DECODE[dtype])
 
 
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
@@ -66,7 +69,7 @@ def test_decode_splits_and_batches(kind, dtype, contexts):
         got = hip_quantized_decode(q, *twin.tensors, ints(tables), ints(contexts), plan=plan,
                                    scale=0.11)
         check_attention(got, q, twin, tables, contexts, list(range(len(contexts) + 1)), 0.11,
-                        WEIGHT_BITS[dtype])
+                        DECODE[dtype])
 
 
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
@@ -92,7 +95,7 @@ def test_what_the_context_ends_before_does_not_matter(kind):
         wide = [row + [page] * 2 for row, page in zip(tables, (0, 1, 2, 3))]
         got = hip_quantized_decode(query, *twin.tensors, ints(wide), ints(contexts))
         check_attention(got, query, twin, tables, contexts, list(range(5)),
-                        1 / math.sqrt(shape[2]), 16)
+                        1 / math.sqrt(shape[2]), DECODE["bf16"])
 
 
 @pytest.mark.parametrize("shape", [(4, 2, 128, 16, "paired"), (4, 2, 64, 16, "paired"),
@@ -110,7 +113,7 @@ def test_blocks_outside_the_pool_are_masked(shape):
     got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
     assert not got[2].any()
     check_attention(got, query, twin, tables, contexts, list(range(5)), 1 / math.sqrt(shape[2]),
-                    16)
+                    DECODE["f16"])
 
 
 @pytest.mark.parametrize("dim", [128, 64, 32])
@@ -155,13 +158,13 @@ def test_scales_far_apart():
             query = 3 * query_of(rng, 2, hq, dim, dtype)
             got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
             check_attention(got, query, twin, tables, contexts, [0, 1, 2], dim ** -0.5,
-                            WEIGHT_BITS[dtype])
+                            DECODE[dtype])
             cu_q = [0, 40, 41]
             query = 3 * query_of(rng, 41, hq, dim, dtype)
             got = hip_quantized_prefill(query, *twin.tensors, ints(cu_q), ints([0, 400, 470]),
                                         ints(tables), max_seqlen_q=40)
             check_attention(got, query, twin, tables, contexts, cu_q, dim ** -0.5,
-                            WEIGHT_BITS[dtype])
+                            VARLEN[dtype])
 
 
 def prefill(query, twin, tables, contexts, lengths, planned=False, **kw):
@@ -190,7 +193,7 @@ def test_prefill(kind, dtype, shape):
         got, cu_q = prefill(query, twin, tables, contexts, lengths, planned)
         assert got.dtype == query.dtype
         check_attention(got, query, twin, tables, contexts, cu_q, 1 / math.sqrt(dim),
-                        WEIGHT_BITS[dtype])
+                        VARLEN[dtype])
 
 
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
@@ -203,7 +206,7 @@ def test_prefill_lengths(kind, contexts, lengths):
     query = query_of(rng, sum(lengths), 8, 128, "bf16")
     for planned in (False, True):
         got, cu_q = prefill(query, twin, tables, contexts, lengths, planned, scale=0.07)
-        check_attention(got, query, twin, tables, contexts, cu_q, 0.07, 16)
+        check_attention(got, query, twin, tables, contexts, cu_q, 0.07, VARLEN["bf16"])
 
 
 def test_prefill_rows_that_see_nothing_are_zeros():
@@ -218,7 +221,7 @@ def test_prefill_rows_that_see_nothing_are_zeros():
             got, cu_q = prefill(query, twin, tables, contexts, lengths, planned)
             assert not got[:4].any() and not got[9:12].any() and not got[14:].any()
             check_attention(got, query, twin, tables, contexts, cu_q, 1 / math.sqrt(shape[2]),
-                            16)
+                            VARLEN["bf16"])
 
 
 def test_strides_of_queries():
@@ -229,10 +232,10 @@ def test_strides_of_queries():
     for query in (fused[:, 2:6], query_of(rng, 2, 4, 130, "bf16")[..., 1:129],
                   query_of(rng, 4, 2, 128, "bf16").transpose(0, 1)):
         got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
-        check_attention(got, query, twin, tables, contexts, [0, 1, 2], 128 ** -0.5, 16)
+        check_attention(got, query, twin, tables, contexts, [0, 1, 2], 128 ** -0.5, DECODE["bf16"])
         got = hip_quantized_prefill(query, *twin.tensors, ints([0, 1, 2]), ints([0, 90, 121]),
                                     ints(tables), max_seqlen_q=1)
-        check_attention(got, query, twin, tables, contexts, [0, 1, 2], 128 ** -0.5, 16)
+        check_attention(got, query, twin, tables, contexts, [0, 1, 2], 128 ** -0.5, VARLEN["bf16"])
 
 
 def test_decode_graphs_and_eager_calls_share_nothing():
@@ -295,7 +298,8 @@ def test_decode_replays_with_other_lengths():
         lens.copy_(ints(contexts))
         graph.replay()
         torch.cuda.synchronize()
-        check_attention(out, query, twin, tables, contexts, [0, 1, 2, 3], 128 ** -0.5, 16)
+        check_attention(out, query, twin, tables, contexts, [0, 1, 2, 3], 128 ** -0.5,
+                        DECODE["f16"])
 
 
 def test_results_repeat():

@@ -54,7 +54,8 @@ def test_attention_of_one_position_is_its_value():
     k, v = rng.integers(-5, 6, (2, 3, 4, 2, 16)).astype(np.float64)
     scales = np.full((3, 2), 0.5)
     q = rng.standard_normal((2, 4, 16))
-    out, around, _ = oracle.attention(q, k, v, scales, scales, [[2, 1], [-1, 0]], [1, 4],
+    out, around, _, peak = oracle.attention(q, k, v, scales, scales, [[2, 1], [-1, 0]], [1, 4],
                                       [0, 1, 2], 0.25)
     np.testing.assert_array_equal(out[0], np.repeat(v[2, 0] * 0.5, 2, axis=0))
+    assert (peak[0] == 0.5).all()
     assert not out[1].any() and not around[1].any()  # its only block is not there

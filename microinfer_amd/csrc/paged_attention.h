@@ -83,19 +83,6 @@ int32_t launch_prefill_plan(const AttnArgs& args, void* workspace, hipStream_t s
 int32_t launch_prefill_mfma_planned(AttnArgs args, int32_t dtype, void* workspace,
                                     bool plan_ready, hipStream_t stream);
 
-// The same plan for other kernels over blocks of `block_rows` query rows and
-// tiles of 32 keys, of paged contexts of at most ctx_cap positions: items,
-// their number in count[0], prefill_counters() counters zeroed. At most
-// prefill_items_max() items (0: the sizes take no plan), parts in
-// prefill_items_slots() slots.
-int32_t prefill_items_max(int32_t num_rows, int32_t num_seqs, int32_t block_rows,
-                          int32_t num_kv_heads);
-int32_t prefill_items_slots(int32_t num_kv_heads);
-int32_t launch_prefill_items(const int32_t* cu_q, const int32_t* cu_k, int32_t num_rows,
-                             int32_t num_seqs, int32_t block_rows, int32_t num_kv_heads,
-                             int32_t ctx_cap, PrefillItem* items, int32_t* count,
-                             int32_t* counters, hipStream_t stream);
-
 // float32 MFMA varlen kernel (paged_prefill_f32.hip): float32 with head_dim
 // 128, contiguous K/V or a block size of at least 16; preferred where it is
 // the faster one.

@@ -1277,35 +1277,6 @@ int32_t launch_prefill_plan(const AttnArgs& a, void* workspace, hipStream_t stre
   return check_launch("paged prefill plan");
 }
 
-int32_t prefill_items_max(int32_t num_rows, int32_t num_seqs, int32_t block_rows,
-                          int32_t num_kv_heads) {
-  const int64_t blocks = (static_cast<int64_t>(num_rows) + block_rows - 1) / block_rows + num_seqs;
-  if (num_seqs > kMaxPlanReqs || blocks > kMaxPlanBlocks) return 0;
-  return static_cast<int32_t>(blocks) + part_cap_of(num_kv_heads);
-}
-
-int32_t prefill_items_slots(int32_t num_kv_heads) { return part_cap_of(num_kv_heads); }
-
-int32_t launch_prefill_items(const int32_t* cu_q, const int32_t* cu_k, int32_t num_rows,
-                             int32_t num_seqs, int32_t block_rows, int32_t num_kv_heads,
-                             int32_t ctx_cap, PrefillItem* items, int32_t* count,
-                             int32_t* counters, hipStream_t stream) {
-  const int32_t max_items = prefill_items_max(num_rows, num_seqs, block_rows, num_kv_heads);
-  if (max_items == 0) return MI_ERR_UNSUPPORTED;
-  auto go = [&](auto kernel) {
-    // Contiguous rows without an end: a request of one row is one like others.
-    kernel<<<1, kPlanThreads, 0, stream>>>(cu_q, cu_k, num_seqs, block_rows, ctx_cap,
-                                           int64_t(1) << 40, device_cus(), num_kv_heads,
-                                           part_cap_of(num_kv_heads), max_items, items, count,
-                                           counters, prefill_counters(num_kv_heads));
-  };
-  if (max_items - part_cap_of(num_kv_heads) <= kPlanThreads)
-    go(prefill_plan_kernel<1>);
-  else
-    go(prefill_plan_kernel<kPlanPer>);
-  return check_launch("paged prefill plan");
-}
-
 int32_t launch_prefill_mfma_planned(AttnArgs a, int32_t dtype, void* workspace, bool plan_ready,
                                     hipStream_t stream) {
   if (!prefill_mfma_supported(a, dtype) ||

@@ -8,11 +8,11 @@
 //  * Workgroup = plan item (request, block of query rows, range of key tiles) x
 //    KV head. The block's tokens times the group's heads are its rows, up to 128:
 //    four waves of 32, so a key tile serves all heads of the group.
-//  * A tile of 32 keys is widened to 16-bit floats (exactly) once for the four
-//    waves: a thread loads 16 codes of K and of V and writes them, a tile later,
-//    to the one of two LDS buffers that is not read. Rows of V that nothing may
-//    see are written as zeros. K runs a tile ahead: the scores of a tile are
-//    computed while the softmax of the one before is.
+//  * 64 keys (32 for f32 with D = 128) are a step: a thread loads its codes of K and V, and a
+//    step later widens them to 16-bit floats (exactly) and writes them to the one
+//    of two LDS buffers that is not read. Keys that nothing may see have V rows of
+//    zeros. Where the halves of 16 keys lie, and their scales, is looked up for
+//    32 steps at once, a thread for a half.
 //  * S^T = K . Q^T on 32x32x16 MFMA: bf16 queries with codes as bf16, f16 with
 //    codes as f16, f32 ones in three bf16 parts, which hold all of their bits.
 //    The K scale meets the scores in float32. A lane owns 16 keys of one row, so
@@ -26,6 +26,7 @@
 //    output is as fine, have two such parts; f32 ones three in bf16.
 //  * Row blocks whose keys are split publish theirs; the last arrival merges
 //    them in order.
+#include <algorithm>
 #include <climits>
 
 #include "quant_mfma.h"
@@ -33,7 +34,7 @@
 namespace mi {
 namespace {
 
-constexpr int kKeys = 32;
+constexpr int kTile = 32;  // keys of an MFMA, and of the plan's tiles
 constexpr int kRows = 32;  // of a wave
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
@@ -66,14 +67,6 @@ __device__ __forceinline__ int swz_v(int key) {
   return D == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 }
 
-#ifndef VAR
-#define VAR 0
-#endif
-// Workgroups of a CU, by the registers of the query's parts.
-template <typename E>
-constexpr int kResident = VAR == 1 && std::is_same<E, BF16>::value ? 3 : 2;
-template <typename E>
-constexpr bool kOverlap = !std::is_same<E, F32>::value && VAR != 1 && VAR != 2;
 
 // How an element type's queries meet K (parts of the query), and its weights V.
 template <typename E>
@@ -95,6 +88,14 @@ struct Meets<F32> {
   static constexpr int kQueries = 3, kWeights = 3;
 };
 
+// What is known of 16 keys: the factor of their scores, the V scale and its
+// logarithm, whether they are in a block of the pool.
+struct alignas(16) Half {
+  float factor, vs, log_vs;
+  int ok;
+};
+constexpr int kInfo = 256;  // halves looked up, a ring of two parts
+
 __device__ __forceinline__ f32x16_t mma(bf16x8_t a, bf16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
@@ -110,8 +111,12 @@ __device__ __forceinline__ V widen(uint32_t lo, uint32_t hi) {
     return widen_operand_f16<C>(lo, hi);
 }
 
+// Tiles of a step, by the registers of the query's parts.
+template <typename E, int D>
+constexpr int kTiles = std::is_same<E, F32>::value && D == 128 ? 1 : 2;
+
 template <typename E, typename C, int D>
-__global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
+__global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
     const QuantPrefillArgs a) {
   using R = typename E::raw;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
@@ -119,12 +124,16 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
   using Query = typename Meets<E>::Query;
   using Weight = typename Meets<E>::Weight;
   constexpr int kQueries = Meets<E>::kQueries, kWeights = Meets<E>::kWeights;
-  constexpr int kTileElems = kKeys * D;
+  constexpr int NT = kTiles<E, D>;
+  constexpr int kKeys = NT * kTile, kHalves = 2 * NT;
   constexpr int kAccFloats = D / 32 * 16;  // of a lane
-  // A thread's 16 codes: with D = 128 of K and of V, with D = 64 of one of them.
-  constexpr bool kBoth = D == 128;
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][kTileElems];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kTileElems];
+  constexpr int kLoads = kKeys * D / 16 / kThreads;  // of 16 codes a thread, for K and for V
+  constexpr int kSpread = kThreads * 16 / D;         // keys between them
+  static_assert(kLoads * kSpread == kKeys, "every key is loaded");
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][kKeys * D];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[2][kKeys * D];
+  __shared__ int64_t s_at[kInfo];
+  __shared__ Half s_half[kInfo];
   __shared__ int s_arrived;
 
   const QuantCache& c = a.c;
@@ -138,7 +147,6 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
   if (item >= *(const ConstI32*)(a.count)) return;  // surplus (uniform)
   const ConstI32* it = (const ConstI32*)(a.items + item);
   const int req = it[0], rblock = it[1], part = it[4], nparts = it[5], slot = it[6];
-  int t_begin = it[2];
   const int t_limit = it[3], counter = it[7];
   const ConstI32* cu_q = (const ConstI32*)(a.cu_q);
   const ConstI32* cu_k = (const ConstI32*)(a.cu_k);
@@ -149,71 +157,64 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
   const int ctx = cu_k[req + 1] - cu_k[req];
   const int tok0 = rblock * tokens;
   const int tok_last = min(q_len, tok0 + tokens) - 1;
-  // Keys of the block: up to the causal limit of its last token.
+  // Keys of the block: up to the causal limit of its last token; of the item.
   const int kv_end = max(0, min(ctx - q_len + tok_last + 1, a.t_width << c.log2_block));
-  const int ntiles = min((kv_end + kKeys - 1) / kKeys, t_limit);
-  t_begin = min(t_begin, ntiles);
+  const int key0 = min(it[2] * kTile, kv_end);
+  const int key_end = static_cast<int>(min(static_cast<int64_t>(t_limit) * kTile,
+                                           static_cast<int64_t>(kv_end)));
+  const int nsteps = key_end > key0 ? (key_end - key0 + kKeys - 1) / kKeys : 0;
 
   const int r = wave * kRows + col;
   const int token = tok0 + r / G, g = r % G;
   const bool row_ok = r < tokens * G && token < q_len;
   const int qpos = ctx - q_len + token;  // the row sees keys 0 .. qpos
-  // Of the wave's rows: tiles below nint need no mask, from nend on they see
+  // Of the wave's rows: steps below nint need no mask, from nend on they see
   // nothing.
   const int wave_tok0 = tok0 + wave * kRows / G;
   const int wave_tok1 = min(tok_last, tok0 + (wave * kRows + kRows - 1) / G);
   const bool wave_ok = wave * kRows < tokens * G && wave_tok0 < q_len;
-  const int nint = min(kv_end / kKeys, max(ctx - q_len + wave_tok0 + 1, 0) / kKeys);
+  const int nint = (min(key_end, ctx - q_len + wave_tok0 + 1) - key0) / kKeys;
   const int nend =
-      wave_ok ? min((max(ctx - q_len + wave_tok1 + 1, 0) + kKeys - 1) / kKeys, ntiles) : 0;
+      wave_ok ? (min(key_end, ctx - q_len + wave_tok1 + 1) - key0 + kKeys - 1) / kKeys : 0;
 
-  // Staging: this thread's key of a tile, its 16 codes, and where they go.
-  const bool is_v = !kBoth && wave >= 2;
-  const int key = kBoth ? tid / 8 : tid % 128 / 4;
-  const int chunk = 2 * (kBoth ? tid % 8 : tid % 4);  // of 8 codes
-  const int wave_half = kBoth ? wave / 2 : wave % 2;  // of the tile, the wave's
+  // Staging: a thread's first key of a step, its 16 codes, and where they go.
+  const int key = tid * 16 / D;
+  const int chunk = tid % (D / 16) * 2;  // of 8 codes
   const int64_t lane_off = head * c.hs + key % 16 * c.ts + chunk * 8;
   const uint8_t* kc = c.k + lane_off;
   const uint8_t* vc = c.v + lane_off;
-  const float* ks_head = c.ks + head * c.s_hs;
-  const float* vs_head = c.vs + head * c.s_hs;
-  const ConstI32* table = (const ConstI32*)(a.tables + req * a.t_stride);
+  const int32_t* table = a.tables + req * a.t_stride;
+  const float scale_log2 = fabsf(a.scale_log2);
 
-  // What is known of a tile, from its ids (read a step before they are used)
-  // to its scales.
-  struct Ids {
-    int id[2];
+  // Looks up half `h` of the item.
+  auto look_up = [&](int h) {
+    const int pos = key0 + 16 * h;
+    Half x{0x1p-126f, 0.f, 0.f, 0};
+    int64_t at = 0;  // an invalid block reads block 0
+    if (pos < key_end) {
+      const int blk = table[pos >> c.log2_block];
+      if (blk >= 0 && blk < c.num_blocks) {
+        at = blk * c.bs + (pos & (c.block_size - 1)) * c.ts;
+        const int64_t s = blk * c.s_bs + head * c.s_hs;
+        x.factor = c.ks[s] * scale_log2;
+        // Masked scores are -inf, which 0 would make NaN.
+        if (x.factor == 0.f) x.factor = 0x1p-126f;
+        x.vs = c.vs[s];
+        x.log_vs = __builtin_amdgcn_logf(x.vs);
+        x.ok = 1;
+      }
+    }
+    s_at[h % kInfo] = at;
+    s_half[h % kInfo] = x;
   };
-  struct Page {
-    int64_t at;  // byte offset of this wave's half
-    int mask;    // bit h: half h is in a block of the pool
-    float ks[2], vs[2];
-  };
-  auto load_ids = [&](int tile) __attribute__((always_inline)) {
-    const int t0 = min(tile, ntiles - 1) * kKeys;
-    const int e0 = t0 >> c.log2_block;
-    // The second half's entry; past the keys, the first's again.
-    const int e1 = t0 + 16 < kv_end ? (t0 + 16) >> c.log2_block : e0;
-    return Ids{table[e0], table[e1]};
-  };
-  auto load_page = [&](int tile, const Ids& ids) __attribute__((always_inline)) {
-    const bool ok0 = static_cast<uint32_t>(ids.id[0]) < static_cast<uint32_t>(c.num_blocks);
-    const bool ok1 = static_cast<uint32_t>(ids.id[1]) < static_cast<uint32_t>(c.num_blocks);
-    const uint32_t p0 = ok0 ? ids.id[0] : 0, p1 = ok1 ? ids.id[1] : 0;
-    const int t0 = min(tile, ntiles - 1) * kKeys;
-    Page p;
-    p.mask = (ok0 ? 1 : 0) | (ok1 ? 2 : 0);
-    p.at = (wave_half ? p1 : p0) * static_cast<uint64_t>(c.bs) +
-           static_cast<uint32_t>((t0 + 16 * wave_half) & (c.block_size - 1)) *
-               static_cast<uint64_t>(c.ts);
-    p.ks[0] = ((const ConstF32*)ks_head)[p0 * c.s_bs];
-    p.ks[1] = ((const ConstF32*)ks_head)[p1 * c.s_bs];
-    p.vs[0] = ((const ConstF32*)vs_head)[p0 * c.s_bs];
-    p.vs[1] = ((const ConstF32*)vs_head)[p1 * c.s_bs];
-    return p;
-  };
-  auto load16 = [&](const uint8_t* base, const Page& p) __attribute__((always_inline)) {
-    return *reinterpret_cast<const Word4*>(base + p.at);
+  Word4 k_reg[kLoads], v_reg[kLoads];
+  auto load_step = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t at = s_at[(t * kHalves + (key + u * kSpread) / 16) % kInfo];
+      k_reg[u] = *reinterpret_cast<const Word4*>(kc + at);
+      v_reg[u] = *reinterpret_cast<const Word4*>(vc + at);
+    }
   };
   // `first`: which of the two chunks goes first, for the banks.
   auto put = [&](auto lo, auto hi, uint16_t* row, int swz, int first)
@@ -222,24 +223,28 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
     *reinterpret_cast<V*>(row + ((chunk + first) ^ swz) * 8) = first ? hi : lo;
     *reinterpret_cast<V*>(row + ((chunk + 1 - first) ^ swz) * 8) = first ? lo : hi;
   };
-  auto land_k = [&](const Word4& w, int buf) __attribute__((always_inline)) {
-    put(widen<Query, C>(w.w[0], w.w[1]), widen<Query, C>(w.w[2], w.w[3]), s_k[buf] + key * D,
-        swz_k<D>(key), 0);
-  };
-  // Keys that nothing may see may be NaN, which 0 times does not make 0.
-  auto land_v = [&](Word4 w, int tile, const Page& p, int buf) __attribute__((always_inline)) {
-    const bool there = tile * kKeys + key < kv_end && (p.mask >> wave_half & 1);
+  auto land_step = [&](int t, int buf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w.w[i] = there ? w.w[i] : 0;
-    put(widen<Weight, C>(w.w[0], w.w[1]), widen<Weight, C>(w.w[2], w.w[3]), s_v[buf] + key * D,
-        swz_v<D>(key), kBoth ? key & 1 : 0);
+    for (int u = 0; u < kLoads; ++u) {
+      const int k = key + u * kSpread;
+      const Word4& w = k_reg[u];
+      put(widen<Query, C>(w.w[0], w.w[1]), widen<Query, C>(w.w[2], w.w[3]), s_k[buf] + k * D,
+          swz_k<D>(k), 0);
+      // Keys that nothing may see may be NaN, which 0 times does not make 0.
+      const bool there =
+          key0 + t * kKeys + k < key_end && s_half[(t * kHalves + k / 16) % kInfo].ok;
+      Word4 v = v_reg[u];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v.w[i] = there ? v.w[i] : 0;
+      put(widen<Weight, C>(v.w[0], v.w[1]), widen<Weight, C>(v.w[2], v.w[3]), s_v[buf] + k * D,
+          swz_v<D>(k), D == 128 ? k & 1 : 0);
+    }
   };
 
   // Query operand: step s holds dims 16 s + 8 half .. + 7 of the lane's row. A
   // negative softmax scale goes into the query, so that the factors of the
   // scores are positive.
   Query qf[kQueries][D / 16];
-  const float scale_log2 = fabsf(a.scale_log2);
   {
     const R* row = static_cast<const R*>(a.q) + static_cast<int64_t>(q_begin + token) * a.q_ts +
                    static_cast<int64_t>(head * G + g) * a.q_hs;
@@ -280,43 +285,49 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
   // sum of this lane's half of the keys.
   float m = -INFINITY, mo = -INFINITY, l = 0.f;
 
-  // s[i]: key i / 4 * 8 + half * 4 + i % 4 of the row, in half i / 8 of the tile.
-  auto scores = [&](int buf) __attribute__((always_inline)) {
-    f32x16_t s;
+  // s[n][i]: key 32 n + i / 4 * 8 + half * 4 + i % 4 of the row, in half 2 n + i / 8.
+  auto compute = [&](int t, int buf) __attribute__((always_inline)) {
+    Half hf[kHalves];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+    for (int h = 0; h < kHalves; ++h) hf[h] = s_half[(t * kHalves + h) % kInfo];
+    f32x16_t s[NT];
 #pragma unroll
-    for (int x = 0; x < D / 16; ++x) {
-      const Query kf = *reinterpret_cast<const Query*>(
-          s_k[buf] + col * D + ((2 * x + half) ^ swz_k<D>(col)) * 8);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < kQueries; ++n) s = mma(kf, qf[n][x], s);
+      for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int k = 32 * n + col;
+        const Query kf = *reinterpret_cast<const Query*>(
+            s_k[buf] + k * D + ((2 * x + half) ^ swz_k<D>(k)) * 8);
+#pragma unroll
+        for (int q = 0; q < kQueries; ++q) s[n] = mma(kf, qf[q][x], s[n]);
+      }
+    int all = 1;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) all &= hf[h].ok;
+    if (t >= nint || !__builtin_amdgcn_readfirstlane(all)) {
+      const int last = min(qpos, key_end - 1) - key0 - t * kKeys - half * 4;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[n][i] = 32 * n + i / 4 * 8 + i % 4 <= last && hf[2 * n + i / 8].ok ? s[n][i]
+                                                                               : -INFINITY;
     }
-    return s;
-  };
-  auto mask_scores = [&](int tile, const Page& p, f32x16_t& s) __attribute__((always_inline)) {
-    const int last = min(qpos, kv_end - 1) - tile * kKeys - half * 4;
+    // The references move where the step's scores lie too far above them.
+    float smax = -INFINITY, wmax = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      s[i] = i / 4 * 8 + i % 4 <= last && (p.mask >> (i / 8) & 1) ? s[i] : -INFINITY;
-  };
-  // Masked scores are -inf, which 0 would make NaN.
-  auto factor_of = [&](float ks) __attribute__((always_inline)) {
-    const float f = ks * scale_log2;
-    return f == 0.f ? 0x1p-126f : f;
-  };
-  // Moves the references where the tile's scores lie too far above them.
-  auto look = [&](const Page& p, const f32x16_t& s) __attribute__((always_inline)) {
-    float high[2], weigh[2];
+    for (int h = 0; h < kHalves; ++h) {
+      float x = s[h / 2][8 * (h % 2)];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float x = s[8 * h];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[8 * h + i]);
-      high[h] = x * factor_of(p.ks[h]);
-      weigh[h] = high[h] + __builtin_amdgcn_logf(p.vs[h]);
+      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[h / 2][8 * (h % 2) + i]);
+      x *= hf[h].factor;
+      smax = fmaxf(smax, x);
+      wmax = fmaxf(wmax, x + hf[h].log_vs);
     }
-    const float smax = fmaxf(high[0], high[1]), wmax = fmaxf(weigh[0], weigh[1]);
     if (__ballot(smax > m + kRescaleSlack || wmax > mo + kMostWeight) != 0) {
       const float mnew = fmaxf(m, fmaxf(smax, lane_xor32(smax, lane)));
       l *= mnew == -INFINITY ? 1.f : fast_exp2(m - mnew);
@@ -329,41 +340,40 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
         for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
       mo = monew;
     }
-  };
-  auto weigh = [&](const Page& p, const f32x16_t& s, Weight (&pf)[2][kWeights])
-      __attribute__((always_inline)) {
     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float factor = factor_of(p.ks[h]);
-      // A half that is not there has a scale that is not its own.
-      // Without a reference all scales were 0 or NaN so far, and so it stays.
-      const float power = __builtin_amdgcn_logf(p.vs[h]) + (base - mo);
-      float up = fast_exp2(power);
-      up = mo > -INFINITY ? up : p.vs[h];
-      up = p.mask >> h & 1 ? up : 0.f;
-      float weight[8];
+    for (int n = 0; n < NT; ++n) {
+      // V's fragments come while the weights are computed. Slots 0 - 3 of a half's
+      // 8 are keys 16 h + 4 half .. + 3, the others eight keys on.
+      Weight vf[2][D / 32];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float e = fast_exp2(fmaf(s[8 * h + i], factor, -base));
-        l += e;
-        weight[i] = e * up;
-      }
-      split8<kWeights>(weight, pf[h]);
-    }
-  };
-  // Slots 0 - 3 of a half's 8 are keys 16 h + 4 half .. + 3, the others eight
-  // keys on.
-  auto gather = [&](const Weight (&pf)[2][kWeights], int buf) __attribute__((always_inline)) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
+        for (int db = 0; db < D / 32; ++db) {
+          const uint16_t* at = s_v[buf] + v_rd[db] + (32 * n + 16 * h) * D;
+          const short4_t both[2] = {read_tr16(at), read_tr16(at + 8 * D)};
+          vf[h][db] = __builtin_bit_cast(Weight, both);
+        }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint16_t* at = s_v[buf] + v_rd[db] + 16 * h * D;
-        const short4_t both[2] = {read_tr16(at), read_tr16(at + 8 * D)};
-        const Weight vf = __builtin_bit_cast(Weight, both);
+        const Half& x = hf[2 * n + h];
+        // Without a reference all scales were 0 or NaN so far, and so it stays.
+        float up = fast_exp2(x.log_vs + (base - mo));
+        up = mo > -INFINITY ? up : x.vs;
+        up = x.ok ? up : 0.f;
+        float weight[8];
 #pragma unroll
-        for (int n = 0; n < kWeights; ++n) o[db] = mma(vf, pf[h][n], o[db]);
+        for (int i = 0; i < 8; ++i) {
+          const float e = fast_exp2(fmaf(s[n][8 * h + i], x.factor, -base));
+          l += e;
+          weight[i] = e * up;
+        }
+        Weight pf[kWeights];
+        split8<kWeights>(weight, pf);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+          for (int w = 0; w < kWeights; ++w) o[db] = mma(vf[h][db], pf[w], o[db]);
       }
     }
   };
@@ -375,71 +385,21 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
     __builtin_amdgcn_s_barrier();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
   };
-  // Step t: K of t + 2 and V of t + 1 go to LDS, K of t + 3 and V of t + 2 are
-  // loaded, the scores of t + 1 and the rest of t computed. Tiles past the last
-  // are the last once more.
-  if (t_begin < ntiles) {
-    Page p0 = load_page(t_begin, load_ids(t_begin));
-    Page p1 = load_page(t_begin + 1, load_ids(t_begin + 1));
-    Page p2 = load_page(t_begin + 2, load_ids(t_begin + 2));
-    Ids ids = load_ids(t_begin + 3);
-    Word4 k_reg, v_reg;
-    if constexpr (kBoth) {
-      const Word4 k0 = load16(kc, p0), v0 = load16(vc, p0), k1 = load16(kc, p1);
-      k_reg = load16(kc, p2);
-      v_reg = load16(vc, p1);
-      land_k(k0, 0);
-      land_v(v0, t_begin, p0, 0);
-      land_k(k1, 1);
-    } else if (is_v) {
-      const Word4 v0 = load16(vc, p0);
-      v_reg = load16(vc, p1);
-      land_v(v0, t_begin, p0, 0);
-    } else {
-      const Word4 k0 = load16(kc, p0), k1 = load16(kc, p1);
-      k_reg = load16(kc, p2);
-      land_k(k0, 0);
-      land_k(k1, 1);
-    }
+  if (nsteps > 0) {
+    constexpr int kPart = kInfo / 2;
+    if (tid < kInfo) look_up(tid);
+    __syncthreads();
+    load_step(0);
+    land_step(0, 0);
+    if (nsteps > 1) load_step(1);
     sync_lds();
-    f32x16_t s;
-    if (t_begin < nend) s = scores(0);
-    // K's first buffer is written next.
-    sync_lds();
-    for (int t = t_begin; t < ntiles; ++t) {
-      const int even = (t - t_begin) & 1;
-      const Page p3 = load_page(t + 3, ids);
-      ids = load_ids(t + 4);
-      if constexpr (kBoth) {
-        land_k(k_reg, even);
-        land_v(v_reg, t + 1, p1, even ^ 1);
-        k_reg = load16(kc, p3);
-        v_reg = load16(vc, p2);
-      } else if (is_v) {
-        land_v(v_reg, t + 1, p1, even ^ 1);
-        v_reg = load16(vc, p2);
-      } else {
-        land_k(k_reg, even);
-        k_reg = load16(kc, p3);
-      }
-      if (t < nend) {
-        if (t >= nint || p0.mask != 3) mask_scores(t, p0, s);
-        look(p0, s);
-        Weight pf[2][kWeights];
-        if constexpr (kOverlap<E>) {
-          const f32x16_t ahead = scores(even ^ 1);
-          weigh(p0, s, pf);
-          gather(pf, even);
-          s = ahead;
-        } else {
-          weigh(p0, s, pf);
-          gather(pf, even);
-          s = scores(even ^ 1);
-        }
-      }
-      p0 = p1;
-      p1 = p2;
-      p2 = p3;
+    for (int t = 0; t < nsteps; ++t) {
+      // The other buffer was last read before the barrier; so was the part of the
+      // ring before this step's.
+      if (t + 1 < nsteps) land_step(t + 1, (t + 1) & 1);
+      if (t + 2 < nsteps) load_step(t + 2);
+      if (t > 0 && t * kHalves % kPart == 0 && tid < kPart) look_up(t * kHalves + kPart + tid);
+      if (t < nend) compute(t, t & 1);
       sync_lds();
     }
   }
@@ -513,19 +473,198 @@ __global__ __launch_bounds__(kThreads, kResident<E>) void quant_prefill_kernel(
     }
 }
 
+// ---------------------------------------------------------------------------
+// The plan: every (request, row block), cut along its keys into parts of at most
+// `target` tiles, largest first. With equal parts a launch takes as many rounds
+// of resident workgroups as they fill, so 552 of 63 tiles on 512 places take
+// twice as long as 512 of 68: the target is chosen among kCandidates by that,
+// with what a part costs by itself counted as kPartTiles.
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 256;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int kMaxPlanBlocks = 4096;
+constexpr int kMaxPlanReqs = 2048;
+constexpr int kMaxParts = 16;
+constexpr int kMinPartTiles = 8;
+constexpr int kPartTiles = 6;
+constexpr int kCandidates = 16;   // targets of 4/8 .. 19/8 of an even share
+constexpr int kSlots = 1024;      // partial slots (part x KV head)
+constexpr int kResident = 2;      // workgroups of a CU
+constexpr int kBuckets = 2 * kPlanThreads;  // sizes >= 511 share the first
+
+__device__ __forceinline__ int parts_of(int tiles, int target) {
+  return tiles > target ? min(kMaxParts, (tiles + target - 1) / target) : 1;
+}
+
+// Exclusive scan over the workgroup, and the total.
+__device__ __forceinline__ int scan(int v, int* s_wave, int& total) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int incl = wave_inclusive_scan(v, lane);
+  if (lane == kWave - 1) s_wave[wave] = incl;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    before += w < wave ? s_wave[w] : 0;
+    total += s_wave[w];
+  }
+  __syncthreads();
+  return before + incl - v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void quant_prefill_plan_kernel(
+    const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int num_seqs, int tokens,
+    int places, int heads, int max_slots, int max_items, PrefillItem* __restrict__ items,
+    int32_t* __restrict__ count, int32_t* __restrict__ counters, int num_counters) {
+  __shared__ int s_first[kMaxPlanReqs + 1];  // request -> first row block
+  __shared__ int s_tiles[kMaxPlanBlocks];
+  __shared__ int16_t s_req[kMaxPlanBlocks];
+  __shared__ int s_hist[kBuckets];
+  __shared__ int s_wave[kPlanWaves];
+  __shared__ int s_best[kPlanWaves][2];  // estimate, target
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave, wave = tid / kWave;
+  for (int i = tid; i < num_counters; i += kPlanThreads) counters[i] = 0;
+  for (int i = tid; i < kBuckets; i += kPlanThreads) s_hist[i] = 0;
+  // Row blocks, in the order of their requests.
+  const int per = (num_seqs + kPlanThreads - 1) / kPlanThreads;
+  const int r0 = min(num_seqs, tid * per), r1 = min(num_seqs, r0 + per);
+  int run = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int n = (max(cu_q[r + 1] - cu_q[r], 0) + tokens - 1) / tokens;
+    s_first[r] = n;
+    run += n;
+  }
+  int blocks;
+  int first = scan(run, s_wave, blocks);
+  for (int r = r0; r < r1; ++r) {
+    const int n = s_first[r];
+    s_first[r] = first;
+    first += n;
+  }
+  if (tid == 0) s_first[num_seqs] = blocks;
+  __syncthreads();
+  blocks = min(blocks, min(max_items - max_slots, kMaxPlanBlocks));
+  int sum = 0;
+  for (int q = tid; q < blocks; q += kPlanThreads) {
+    int lo = 0, hi = num_seqs - 1;  // the last request whose first block <= q
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (s_first[mid] <= q) lo = mid; else hi = mid - 1;
+    }
+    const int q_len = cu_q[lo + 1] - cu_q[lo];
+    const int64_t ctx = static_cast<int64_t>(cu_k[lo + 1]) - cu_k[lo];
+    const int last = min(q_len, (q - s_first[lo] + 1) * tokens);
+    const int keys = static_cast<int>(max(int64_t(0), min(ctx - q_len + last, int64_t(1) << 30)));
+    s_tiles[q] = (keys + kTile - 1) / kTile;
+    s_req[q] = static_cast<int16_t>(lo);
+    sum += s_tiles[q];
+  }
+  int total;
+  scan(sum, s_wave, total);
+  const int64_t share = (static_cast<int64_t>(total) * heads + places - 1) / places;
+  // Each wave tries every fourth target.
+  int best = INT_MAX, best_target = INT_MAX / 2;
+  for (int j = wave; j < kCandidates; j += kPlanWaves) {
+    const int target = max(kMinPartTiles, static_cast<int>(
+        min<int64_t>((share * (4 + j) + 7) / 8, INT_MAX / 4)));
+    int n = 0, split = 0, longest = 0;
+    for (int q = lane; q < blocks; q += kWave) {
+      const int tiles = s_tiles[q], p = parts_of(tiles, target);
+      n += p;
+      split += p > 1 ? p : 0;
+      longest = max(longest, (tiles + p - 1) / p);
+    }
+    n = wave_sum_int(n);
+    split = wave_sum_int(split);
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) longest = max(longest, __shfl_xor(longest, o, kWave));
+    if (split > max_slots) continue;
+    // Rounds of average parts, and no less than the longest.
+    const int64_t rounds = (static_cast<int64_t>(n) * heads + places - 1) / places;
+    const int64_t mean = (static_cast<int64_t>(total) + max(n, 1) - 1) / max(n, 1);
+    const int64_t estimate =
+        max(rounds * (mean + kPartTiles), static_cast<int64_t>(longest) + kPartTiles);
+    if (estimate < best) {
+      best = static_cast<int>(min<int64_t>(estimate, INT_MAX - 1));
+      best_target = target;
+    }
+  }
+  if (lane == 0) {
+    s_best[wave][0] = best;
+    s_best[wave][1] = best_target;
+  }
+  __syncthreads();
+  int target = s_best[0][1];
+  best = s_best[0][0];
+#pragma unroll
+  for (int w = 1; w < kPlanWaves; ++w)
+    // Of equal ones the larger parts.
+    if (s_best[w][0] < best || (s_best[w][0] == best && s_best[w][1] > target)) {
+      best = s_best[w][0];
+      target = s_best[w][1];
+    }
+  // Part p of n covers tiles [p * tiles / n, (p + 1) * tiles / n).
+  auto bucket_of = [](int size) { return kBuckets - 1 - min(size, kBuckets - 1); };
+  int nsplit = 0, nslots = 0;
+  for (int q = tid; q < blocks; q += kPlanThreads) {
+    const int tiles = s_tiles[q], n = parts_of(tiles, target);
+    for (int p = 0; p < n; ++p)
+      atomicAdd(&s_hist[bucket_of((p + 1) * tiles / n - p * tiles / n)], 1);
+    nsplit += n > 1;
+    nslots += n > 1 ? n : 0;
+  }
+  int all;
+  int unit = scan(nsplit, s_wave, all);
+  int slot = scan(nslots, s_wave, all);
+  const int h0 = s_hist[2 * tid], h1 = s_hist[2 * tid + 1];
+  const int start = scan(h0 + h1, s_wave, all);
+  s_hist[2 * tid] = start;
+  s_hist[2 * tid + 1] = start + h0;
+  if (tid == 0) count[0] = min(all, max_items);
+  __syncthreads();
+  for (int q = tid; q < blocks; q += kPlanThreads) {
+    const int tiles = s_tiles[q], n = parts_of(tiles, target);
+    for (int p = 0; p < n; ++p) {
+      PrefillItem it;
+      it.req = s_req[q];
+      it.qblock = q - s_first[it.req];
+      it.tile_begin = p * tiles / n;
+      it.tile_end = (p + 1) * tiles / n;
+      it.part = p;
+      it.nparts = n;
+      it.slot = n > 1 ? slot : 0;
+      it.counter = n > 1 ? unit : 0;
+      const int pos = atomicAdd(&s_hist[bucket_of(it.tile_end - it.tile_begin)], 1);
+      if (pos < max_items) items[pos] = it;
+    }
+    if (n > 1) {
+      slot += n;
+      ++unit;
+    }
+  }
+}
+
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // Workspace: [count][counters][items][m, l, mo][o].
 struct Layout {
   int64_t counters, items, ml, acc, total;
-  int32_t max_items;
+  int32_t max_items, max_slots, num_counters;
 };
+// max_items 0: too many requests or row blocks.
 Layout layout_of(int32_t num_rows, int32_t num_seqs, int32_t group, int32_t heads, int32_t dim) {
   Layout l{};
-  l.max_items = prefill_items_max(num_rows, num_seqs, kBlockRows / group, heads);
-  const int64_t regions = static_cast<int64_t>(prefill_items_slots(heads)) * heads * kWaves;
+  const int tokens = kBlockRows / group;
+  const int64_t blocks = (static_cast<int64_t>(num_rows) + tokens - 1) / tokens + num_seqs;
+  if (num_seqs > kMaxPlanReqs || blocks > kMaxPlanBlocks) return l;
+  l.max_slots = std::max(2, kSlots / heads);
+  l.max_items = static_cast<int32_t>(blocks) + l.max_slots;
+  l.num_counters = l.max_slots / 2 * heads;
+  const int64_t regions = static_cast<int64_t>(l.max_slots) * heads * kWaves;
   l.counters = 256;
-  l.items = l.counters + round256(int64_t(4) * prefill_counters(heads));
+  l.items = l.counters + round256(int64_t(4) * l.num_counters);
   l.ml = l.items + round256(l.max_items * static_cast<int64_t>(sizeof(PrefillItem)));
   l.acc = l.ml + round256(regions * 4 * kWave * 4);
   l.total = l.acc + regions * (dim / 2) * kWave * 4;
@@ -556,10 +695,11 @@ int32_t launch_quant_prefill_plan(const int32_t* cu_q, const int32_t* cu_k, int3
                                   void* workspace, hipStream_t stream) {
   const Layout l = layout_of(num_rows, num_seqs, group, heads, dim);
   char* ws = static_cast<char*>(workspace);
-  return launch_prefill_items(cu_q, cu_k, num_rows, num_seqs, kBlockRows / group, heads, INT_MAX,
-                              reinterpret_cast<PrefillItem*>(ws + l.items),
-                              reinterpret_cast<int32_t*>(ws),
-                              reinterpret_cast<int32_t*>(ws + l.counters), stream);
+  quant_prefill_plan_kernel<<<1, kPlanThreads, 0, stream>>>(
+      cu_q, cu_k, num_seqs, kBlockRows / group, kResident * device_cus(), heads, l.max_slots,
+      l.max_items, reinterpret_cast<PrefillItem*>(ws + l.items), reinterpret_cast<int32_t*>(ws),
+      reinterpret_cast<int32_t*>(ws + l.counters), l.num_counters);
+  return check_launch("quantized prefill plan");
 }
 
 int32_t launch_quant_prefill_mfma(const QuantAttnArgs& args, int32_t dtype, int32_t code,

@@ -393,14 +393,19 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
     land_step(0, 0);
     if (nsteps > 1) load_step(1);
     sync_lds();
-    for (int t = 0; t < nsteps; ++t) {
+    auto step = [&](int t, auto parity) __attribute__((always_inline)) {
+      constexpr int kBuf = decltype(parity)::value;  // LDS addresses are immediates
       // The other buffer was last read before the barrier; so was the part of the
       // ring before this step's.
-      if (t + 1 < nsteps) land_step(t + 1, (t + 1) & 1);
+      if (t + 1 < nsteps) land_step(t + 1, kBuf ^ 1);
       if (t + 2 < nsteps) load_step(t + 2);
       if (t > 0 && t * kHalves % kPart == 0 && tid < kPart) look_up(t * kHalves + kPart + tid);
-      if (t < nend) compute(t, t & 1);
+      if (t < nend) compute(t, kBuf);
       sync_lds();
+    };
+    for (int t = 0; t < nsteps; t += 2) {
+      step(t, std::integral_constant<int, 0>());
+      if (t + 1 < nsteps) step(t + 1, std::integral_constant<int, 1>());
     }
   }
 

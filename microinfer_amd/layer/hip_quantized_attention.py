@@ -15,8 +15,8 @@ from dataclasses import dataclass, field
 import torch
 
 from microinfer_amd import _lib
-from microinfer_amd.layer.hip_paged_attention import _index32
-from microinfer_amd.worker.hip_quantized_kv import check_quantized_cache, whole_vectors
+from microinfer_amd.worker.hip_quantized_kv import (check_quantized_cache, index32,
+                                                    whole_vectors)
 
 MAX_SEQS = 4096
 _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
@@ -36,6 +36,7 @@ class QuantizedDecodePlan:
     counters: torch.Tensor  # zero, for calls in the place that made the plan
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
     place: tuple
+    bytes: int
     workspace_bytes: int
     _workspaces: dict = field(default_factory=dict, repr=False, compare=False)
 
@@ -74,7 +75,7 @@ def quantized_decode_plan(context_lens: torch.Tensor, *, num_q_heads: int, num_k
     num_seqs, device = context_lens.numel(), context_lens.device
     if num_seqs > MAX_SEQS:
         raise ValueError(f"at most {MAX_SEQS} sequences")
-    context_lens = _index32(context_lens)
+    context_lens = index32(context_lens)
     lib = _lib.load()
     with _lib.on_device(device):
         nbytes = lib.mi_quant_decode_plan_bytes(num_seqs, num_kv_heads)
@@ -88,22 +89,24 @@ def quantized_decode_plan(context_lens: torch.Tensor, *, num_q_heads: int, num_k
         place = _call_place(device)
     return QuantizedDecodePlan(
         buffer, counters, (num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size,
-                           block_table_width), place,
+                           block_table_width), place, nbytes,
         lib.mi_quant_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim))
 
 
-def _check_query(query: torch.Tensor, key_cache: torch.Tensor, what: str) -> None:
-    if query.ndim != 3:
-        raise ValueError(f"query must have shape [{what}, Hq, D]")
+def _check_query(query: torch.Tensor, key_cache: torch.Tensor, device: int, rows: str):
+    """ValueError unless the query fits the cache; its shape and the cache's."""
+    shape, cache = query.shape, key_cache.shape
+    if len(shape) != 3:
+        raise ValueError(f"query must have shape [{rows}, Hq, D]")
     if query.dtype not in _FLOAT_DTYPES:
         raise ValueError("unsupported query dtype")
-    _, num_q_heads, head_dim = query.shape
-    if query.device != key_cache.device:
+    if query.get_device() != device:
         raise ValueError("query and cache must share a device")
-    if key_cache.shape[3] != head_dim:
+    if cache[3] != shape[2]:
         raise ValueError("query and cache head dimensions differ")
-    if num_q_heads == 0 or num_q_heads % key_cache.shape[2]:
+    if shape[1] == 0 or shape[1] % cache[2]:
         raise ValueError("Hq must be divisible by Hkv")
+    return shape, cache
 
 
 def hip_quantized_decode(query: torch.Tensor, key_cache: torch.Tensor,
@@ -121,43 +124,42 @@ def hip_quantized_decode(query: torch.Tensor, key_cache: torch.Tensor,
     own. Sequences of length 0 give zeros, block ids outside the pool are
     masked.
     """
-    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
-                                        "hip_quantized_decode")
-    _check_query(query, key_cache, "requests")
-    num_seqs, num_q_heads, head_dim = query.shape
-    num_blocks, block_size, num_kv_heads, _ = key_cache.shape
-    device = query.device
+    cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
+                                                value_scales, "hip_quantized_decode")
+    ((num_seqs, num_q_heads, head_dim),
+     (num_blocks, block_size, num_kv_heads, _)) = _check_query(query, key_cache, device,
+                                                               "requests")
     if block_tables.ndim != 2 or block_tables.shape[0] != num_seqs:
         raise ValueError("block_tables must have one row per request")
     if context_lens.numel() != num_seqs:
         raise ValueError("context_lens must have one entry per request")
-    _lib.require_device(block_tables, context_lens, what="hip_quantized_decode")
-    if block_tables.device != device or context_lens.device != device:
+    if block_tables.get_device() != device or context_lens.get_device() != device:
+        _lib.require_device(block_tables, context_lens, what="hip_quantized_decode")
         raise ValueError("block_tables and context_lens must be on the query's device")
-    width = block_tables.shape[1]
-    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, query.dtype, block_size, width)
+    width, dtype = block_tables.shape[1], query.dtype
     if plan is None:
         plan = quantized_decode_plan(
             context_lens.reshape(-1), num_q_heads=num_q_heads, num_kv_heads=num_kv_heads,
-            head_dim=head_dim, dtype=query.dtype, block_size=block_size,
-            block_table_width=width)
-    elif not isinstance(plan, QuantizedDecodePlan) or plan.sizes != sizes:
+            head_dim=head_dim, dtype=dtype, block_size=block_size, block_table_width=width)
+    elif not isinstance(plan, QuantizedDecodePlan) or plan.sizes != (
+            num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size, width):
         raise ValueError("plan must come from quantized_decode_plan() for this call's sizes")
-    elif plan.buffer.device != device:
+    elif plan.buffer.get_device() != device:
         raise ValueError("plan must be on the query's device")
-    query, tables = whole_vectors(query), _index32(block_tables)
-    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    query, tables = whole_vectors(query), index32(block_tables)
+    out = query.new_empty((num_seqs, num_q_heads, head_dim))
     if num_seqs == 0:
         return out
-    with _lib.on_device(device):
-        partials, counters = plan.workspace(device)
+    strides = query.stride()
+    with _lib.on_device(query.device):
+        partials, counters = plan.workspace(query.device)
         status = _lib.load().mi_quant_decode(
-            query.data_ptr(), *query.stride()[:2], *cache, tables.data_ptr(), tables.stride(0),
-            width, plan.buffer.data_ptr(), plan.buffer.numel(), out.data_ptr(),
-            num_q_heads * head_dim, head_dim, partials.data_ptr(), partials.numel(),
-            counters.data_ptr(), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
-            num_blocks, float(head_dim ** -0.5 if scale is None else scale),
-            _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(device))
+            query.data_ptr(), strides[0], strides[1], *cache, tables.data_ptr(), width, width,
+            plan.buffer.data_ptr(), plan.bytes, out.data_ptr(), num_q_heads * head_dim, head_dim,
+            partials.data_ptr(), plan.workspace_bytes, counters.data_ptr(), num_seqs,
+            num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+            head_dim ** -0.5 if scale is None else float(scale), _lib.DTYPE_CODES[dtype], code,
+            _lib.stream_handle(query.device))
     _lib.check(status, "mi_quant_decode")
     return out
 
@@ -212,7 +214,7 @@ def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tenso
     nbytes = _lib.load().mi_quant_prefill_workspace_bytes(*sizes)
     if nbytes == 0:
         return None
-    plan = QuantizedPrefillPlan(_index32(cu_seqlens_q), _index32(cu_seqlens_k), sizes, nbytes)
+    plan = QuantizedPrefillPlan(index32(cu_seqlens_q), index32(cu_seqlens_k), sizes, nbytes)
     with _lib.on_device(device):
         plan.workspace(device)
     return plan
@@ -232,12 +234,10 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
     for these lengths and sizes; without it the call makes its own. Rows that
     see nothing give zeros.
     """
-    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
-                                        "hip_quantized_prefill")
-    _check_query(query, key_cache, "tokens")
-    num_tokens, num_q_heads, head_dim = query.shape
-    num_blocks, block_size, num_kv_heads, _ = key_cache.shape
-    device = query.device
+    cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
+                                                value_scales, "hip_quantized_prefill")
+    ((num_tokens, num_q_heads, head_dim),
+     (num_blocks, block_size, num_kv_heads, _)) = _check_query(query, key_cache, device, "tokens")
     if block_tables.ndim != 2:
         raise ValueError("block_tables must have one row per request")
     num_requests, width = block_tables.shape
@@ -246,19 +246,20 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
             raise ValueError(f"{name} must have num_requests + 1 entries")
     if max_seqlen_q <= 0 and num_tokens:
         raise ValueError("max_seqlen_q must be positive")
-    _lib.require_device(cu_seqlens_q, cu_seqlens_k, block_tables, what="hip_quantized_prefill")
-    if any(t.device != device for t in (cu_seqlens_q, cu_seqlens_k, block_tables)):
+    if any(t.get_device() != device for t in (cu_seqlens_q, cu_seqlens_k, block_tables)):
+        _lib.require_device(cu_seqlens_q, cu_seqlens_k, block_tables,
+                            what="hip_quantized_prefill")
         raise ValueError("cu_seqlens and block_tables must be on the query's device")
     sizes = num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim, block_size
     if plan is not None and (not isinstance(plan, QuantizedPrefillPlan) or plan.sizes != sizes):
         raise ValueError("plan must come from quantized_prefill_plan() for this call's sizes")
-    if plan is not None and plan.cu_seqlens_q.device != device:
+    if plan is not None and plan.cu_seqlens_q.get_device() != device:
         raise ValueError("plan must be on the query's device")
     if num_tokens and not num_requests:
         raise ValueError("tokens without requests")
-    query, tables = whole_vectors(query), _index32(block_tables)
-    cu_q, cu_k = _index32(cu_seqlens_q), _index32(cu_seqlens_k)
-    out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    query, tables = whole_vectors(query), index32(block_tables)
+    cu_q, cu_k = index32(cu_seqlens_q), index32(cu_seqlens_k)
+    out = query.new_empty((num_tokens, num_q_heads, head_dim))
     if num_tokens == 0:
         return out
     if plan is None:
@@ -266,15 +267,16 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
             cu_q, cu_k, num_tokens=num_tokens, num_q_heads=num_q_heads,
             num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=query.dtype,
             block_size=block_size, block_table_width=width)
-    with _lib.on_device(device):
+    strides = query.stride()
+    with _lib.on_device(query.device):
         workspace, nbytes = None, 0
         if plan is not None:
-            workspace, nbytes = plan.workspace(device).data_ptr(), plan.workspace_bytes
+            workspace, nbytes = plan.workspace(query.device).data_ptr(), plan.workspace_bytes
         status = _lib.load().mi_quant_prefill(
-            query.data_ptr(), *query.stride()[:2], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
-            tables.data_ptr(), tables.stride(0), width, out.data_ptr(), num_q_heads * head_dim,
-            head_dim, workspace, nbytes, num_tokens, num_requests, num_q_heads, num_kv_heads,
-            head_dim, block_size, num_blocks, float(head_dim ** -0.5 if scale is None else scale),
-            _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(device))
+            query.data_ptr(), strides[0], strides[1], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
+            tables.data_ptr(), width, width, out.data_ptr(), num_q_heads * head_dim, head_dim,
+            workspace, nbytes, num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim,
+            block_size, num_blocks, head_dim ** -0.5 if scale is None else float(scale),
+            _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(query.device))
     _lib.check(status, "mi_quant_prefill")
     return out

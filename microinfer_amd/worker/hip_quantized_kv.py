@@ -32,7 +32,28 @@ _INDEX_DTYPES = (torch.int32, torch.int64)
 
 def check_quantized_cache(key_cache, value_cache, key_scales, value_scales, what: str):
     """ValueError / RuntimeError unless the four are an 8-bit cache on the GPU;
-    the arguments that describe it to the library, and its code."""
+    the arguments that describe it to the library, its code and its device's
+    index. One look at each property: this is most of a small call's time."""
+    shape, strides, dtype = key_cache.shape, key_cache.stride(), key_cache.dtype
+    scale_strides, device = key_scales.stride(), key_cache.get_device()
+    keys, values = key_cache.data_ptr(), value_cache.data_ptr()
+    if (len(shape) != 4 or dtype not in _CODES or value_cache.shape != shape
+            or value_cache.dtype != dtype or value_cache.stride() != strides
+            or strides[3] != 1 or key_scales.shape != (shape[0], shape[2])
+            or value_scales.shape != key_scales.shape or key_scales.dtype != torch.float32
+            or value_scales.dtype != torch.float32 or value_scales.stride() != scale_strides
+            or device < 0 or value_cache.get_device() != device
+            or key_scales.get_device() != device or value_scales.get_device() != device
+            or shape[1] & (shape[1] - 1) or not shape[1]
+            or shape[3] & (shape[3] - 1) or not 16 <= shape[3] <= 256
+            or (keys | values | strides[0] | strides[1] | strides[2]) & 7):
+        _refuse(key_cache, value_cache, key_scales, value_scales, what)
+    return (keys, values, strides[0], strides[1], strides[2], key_scales.data_ptr(),
+            value_scales.data_ptr(), *scale_strides), _CODES[dtype], device
+
+
+def _refuse(key_cache, value_cache, key_scales, value_scales, what: str):
+    """Raises what ``check_quantized_cache`` found."""
     _lib.require_device(key_cache, value_cache, key_scales, value_scales, what=what)
     if key_cache.ndim != 4 or value_cache.shape != key_cache.shape:
         raise ValueError("key/value caches must have matching [blocks, B, Hkv, D] shapes")
@@ -46,19 +67,20 @@ def check_quantized_cache(key_cache, value_cache, key_scales, value_scales, what
         raise ValueError("K/V caches must share one layout")
     if key_cache.stride(-1) != 1:
         raise ValueError("cache head_dim must be contiguous")
-    device = key_cache.device
-    if any(t.device != device for t in (value_cache, key_scales, value_scales)):
+    if any(t.device != key_cache.device for t in (value_cache, key_scales, value_scales)):
         raise ValueError("caches and scales must share a device")
     if block_size <= 0 or block_size & (block_size - 1):
         raise ValueError("paged kernels require a power-of-two block size")
     if head_dim & (head_dim - 1) or not 16 <= head_dim <= 256:
         raise ValueError("8-bit caches need a power-of-two head_dim from 16 to 256")
-    block_stride, token_stride, head_stride, _ = key_cache.stride()
-    pointers = key_cache.data_ptr(), value_cache.data_ptr()
-    if (pointers[0] | pointers[1] | block_stride | token_stride | head_stride) & 7:
-        raise ValueError("8-bit cache rows must be 8-byte aligned")
-    return (*pointers, block_stride, token_stride, head_stride, key_scales.data_ptr(),
-            value_scales.data_ptr(), *key_scales.stride()), _CODES[key_cache.dtype]
+    raise ValueError("8-bit cache rows must be 8-byte aligned")
+
+
+def index32(tensor: torch.Tensor) -> torch.Tensor:
+    """An index tensor as the kernels read it."""
+    if tensor.dtype != torch.int32:
+        tensor = tensor.to(torch.int32)
+    return tensor if tensor.is_contiguous() else tensor.contiguous()
 
 
 def whole_vectors(rows: torch.Tensor) -> torch.Tensor:
@@ -73,7 +95,7 @@ def whole_vectors(rows: torch.Tensor) -> torch.Tensor:
 def _slots(slot_mapping: torch.Tensor) -> torch.Tensor:
     if slot_mapping.ndim != 1 or slot_mapping.dtype not in _INDEX_DTYPES:
         raise ValueError("slots must be a 1-D integer tensor")
-    return slot_mapping.contiguous()
+    return slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
 
 
 @dataclass(frozen=True)
@@ -117,21 +139,23 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
     ``quantized_append_plan`` for these slots; without it a call of more than
     1024 rows makes its own.
     """
-    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
-                                        "quantized_append")
-    _lib.require_device(slot_mapping, keys, values, what="quantized_append")
+    cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
+                                                value_scales, "quantized_append")
     num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
-    if keys.ndim != 3 or values.shape != keys.shape:
+    shape, dtype = keys.shape, keys.dtype
+    if len(shape) != 3 or values.shape != shape:
         raise ValueError("K/V must have matching [tokens, Hkv, D] shapes")
-    if keys.shape[1:] != key_cache.shape[2:]:
+    tokens = shape[0]
+    if shape[1] != num_kv_heads or shape[2] != head_dim:
         raise ValueError("K/V heads must match the cache")
-    if keys.dtype not in _FLOAT_DTYPES or values.dtype != keys.dtype:
+    if dtype not in _FLOAT_DTYPES or values.dtype != dtype:
         raise ValueError("K/V must be float16, bfloat16 or float32, both alike")
-    tokens, device = keys.shape[0], key_cache.device
     slots = _slots(slot_mapping)
     if slots.numel() != tokens:
         raise ValueError("one slot per token is required")
-    if any(t.device != device for t in (slots, keys, values)):
+    if (slots.get_device() != device or keys.get_device() != device
+            or values.get_device() != device):
+        _lib.require_device(slots, keys, values, what="quantized_append")
         raise ValueError("slots and K/V must be on the cache device")
     if block_size > 1024:
         raise ValueError("8-bit caches are written in blocks of at most 1024 tokens")
@@ -143,16 +167,17 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
     elif not isinstance(plan, QuantizedAppendPlan) or plan.sizes != (tokens, block_size,
                                                                      num_blocks):
         raise ValueError("plan must come from quantized_append_plan() for this call's sizes")
-    elif plan.rows.device != device:
+    elif plan.rows.get_device() != device:
         raise ValueError("plan must be on the cache device")
     keys, values = whole_vectors(keys), whole_vectors(values)
-    with _lib.on_device(device):
+    k_strides, v_strides = keys.stride(), values.stride()
+    with _lib.on_device(key_cache.device):
         status = _lib.load().mi_quant_append(
-            keys.data_ptr(), *keys.stride()[:2], values.data_ptr(), *values.stride()[:2], *cache,
-            slots.data_ptr(), int(slots.dtype == torch.int64),
+            keys.data_ptr(), k_strides[0], k_strides[1], values.data_ptr(), v_strides[0],
+            v_strides[1], *cache, slots.data_ptr(), slots.dtype == torch.int64,
             None if plan is None else plan.rows.data_ptr(), tokens, num_kv_heads, head_dim,
-            block_size, num_blocks, _lib.DTYPE_CODES[keys.dtype], code,
-            _lib.stream_handle(device))
+            block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
+            _lib.stream_handle(key_cache.device))
     _lib.check(status, "mi_quant_append")
 
 
@@ -163,33 +188,30 @@ def quantized_gather(key_cache: torch.Tensor, value_cache: torch.Tensor,
     """Each request's first rows as contiguous K/V ``[total_rows, Hkv, D]`` of
     ``dtype``: request r's are rows ``cu_seqlens_k[r] : cu_seqlens_k[r + 1]``.
     Rows of blocks outside the pool or the table are zeros."""
-    cache, code = check_quantized_cache(key_cache, value_cache, key_scales, value_scales,
-                                        "quantized_gather")
-    _lib.require_device(block_tables, cu_seqlens_k, what="quantized_gather")
+    cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
+                                                value_scales, "quantized_gather")
     if dtype not in _FLOAT_DTYPES:
         raise ValueError("rows are read as float16, bfloat16 or float32")
     if block_tables.ndim != 2 or cu_seqlens_k.numel() != block_tables.shape[0] + 1:
         raise ValueError("cu_seqlens_k must have one entry more than block_tables has rows")
-    device = key_cache.device
-    if block_tables.device != device or cu_seqlens_k.device != device:
+    if block_tables.get_device() != device or cu_seqlens_k.get_device() != device:
+        _lib.require_device(block_tables, cu_seqlens_k, what="quantized_gather")
         raise ValueError("block_tables and cu_seqlens_k must be on the cache device")
     if type(total_rows) is not int or total_rows < 0:
         raise ValueError("total_rows must be a nonnegative integer")
     num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
-    shape = (total_rows, num_kv_heads, head_dim)
-    keys = torch.empty(shape, dtype=dtype, device=device)
+    keys = key_cache.new_empty((total_rows, num_kv_heads, head_dim), dtype=dtype)
     values = torch.empty_like(keys)
     if total_rows == 0:
         return keys, values
     if block_tables.shape[0] == 0:
         raise ValueError("rows without requests")
-    tables = block_tables.to(torch.int32).contiguous()
-    offsets = cu_seqlens_k.to(torch.int32).contiguous()
-    with _lib.on_device(device):
+    tables, offsets = index32(block_tables), index32(cu_seqlens_k)
+    requests, width = tables.shape
+    with _lib.on_device(key_cache.device):
         status = _lib.load().mi_quant_gather(
-            *cache, tables.data_ptr(), tables.stride(0), tables.shape[1], offsets.data_ptr(),
-            tables.shape[0], total_rows, keys.data_ptr(), values.data_ptr(), num_kv_heads,
-            head_dim, block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
-            _lib.stream_handle(device))
+            *cache, tables.data_ptr(), width, width, offsets.data_ptr(), requests, total_rows,
+            keys.data_ptr(), values.data_ptr(), num_kv_heads, head_dim, block_size, num_blocks,
+            _lib.DTYPE_CODES[dtype], code, _lib.stream_handle(key_cache.device))
     _lib.check(status, "mi_quant_gather")
     return keys, values

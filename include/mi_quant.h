@@ -51,9 +51,10 @@ extern "C" {
  * becomes NaN, until the block begins anew. Of rows with the same slot one is
  * written, whichever.
  *
- * rows: what mi_quant_append_plan made of these slots (it serves every layer
- * of a step), or NULL, with at most 1024 tokens. block_size at most 1024.
- * keys and values are 16-byte aligned, with strides of whole 16-byte vectors.
+ * plan: what mi_quant_append_plan made of these slots (it serves every layer
+ * of a step), or NULL, with at most 1024 tokens (the faster of the two up to
+ * some hundred). block_size at most 1024. keys and values are 16-byte aligned,
+ * with strides of whole 16-byte vectors.
  */
 int32_t mi_quant_append(const void* keys, int64_t key_token_stride, int64_t key_head_stride,
                         const void* values, int64_t value_token_stride,
@@ -61,19 +62,19 @@ int32_t mi_quant_append(const void* keys, int64_t key_token_stride, int64_t key_
                         int64_t cache_block_stride, int64_t cache_token_stride,
                         int64_t cache_head_stride, float* key_scales, float* value_scales,
                         int64_t scale_block_stride, int64_t scale_head_stride,
-                        const void* slots, int32_t slots_are_int64, const int32_t* rows,
-                        int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
-                        int32_t block_size, int32_t num_blocks, int32_t dtype, int32_t code,
-                        void* stream);
+                        const void* slots, int32_t slots_are_int64, const void* plan,
+                        int64_t plan_bytes, int32_t num_tokens, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t dtype,
+                        int32_t code, void* stream);
 
 /*
- * rows[slot] = a row written at slot, for every slot that is written; the
- * other entries keep what they held (they need no initialisation: a reader
- * checks an entry against the slot list). rows: num_blocks * block_size int32.
+ * The blocks that these slots write to, and their rows, found on the device.
+ * plan: mi_quant_append_plan_bytes() bytes, 8-byte aligned, no initialisation.
  */
+int64_t mi_quant_append_plan_bytes(int32_t num_tokens, int32_t block_size, int32_t num_blocks);
 int32_t mi_quant_append_plan(const void* slots, int32_t slots_are_int64, int32_t num_tokens,
-                             int32_t block_size, int32_t num_blocks, int32_t* rows,
-                             void* stream);
+                             int32_t block_size, int32_t num_blocks, void* plan,
+                             int64_t plan_bytes, void* stream);
 
 /*
  * Read back: output row i (of total_rows) is position i - cu_seqlens_k[r] of

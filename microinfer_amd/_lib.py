@@ -137,11 +137,12 @@ SIGNATURES = {
         [_P, _I64, _I32, _I32, _I32, _P, _P, _I64, _I32, _P, _P, _P, _P, _I32, _P, _I64, _P,
          _P],
     ),
-    "mi_quant_append_plan": (_I32, [_P, _I32, _I32, _I32, _I32, _P, _P]),
+    "mi_quant_append_plan_bytes": (_I64, [_I32, _I32, _I32]),
+    "mi_quant_append_plan": (_I32, [_P, _I32, _I32, _I32, _I32, _P, _I64, _P]),
     "mi_quant_append": (
         _I32,
-        [_P, _I64, _I64, _P, _I64, _I64, *_QUANT_CACHE, _P, _I32, _P, _I32, _I32, _I32, _I32,
-         _I32, _I32, _I32, _P],
+        [_P, _I64, _I64, _P, _I64, _I64, *_QUANT_CACHE, _P, _I32, _P, _I64, _I32, _I32, _I32,
+         _I32, _I32, _I32, _I32, _P],
     ),
     "mi_quant_gather": (
         _I32,

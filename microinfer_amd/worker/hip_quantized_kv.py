@@ -23,7 +23,9 @@ import torch
 from microinfer_amd import _lib
 
 QUANTIZED_DTYPES = (torch.float8_e4m3fn, torch.int8)
-MAX_SCANNED_TOKENS = 1024  # a larger call needs a plan, and makes one itself
+# Calls of so many rows find a block's rows in the slot list themselves; larger
+# ones have them from a plan.
+MAX_SCANNED_TOKENS = 256
 
 _CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
@@ -102,27 +104,33 @@ def _slots(slot_mapping: torch.Tensor) -> torch.Tensor:
 class QuantizedAppendPlan:
     """Where a step's rows go (``quantized_append_plan``), for every layer."""
 
-    rows: torch.Tensor
+    buffer: torch.Tensor | None  # None: few rows, which need no plan
     sizes: tuple  # tokens, block size, blocks
+    bytes: int
 
 
 def quantized_append_plan(slot_mapping: torch.Tensor, *, block_size: int,
                           num_blocks: int) -> QuantizedAppendPlan:
     """The plan of ``quantized_append`` calls with these slots, made on the
     device (capture-safe)."""
-    _lib.require_device(slot_mapping, what="quantized_append_plan")
     slots = _slots(slot_mapping)
+    if not slots.is_cuda:
+        _lib.require_device(slots, what="quantized_append_plan")
     if block_size <= 0 or block_size & (block_size - 1):
         raise ValueError("paged kernels require a power-of-two block size")
     if num_blocks <= 0:
         raise ValueError("num_blocks must be positive")
-    rows = torch.empty(num_blocks * block_size, dtype=torch.int32, device=slots.device)
-    with _lib.on_device(slots.device):
-        status = _lib.load().mi_quant_append_plan(
-            slots.data_ptr(), int(slots.dtype == torch.int64), slots.numel(), block_size,
-            num_blocks, rows.data_ptr(), _lib.stream_handle(slots.device))
+    sizes = slots.numel(), block_size, num_blocks
+    if sizes[0] <= MAX_SCANNED_TOKENS:
+        return QuantizedAppendPlan(None, sizes, 0)
+    lib, device = _lib.load(), slots.device
+    nbytes = lib.mi_quant_append_plan_bytes(*sizes)
+    buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with _lib.on_device(device):
+        status = lib.mi_quant_append_plan(slots.data_ptr(), slots.dtype == torch.int64, *sizes,
+                                          buffer.data_ptr(), nbytes, _lib.stream_handle(device))
     _lib.check(status, "mi_quant_append_plan")
-    return QuantizedAppendPlan(rows, (slots.numel(), block_size, num_blocks))
+    return QuantizedAppendPlan(buffer, sizes, nbytes)
 
 
 def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -136,8 +144,8 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
     block, rows below the lowest offset written stay (rounded again where the
     scale rises); the others stand for something only once they are written.
     Of rows with equal slots one is written, whichever. ``plan``: of
-    ``quantized_append_plan`` for these slots; without it a call of more than
-    1024 rows makes its own.
+    ``quantized_append_plan`` for these slots; without it a call of many rows
+    makes its own.
     """
     cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
                                                 value_scales, "quantized_append")
@@ -162,12 +170,11 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
     if tokens == 0:
         return
     if plan is None:
-        if tokens > MAX_SCANNED_TOKENS:
-            plan = quantized_append_plan(slots, block_size=block_size, num_blocks=num_blocks)
+        plan = quantized_append_plan(slots, block_size=block_size, num_blocks=num_blocks)
     elif not isinstance(plan, QuantizedAppendPlan) or plan.sizes != (tokens, block_size,
                                                                      num_blocks):
         raise ValueError("plan must come from quantized_append_plan() for this call's sizes")
-    elif plan.rows.get_device() != device:
+    elif plan.buffer is not None and plan.buffer.get_device() != device:
         raise ValueError("plan must be on the cache device")
     keys, values = whole_vectors(keys), whole_vectors(values)
     k_strides, v_strides = keys.stride(), values.stride()
@@ -175,8 +182,8 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
         status = _lib.load().mi_quant_append(
             keys.data_ptr(), k_strides[0], k_strides[1], values.data_ptr(), v_strides[0],
             v_strides[1], *cache, slots.data_ptr(), slots.dtype == torch.int64,
-            None if plan is None else plan.rows.data_ptr(), tokens, num_kv_heads, head_dim,
-            block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
+            None if plan.buffer is None else plan.buffer.data_ptr(), plan.bytes, tokens,
+            num_kv_heads, head_dim, block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
             _lib.stream_handle(key_cache.device))
     _lib.check(status, "mi_quant_append")
 

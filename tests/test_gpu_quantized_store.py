@@ -6,8 +6,10 @@ import numpy as np
 import pytest
 import torch
 
-from microinfer_amd.worker.hip_quantized_kv import (quantized_append, quantized_append_plan,
-                                                    quantized_gather)
+from microinfer_amd import _lib
+from microinfer_amd.worker import hip_quantized_kv
+from microinfer_amd.worker.hip_quantized_kv import (QuantizedAppendPlan, quantized_append,
+                                                    quantized_append_plan, quantized_gather)
 from tests.quantized_support import CODES, DTYPES, Twin, ints, tables_of
 from oracle import quantized as oracle
 
@@ -19,14 +21,20 @@ def rows_of(gen, tokens, heads, dim, dtype, size=1.0):
     return [t.to(dtype).cuda() for t in x]
 
 
-def write(twin, slots, keys, values, planned=None, index=torch.int32):
+@pytest.fixture(params=[False, True], ids=["scanned", "planned"])
+def planned(request, monkeypatch):
+    """Small calls find their rows in the list, or have them from a plan."""
+    monkeypatch.setattr(hip_quantized_kv, "MAX_SCANNED_TOKENS", 0 if request.param else 1024)
+    return request.param
+
+
+def write(twin, slots, keys, values, plan=True, index=torch.int32):
     """Through the library and through the twin."""
     where = torch.tensor(slots, dtype=index, device="cuda")
-    plan = None
-    if planned:
-        blocks, block = twin.k.shape[:2]
-        plan = quantized_append_plan(where, block_size=block, num_blocks=blocks)
-    quantized_append(*twin.tensors, where, keys, values, plan=plan)
+    blocks, block = twin.k.shape[:2]
+    quantized_append(*twin.tensors, where, keys, values,
+                     plan=quantized_append_plan(where, block_size=block, num_blocks=blocks)
+                     if plan else None)
     twin.expect(slots, keys, values)
 
 
@@ -35,7 +43,7 @@ def write(twin, slots, keys, values, planned=None, index=torch.int32):
 @pytest.mark.parametrize("heads,dim,block,layout", [
     (8, 128, 16, "paired"), (3, 64, 32, "head_major"), (2, 16, 4, "token_major"),
     (1, 256, 64, "paired"), (5, 32, 1, "token_major"), (2, 128, 256, "paired")])
-def test_blocks_fill_over_several_calls(kind, dtype, heads, dim, block, layout):
+def test_blocks_fill_over_several_calls(kind, dtype, heads, dim, block, layout, planned):
     gen = torch.Generator().manual_seed(heads + dim)
     blocks = 12
     twin = Twin(blocks, block, heads, dim, kind, layout)
@@ -53,7 +61,7 @@ def test_blocks_fill_over_several_calls(kind, dtype, heads, dim, block, layout):
         where = [s for seq, n in enumerate(news)
                  for s in slots(seq, lengths[seq], lengths[seq] + n)]
         keys, values = rows_of(gen, len(where), heads, dim, DTYPES[dtype], size)
-        write(twin, where, keys, values, planned=step % 2,
+        write(twin, where, keys, values, plan=step % 2,
               index=torch.int64 if step == 2 else torch.int32)
         lengths = [length + n for length, n in zip(lengths, news)]
         twin.check()
@@ -61,19 +69,18 @@ def test_blocks_fill_over_several_calls(kind, dtype, heads, dim, block, layout):
 
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
 @pytest.mark.parametrize("tokens", [1, 7, 64, 1024, 1025, 3000])
-def test_any_order_of_slots(kind, tokens):
+def test_any_order_of_slots(kind, tokens, planned):
     """Scanned and planned calls find a block's rows wherever they stand."""
     gen = torch.Generator().manual_seed(tokens)
     rng = np.random.default_rng(tokens)
     blocks, block = max(2 * tokens // 16, 4), 16
-    twins = [Twin(blocks, block, 2, 64, kind) for _ in range(2)]
+    twin = Twin(blocks, block, 2, 64, kind)
     slots = rng.permutation(blocks * block)[:tokens]
     slots[rng.random(tokens) < 0.05] = -1
     slots[rng.random(tokens) < 0.05] = blocks * block + 3
     keys, values = rows_of(gen, tokens, 2, 64, torch.bfloat16)
-    for twin, planned in zip(twins, (False, True)):
-        write(twin, slots.tolist(), keys, values, planned)
-        twin.check()
+    write(twin, slots.tolist(), keys, values, index=torch.int64 if tokens == 64 else torch.int32)
+    twin.check()
 
 
 def test_every_16_bit_value():
@@ -101,7 +108,6 @@ def test_extreme_float32_rows():
 
 
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
-@pytest.mark.parametrize("planned", [False, True])
 def test_values_that_are_not_finite(kind, planned):
     gen = torch.Generator().manual_seed(5)
     twin = Twin(8, 16, 2, 128, kind)
@@ -109,31 +115,27 @@ def test_values_that_are_not_finite(kind, planned):
     keys[3, 1, 7] = float("nan")
     values[18, 0, 0] = float("-inf")
     values[2] = float("inf")
-    write(twin, list(range(30, 50)), keys, values, planned)
+    write(twin, list(range(30, 50)), keys, values)
     twin.check()
     write(twin, [50], keys[:1], values[:1])  # a block that holds NaN
     write(twin, [32], keys[5:6], values[5:6])  # and one that begins anew
     twin.check()
 
 
-def test_rows_with_equal_slots_are_not_mixed():
+def test_rows_with_equal_slots_are_not_mixed(planned):
     gen = torch.Generator().manual_seed(6)
     keys, values = rows_of(gen, 40, 2, 128, torch.float16)
-    slots = [5] * 30 + [6] * 10
-    for planned in (False, True):
-        got = Twin(2, 16, 2, 128, "fp8")
-        where = ints(slots)
-        plan = quantized_append_plan(where, block_size=16, num_blocks=2) if planned else None
-        quantized_append(*got.tensors, where, keys, values, plan=plan)
-        codes = [t.cpu().double().numpy() for t in got.tensors]
-        found = 0
-        for i in range(30):
-            for j in range(30, 40):
-                want = Twin(2, 16, 2, 128, "fp8", device="cpu")
-                want.expect([5, 6], keys[[i, j]], values[[i, j]])
-                found += all(np.array_equal(a, b) for a, b in
-                             zip(codes, (want.k, want.v, want.ks, want.vs)))
-        assert found >= 1
+    got = Twin(2, 16, 2, 128, "fp8")
+    quantized_append(*got.tensors, ints([5] * 30 + [6] * 10), keys, values)
+    codes = [t.cpu().double().numpy() for t in got.tensors]
+    found = 0
+    for i in range(30):
+        for j in range(30, 40):
+            want = Twin(2, 16, 2, 128, "fp8", device="cpu")
+            want.expect([5, 6], keys[[i, j]], values[[i, j]])
+            found += all(np.array_equal(a, b) for a, b in
+                         zip(codes, (want.k, want.v, want.ks, want.vs)))
+    assert found >= 1
 
 
 def test_fused_rows_and_strides():
@@ -167,23 +169,51 @@ def test_checked_and_fast_writes_of_a_cache():
     twin.check()
 
 
-def test_a_plan_with_nothing_of_these_slots_is_safe():
-    """Entries that are not of this call's slots are looked through."""
+def test_what_a_plan_held_before_does_not_matter(monkeypatch):
+    """A plan's memory of an earlier step, and of anything else."""
+    monkeypatch.setattr(hip_quantized_kv, "MAX_SCANNED_TOKENS", 0)
+    gen = torch.Generator().manual_seed(9)
+    rng = np.random.default_rng(0)
+    twin = Twin(6, 16, 2, 64, "int8")
+    keys, values = rows_of(gen, 20, 2, 64, torch.bfloat16)
+    lib = _lib.load()
+    nbytes = lib.mi_quant_append_plan_bytes(20, 16, 6)
+    noise = torch.from_numpy(rng.integers(-9, 30, nbytes // 4).astype(np.int32)).cuda()
+    for begin in (40, 33, 61):
+        where = list(range(begin, begin + 20))
+        slots = ints(where)
+        lib.mi_quant_append_plan(slots.data_ptr(), 0, 20, 16, 6, noise.data_ptr(), nbytes,
+                                 _lib.stream_handle(slots.device))
+        plan = QuantizedAppendPlan(noise.view(torch.uint8), (20, 16, 6), nbytes)
+        quantized_append(*twin.tensors, slots, keys, values, plan=plan)
+        twin.expect(where, keys, values)
+        twin.check()
+
+
+def test_calls_refuse_plans_of_other_sizes():
     gen = torch.Generator().manual_seed(9)
     twin = Twin(6, 16, 2, 64, "int8")
     keys, values = rows_of(gen, 20, 2, 64, torch.bfloat16)
-    where = ints(list(range(40, 60)))
-    plan = quantized_append_plan(where, block_size=16, num_blocks=6)
-    rng = np.random.default_rng(0)
-    noise = torch.from_numpy(rng.integers(-9, 30, 96).astype(np.int32)).cuda()
-    noise[40:60] = plan.rows[40:60]
-    plan.rows.copy_(noise)
-    quantized_append(*twin.tensors, where, keys, values, plan=plan)
-    twin.expect(where.tolist(), keys, values)
+    slots = ints(list(range(20)))
+    for sizes in ((19, 16, 6), (20, 32, 6), (20, 16, 5)):
+        plan = quantized_append_plan(slots[:sizes[0]], block_size=sizes[1], num_blocks=sizes[2])
+        with pytest.raises(ValueError, match="plan"):
+            quantized_append(*twin.tensors, slots, keys, values, plan=plan)
+    with pytest.raises(ValueError, match="one slot"):
+        quantized_append(*twin.tensors, slots[1:], keys, values)
+    with pytest.raises(ValueError, match="alike"):
+        quantized_append(*twin.tensors, slots, keys, values.float())
+    with pytest.raises(ValueError, match="heads"):
+        quantized_append(*twin.tensors, slots, keys[:, :1], values[:, :1])
+    with pytest.raises(ValueError, match="layout"):
+        quantized_append(twin.layer.keys, twin.layer.values.contiguous(), *twin.tensors[2:],
+                         slots, keys, values)
+    with pytest.raises(ValueError, match="scales"):
+        quantized_append(*twin.tensors[:2], *(t.double() for t in twin.tensors[2:]), slots, keys,
+                         values)
     twin.check()
 
 
-@pytest.mark.parametrize("planned", [False, True])
 def test_captured_writes_replay_with_other_rows(planned):
     gen = torch.Generator().manual_seed(10)
     twin = Twin(16, 16, 2, 128, "fp8")
@@ -191,7 +221,7 @@ def test_captured_writes_replay_with_other_rows(planned):
     keys, values = rows_of(gen, 40, 2, 128, torch.bfloat16)
 
     def call():
-        plan = quantized_append_plan(slots, block_size=16, num_blocks=16) if planned else None
+        plan = quantized_append_plan(slots, block_size=16, num_blocks=16)
         quantized_append(*twin.tensors, slots, keys, values, plan=plan)
 
     call()

@@ -72,7 +72,7 @@ def _args(order, over):
 
 def _append(lib, **over):
     order = dict(rows_k=4096, kts=256, khs=128, rows_v=8192, vts=256, vhs=128, **CACHE, slots=4096,
-                 is64=0, rows=None, tokens=3, heads=2, dim=128, block=16, blocks=8, dtype=2,
+                 is64=0, plan=None, plan_bytes=0, tokens=3, heads=2, dim=128, block=16, blocks=8, dtype=2,
                  code=0)
     return lib.mi_quant_append(*_args(order, over), None)
 
@@ -129,10 +129,18 @@ def test_c_append_validates_the_rows():
     assert _append(lib, tokens=1025) == 2 and "plan" in _lib.last_error()
     assert _append(lib, block=2048) == 2
     assert _append(lib, tokens=0, rows_k=None) == 0
-    assert lib.mi_quant_append_plan(4096, 0, 3, 12, 8, 4096, None) == 1
-    assert lib.mi_quant_append_plan(4096, 0, -3, 16, 8, 4096, None) == 1
-    assert lib.mi_quant_append_plan(None, 0, 3, 16, 8, 4096, None) == 1
-    assert lib.mi_quant_append_plan(None, 0, 0, 16, 8, None, None) == 0
+    need = lib.mi_quant_append_plan_bytes(2000, 16, 8)
+    assert need > 8 * 16 * 4 and lib.mi_quant_append_plan_bytes(0, 16, 8) == 0
+    assert _append(lib, tokens=2000, plan=4096, plan_bytes=need - 1) == 3
+    assert _append(lib, tokens=2000, plan=4100, plan_bytes=need) == 3
+
+    def plan(slots=4096, tokens=2000, block=16, blocks=8, buffer=4096, nbytes=need):
+        return lib.mi_quant_append_plan(slots, 0, tokens, block, blocks, buffer, nbytes, None)
+
+    assert plan(block=12) == 1 and plan(tokens=-3) == 1 and plan(blocks=0) == 1
+    assert plan(slots=None) == 1 and plan(buffer=None) == 1
+    assert plan(nbytes=need - 1) == 3 and plan(buffer=4100) == 3
+    assert plan(tokens=0, slots=None, buffer=None) == 0
 
 
 def test_c_gather_validates_its_rows():

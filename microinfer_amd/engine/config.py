@@ -5,8 +5,9 @@ fields of ``EngineConfig`` (microinfer/config/engine.py:6-68) that this
 engine acts on, with the same validation errors. The reference's switches
 for torch.compile and n-gram speculative decoding have no counterpart here:
 decode runs from hipGraphs of the HIP kernels, and speculation is not part
-of the attention path. ``SampleParameter.logprobs`` and
-``EngineConfig.shared_prefix_decode`` have no counterpart in the reference.
+of the attention path. ``SampleParameter.logprobs``,
+``EngineConfig.shared_prefix_decode`` and ``EngineConfig.kv_cache_dtype`` have no
+counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -14,7 +15,10 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass
 
+import torch
 
+# What EngineConfig.kv_cache_dtype may be (None: the model's type).
+KV_CACHE_DTYPES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8}
 MAX_LOGPROBS = 32  # alternatives that mi_token_logprobs gives
 
 
@@ -54,6 +58,10 @@ class EngineConfig:
     # Decode batches whose sequences share enough cache blocks (forks, common
     # prompts) read them together; captures a second graph per bucket.
     shared_prefix_decode: bool = False
+    # "fp8" or "int8": the K/V cache in 8 bits, half of a 16-bit one's memory,
+    # with a scale for each block and KV head. Sequences then read shared blocks
+    # each for itself.
+    kv_cache_dtype: str | None = None
 
     def __post_init__(self):
         for name in ("max_num_seqs", "max_num_batched_tokens", "max_num_prefill_tokens",
@@ -67,3 +75,5 @@ class EngineConfig:
         for name in ("debug_mode", "use_cuda_graph", "mixed_batch", "shared_prefix_decode"):
             if type(getattr(self, name)) is not bool:
                 raise ValueError(f"{name} must be a boolean")
+        if self.kv_cache_dtype is not None and self.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype must be None or one of {tuple(KV_CACHE_DTYPES)}")

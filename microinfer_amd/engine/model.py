@@ -11,7 +11,8 @@ last row on prefill (qwen3.py:57-65).
 
 On this path the per-layer Q/K norm + RoPE + KV append is one HIP launch
 (``mi_qk_norm_rope_append``; in decode steps part of the attention's,
-``mi_paged_decode_qkv``), attention is the HIP paged decode / varlen
+``mi_paged_decode_qkv``; with 8-bit caches the norm and rotation, then the
+quantising append), attention is the HIP paged decode / varlen
 prefill (``paged_attention_meta`` / ``varlen_attention``), and RMSNorm with
 its residual sum and the SwiGLU gate are HIP launches too (``hip_dense``:
 the counterparts of the reference's compiled ``_compiled_add_rms_norm`` /
@@ -172,6 +173,22 @@ class Qwen3Model:
                 plan=metadata.decode_plan(c.num_kv_head, cache.block_size))
             return attn.reshape(tokens, c.num_q_head * c.head_dim)
         direct = metadata.is_prefill and metadata.direct_prefill
+        if cache.quantized:
+            q, k = qk_norm_rope_append(
+                qkv, q_weight=layer.q_norm, k_weight=layer.k_norm, eps=c.norm_eps,
+                cos_table=self.cos, sin_table=self.sin, positions=positions,
+                num_q_heads=c.num_q_head, num_kv_heads=c.num_kv_head, head_dim=c.head_dim,
+                interleaved=c.rope_interleaved, return_k=True)
+            v = qkv[:, (c.num_q_head + c.num_kv_head) * c.head_dim:]
+            v = v.view(tokens, c.num_kv_head, c.head_dim)
+            cache.write_slots(metadata.slot_mapping, k, v, plan=metadata.append_plan(cache.keys))
+            if direct:  # over this step's own rows, before they were quantised
+                attn = varlen_attention(q, k, v.contiguous(), metadata)
+            else:
+                attn = paged_attention_meta(q, cache.keys, cache.values, metadata,
+                                            key_scales=cache.key_scales,
+                                            value_scales=cache.value_scales)
+            return attn.reshape(tokens, c.num_q_head * c.head_dim)
         rotated = qk_norm_rope_append(
             qkv, q_weight=layer.q_norm, k_weight=layer.k_norm, eps=c.norm_eps,
             cos_table=self.cos, sin_table=self.sin, positions=positions,

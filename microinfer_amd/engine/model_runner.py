@@ -11,6 +11,10 @@ The KV pool has one block more than the block manager hands out: the pad
 rows of graph buckets write their K/V there. With ``EngineConfig.debug_mode``
 each step's metadata is validated before launch (``runner.validate_step``).
 
+With ``EngineConfig.kv_cache_dtype`` the pool is in 8 bits: rows are quantised
+as they are appended and attention reads the codes (``hip_quantized_kv``,
+``hip_quantized_attention``).
+
 With ``EngineConfig.shared_prefix_decode`` a decode batch whose sequences
 share enough blocks (forks of a request, common prompts) reads them together
 (``hip_shared_decode``), from a second set of graphs; sequences that ask for
@@ -22,7 +26,7 @@ from __future__ import annotations
 
 import torch
 
-from microinfer_amd.engine.config import EngineConfig
+from microinfer_amd.engine.config import KV_CACHE_DTYPES, EngineConfig
 from microinfer_amd.engine.sequence import TokenLogprob
 from microinfer_amd.layer.hip_logprobs import token_logprobs
 from microinfer_amd.layer.hip_sampler import Sampler, greedy_argmax
@@ -40,17 +44,17 @@ class ModelRunner:
         self.model, self.config = model, config
         self.num_blocks, self.block_size = num_blocks, block_size
         self.kv_cache = KVCache(c.num_hidden_layer, num_blocks + 1, block_size, c.num_kv_head,
-                                c.head_dim, dtype=model.dtype, device=model.device,
-                                layout=layout)
+                                c.head_dim, device=model.device, layout=layout,
+                                dtype=KV_CACHE_DTYPES.get(config.kv_cache_dtype, model.dtype))
         model.bind_caches([self.kv_cache.layer(i) for i in range(c.num_hidden_layer)])
         self.builder = StepMetadataBuilder(block_size, model.device, pad_block_id=num_blocks,
                                            debug_mode=config.debug_mode, num_blocks=num_blocks,
                                            max_pos_embed=c.max_pos_embed,
                                            vocab_size=c.vocab_size)
         self.sampler = Sampler()
-        self.share = config.shared_prefix_decode and supported_shared_decode(
-            c.num_q_head, c.num_kv_head, c.head_dim, model.dtype, block_size,
-            config.max_num_seqs)
+        self.share = (config.shared_prefix_decode and not self.kv_cache.quantized
+                      and supported_shared_decode(c.num_q_head, c.num_kv_head, c.head_dim,
+                                                  model.dtype, block_size, config.max_num_seqs))
         self.graphs = self.shared_graphs = None
         if config.use_cuda_graph:
             buckets = dict(max_num_seqs=config.max_num_seqs, table_width=num_blocks + 1,

@@ -3,7 +3,8 @@
 Mirrors ``CachedAttention`` (microinfer/layer/cached_attention.py:56-101):
 append this step's K/V first (checked or fast), then attend, so attention
 sees the current tokens. The no-prefix prefill runs the same HIP varlen
-kernel on the contiguous K/V instead of FlashAttention or an SDPA loop.
+kernel on the contiguous K/V instead of FlashAttention or an SDPA loop. An 8-bit
+cache quantises what is appended, and is attended over as it then stands.
 """
 
 from __future__ import annotations
@@ -33,10 +34,15 @@ class CachedAttention(nn.Module):
                 raise ValueError("bound cache requires slot_mapping")
             if metadata.validate_cache_write:
                 cache.write_checked(metadata.slot_mapping, k, v)
+            elif cache.quantized:
+                cache.write_slots(metadata.slot_mapping, k, v,
+                                  plan=metadata.append_plan(cache.keys))
             else:
                 cache.write_slots(metadata.slot_mapping, k, v)
         if not direct:
-            return paged_attention_meta(q, cache.keys, cache.values, metadata)
+            return paged_attention_meta(q, cache.keys, cache.values, metadata,
+                                        key_scales=cache.key_scales,
+                                        value_scales=cache.value_scales)
         if q.shape[1] % k.shape[1]:
             raise ValueError("query heads must be divisible by KV heads")
         return varlen_attention(q, k, v, metadata)

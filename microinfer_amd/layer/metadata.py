@@ -49,6 +49,7 @@ class AttentionMetadata:
     _decode_plans: dict = field(default_factory=dict, repr=False)
     _prefill_plans: dict = field(default_factory=dict, repr=False)
     _shared_plans: dict = field(default_factory=dict, repr=False)
+    _append_plans: dict = field(default_factory=dict, repr=False)
 
     @classmethod
     def build(
@@ -163,6 +164,40 @@ class AttentionMetadata:
                 num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=query.dtype,
                 block_size=block_size, block_table_width=width, num_kv_rows=rows, paged=paged)
         return self._prefill_plans[key]
+
+    def append_plan(self, key_cache: torch.Tensor):
+        """Where this step's rows go in 8-bit caches of this size, found once
+        for every layer."""
+        if self.slot_mapping is None:
+            raise ValueError("metadata has no slot_mapping")
+        from microinfer_amd.worker.hip_quantized_kv import quantized_append_plan
+
+        key = key_cache.shape[:2]
+        if key not in self._append_plans:
+            self._append_plans[key] = quantized_append_plan(
+                self.slot_mapping, num_blocks=key[0], block_size=key[1])
+        return self._append_plans[key]
+
+    def quantized_plan(self, query: torch.Tensor, key_cache: torch.Tensor):
+        """Device plan of this step's attention over 8-bit caches, built once
+        and reused by every layer (None where such calls run unplanned)."""
+        if self.block_tables is None:
+            raise ValueError("paged attention needs block_tables")
+        from microinfer_amd.layer.hip_quantized_attention import (quantized_decode_plan,
+                                                                  quantized_prefill_plan)
+
+        num_tokens, num_q_heads, head_dim = query.shape
+        _, block_size, num_kv_heads, _ = key_cache.shape
+        sizes = dict(num_q_heads=num_q_heads, num_kv_heads=num_kv_heads, head_dim=head_dim,
+                     dtype=query.dtype, block_size=block_size,
+                     block_table_width=self.block_tables.shape[1])
+        plans = self._decode_plans if self.is_decode else self._prefill_plans
+        key = ("8-bit", num_tokens, *sizes.values())
+        if key not in plans:
+            plans[key] = (quantized_decode_plan(self.context_lens, **sizes) if self.is_decode else
+                          quantized_prefill_plan(self.cu_seqlens_q, self.cu_seqlens_k,
+                                                 num_tokens=num_tokens, **sizes))
+        return plans[key]
 
     @property
     def cu_q_cpu(self) -> tuple[int, ...]:

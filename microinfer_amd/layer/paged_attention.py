@@ -11,6 +11,10 @@ here every route is a gfx950 kernel and nothing falls back to the CPU:
   so the reference's ``Σctx >= 4 Σq`` choice between in-place and gathered
   prefill, :104-139, disappears)
 
+8-bit caches come with their scales and take ``hip_quantized_decode`` and
+``hip_quantized_prefill`` (``quantized_gather`` for rows); groups of sequences
+read their blocks there each for itself, with the same result.
+
 ``gather_paged_kv`` (also under the reference's name ``_gather_paged_kv``)
 keeps the reference's signature for callers that need contiguous varlen K/V;
 it is one launch instead of two ``index_select`` per request plus ``cat``.
@@ -30,20 +34,25 @@ from microinfer_amd.layer.hip_paged_attention import (
     hip_paged_prefill,
     vector_heads,
 )
+from microinfer_amd.layer.hip_quantized_attention import (hip_quantized_decode,
+                                                          hip_quantized_prefill)
 from microinfer_amd.layer.hip_shared_decode import hip_shared_decode
 from microinfer_amd.layer.metadata import AttentionMetadata
+from microinfer_amd.worker.hip_quantized_kv import QUANTIZED_DTYPES, quantized_gather
 
 
 _INT32_MAX = 2 ** 31 - 1
 
 
-def gather_paged_kv(key_cache, value_cache, block_tables, contexts, block_size):
+def gather_paged_kv(key_cache, value_cache, block_tables, contexts, block_size, *,
+                    key_scales=None, value_scales=None, dtype=torch.bfloat16):
     """Materialise each request's first ``contexts[r]`` rows as varlen K/V.
 
     Same arguments as ``_gather_paged_kv`` (paged_attention.py:76): host-side
     ``contexts``; returns ``(keys, values)`` of shape ``[sum(contexts), Hkv, D]``.
     Not under graph capture, which would fix the lengths: ``hip_gather_kv``
-    takes them from the device.
+    takes them from the device. Rows of 8-bit caches, given with their scales,
+    come as ``dtype``.
     """
     if block_size != key_cache.shape[1]:
         raise ValueError("block_size does not match the cache")
@@ -59,6 +68,12 @@ def gather_paged_kv(key_cache, value_cache, block_tables, contexts, block_size):
     if key_cache.is_cuda and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("gather_paged_kv takes its lengths from the host: not under capture")
     tables = block_tables[: len(contexts)]
+    if key_cache.dtype in QUANTIZED_DTYPES:
+        if key_scales is None or value_scales is None:
+            raise ValueError("8-bit caches need their scales")
+        cu_k = torch.tensor(offsets, dtype=torch.int32, device=key_cache.device)
+        return quantized_gather(key_cache, value_cache, key_scales, value_scales, tables, cu_k,
+                                offsets[-1], dtype=dtype)
     if (len(contexts) == tables.shape[0] <= GATHER_HOST_REQUESTS
             and offsets[-1] <= _INT32_MAX):
         return hip_gather_kv_host(key_cache, value_cache, tables, offsets)
@@ -77,8 +92,11 @@ def paged_attention_meta(
     metadata: AttentionMetadata,
     *,
     scale: float | None = None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """Kernel dispatch for validated metadata; no host validation or tolist."""
+    """Kernel dispatch for validated metadata; no host validation or tolist.
+    ``key_scales`` / ``value_scales``: those of 8-bit caches."""
     if query.shape[0] == 0:
         return torch.empty_like(query)
     if scale is None:
@@ -90,6 +108,9 @@ def paged_attention_meta(
         )
     if metadata.block_tables is None:
         raise RuntimeError("paged attention requires block_tables")
+    if key_cache.dtype in QUANTIZED_DTYPES:
+        return _quantized_attention(query, key_cache, value_cache, key_scales, value_scales,
+                                    metadata, scale)
 
     if metadata.is_decode:
         if metadata.context_lens is None:
@@ -129,6 +150,28 @@ def paged_attention_meta(
         scale=scale,
         plan=metadata.prefill_plan(query, key_cache),
     )
+
+
+def _quantized_attention(query, key_cache, value_cache, key_scales, value_scales, metadata,
+                         scale):
+    """``paged_attention_meta`` over 8-bit caches."""
+    if key_scales is None or value_scales is None:
+        raise ValueError("8-bit caches need their scales")
+    cache = key_cache, value_cache, key_scales, value_scales
+    if metadata.is_decode:
+        if metadata.context_lens is None:
+            raise RuntimeError("decode metadata requires context_lens")
+        plan = metadata.quantized_plan(query, key_cache)
+        return hip_quantized_decode(query, *cache, metadata.block_tables, metadata.context_lens,
+                                    scale=scale, plan=plan)
+    if metadata.cu_seqlens_q is None or metadata.cu_seqlens_k is None:
+        raise RuntimeError("prefill metadata requires cu_seqlens_q and cu_seqlens_k")
+    max_q = metadata.max_seqlen_q
+    if max_q <= 0:
+        max_q = max(metadata.q_lens_cpu, default=0)
+    return hip_quantized_prefill(query, *cache, metadata.cu_seqlens_q, metadata.cu_seqlens_k,
+                                 metadata.block_tables, max_seqlen_q=max_q, scale=scale,
+                                 plan=metadata.quantized_plan(query, key_cache))
 
 
 def varlen_attention(query, keys, values, metadata: AttentionMetadata, *, scale=None):

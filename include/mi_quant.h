@@ -132,21 +132,25 @@ int32_t mi_quant_decode(const void* query, int64_t q_token_stride, int64_t q_hea
  * Varlen attention: mi_paged_prefill over an 8-bit cache. Request r's query
  * rows are cu_seqlens_q[r] .. cu_seqlens_q[r + 1], its context
  * cu_seqlens_k[r + 1] - cu_seqlens_k[r] positions, the mask causal and
- * bottom-right aligned. Rows that see no position give zeros.
+ * bottom-right aligned. Rows that see no position give zeros. max_seqlen_q
+ * bounds the query rows of any request: rows past it may stay unwritten.
  *
  * Where mi_quant_prefill_workspace_bytes() is not 0, calls of these sizes take
  * a workspace of so many bytes (256-byte aligned) in which
  * mi_quant_prefill_plan has laid out the step, on the device, from the
- * cu_seqlens; the plan serves all layers, one call after the other. Calls that
- * may run concurrently need workspaces of their own.
+ * cu_seqlens, for the same sizes, max_seqlen_q and table width; the plan serves
+ * all layers, one call after the other. Calls that may run concurrently need
+ * workspaces of their own.
  */
 int64_t mi_quant_prefill_workspace_bytes(int32_t num_tokens, int32_t num_requests,
-                                         int32_t num_q_heads, int32_t num_kv_heads,
-                                         int32_t head_dim, int32_t block_size);
+                                         int32_t max_seqlen_q, int32_t num_q_heads,
+                                         int32_t num_kv_heads, int32_t head_dim,
+                                         int32_t block_size);
 int32_t mi_quant_prefill_plan(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                              int32_t num_tokens, int32_t num_requests, int32_t num_q_heads,
-                              int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-                              void* workspace, int64_t workspace_bytes, void* stream);
+                              int32_t num_tokens, int32_t num_requests, int32_t max_seqlen_q,
+                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                              int32_t block_size, int32_t block_table_width, void* workspace,
+                              int64_t workspace_bytes, void* stream);
 int32_t mi_quant_prefill(const void* query, int64_t q_token_stride, int64_t q_head_stride,
                          const void* key_cache, const void* value_cache,
                          int64_t cache_block_stride, int64_t cache_token_stride,
@@ -157,9 +161,9 @@ int32_t mi_quant_prefill(const void* query, int64_t q_token_stride, int64_t q_he
                          int64_t block_table_stride, int32_t block_table_width, void* out,
                          int64_t out_token_stride, int64_t out_head_stride, void* workspace,
                          int64_t workspace_bytes, int32_t num_tokens, int32_t num_requests,
-                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                         int32_t block_size, int32_t num_blocks, float scale, int32_t dtype,
-                         int32_t code, void* stream);
+                         int32_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t block_size, int32_t num_blocks, float scale,
+                         int32_t dtype, int32_t code, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -158,13 +158,12 @@ SIGNATURES = {
         [_P, _I64, _I64, *_QUANT_CACHE, _P, _I64, _I32, _P, _I64, _P, _I64, _I64, _P, _I64, _P,
          _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
     ),
-    "mi_quant_prefill_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32, _I32]),
-    "mi_quant_prefill_plan": (
-        _I32, [_P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P]),
+    "mi_quant_prefill_workspace_bytes": (_I64, [_I32] * 7),
+    "mi_quant_prefill_plan": (_I32, [_P, _P, *[_I32] * 8, _P, _I64, _P]),
     "mi_quant_prefill": (
         _I32,
         [_P, _I64, _I64, *_QUANT_CACHE, _P, _P, _P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I32,
-         _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
+         _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
     ),
 }
 

@@ -108,11 +108,15 @@ struct QuantAttnArgs {
   const int32_t* cu_k;
   void* out;
   int64_t o_ts, o_hs;
-  float* ws_acc;  // partials: [items, Hkv, G, D] unnormalised sums
-  float* ws_ml;   // [items, Hkv, G, 2]: log2-domain maximum, sum
-  int32_t* counters;     // [num_seqs, Hkv], zero on entry and exit
+  float* ws_acc;  // partials: [items, Hkv, rows, D] unnormalised sums
+  float* ws_ml;   // [items, Hkv, rows, 2]: log2-domain maximum, sum
+  int32_t* counters;  // [num_seqs, row groups, Hkv], zero on entry and exit
   const PlanItem* plan;  // decode: [max_items]
   int32_t num_seqs, num_rows, group, max_items;
+  // MFMA kernel of few rows: at most so many of a sequence's at a KV head, in
+  // so many groups.
+  int32_t head_rows, row_groups;
+  uint32_t group_inverse;  // 2^24 / group, rounded up
   float scale_log2;
 };
 

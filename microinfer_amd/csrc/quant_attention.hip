@@ -1,5 +1,6 @@
 // C entry points of attention over an 8-bit K/V cache.
-#include <cmath>
+#include <algorithm>
+#include <climits>
 
 #include "quant_mfma.h"
 
@@ -23,13 +24,70 @@ int32_t check_table(const std::string& fn, const int32_t* tables, int32_t width,
   return MI_OK;
 }
 
-int32_t check_prefill_workspace(const std::string& fn, int32_t num_tokens, int32_t num_requests,
-                                int32_t group, int32_t num_kv_heads, int32_t head_dim,
-                                int32_t block_size, const void* workspace, int64_t bytes) {
-  const int64_t need = quant_prefill_workspace(num_tokens, num_requests, group, num_kv_heads,
-                                               head_dim, block_size);
-  if (workspace == nullptr || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
-    return fail(MI_ERR_WORKSPACE, fn + ": workspace needs " + std::to_string(need) +
+// Whether decode steps go to the MFMA kernel, cache alignment aside.
+bool decode_on_mfma(int32_t head_dim, int32_t group, int32_t block_size) {
+  return quant_decode_mfma_takes(head_dim, block_size) && quant_decode_row_groups(group) == 1;
+}
+
+// Varlen calls of at most kFewRows rows of a request at a KV head, or kFewInAll of
+// all requests, are laid out and run like decode steps. Four layers of 32 query
+// and 8 KV heads of 128, us like that / as longer ones: a token on 16000
+// positions (one query head a KV head) 72 / 248, 8 tokens 122 / 249, 16 on 8000
+// 108 / 200, 32 on 8000 159 / 202, 64 on 8000 260 / 212; 16 requests of 4 tokens
+// on 4000 155 / 200, 32 of 8 on 2000 160 / 193, 64 of 4 234 / 277, 64 of 8 295 /
+// 279, 8 of 16 on 4000 199 / 183, 32 of 16 on 2000 255 / 221.
+constexpr int32_t kFewRows = 32;
+constexpr int32_t kFewInAll = 128;
+
+// A varlen call's sizes and where its workspace holds what.
+struct VarlenLayout {
+  bool few;
+  int32_t rows;  // few: of a request at a KV head, at most
+  int32_t items;
+  int64_t num_counters;
+  int64_t lens, counters, plan, acc, ml;  // few: offsets
+  int64_t total;  // 0: these sizes take no plan
+};
+
+VarlenLayout varlen_layout(int32_t num_tokens, int32_t num_requests, int32_t max_seqlen_q,
+                           int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                           int32_t block_size) {
+  VarlenLayout l{};
+  if (num_tokens <= 0 || num_requests <= 0 || max_seqlen_q <= 0 || num_kv_heads <= 0 ||
+      num_q_heads <= 0 || num_q_heads % num_kv_heads != 0)
+    return l;
+  const int32_t group = num_q_heads / num_kv_heads;
+  const int64_t rows = static_cast<int64_t>(std::min(max_seqlen_q, num_tokens)) * group;
+  l.few = (rows <= kFewRows || rows * num_requests <= kFewInAll) &&
+          num_requests <= kMaxPlanSeqs && quant_decode_mfma_takes(head_dim, block_size);
+  if (!l.few) {
+    l.total = quant_prefill_workspace(num_tokens, num_requests, group, num_kv_heads, head_dim,
+                                      block_size);
+    return l;
+  }
+  l.rows = static_cast<int32_t>(rows);
+  l.items = decode_max_items(num_requests, num_kv_heads, 0);
+  l.num_counters =
+      static_cast<int64_t>(num_requests) * num_kv_heads * quant_decode_row_groups(l.rows);
+  if (l.num_counters > INT_MAX) return l;
+  auto room = [&](int64_t bytes) {
+    const int64_t at = l.total;
+    l.total += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const int64_t slots = static_cast<int64_t>(l.items) * num_kv_heads * rows;
+  l.lens = room(num_requests * int64_t(4));
+  l.counters = room(l.num_counters * 4);
+  l.plan = room(decode_plan_bytes(num_requests, num_kv_heads, 0));
+  l.acc = room(slots * head_dim * 4);
+  l.ml = room(slots * 2 * 4);
+  return l;
+}
+
+int32_t check_varlen_workspace(const std::string& fn, const VarlenLayout& l,
+                               const void* workspace, int64_t bytes) {
+  if (workspace == nullptr || bytes < l.total || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
+    return fail(MI_ERR_WORKSPACE, fn + ": workspace needs " + std::to_string(l.total) +
                                       " bytes, 256-byte aligned");
   return MI_OK;
 }
@@ -76,8 +134,7 @@ extern "C" int32_t mi_quant_decode_plan(const int32_t* context_lens, int32_t num
     return fail(MI_ERR_WORKSPACE, fn + ": plan buffer too small or misaligned");
   return launch_decode_plan(context_lens, num_seqs, num_kv_heads, block_size, block_table_width,
                             0,
-                            !quant_decode_mfma_takes(head_dim, num_q_heads / num_kv_heads,
-                                                     block_size),
+                            !decode_on_mfma(head_dim, num_q_heads / num_kv_heads, block_size),
                             static_cast<PlanItem*>(plan), counters,
                             static_cast<hipStream_t>(stream));
 }
@@ -141,41 +198,57 @@ extern "C" int32_t mi_quant_decode(
   a.group = num_q_heads / num_kv_heads;
   a.scale_log2 = scale * kLog2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (quant_decode_mfma_supported(a)) return launch_quant_decode_mfma(a, dtype, code, s);
+  if (decode_on_mfma(head_dim, a.group, block_size) && quant_mfma_aligned(a.c))
+    return launch_quant_decode_mfma(a, a.group, dtype, code, s);
   return launch_quant_vector(a, dtype, code, s);
 }
 
 extern "C" int64_t mi_quant_prefill_workspace_bytes(int32_t num_tokens, int32_t num_requests,
-                                                    int32_t num_q_heads, int32_t num_kv_heads,
-                                                    int32_t head_dim, int32_t block_size) {
-  if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return 0;
-  return mi::quant_prefill_workspace(num_tokens, num_requests, num_q_heads / num_kv_heads,
-                                     num_kv_heads, head_dim, block_size);
+                                                    int32_t max_seqlen_q, int32_t num_q_heads,
+                                                    int32_t num_kv_heads, int32_t head_dim,
+                                                    int32_t block_size) {
+  return mi::varlen_layout(num_tokens, num_requests, max_seqlen_q, num_q_heads, num_kv_heads,
+                           head_dim, block_size).total;
 }
 
 extern "C" int32_t mi_quant_prefill_plan(const int32_t* cu_seqlens_q,
                                          const int32_t* cu_seqlens_k, int32_t num_tokens,
-                                         int32_t num_requests, int32_t num_q_heads,
-                                         int32_t num_kv_heads, int32_t head_dim,
-                                         int32_t block_size, void* workspace,
+                                         int32_t num_requests, int32_t max_seqlen_q,
+                                         int32_t num_q_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, int32_t block_size,
+                                         int32_t block_table_width, void* workspace,
                                          int64_t workspace_bytes, void* stream) {
   using namespace mi;
   clear_error();
   const std::string fn = "mi_quant_prefill_plan";
   int32_t st = check_heads(fn, num_q_heads, num_kv_heads);
   if (st != MI_OK) return st;
-  const int32_t group = num_q_heads / num_kv_heads;
-  if (quant_prefill_workspace(num_tokens, num_requests, group, num_kv_heads, head_dim,
-                              block_size) == 0)
-    return fail(MI_ERR_UNSUPPORTED, fn + ": these sizes take no plan");
+  const VarlenLayout l = varlen_layout(num_tokens, num_requests, max_seqlen_q, num_q_heads,
+                                       num_kv_heads, head_dim, block_size);
+  if (l.total == 0) return fail(MI_ERR_UNSUPPORTED, fn + ": these sizes take no plan");
+  if (!is_pow2(block_size))
+    return fail(MI_ERR_INVALID_ARGUMENT, fn + ": block_size must be a power of two");
+  if (block_table_width < 0)
+    return fail(MI_ERR_INVALID_ARGUMENT, fn + ": negative table width");
+  if (static_cast<int64_t>(block_table_width) * block_size > (int64_t(1) << 30))
+    return fail(MI_ERR_UNSUPPORTED, fn + ": tables of more than 2^30 positions");
   if (!cu_seqlens_q || !cu_seqlens_k)
     return fail(MI_ERR_INVALID_ARGUMENT, fn + ": null pointer");
-  st = check_prefill_workspace(fn, num_tokens, num_requests, group, num_kv_heads, head_dim,
-                               block_size, workspace, workspace_bytes);
+  st = check_varlen_workspace(fn, l, workspace, workspace_bytes);
   if (st != MI_OK) return st;
-  return launch_quant_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_tokens, num_requests, group,
-                                   num_kv_heads, head_dim, workspace,
-                                   static_cast<hipStream_t>(stream));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!l.few)
+    return launch_quant_prefill_plan(cu_seqlens_q, cu_seqlens_k, num_tokens, num_requests,
+                                     num_q_heads / num_kv_heads, num_kv_heads, head_dim,
+                                     workspace, s);
+  char* ws = static_cast<char*>(workspace);
+  int32_t* lens = reinterpret_cast<int32_t*>(ws + l.lens);
+  st = launch_few_rows(cu_seqlens_q, cu_seqlens_k, num_requests, lens,
+                       reinterpret_cast<int32_t*>(ws + l.counters),
+                       static_cast<int32_t>(l.num_counters), s);
+  if (st != MI_OK) return st;
+  return launch_decode_plan(lens, num_requests, num_kv_heads, block_size, block_table_width, 0,
+                            false, reinterpret_cast<PlanItem*>(ws + l.plan), nullptr, s);
 }
 
 extern "C" int32_t mi_quant_prefill(
@@ -186,8 +259,9 @@ extern "C" int32_t mi_quant_prefill(
     const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t block_table_stride,
     int32_t block_table_width, void* out, int64_t out_token_stride, int64_t out_head_stride,
     void* workspace, int64_t workspace_bytes, int32_t num_tokens, int32_t num_requests,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-    int32_t num_blocks, float scale, int32_t dtype, int32_t code, void* stream) {
+    int32_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int32_t num_blocks, float scale, int32_t dtype, int32_t code,
+    void* stream) {
   using namespace mi;
   clear_error();
   const std::string fn = "mi_quant_prefill";
@@ -202,6 +276,8 @@ extern "C" int32_t mi_quant_prefill(
     return fail(MI_ERR_INVALID_ARGUMENT, fn + ": negative sizes");
   if (num_tokens == 0) return MI_OK;
   if (num_requests == 0) return fail(MI_ERR_INVALID_ARGUMENT, fn + ": tokens without requests");
+  if (max_seqlen_q <= 0)
+    return fail(MI_ERR_INVALID_ARGUMENT, fn + ": max_seqlen_q must be positive");
   if (!query || !out || !cu_seqlens_q || !cu_seqlens_k)
     return fail(MI_ERR_INVALID_ARGUMENT, fn + ": null pointer");
   if (!whole_vectors(query, q_token_stride, q_head_stride, dtype) ||
@@ -227,9 +303,17 @@ extern "C" int32_t mi_quant_prefill(
   a.group = num_q_heads / num_kv_heads;
   a.scale_log2 = scale * kLog2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!quant_prefill_mfma_supported(a)) return launch_quant_vector(a, dtype, code, s);
-  st = check_prefill_workspace(fn, num_tokens, num_requests, a.group, num_kv_heads, head_dim,
-                               block_size, workspace, workspace_bytes);
+  const VarlenLayout l = varlen_layout(num_tokens, num_requests, max_seqlen_q, num_q_heads,
+                                       num_kv_heads, head_dim, block_size);
+  if (l.total == 0 || !quant_mfma_aligned(a.c)) return launch_quant_vector(a, dtype, code, s);
+  st = check_varlen_workspace(fn, l, workspace, workspace_bytes);
   if (st != MI_OK) return st;
-  return launch_quant_prefill_mfma(a, dtype, code, workspace, s);
+  if (!l.few) return launch_quant_prefill_mfma(a, dtype, code, workspace, s);
+  char* ws = static_cast<char*>(workspace);
+  a.max_items = l.items;
+  a.plan = reinterpret_cast<const PlanItem*>(ws + l.plan);
+  a.counters = reinterpret_cast<int32_t*>(ws + l.counters);
+  a.ws_acc = reinterpret_cast<float*>(ws + l.acc);
+  a.ws_ml = reinterpret_cast<float*>(ws + l.ml);
+  return launch_quant_decode_mfma(a, l.rows, dtype, code, s);
 }

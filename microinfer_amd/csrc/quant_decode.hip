@@ -1,22 +1,24 @@
-// Decode attention over an 8-bit K/V cache on MFMA: head_dim 64 or 128, up to
-// 16 query heads per KV head, blocks of at least 16, queries of any type.
+// Attention of few query rows over an 8-bit K/V cache on MFMA: decode steps, and
+// requests of a few tokens (drafts to verify, ends of prompts). head_dim 64 or
+// 128, blocks of at least 16, queries of any type.
 //
 // out = softmax(scale * q . (k * ks)) (v * vs), with one ks and vs for each
 // block and KV head. Bound by HBM for long contexts (two bytes a position and
 // dim), by latency for few short ones.
 //
-//  * Workgroup = plan item (sequence, block range) x KV head, all its query
-//    heads, so a cache row is read once. Its waves take tiles of 32 positions
-//    in turn: two halves of 16, each in one block.
+//  * A sequence's rows at a KV head are its tokens times the group's query heads.
+//    Workgroup = plan item (sequence, block range) x KV head x up to 16 NC of
+//    them, so a cache row is read once for those. Its waves take tiles of 32
+//    positions in turn: two halves of 16, each in one block.
 //  * Tiles come into a ring of LDS slots of the wave's own by direct loads
 //    (waited for by count, so a slot per wave stays in flight), the four scales
 //    of a tile with them.
-//  * Scores S^T[pos][head] = K . Q^T on v_mfma_f32_16x16x32_bf16, a half at a
+//  * Scores S^T[pos][row] = K . Q^T on v_mfma_f32_16x16x32_bf16, a half at a
 //    time; codes are widened to bf16 on their way from LDS, which loses nothing,
 //    and a query comes in as many bf16 parts as hold all of its bits (1 for
 //    bf16, 2 for f16, 3 for f32). The K scale meets the score in float32.
 //  * The lanes that hold a tile's scores hold the weights that
-//    O^T[dim][head] += V^T . P^T wants from them, with V's bytes transposed on
+//    O^T[dim][row] += V^T . P^T wants from them, with V's bytes transposed on
 //    their way out of LDS (ds_read_b64_tr_b8). A weight times the V scale goes
 //    in as two bf16 parts (three for f32 queries), so that it loses less than
 //    the output's rounding: in bf16, whose range is float32's, however far
@@ -24,6 +26,9 @@
 //  * Online softmax in the log2 domain; the reference moves only when a score
 //    exceeds it by more than 15.
 //  * Waves are joined through LDS, partitions by their last arrival, in order.
+#include <algorithm>
+#include <climits>
+
 #include "quant_mfma.h"
 
 namespace mi {
@@ -31,20 +36,15 @@ namespace {
 
 constexpr int kHalf = 16;   // positions of a half: one block's
 constexpr int kTile = 32;   // positions of a tile
-constexpr int kHeads = 16;  // MFMA columns
+constexpr int kCols = 16;   // MFMA columns: query rows
 constexpr float kRescaleSlack = 15.f;
 
-// One step of the running merge of partitions, in the log2 domain; an empty
-// partition (mb = -inf) weighs nothing.
-__device__ __forceinline__ void merge_step(float& mx, float& ls, float& os, float mb, float lb,
-                                           float ob) {
-  if (mb == -INFINITY) return;
-  const float mnew = fmaxf(mx, mb);
-  const float fo = mx == -INFINITY ? 0.f : fast_exp2(mx - mnew);
-  const float fb = fast_exp2(mb - mnew);
-  ls = fmaf(ls, fo, lb * fb);
-  os = fmaf(os, fo, ob * fb);
-  mx = mnew;
+// Maximum over aligned groups of 16 lanes.
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  return fmaxf(v, dpp_move<0x140>(v));
 }
 
 // LDS: a half's rows are D bytes, 16-byte chunk c of row r at cell
@@ -60,8 +60,9 @@ __device__ __forceinline__ int swz_v(int r, int half) {
   return D == 128 ? ((r >> 1) & 3) ^ (4 * half) : ((r >> 2) & 1) ^ (2 * half);
 }
 
-template <typename E, typename C, int D, int NW, int NS>
-__global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kernel(const QuantAttnArgs a) {
+template <typename E, typename C, int D, int NC, int NW, int NS>
+__global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kernel(
+    const QuantAttnArgs a) {
   using R = typename E::raw;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
   constexpr int kParts = kQueryParts<E>;
@@ -74,11 +75,12 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
   constexpr int kChunks = D / 16;
   constexpr int kSteps = D / 32;  // MFMAs of a half's scores
   constexpr int kRowsPerLoad = 1024 / D;
-  static_assert(NS >= 1 && NS <= 2 && kHeads * D * 4 <= NS * kSlotBytes, "ring");
+  static_assert(NS >= 1 && NS <= 2 && NC * kCols * D * 4 <= NS * kSlotBytes, "ring");
 
   __shared__ __attribute__((aligned(16))) char s_ring[NW * NS * kSlotBytes];
-  __shared__ float s_m[NW][kHeads];
-  __shared__ float s_l[NW][kHeads];
+  __shared__ __attribute__((aligned(16))) float s_m[NC * kCols][NW];
+  __shared__ __attribute__((aligned(16))) float s_l[NC * kCols][NW];
+  __shared__ float s_row[2][NC * kCols];
   __shared__ int s_arrived;
 
   const QuantCache& c = a.c;
@@ -86,7 +88,8 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
   const int lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int head = blockIdx.x % c.heads;
-  const int w = blockIdx.x / c.heads;
+  const int group = blockIdx.x / c.heads % a.row_groups;
+  const int w = blockIdx.x / c.heads / a.row_groups;
   const int G = a.group;
   const int col = lane % 16;
   const int quad = lane / 16;
@@ -105,6 +108,21 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
   const int blk_begin = max(it.blk_begin, 0);
   const int blk_end = min(it.blk_end, a.t_width);
   const int nparts = it.nparts;
+  // The rows: of a decode step, or of a request's tokens, which see less of its
+  // end the earlier they are.
+  int q_begin = seq, q_len = 1, seen = INT_MAX;  // by the first token
+  if (a.cu_q != nullptr) {
+    const ConstI32* cu_q = (const ConstI32*)(a.cu_q);
+    const ConstI32* cu_k = (const ConstI32*)(a.cu_k);
+    q_begin = max(cu_q[seq], 0);
+    q_len = cu_q[seq + 1] - q_begin;
+    seen = cu_k[seq + 1] - cu_k[seq] - q_len + 1;
+    q_len = min(q_len, a.num_rows - q_begin);
+  }
+  const int row0 = group * NC * kCols;
+  const int rows =
+      min(static_cast<int>(min(int64_t(q_len) * G, int64_t(a.head_rows))) - row0, NC * kCols);
+  if (rows <= 0) return;  // in every part
   const int pos_begin = blk_begin << lb;
   const int pos_end = min(ctx, blk_end << lb);
   const int ntiles = pos_end > pos_begin ? (pos_end - pos_begin + kTile - 1) / kTile : 0;
@@ -159,27 +177,47 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
     return mask;
   };
 
+  // Row r's token: r and G are small enough for this to be r / G.
+  auto token_of = [&](int r) { return static_cast<int>(uint32_t(r) * a.group_inverse >> 24); };
   // Query operand of MFMA step 2 j + h: dims 16 (quad + 4 j) + 8 h .. + 7 of
-  // head `col`, the order in which a lane reads K.
-  bf16x8_t qf[kParts][kSteps];
+  // row `col`, the order in which a lane reads K.
+  bf16x8_t qf[NC][kParts][kSteps];
+  int limit[NC];  // the row sees positions below
   auto load_q = [&]() {
-    const R* row = static_cast<const R*>(a.q) + seq * a.q_ts +
-                   static_cast<int64_t>(head * G + col) * a.q_hs;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      float x[8] = {};
-      if (col < G) load8<E>(row + 16 * (quad + 4 * (s / 2)) + 8 * (s % 2), x);
-      bf16x8_t part[kParts];
-      split8<kParts>(x, part);
+    for (int n = 0; n < NC; ++n) {
+      const bool there = n * kCols + col < rows;
+      const int r = row0 + (there ? n * kCols + col : 0);
+      const int token = token_of(r), g = r - token * G;
+      limit[n] = there ? min(static_cast<int>(min(static_cast<int64_t>(seen) + token,
+                                                  int64_t(INT_MAX))), pos_end) : 0;
+      const R* row = static_cast<const R*>(a.q) + static_cast<int64_t>(q_begin + token) * a.q_ts +
+                     static_cast<int64_t>(head * G + g) * a.q_hs;
+      float x[kSteps][8];  // loads that wait for no branch
 #pragma unroll
-      for (int n = 0; n < kParts; ++n) qf[n][s] = part[n];
+      for (int s = 0; s < kSteps; ++s)
+        load8<E>(row + 16 * (quad + 4 * (s / 2)) + 8 * (s % 2), x[s]);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[s][i] = there ? x[s][i] : 0.f;
+        bf16x8_t part[kParts];
+        split8<kParts>(x[s], part);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) qf[n][p][s] = part[p];
+      }
     }
   };
 
-  f32x4_t o[D / 16];
+  f32x4_t o[NC][D / 16];
+  float m[NC], l[NC];
 #pragma unroll
-  for (int db = 0; db < D / 16; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  for (int n = 0; n < NC; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) o[n][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
 
   auto compute = [&](int k, const char* slot, int mask) {
     const f32x4_t scales = *reinterpret_cast<const f32x4_t*>(slot + 4 * kHalfBytes);
@@ -200,54 +238,65 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
         vw[db] = read_tr8(base + (db ^ swz_v<D>(row, half)) * 16);
     }
     const int p = pos_begin + k * kTile + 4 * quad;
-    float sc[8];
-    float tmax = -INFINITY;
+    float sc[NC][8];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+      f32x4_t s[NC];
+#pragma unroll
+      for (int n = 0; n < NC; ++n) s[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const bf16x8_t kf =
             widen_operand<C>(kw[j][i / 2].w[2 * (i % 2)], kw[j][i / 2].w[2 * (i % 2) + 1]);
 #pragma unroll
-        for (int n = 0; n < kParts; ++n)
-          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][i], s, 0, 0, 0);
+        for (int n = 0; n < NC; ++n)
+#pragma unroll
+          for (int q = 0; q < kParts; ++q)
+            s[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][q][i], s[n], 0, 0, 0);
       }
       const float factor = scales[j] * a.scale_log2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[4 * j + i] =
-            (mask >> j & 1) && p + kHalf * j + i < pos_end ? s[i] * factor : -INFINITY;
-        tmax = fmaxf(tmax, sc[4 * j + i]);
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sc[n][4 * j + i] =
+              (mask >> j & 1) && p + kHalf * j + i < limit[n] ? s[n][i] * factor : -INFINITY;
+    }
+    bf16x8_t pf[NC][kWeights];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float tmax = sc[n][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) tmax = fmaxf(tmax, sc[n][i]);
+      tmax = fmaxf(tmax, lane_xor16(tmax, lane));
+      tmax = fmaxf(tmax, lane_xor32(tmax, lane));
+      if (__ballot(tmax > m[n] + kRescaleSlack) != 0) {
+        const float mnew = fmaxf(m[n], tmax);
+        const float alpha = mnew == -INFINITY ? 1.f : fast_exp2(m[n] - mnew);
+        l[n] *= alpha;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) o[n][db] *= alpha;
+        m[n] = mnew;
       }
-    }
-    tmax = fmaxf(tmax, lane_xor16(tmax, lane));
-    tmax = fmaxf(tmax, lane_xor32(tmax, lane));
-    if (__ballot(tmax > m + kRescaleSlack) != 0) {
-      const float mnew = fmaxf(m, tmax);
-      const float alpha = mnew == -INFINITY ? 1.f : fast_exp2(m - mnew);
-      l *= alpha;
+      const float base = m[n] == -INFINITY ? 0.f : m[n];
+      float weight[8];
 #pragma unroll
-      for (int db = 0; db < D / 16; ++db) o[db] *= alpha;
-      m = mnew;
+      for (int i = 0; i < 8; ++i) {
+        const float e = fast_exp2(sc[n][i] - base);
+        l[n] += e;
+        // A half that is not there has a scale that is not its own.
+        weight[i] = e * (mask >> (i / 4) & 1 ? scales[2 + i / 4] : 0.f);
+      }
+      split8<kWeights>(weight, pf[n]);
     }
-    const float base = m == -INFINITY ? 0.f : m;
-    float weight[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float e = fast_exp2(sc[i] - base);
-      l += e;
-      // A half that is not there has a scale that is not its own.
-      weight[i] = e * (mask >> (i / 4) & 1 ? scales[2 + i / 4] : 0.f);
-    }
-    bf16x8_t pf[kWeights];
-    split8<kWeights>(weight, pf);
 #pragma unroll
     for (int db = 0; db < D / 16; ++db) {
       const bf16x8_t vf = widen_operand<C>(vw[db].x, vw[db].y);
 #pragma unroll
-      for (int n = 0; n < kWeights; ++n)
-        o[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], o[db], 0, 0, 0);
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int q = 0; q < kWeights; ++q)
+          o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][q], o[n][db], 0, 0, 0);
     }
   };
 
@@ -299,79 +348,89 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
   __builtin_amdgcn_s_waitcnt(0x0070);
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 
-  l += lane_xor16(l, lane);
-  l += lane_xor32(l, lane);
-  if (!(l == l)) m = 0.f;  // NaN counts, whatever the maximum
-
-  // The wave's state into its own drained ring: acc[h][d].
-  float* my_acc = reinterpret_cast<float*>(my_ring);
-  if (col < G) {
 #pragma unroll
-    for (int db = 0; db < D / 16; ++db)
-      *reinterpret_cast<f32x4_t*>(my_acc + col * D + db * 16 + 4 * quad) = o[db];
+  for (int n = 0; n < NC; ++n) {
+    l[n] += lane_xor16(l[n], lane);
+    l[n] += lane_xor32(l[n], lane);
+    if (!(l[n] == l[n])) m[n] = 0.f;  // NaN counts, whatever the maximum
+    if (lane < kCols) {
+      s_m[n * kCols + lane][wave] = m[n];
+      s_l[n * kCols + lane][wave] = l[n];
+    }
   }
-  if (lane < kHeads) {
-    s_m[wave][lane] = m;
-    s_l[wave][lane] = l;
+  // The waves' sums into their own drained rings, acc[row][d] with four dims at
+  // cell (d / 4) ^ (row % 16) of the row, joined by all threads: a thread's pair
+  // of dims `dim`, of rows row_of(0), row_of(1), ...
+  constexpr int kThreads = NW * kWave;
+  constexpr int kStep = 2 * kThreads / D;  // rows that the threads cover at once
+  constexpr int kPairs = NC * kCols / kStep;
+  const int dim = 2 * (tid % (D / 2));
+  auto row_of = [&](int j) { return j * kStep + tid / (D / 2); };
+  {
+    float* acc = reinterpret_cast<float*>(my_ring);
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db)
+        if (n * kCols + col < rows)
+          *reinterpret_cast<f32x4_t*>(acc + (n * kCols + col) * D +
+                                      4 * ((db * 4 + quad) ^ col)) = o[n][db];
   }
   __syncthreads();
-
-  const int elems = G * D;
-  constexpr int kThreads = NW * kWave;
-  constexpr int kPer = kHeads * D / kThreads;
-  float acc_v[kPer], m_v[kPer], l_v[kPer];
+  Float2 sum[kPairs];
+  float top[kPairs], total[kPairs];  // a row's maximum and sum
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = tid + j * kThreads;
-    acc_v[j] = 0.f;
-    m_v[j] = -INFINITY;
-    l_v[j] = 0.f;
-    if (e < elems) {
-      const int h = e / D, d = e % D;
-      float mx = -INFINITY;
+  for (int j = 0; j < kPairs; ++j) {
+    const float* ms = s_m[row_of(j)];
+    const float* lw = s_l[row_of(j)];
+    top[j] = -INFINITY;
+    total[j] = 0.f;
+    sum[j] = Float2{0.f, 0.f};
+    if (row_of(j) >= rows) continue;
+    const int at = row_of(j) * D + 4 * ((dim / 4) ^ (row_of(j) % 16)) + dim % 4;
 #pragma unroll
-      for (int wv = 0; wv < NW; ++wv) mx = fmaxf(mx, s_m[wv][h]);
-      float ls = 0.f, os = 0.f;
+    for (int wv = 0; wv < NW; ++wv) top[j] = fmaxf(top[j], ms[wv]);
 #pragma unroll
-      for (int wv = 0; wv < NW; ++wv) {
-        const float mw = s_m[wv][h];
-        const float f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
-        ls = fmaf(f, s_l[wv][h], ls);
-        os = fmaf(f, reinterpret_cast<const float*>(s_ring + wv * NS * kSlotBytes)[h * D + d], os);
-      }
-      acc_v[j] = os;
-      m_v[j] = mx;
-      l_v[j] = ls;
+    for (int wv = 0; wv < NW; ++wv) {
+      const Float2 y =
+          *reinterpret_cast<const Float2*>(s_ring + wv * NS * kSlotBytes + at * 4);
+      const float f = ms[wv] == -INFINITY ? 0.f : fast_exp2(ms[wv] - top[j]);
+      total[j] = fmaf(f, lw[wv], total[j]);
+      sum[j].x = fmaf(f, y.x, sum[j].x);
+      sum[j].y = fmaf(f, y.y, sum[j].y);
     }
   }
-
-  R* out = static_cast<R*>(a.out) + seq * a.o_ts + static_cast<int64_t>(head * G) * a.o_hs;
+  auto put = [&](int r, Float2 x, float ls) {
+    const int token = token_of(row0 + r);
+    const float inv = ls != 0.f ? 1.f / ls : 0.f;
+    struct alignas(2 * sizeof(R)) Pair {
+      R x, y;
+    };
+    *reinterpret_cast<Pair*>(static_cast<R*>(a.out) +
+                             static_cast<int64_t>(q_begin + token) * a.o_ts +
+                             static_cast<int64_t>(head * G + row0 + r - token * G) * a.o_hs +
+                             dim) =
+        Pair{E::store(x.x * inv), E::store(x.y * inv)};
+  };
   if (nparts == 1) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int e = tid + j * kThreads;
-      if (e < elems) {
-        const float inv = l_v[j] != 0.f ? 1.f / l_v[j] : 0.f;
-        out[(e / D) * a.o_hs + e % D] = E::store(acc_v[j] * inv);
-      }
-    }
+    for (int j = 0; j < kPairs; ++j)
+      if (row_of(j) < rows) put(row_of(j), sum[j], total[j]);
     return;
   }
 
-  int32_t* counter = a.counters + static_cast<int64_t>(seq) * c.heads + head;
-  const int64_t base = (static_cast<int64_t>(it.first_item + it.part) * c.heads + head) * G;
+  int32_t* counter =
+      a.counters + (static_cast<int64_t>(seq) * a.row_groups + group) * c.heads + head;
+  // Row r of partition p.
+  auto slot_of = [&](int p, int r) {
+    return (static_cast<int64_t>(it.first_item + p) * c.heads + head) * a.head_rows + row0 + r;
+  };
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = tid + j * kThreads;
-    if (e < elems) {
-      const int h = e / D, d = e % D;
-      store_coherent(a.ws_acc + (base + h) * D + d, acc_v[j]);
-      if (d == 0) {
-        store_coherent(a.ws_ml + (base + h) * 2, m_v[j]);
-        store_coherent(a.ws_ml + (base + h) * 2 + 1, l_v[j]);
-      }
+  for (int j = 0; j < kPairs; ++j)
+    if (row_of(j) < rows) {
+      store_coherent2(a.ws_acc + slot_of(it.part, row_of(j)) * D + dim, sum[j].x, sum[j].y);
+      if (dim == 0) store_coherent2(a.ws_ml + slot_of(it.part, row_of(j)) * 2, top[j], total[j]);
     }
-  }
   wait_stores();
   __syncthreads();  // every thread's partials are at the coherent level
   if (tid == 0)
@@ -379,64 +438,177 @@ __global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kern
   __syncthreads();
   if (s_arrived != nparts - 1) return;
 
-  constexpr int kBatch = 8;  // partitions whose loads are in flight together
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = tid + j * kThreads;
-    if (e >= elems) continue;
-    const int h = e / D, d = e % D;
-    float mx = -INFINITY, ls = 0.f, os = 0.f;
-    for (int p0 = 0; p0 < nparts; p0 += kBatch) {
-      float mb[kBatch], lbv[kBatch], ob[kBatch];
+  // What a merge takes is its loads' latency, so many are in flight at once.
+  if (rows <= kStep) {  // a row a thread
+    const int r = row_of(0);
+    constexpr int kBatch = 8;
+    float mx = -INFINITY, ls = 0.f;
+    Float2 x{0.f, 0.f};
+    for (int p0 = 0; p0 < nparts && r < rows; p0 += kBatch) {
+      Float2 ml[kBatch], y[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const int p = min(p0 + b, nparts - 1);
-        const int64_t row = (static_cast<int64_t>(it.first_item + p) * c.heads + head) * G + h;
-        mb[b] = load_coherent(a.ws_ml + row * 2);
-        lbv[b] = load_coherent(a.ws_ml + row * 2 + 1);
-        ob[b] = load_coherent(a.ws_acc + row * D + d);
+        const int64_t at = slot_of(min(p0 + b, nparts - 1), r);
+        ml[b] = load_coherent2(a.ws_ml + at * 2);
+        y[b] = load_coherent2(a.ws_acc + at * D + dim);
       }
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b)
-        if (p0 + b < nparts) merge_step(mx, ls, os, mb[b], lbv[b], ob[b]);
+      for (int b = 0; b < kBatch; ++b) {
+        if (p0 + b >= nparts || ml[b].x == -INFINITY) continue;  // nothing was seen
+        const float now = fmaxf(mx, ml[b].x);
+        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - now);
+        const float f = fast_exp2(ml[b].x - now);
+        ls = fmaf(ls, back, f * ml[b].y);
+        x.x = fmaf(x.x, back, f * y[b].x);
+        x.y = fmaf(x.y, back, f * y[b].y);
+        mx = now;
+      }
     }
-    const float inv = ls != 0.f ? 1.f / ls : 0.f;
-    out[h * a.o_hs + d] = E::store(os * inv);
+    if (r < rows) put(r, x, ls);
+  } else if constexpr (kPairs > 1) {
+    // Several rows a thread: the factors go through LDS, found by 16 lanes a row.
+    constexpr int kChunk = 32;  // partitions at once there
+    constexpr int kBatch = (NS == 1 ? 16 : 32) / kPairs;
+    static_assert(kThreads / 16 >= NC * kCols, "16 lanes for a row's factors");
+    const int frow = tid / 16, sub = tid % 16;
+    float(*s_f)[NC * kCols] = reinterpret_cast<float(*)[NC * kCols]>(s_ring);
+    float mx = -INFINITY, ls = 0.f;
+    Float2 x[kPairs] = {};
+    for (int p0 = 0; p0 < nparts; p0 += kChunk) {
+      const int n = min(kChunk, nparts - p0);
+      Float2 y[kBatch][kPairs];
+      auto load = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j)
+            y[b][j] = load_coherent2(
+                a.ws_acc + slot_of(p0 + min(q + b, n - 1), min(row_of(j), rows - 1)) * D + dim);
+      };
+      Float2 ml[kChunk / 16];
+#pragma unroll
+      for (int i = 0; i < kChunk / 16; ++i)
+        ml[i] = load_coherent2(
+            a.ws_ml + slot_of(p0 + min(sub + 16 * i, n - 1), min(frow, rows - 1)) * 2);
+      load(0);
+      if (p0 > 0) __syncthreads();  // the last factors are read
+      if (frow < NC * kCols) {
+        float now = mx;
+#pragma unroll
+        for (int i = 0; i < kChunk / 16; ++i) now = fmaxf(now, max16(ml[i].x));
+        float lsum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kChunk / 16; ++i) {
+          // Below zero: nothing was seen.
+          const float f = ml[i].x == -INFINITY ? -1.f : fast_exp2(ml[i].x - now);
+          lsum += f < 0.f || sub + 16 * i >= n ? 0.f : f * ml[i].y;
+          s_f[sub + 16 * i][frow] = f;
+        }
+        const float back = mx == -INFINITY ? 0.f : fast_exp2(mx - now);
+        ls = fmaf(ls, back, group_sum<16>(lsum));
+        mx = now;
+        if (sub == 0) {
+          s_row[0][frow] = back;
+          s_row[1][frow] = ls;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        const float back = s_row[0][row_of(j)];
+        x[j].x *= back;
+        x[j].y *= back;
+      }
+      for (int q = 0; q < n; q += kBatch) {
+        if (q > 0) load(q);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) {
+            const float f = s_f[min(q + b, kChunk - 1)][row_of(j)];
+            const bool weighs = q + b < n && f >= 0.f;
+            x[j].x = weighs ? fmaf(f, y[b][j].x, x[j].x) : x[j].x;
+            x[j].y = weighs ? fmaf(f, y[b][j].y, x[j].y) : x[j].y;
+          }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j)
+      if (row_of(j) < rows) put(row_of(j), x[j], s_row[1][row_of(j)]);
   }
   if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// The lengths of requests as decode sequences (0: no rows), and the counters of
+// their rows cleared.
+__global__ __launch_bounds__(256) void few_rows_kernel(const int32_t* __restrict__ cu_q,
+                                                       const int32_t* __restrict__ cu_k,
+                                                       int num_seqs, int32_t* __restrict__ lens,
+                                                       int32_t* __restrict__ counters,
+                                                       int num_counters) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < num_seqs) lens[i] = cu_q[i + 1] > cu_q[i] ? max(cu_k[i + 1] - cu_k[i], 0) : 0;
+  if (i < num_counters) counters[i] = 0;
+}
+
 }  // namespace
 
-bool quant_decode_mfma_takes(int32_t head_dim, int32_t group, int32_t block_size) {
-  return (head_dim == 128 || head_dim == 64) && group <= kHeads && block_size >= kHalf;
+bool quant_decode_mfma_takes(int32_t head_dim, int32_t block_size) {
+  return (head_dim == 128 || head_dim == 64) && block_size >= kHalf;
 }
 
-bool quant_decode_mfma_supported(const QuantAttnArgs& a) {
-  const QuantCache& c = a.c;
+bool quant_mfma_aligned(const QuantCache& c) {
   const auto low = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | c.bs |
                    c.ts | c.hs;
-  return quant_decode_mfma_takes(c.dim, a.group, c.block_size) && low % 16 == 0 &&
-         c.ts < (int64_t(1) << 26);
+  return low % 16 == 0 && c.ts < (int64_t(1) << 26);
 }
 
-int32_t launch_quant_decode_mfma(const QuantAttnArgs& a, int32_t dtype, int32_t code,
+int32_t quant_decode_row_groups(int32_t rows) {
+  return rows <= kCols ? 1 : (rows - 1) / (2 * kCols) + 1;
+}
+
+int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, int32_t code,
                                  hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(a.max_items) * a.c.heads);
-  const bool narrow = static_cast<int64_t>(a.num_seqs) * a.c.heads > device_cus();
+  a.head_rows = rows;
+  a.row_groups = quant_decode_row_groups(rows);
+  // r * inverse >> 24 is r / group for r * group < 2^24, with no overflow for
+  // r < 2^8.
+  if (rows > 256) return fail(MI_ERR_UNSUPPORTED, "quantized decode: too many rows");
+  a.group_inverse = ((1u << 24) + a.group - 1) / a.group;
+  const int64_t grid = static_cast<int64_t>(a.max_items) * a.c.heads * a.row_groups;
+  if (grid > INT_MAX)
+    return fail(MI_ERR_UNSUPPORTED, "quantized attention: too many rows for one launch");
+  // Many workgroups: two a CU with a slot a wave, where they fit the registers
+  // that leaves them (four layers of 128 sequences of 500 tokens 144 us, 173 with
+  // one of two slots; 64 of 1000 with heads of 64 77 / 80, float32 80 / 84. Heads
+  // of 128 spill: f16 64 of 1000 166 / 136, float32 376 / 141).
+  const bool narrow =
+      static_cast<int64_t>(a.num_seqs) * a.c.heads * a.row_groups > device_cus();
   return with_types(dtype, code, [&](auto e, auto co) {
     using E = decltype(e);
     using C = decltype(co);
     auto go = [&](auto kernel) {
-      kernel<<<grid, kWave * 8, 0, stream>>>(a);
+      kernel<<<static_cast<uint32_t>(grid), kWave * 8, 0, stream>>>(a);
       return check_launch("quantized decode");
     };
-    if (a.c.dim == 128)
-      return narrow ? go(quant_decode_kernel<E, C, 128, 8, 1>)
-                    : go(quant_decode_kernel<E, C, 128, 8, 2>);
-    return narrow ? go(quant_decode_kernel<E, C, 64, 8, 1>)
-                  : go(quant_decode_kernel<E, C, 64, 8, 2>);
+    const bool wide = a.c.dim == 128;
+    if (rows > kCols)
+      return wide ? go(quant_decode_kernel<E, C, 128, 2, 8, 2>)
+                  : go(quant_decode_kernel<E, C, 64, 2, 8, 2>);
+    if (narrow && !wide) return go(quant_decode_kernel<E, C, 64, 1, 8, 1>);
+    if constexpr (std::is_same<E, BF16>::value)
+      if (narrow) return go(quant_decode_kernel<E, C, 128, 1, 8, 1>);
+    return wide ? go(quant_decode_kernel<E, C, 128, 1, 8, 2>)
+                : go(quant_decode_kernel<E, C, 64, 1, 8, 2>);
   });
+}
+
+int32_t launch_few_rows(const int32_t* cu_q, const int32_t* cu_k, int32_t num_seqs, int32_t* lens,
+                        int32_t* counters, int32_t num_counters, hipStream_t stream) {
+  const int n = std::max(num_seqs, num_counters);
+  few_rows_kernel<<<(n - 1) / 256 + 1, 256, 0, stream>>>(cu_q, cu_k, num_seqs, lens, counters,
+                                                         num_counters);
+  return check_launch("quantized attention plan");
 }
 
 }  // namespace mi

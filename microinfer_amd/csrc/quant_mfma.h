@@ -119,17 +119,21 @@ __device__ __forceinline__ int2v_t read_tr8(const void* lds) {
 // calls of these sizes), its plan in the workspace, and its launch with that.
 int64_t quant_prefill_workspace(int32_t num_rows, int32_t num_seqs, int32_t group, int32_t heads,
                                 int32_t dim, int32_t block_size);
-bool quant_prefill_mfma_supported(const QuantAttnArgs& a);
 int32_t launch_quant_prefill_plan(const int32_t* cu_q, const int32_t* cu_k, int32_t num_rows,
                                   int32_t num_seqs, int32_t group, int32_t heads, int32_t dim,
                                   void* workspace, hipStream_t stream);
 int32_t launch_quant_prefill_mfma(const QuantAttnArgs& a, int32_t dtype, int32_t code,
                                   void* workspace, hipStream_t stream);
 
-// Whether the MFMA decode kernel takes calls of this shape, and its launch.
-bool quant_decode_mfma_takes(int32_t head_dim, int32_t group, int32_t block_size);
-bool quant_decode_mfma_supported(const QuantAttnArgs& a);
-int32_t launch_quant_decode_mfma(const QuantAttnArgs& a, int32_t dtype, int32_t code,
+// MFMA kernel of few rows (quant_decode.hip): whether it takes caches of this
+// shape, the workgroups that share a sequence's `rows` at a KV head, the launch;
+// the lengths of requests for its plan.
+bool quant_decode_mfma_takes(int32_t head_dim, int32_t block_size);
+bool quant_mfma_aligned(const QuantCache& c);
+int32_t quant_decode_row_groups(int32_t rows);
+int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, int32_t code,
                                  hipStream_t stream);
+int32_t launch_few_rows(const int32_t* cu_q, const int32_t* cu_k, int32_t num_seqs, int32_t* lens,
+                        int32_t* counters, int32_t num_counters, hipStream_t stream);
 
 }  // namespace mi

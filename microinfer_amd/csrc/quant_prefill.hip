@@ -687,14 +687,6 @@ int64_t quant_prefill_workspace(int32_t num_rows, int32_t num_seqs, int32_t grou
   return l.max_items == 0 ? 0 : l.total;
 }
 
-bool quant_prefill_mfma_supported(const QuantAttnArgs& a) {
-  const QuantCache& c = a.c;
-  const auto low = reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v) | c.bs |
-                   c.ts | c.hs;
-  return low % 16 == 0 &&
-         quant_prefill_workspace(a.num_rows, a.num_seqs, a.group, c.heads, c.dim, c.block_size) > 0;
-}
-
 int32_t launch_quant_prefill_plan(const int32_t* cu_q, const int32_t* cu_k, int32_t num_rows,
                                   int32_t num_seqs, int32_t group, int32_t heads, int32_t dim,
                                   void* workspace, hipStream_t stream) {

@@ -170,7 +170,8 @@ class QuantizedPrefillPlan:
 
     cu_seqlens_q: torch.Tensor
     cu_seqlens_k: torch.Tensor
-    sizes: tuple  # tokens, requests, Hq, Hkv, head_dim, block size
+    sizes: tuple  # tokens, requests, Hq, Hkv, head_dim, block size, table width
+    max_seqlen_q: int
     workspace_bytes: int
     _workspaces: dict = field(default_factory=dict, repr=False, compare=False)
 
@@ -182,11 +183,10 @@ class QuantizedPrefillPlan:
         have = self._workspaces.get(place)
         if have is None:
             have = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
-            tokens, requests, num_q_heads, num_kv_heads, head_dim, block_size = self.sizes
+            tokens, requests, *sizes = self.sizes
             status = _lib.load().mi_quant_prefill_plan(
                 self.cu_seqlens_q.data_ptr(), self.cu_seqlens_k.data_ptr(), tokens, requests,
-                num_q_heads, num_kv_heads, head_dim, block_size, have.data_ptr(),
-                self.workspace_bytes, place[1])
+                self.max_seqlen_q, *sizes, have.data_ptr(), self.workspace_bytes, place[1])
             _lib.check(status, "mi_quant_prefill_plan")
             if not place[2] or not self._workspaces:
                 self._workspaces[place] = have
@@ -195,11 +195,13 @@ class QuantizedPrefillPlan:
 
 def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, *,
                            num_tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
-                           dtype: torch.dtype, block_size: int,
-                           block_table_width: int) -> QuantizedPrefillPlan | None:
+                           dtype: torch.dtype, block_size: int, block_table_width: int,
+                           max_seqlen_q: int | None = None) -> QuantizedPrefillPlan | None:
     """The plan of one step's ``hip_quantized_prefill`` calls (shared by its
     layers), from the cu_seqlens on the device (capture-safe). None: calls of
-    these sizes run without one."""
+    these sizes run without one. ``max_seqlen_q`` bounds the new tokens of any
+    request (``num_tokens`` by default): where it is small, the step is laid out
+    for few rows a request."""
     _lib.require_device(cu_seqlens_q, cu_seqlens_k, what="quantized_prefill_plan")
     if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
         raise ValueError("Hq must be divisible by Hkv")
@@ -210,11 +212,16 @@ def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tenso
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have num_requests + 1 entries")
     if cu_seqlens_k.device != device:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must share a device")
-    sizes = num_tokens, requests, num_q_heads, num_kv_heads, head_dim, block_size
-    nbytes = _lib.load().mi_quant_prefill_workspace_bytes(*sizes)
+    longest = num_tokens if max_seqlen_q is None else min(max_seqlen_q, num_tokens)
+    if longest <= 0 and num_tokens:
+        raise ValueError("max_seqlen_q must be positive")
+    sizes = num_q_heads, num_kv_heads, head_dim, block_size
+    nbytes = _lib.load().mi_quant_prefill_workspace_bytes(num_tokens, requests, longest, *sizes)
     if nbytes == 0:
         return None
-    plan = QuantizedPrefillPlan(index32(cu_seqlens_q), index32(cu_seqlens_k), sizes, nbytes)
+    plan = QuantizedPrefillPlan(index32(cu_seqlens_q), index32(cu_seqlens_k),
+                                (num_tokens, requests, *sizes, block_table_width), longest,
+                                nbytes)
     with _lib.on_device(device):
         plan.workspace(device)
     return plan
@@ -230,9 +237,9 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
 
     ``query [T, Hq, D]``; request r owns query rows ``cu_seqlens_q[r]..`` and
     context ``cu_seqlens_k[r+1] - cu_seqlens_k[r]`` (it includes the new rows,
-    which the caller appended first). ``plan``: of ``quantized_prefill_plan``
-    for these lengths and sizes; without it the call makes its own. Rows that
-    see nothing give zeros.
+    which the caller appended first). ``max_seqlen_q`` bounds the query rows of
+    any request. ``plan``: of ``quantized_prefill_plan`` for these lengths and
+    sizes; without it the call makes its own. Rows that see nothing give zeros.
     """
     cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
                                                 value_scales, "hip_quantized_prefill")
@@ -250,8 +257,10 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
         _lib.require_device(cu_seqlens_q, cu_seqlens_k, block_tables,
                             what="hip_quantized_prefill")
         raise ValueError("cu_seqlens and block_tables must be on the query's device")
-    sizes = num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim, block_size
-    if plan is not None and (not isinstance(plan, QuantizedPrefillPlan) or plan.sizes != sizes):
+    sizes = num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim, block_size, width
+    longest = min(max_seqlen_q, num_tokens)
+    if plan is not None and (not isinstance(plan, QuantizedPrefillPlan) or plan.sizes != sizes
+                             or plan.max_seqlen_q < longest):
         raise ValueError("plan must come from quantized_prefill_plan() for this call's sizes")
     if plan is not None and plan.cu_seqlens_q.get_device() != device:
         raise ValueError("plan must be on the query's device")
@@ -266,17 +275,18 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
         plan = quantized_prefill_plan(
             cu_q, cu_k, num_tokens=num_tokens, num_q_heads=num_q_heads,
             num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=query.dtype,
-            block_size=block_size, block_table_width=width)
+            block_size=block_size, block_table_width=width, max_seqlen_q=max_seqlen_q)
     strides = query.stride()
     with _lib.on_device(query.device):
         workspace, nbytes = None, 0
         if plan is not None:
             workspace, nbytes = plan.workspace(query.device).data_ptr(), plan.workspace_bytes
+            longest = plan.max_seqlen_q
         status = _lib.load().mi_quant_prefill(
             query.data_ptr(), strides[0], strides[1], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
             tables.data_ptr(), width, width, out.data_ptr(), num_q_heads * head_dim, head_dim,
-            workspace, nbytes, num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim,
-            block_size, num_blocks, head_dim ** -0.5 if scale is None else float(scale),
+            workspace, nbytes, num_tokens, num_requests, longest, num_q_heads, num_kv_heads,
+            head_dim, block_size, num_blocks, head_dim ** -0.5 if scale is None else float(scale),
             _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(query.device))
     _lib.check(status, "mi_quant_prefill")
     return out

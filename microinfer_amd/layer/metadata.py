@@ -196,7 +196,8 @@ class AttentionMetadata:
         if key not in plans:
             plans[key] = (quantized_decode_plan(self.context_lens, **sizes) if self.is_decode else
                           quantized_prefill_plan(self.cu_seqlens_q, self.cu_seqlens_k,
-                                                 num_tokens=num_tokens, **sizes))
+                                                 num_tokens=num_tokens,
+                                                 max_seqlen_q=self.max_seqlen_q or None, **sizes))
         return plans[key]
 
     @property

@@ -209,6 +209,120 @@ def test_prefill_lengths(kind, contexts, lengths):
         check_attention(got, query, twin, tables, contexts, cu_q, 0.07, VARLEN["bf16"])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("shape,lengths", [
+    ((4, 2, 128, 16, "paired"), [3, 0, 1, 8, 2]),  # up to 16 rows
+    ((8, 2, 64, 32, "head_major"), [7, 8, 0, 1, 5]),  # 32
+    ((12, 2, 128, 16, "paired"), [10, 9, 1, 6, 3]),  # 60, in two groups
+    ((3, 1, 64, 16, "token_major"), [11, 21, 5, 16, 13]),  # 63
+    ((20, 1, 128, 64, "paired"), [1, 3, 2, 0, 3]),
+    ((17, 1, 64, 16, "paired"), [0, 0, 1, 1, 0])])
+def test_few_rows_a_request(kind, dtype, shape, lengths):
+    """Requests laid out like decode steps: whole and in parts, rows in one
+    group and in several, tokens that see less than the last, rows that see
+    nothing, blocks outside the pool."""
+    rng = np.random.default_rng(sum(lengths))
+    hq, hkv, dim, block, _ = shape
+    contexts = [1700, 40, 33, 5, 900]
+    twin, tables, _ = decode_case(rng, contexts, shape, kind, dtype)
+    tables[4][0] = -3
+    query = query_of(rng, sum(lengths), hq, dim, dtype)
+    cu_q = ints(np.cumsum([0] + lengths).tolist())
+    cu_k = ints(np.cumsum([0] + contexts).tolist())
+    plan = quantized_prefill_plan(
+        cu_q, cu_k, num_tokens=query.shape[0], num_q_heads=hq, num_kv_heads=hkv, head_dim=dim,
+        dtype=query.dtype, block_size=block, block_table_width=len(tables[0]),
+        max_seqlen_q=max(lengths) + 1)
+    for q, how, most in ((query, None, max(lengths)), (query, plan, max(lengths) + 1),
+                         (query.flip(0), plan, max(lengths) + 1)):
+        got = hip_quantized_prefill(q, *twin.tensors, cu_q, cu_k, ints(tables),
+                                    max_seqlen_q=max(lengths), plan=how, scale=0.13)
+        few = most * hq // hkv <= 32  # of five requests
+        check_attention(got, q, twin, tables, contexts, cu_q.tolist(), 0.13,
+                        (DECODE if few else VARLEN)[dtype])
+    longer = dict(max_seqlen_q=max(lengths) + 2, plan=plan)
+    if sum(lengths) > max(lengths) + 1:  # more rows than tokens there cannot be
+        with pytest.raises(ValueError, match="plan"):
+            hip_quantized_prefill(query, *twin.tensors, cu_q, cu_k, ints(tables), **longer)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("shape,length,context", [
+    ((8, 2, 128, 16, "paired"), 30, 1900), ((3, 1, 64, 32, "head_major"), 42, 700),
+    ((128, 1, 128, 16, "paired"), 1, 2500), ((16, 2, 64, 16, "paired"), 16, 50)])
+def test_one_request_of_rows_in_several_groups(dtype, shape, length, context):
+    rng = np.random.default_rng(length)
+    hq, hkv, dim, block, _ = shape
+    twin, tables, _ = decode_case(rng, [context], shape, "fp8", dtype)
+    query = query_of(rng, length, hq, dim, dtype)
+    got = hip_quantized_prefill(query, *twin.tensors, ints([0, length]), ints([0, context]),
+                                ints(tables), max_seqlen_q=length)
+    check_attention(got, query, twin, tables, [context], [0, length], dim ** -0.5, DECODE[dtype])
+
+
+@pytest.mark.parametrize("hq,hkv", [(17, 1), (32, 1), (64, 2), (66, 2), (40, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_of_large_groups(hq, hkv, dim):
+    rng = np.random.default_rng(hq)
+    contexts = [1500, 1, 77]
+    shape = (hq, hkv, dim, 16, "paired")
+    for dtype in DTYPES:
+        twin, tables, query = decode_case(rng, contexts, shape, "fp8", dtype)
+        got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+        check_attention(got, query, twin, tables, contexts, [0, 1, 2, 3], dim ** -0.5,
+                        DECODE[dtype])
+
+
+def test_few_rows_in_graphs_and_on_other_streams():
+    """A captured plan with its calls and captured calls of an eager plan,
+    replayed among eager calls, as the lengths on the device change."""
+    rng = np.random.default_rng(21)
+    contexts, lengths = [1800, 500, 60], [4, 1, 3]
+    shape = (8, 2, 128, 16, "paired")
+    twin, tables, _ = decode_case(rng, contexts, shape, "fp8", "bf16")
+    query, other = query_of(rng, 8, 8, 128, "bf16"), query_of(rng, 8, 8, 128, "bf16")
+    cu_q, cu_k = ints([0, 4, 5, 8]), ints(np.cumsum([0] + contexts).tolist())
+    at = ints(tables)
+
+    def planned():
+        return quantized_prefill_plan(cu_q, cu_k, num_tokens=8, num_q_heads=8, num_kv_heads=2,
+                                      head_dim=128, dtype=query.dtype, block_size=16,
+                                      block_table_width=at.shape[1], max_seqlen_q=4)
+
+    def run(q, plan):
+        return hip_quantized_prefill(q, *twin.tensors, cu_q, cu_k, at, max_seqlen_q=4, plan=plan)
+
+    eager = planned()
+    want = run(query, eager).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = planned()
+        first, second = run(query, plan), run(other, plan)
+    held = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(held):
+        third = run(query, eager)
+    side = torch.cuda.Stream()
+    for step in range(3):
+        graph.replay()
+        held.replay()
+        with torch.cuda.stream(side):
+            fourth = run(query, eager)
+        torch.cuda.synchronize()
+        for got, q in ((first, query), (second, other)):
+            check_attention(got, q, twin, tables, contexts, [0, 4, 5, 8], 128 ** -0.5,
+                            DECODE["bf16"])
+        assert torch.equal(third, want) and torch.equal(fourth, want)
+        if step == 1:  # lengths for the captured plan; the eager one keeps its own
+            contexts = [1700, 300, 41]
+            cu_k.copy_(ints(np.cumsum([0] + contexts).tolist()))
+            break
+    graph.replay()
+    torch.cuda.synchronize()
+    check_attention(first, query, twin, tables, contexts, [0, 4, 5, 8], 128 ** -0.5,
+                    DECODE["bf16"])
+
+
 def test_prefill_rows_that_see_nothing_are_zeros():
     """More query rows than positions, contexts of nothing, invalid blocks."""
     rng = np.random.default_rng(7)

@@ -94,8 +94,8 @@ def _decode(lib, **over):
 def _prefill(lib, **over):
     order = dict(q=4096, qts=512, qhs=128, **CACHE, cu_q=4096, cu_k=4096, tables=4096, tstride=4,
                  width=4, out=4096, ots=512, ohs=128, ws=4096, ws_bytes=1 << 30, tokens=9,
-                 requests=2, hq=4, heads=2, dim=128, block=16, blocks=8, scale=0.1, dtype=2,
-                 code=0)
+                 requests=2, longest=9, hq=4, heads=2, dim=128, block=16, blocks=8, scale=0.1,
+                 dtype=2, code=0)
     return lib.mi_quant_prefill(*_args(order, over), None)
 
 
@@ -197,18 +197,26 @@ def test_c_prefill_validates_its_requests():
     for name in ("cu_q", "cu_k"):
         assert _prefill(lib, **{name: None}) == 1 and "null" in _lib.last_error()
     assert _prefill(lib, tokens=0, q=None) == 0
-    need = lib.mi_quant_prefill_workspace_bytes(9, 2, 4, 2, 128, 16)
-    assert need > 0 and _prefill(lib, ws_bytes=need - 1) == 3 and str(need) in _lib.last_error()
-    assert _prefill(lib, ws=None) == 3 and _prefill(lib, ws=4112) == 3
-    for sizes in ((0, 2, 4, 2, 128, 16), (9, 0, 4, 2, 128, 16), (9, 2, 3, 2, 128, 16),
-                  (9, 2, 4, 2, 32, 16), (9, 2, 4, 2, 128, 8), (9, 2, 258, 2, 128, 16)):
+    assert _prefill(lib, longest=0) == 1 and "max_seqlen_q" in _lib.last_error()
+    # Few rows a request, and many.
+    for tokens, longest in ((9, 9), (900, 2), (900, 900)):
+        need = lib.mi_quant_prefill_workspace_bytes(tokens, 2, longest, 4, 2, 128, 16)
+        sizes = dict(tokens=tokens, longest=longest)
+        assert need > 0 and _prefill(lib, ws_bytes=need - 1, **sizes) == 3
+        assert str(need) in _lib.last_error()
+        assert _prefill(lib, ws=None, **sizes) == 3 and _prefill(lib, ws=4112, **sizes) == 3
+    for sizes in ((0, 2, 9, 4, 2, 128, 16), (9, 0, 9, 4, 2, 128, 16), (9, 2, 9, 3, 2, 128, 16),
+                  (9, 2, 0, 4, 2, 128, 16), (9, 2, 9, 4, 2, 32, 16), (9, 2, 9, 4, 2, 128, 8),
+                  (9, 2, 9, 258, 2, 128, 16)):
         assert lib.mi_quant_prefill_workspace_bytes(*sizes) == 0
+    need = lib.mi_quant_prefill_workspace_bytes(9, 2, 9, 4, 2, 128, 16)
 
-    def plan(cu_q=4096, cu_k=4096, tokens=9, requests=2, hq=4, hkv=2, dim=128, block=16, ws=4096,
-             nbytes=1 << 30):
-        return lib.mi_quant_prefill_plan(cu_q, cu_k, tokens, requests, hq, hkv, dim, block, ws,
-                                         nbytes, None)
+    def plan(cu_q=4096, cu_k=4096, tokens=9, requests=2, longest=9, hq=4, hkv=2, dim=128,
+             block=16, width=4, ws=4096, nbytes=1 << 30):
+        return lib.mi_quant_prefill_plan(cu_q, cu_k, tokens, requests, longest, hq, hkv, dim,
+                                         block, width, ws, nbytes, None)
 
     assert plan(hq=3) == 1 and plan(dim=32) == 2 and plan(tokens=0) == 2
+    assert plan(block=24) == 1 and plan(width=-1) == 1 and plan(width=1 << 27) == 2
     assert plan(cu_q=None) == 1 and plan(cu_k=None) == 1
     assert plan(ws=None) == 3 and plan(nbytes=need - 1) == 3 and plan(ws=4104) == 3

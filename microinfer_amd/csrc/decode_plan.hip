@@ -38,7 +38,6 @@ constexpr int32_t kTargetItems = 192;
 // (176) 16.4 / 14.6 / 16.6; 2 KV heads, 4096 31.4 / 31.4 / 40.7, 8192 44 / 38
 // / 44, 32768 (352) 69 / - / 62; head_dim 64 bf16 16.8 / 15.8 / 16.3 at 4096,
 // float32 13.7 / 12.4 / 15.7, head_dim 256 bf16 32.6 / 28.3 / 33.2).
-constexpr int32_t kMinPartPositions = 64;
 constexpr int32_t kMaxMinPart = 512;
 constexpr int32_t kMaxMinPartVector = 256;
 constexpr int32_t kLongPositions = 16384;
@@ -74,10 +73,11 @@ __device__ __forceinline__ int part_blocks(int nb, int split_k, int pb_global, i
 
 // The step's part size from its blocks in all and its longest sequence's.
 __device__ __forceinline__ int step_part_blocks(int64_t total_blocks, int longest, int lb,
-                                                int num_kv_heads, int target, int max_min_part) {
+                                                int num_kv_heads, int target, int min_part,
+                                                int max_min_part) {
   const int64_t want = total_blocks * num_kv_heads;
   const int most = max(max_min_part >> lb, longest / (kLongPositions / max_min_part));
-  const int least = min(max(longest / 8, kMinPartPositions >> lb), most);
+  const int least = min(max(longest / 8, min_part >> lb), most);
   return max(max(least, 1), static_cast<int>((want + target - 1) / target));
 }
 
@@ -89,7 +89,7 @@ __device__ __forceinline__ int whole_blocks(int num_seqs, int num_kv_heads, int 
 
 __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(
     const int32_t* __restrict__ context_lens, int num_seqs, int num_kv_heads, int block_size,
-    int lb, int width, int split_k, int target, int max_min_part, int max_items,
+    int lb, int width, int split_k, int target, int min_part, int max_min_part, int max_items,
     PlanItem* __restrict__ plan, int32_t* __restrict__ counters, int num_counters) {
   __shared__ int s_ctx[kMaxPlanSeqs];
   __shared__ int s_order[kMaxPlanSeqs];  // rank -> sequence
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(
   __syncthreads();
   const int pb_global =
       split_k == 0 ? step_part_blocks(s_total_blocks, s_longest, lb, num_kv_heads, target,
-                                    max_min_part) : 1;
+                                    min_part, max_min_part) : 1;
 
   // Rank sequences by block count, longest first (ties keep batch order).
   const bool sort = num_seqs <= kSortLimit;
@@ -240,7 +240,8 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(
 // 128-2048 8.6 -> 4.5.
 __global__ __launch_bounds__(kPlanThreads) void decode_plan_wave_kernel(
     const int32_t* __restrict__ context_lens, int num_seqs, int num_kv_heads, int block_size,
-    int lb, int width, int target, int max_min_part, int max_items, PlanItem* __restrict__ plan,
+    int lb, int width, int target, int min_part, int max_min_part, int max_items,
+    PlanItem* __restrict__ plan,
     int32_t* __restrict__ counters, int num_counters) {
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_wave_kernel(
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) longest = max(longest, __shfl_xor(longest, o, kWave));
   const int pb = step_part_blocks(wave_sum_int(nb), longest, lb, num_kv_heads, target,
-                                    max_min_part);
+                                    min_part, max_min_part);
   const int np = nb <= whole_blocks(num_seqs, num_kv_heads, lb) ? 1 : (nb + pb - 1) / pb;
   const int last = nb - (np - 1) * pb;  // blocks of the last part, the odd one
   // Over the sequences ahead of this lane's (longer, or as long and earlier
@@ -331,18 +332,19 @@ int64_t decode_plan_bytes(int32_t num_seqs, int32_t num_kv_heads, int32_t split_
 
 int32_t launch_decode_plan(const int32_t* context_lens, int32_t num_seqs, int32_t num_kv_heads,
                            int32_t block_size, int32_t block_table_width, int32_t split_k,
-                           bool vector, PlanItem* plan, int32_t* counters, hipStream_t stream) {
+                           bool vector, PlanItem* plan, int32_t* counters, hipStream_t stream,
+                           int32_t min_part) {
   const int32_t max_min_part = vector ? kMaxMinPartVector : kMaxMinPart;
   if (num_seqs <= kWave && split_k == 0) {
     decode_plan_wave_kernel<<<1, kPlanThreads, 0, stream>>>(
         context_lens, num_seqs, num_kv_heads, block_size, ilog2(block_size), block_table_width,
-        kTargetItems, max_min_part, decode_max_items(num_seqs, num_kv_heads, split_k), plan,
+        kTargetItems, min_part, max_min_part, decode_max_items(num_seqs, num_kv_heads, split_k), plan,
         counters, counters != nullptr ? num_seqs * num_kv_heads : 0);
     return check_launch("decode plan");
   }
   decode_plan_kernel<<<1, kPlanThreads, 0, stream>>>(
       context_lens, num_seqs, num_kv_heads, block_size, ilog2(block_size), block_table_width,
-      split_k, kTargetItems, max_min_part,
+      split_k, kTargetItems, min_part, max_min_part,
       decode_max_items(num_seqs, num_kv_heads, split_k), plan, counters,
       counters != nullptr ? num_seqs * num_kv_heads : 0);
   return check_launch("decode plan");

@@ -165,6 +165,13 @@ int32_t mi_quant_prefill(const void* query, int64_t q_token_stride, int64_t q_he
                          int32_t head_dim, int32_t block_size, int32_t num_blocks, float scale,
                          int32_t dtype, int32_t code, void* stream);
 
+/*
+ * Which capture into a graph the stream is in: *id is 0 outside any, otherwise
+ * the capture's own number. For callers that keep workspaces: two graphs that are
+ * replayed at once must not share one.
+ */
+int32_t mi_stream_capture_id(void* stream, uint64_t* id);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

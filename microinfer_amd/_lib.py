@@ -158,6 +158,7 @@ SIGNATURES = {
         [_P, _I64, _I64, *_QUANT_CACHE, _P, _I64, _I32, _P, _I64, _P, _I64, _I64, _P, _I64, _P,
          _I32, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _I32, _P],
     ),
+    "mi_stream_capture_id": (_I32, [_P, _P]),
     "mi_quant_prefill_workspace_bytes": (_I64, [_I32] * 7),
     "mi_quant_prefill_plan": (_I32, [_P, _P, *[_I32] * 8, _P, _I64, _P]),
     "mi_quant_prefill": (

@@ -324,3 +324,17 @@ extern "C" int32_t mi_quant_prefill(
   a.ws_ml = reinterpret_cast<float*>(ws + l.ml);
   return launch_quant_decode_mfma(a, l.rows, dtype, code, s);
 }
+
+extern "C" int32_t mi_stream_capture_id(void* stream, uint64_t* id) {
+  using namespace mi;
+  clear_error();
+  if (id == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "mi_stream_capture_id: null pointer");
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long number = 0;
+  const hipError_t err =
+      hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &number);
+  if (err != hipSuccess)
+    return fail(MI_ERR_HIP, std::string("mi_stream_capture_id: ") + hipGetErrorString(err));
+  *id = status == hipStreamCaptureStatusNone ? 0 : number;
+  return MI_OK;
+}

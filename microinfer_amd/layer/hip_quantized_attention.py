@@ -9,6 +9,7 @@ and the softmax weights (V) in float32.
 
 from __future__ import annotations
 
+import ctypes
 import threading
 from dataclasses import dataclass, field
 
@@ -23,9 +24,15 @@ _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
 def _call_place(device: torch.device) -> tuple:
-    """What calls that run one after the other have in common."""
-    return (threading.get_ident(), _lib.stream_handle(device),
-            torch.cuda.is_current_stream_capturing())
+    """What calls that run one after the other have in common: thread, stream and
+    the capture that they are in, if any."""
+    stream, capture = _lib.stream_handle(device), 0
+    if torch.cuda.is_current_stream_capturing():
+        number = ctypes.c_uint64()
+        _lib.check(_lib.load().mi_stream_capture_id(stream, ctypes.addressof(number)),
+                   "mi_stream_capture_id")
+        capture = number.value
+    return threading.get_ident(), stream, capture
 
 
 @dataclass(frozen=True)
@@ -188,6 +195,8 @@ class QuantizedPrefillPlan:
                 self.cu_seqlens_q.data_ptr(), self.cu_seqlens_k.data_ptr(), tokens, requests,
                 self.max_seqlen_q, *sizes, have.data_ptr(), self.workspace_bytes, place[1])
             _lib.check(status, "mi_quant_prefill_plan")
+            # A graph keeps what is made in its capture: only the plan's own does
+            # for further calls.
             if not place[2] or not self._workspaces:
                 self._workspaces[place] = have
         return have

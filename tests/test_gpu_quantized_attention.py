@@ -416,6 +416,52 @@ def test_decode_replays_with_other_lengths():
                         DECODE["f16"])
 
 
+def test_graphs_do_not_share_a_plans_workspace():
+    """A plan that one graph holds, called in the capture of another: both are
+    replayed at once, on two streams."""
+    rng = np.random.default_rng(23)
+    contexts, lengths = [1900, 700, 1200], [3, 200, 4]
+    twin, tables, _ = decode_case(rng, contexts, (8, 2, 128, 16, "paired"), "fp8", "bf16")
+    at, lens = ints(tables), ints(contexts)
+    sizes = dict(num_q_heads=8, num_kv_heads=2, head_dim=128, dtype=torch.bfloat16,
+                 block_size=16, block_table_width=at.shape[1])
+    cu_k = ints(np.cumsum([0] + contexts).tolist())
+    one, other = (query_of(rng, 3, 8, 128, "bf16") for _ in range(2))
+    cases = [(one, other, [1, 1, 1], lambda: quantized_decode_plan(lens, **sizes),
+              lambda q, plan: hip_quantized_decode(q, *twin.tensors, at, lens, plan=plan))]
+    for new in ([3, 2, 4], lengths):
+        cu_q = ints(np.cumsum([0] + new).tolist())
+        rows, most = sum(new), max(new)
+        one, other = (query_of(rng, rows, 8, 128, "bf16") for _ in range(2))
+        cases.append((
+            one, other, new,
+            lambda cu_q=cu_q, rows=rows, most=most: quantized_prefill_plan(
+                cu_q, cu_k, num_tokens=rows, max_seqlen_q=most, **sizes),
+            lambda q, plan, cu_q=cu_q, most=most: hip_quantized_prefill(
+                q, *twin.tensors, cu_q, cu_k, at, max_seqlen_q=most, plan=plan)))
+    side = torch.cuda.Stream()
+    for one, other, new, planned, run in cases:
+        held = planned()
+        run(one, held)  # kernels are loaded
+        torch.cuda.synchronize()
+        first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first):
+            plan = planned()
+            mine = run(one, plan)
+        first.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(second):
+            theirs = run(other, plan)
+        for _ in range(10):
+            first.replay()
+            with torch.cuda.stream(side):
+                second.replay()
+        torch.cuda.synchronize()
+        cu_q = np.cumsum([0] + new).tolist()
+        for got, q in ((mine, one), (theirs, other)):
+            check_attention(got, q, twin, tables, contexts, cu_q, 128 ** -0.5, VARLEN["bf16"])
+
+
 def test_results_repeat():
     rng = np.random.default_rng(11)
     contexts = [3000, 40, 1500]

@@ -220,3 +220,8 @@ def test_c_prefill_validates_its_requests():
     assert plan(block=24) == 1 and plan(width=-1) == 1 and plan(width=1 << 27) == 2
     assert plan(cu_q=None) == 1 and plan(cu_k=None) == 1
     assert plan(ws=None) == 3 and plan(nbytes=need - 1) == 3 and plan(ws=4104) == 3
+
+
+def test_capture_id_wants_somewhere_to_put_it():
+    lib = _lib.load()
+    assert lib.mi_stream_capture_id(None, None) == 1 and "null" in _lib.last_error()

@@ -16,7 +16,8 @@
  *   MI_CODE_INT8  -127 .. 127
  * head_dim is a power of two from 16 to 256, block_size a power of two
  * (MI_ERR_UNSUPPORTED / MI_ERR_INVALID_ARGUMENT otherwise). The readers take
- * any float32 scales; mi_quant_append writes powers of two.
+ * any scales that are not negative (a NaN makes NaN of what it scales);
+ * mi_quant_append writes powers of two.
  */
 #ifndef MI_QUANT_H_
 #define MI_QUANT_H_
@@ -133,7 +134,10 @@ int32_t mi_quant_decode(const void* query, int64_t q_token_stride, int64_t q_hea
  * rows are cu_seqlens_q[r] .. cu_seqlens_q[r + 1], its context
  * cu_seqlens_k[r + 1] - cu_seqlens_k[r] positions, the mask causal and
  * bottom-right aligned. Rows that see no position give zeros. max_seqlen_q
- * bounds the query rows of any request: rows past it may stay unwritten.
+ * bounds the query rows of any request: rows past it may stay unwritten. A NaN
+ * makes NaN of the rows that see it; one in V may also do so to earlier rows of
+ * its own request (0 times it is NaN), but to none of another, and what lies
+ * behind a context or outside the pool reaches no row.
  *
  * Where mi_quant_prefill_workspace_bytes() is not 0, calls of these sizes take
  * a workspace of so many bytes (256-byte aligned) in which

@@ -61,7 +61,7 @@ __device__ __forceinline__ Codes8 narrow8(const float* x) {
   return Codes8{C::narrow4(x), C::narrow4(x + 4)};
 }
 
-// Eight neighbouring elements as float32, and back.
+// Eight neighbouring elements as float32.
 template <typename E>
 __device__ __forceinline__ void load8(const typename E::raw* p, float* x) {
   using R = typename E::raw;
@@ -71,18 +71,6 @@ __device__ __forceinline__ void load8(const typename E::raw* p, float* x) {
     const Pack<R, N> v = load_pack<R, N>(p + j);
 #pragma unroll
     for (int i = 0; i < N; ++i) x[j + i] = E::load(v.v[i]);
-  }
-}
-template <typename E>
-__device__ __forceinline__ void store8(typename E::raw* p, const float* x) {
-  using R = typename E::raw;
-  constexpr int N = 16 / sizeof(R);
-#pragma unroll
-  for (int j = 0; j < 8; j += N) {
-    Pack<R, N> v;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v.v[i] = E::store(x[j + i]);
-    store_pack<R, N>(p + j, v);
   }
 }
 

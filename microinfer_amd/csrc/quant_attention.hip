@@ -32,7 +32,8 @@ constexpr int32_t kMinPart = 128;
 
 // Whether decode steps go to the MFMA kernel, cache alignment aside.
 bool decode_on_mfma(int32_t head_dim, int32_t group, int32_t block_size) {
-  return quant_decode_mfma_takes(head_dim, block_size) && quant_decode_row_groups(group) == 1;
+  return quant_decode_mfma_takes(head_dim, block_size) &&
+         quant_decode_row_groups(group, head_dim) == 1;
 }
 
 // Varlen calls of at most kFewRows rows of a request at a KV head, or kFewInAll of
@@ -73,8 +74,8 @@ VarlenLayout varlen_layout(int32_t num_tokens, int32_t num_requests, int32_t max
   }
   l.rows = static_cast<int32_t>(rows);
   l.items = decode_max_items(num_requests, num_kv_heads, 0);
-  l.num_counters =
-      static_cast<int64_t>(num_requests) * num_kv_heads * quant_decode_row_groups(l.rows);
+  l.num_counters = static_cast<int64_t>(num_requests) * num_kv_heads *
+                   quant_decode_row_groups(l.rows, head_dim);
   if (l.num_counters > INT_MAX) return l;
   auto room = [&](int64_t bytes) {
     const int64_t at = l.total;

@@ -1,6 +1,6 @@
 // Attention of few query rows over an 8-bit K/V cache on MFMA: decode steps, and
-// requests of a few tokens (drafts to verify, ends of prompts). head_dim 64 or
-// 128, blocks of at least 16, queries of any type.
+// requests of a few tokens (drafts to verify, ends of prompts). head_dim 64, 128
+// or 256, blocks of at least 16, queries of any type.
 //
 // out = softmax(scale * q . (k * ks)) (v * vs), with one ks and vs for each
 // block and KV head. Bound by HBM for long contexts (two bytes a position and
@@ -53,15 +53,21 @@ __device__ __forceinline__ float max16(float v) {
 // halves.
 template <int D>
 __device__ __forceinline__ int swz_k(int r) {
-  return D == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+  return D == 256 ? r & 15 : D == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
 template <int D>
 __device__ __forceinline__ int swz_v(int r, int half) {
-  return D == 128 ? ((r >> 1) & 3) ^ (4 * half) : ((r >> 2) & 1) ^ (2 * half);
+  return D == 256   ? (r & 7) ^ (8 * half)
+         : D == 128 ? ((r >> 1) & 3) ^ (4 * half)
+                    : ((r >> 2) & 1) ^ (2 * half);
 }
 
+// Waves a SIMD that the registers are kept for: of the workgroups that a CU's LDS
+// has room for.
+constexpr int waves_of(int D, int NS) { return D < 256 && NS == 1 ? 4 : 2; }
+
 template <typename E, typename C, int D, int NC, int NW, int NS>
-__global__ __launch_bounds__(kWave * NW, NS == 1 ? 4 : 2) void quant_decode_kernel(
+__global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kernel(
     const QuantAttnArgs a) {
   using R = typename E::raw;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
@@ -554,7 +560,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const int32_t* __restrict
 }  // namespace
 
 bool quant_decode_mfma_takes(int32_t head_dim, int32_t block_size) {
-  return (head_dim == 128 || head_dim == 64) && block_size >= kHalf;
+  return (head_dim == 256 || head_dim == 128 || head_dim == 64) && block_size >= kHalf;
 }
 
 bool quant_mfma_aligned(const QuantCache& c) {
@@ -563,14 +569,15 @@ bool quant_mfma_aligned(const QuantCache& c) {
   return low % 16 == 0 && c.ts < (int64_t(1) << 26);
 }
 
-int32_t quant_decode_row_groups(int32_t rows) {
+int32_t quant_decode_row_groups(int32_t rows, int32_t head_dim) {
+  if (head_dim == 256) return (rows - 1) / kCols + 1;
   return rows <= kCols ? 1 : (rows - 1) / (2 * kCols) + 1;
 }
 
 int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, int32_t code,
                                  hipStream_t stream) {
   a.head_rows = rows;
-  a.row_groups = quant_decode_row_groups(rows);
+  a.row_groups = quant_decode_row_groups(rows, a.c.dim);
   // r * inverse >> 24 is r / group for r * group < 2^24, with no overflow for
   // r < 2^8.
   if (rows > 256) return fail(MI_ERR_UNSUPPORTED, "quantized decode: too many rows");
@@ -591,6 +598,7 @@ int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, i
       kernel<<<static_cast<uint32_t>(grid), kWave * 8, 0, stream>>>(a);
       return check_launch("quantized decode");
     };
+    if (a.c.dim == 256) return go(quant_decode_kernel<E, C, 256, 1, 8, 1>);
     const bool wide = a.c.dim == 128;
     if (rows > kCols)
       return wide ? go(quant_decode_kernel<E, C, 128, 2, 8, 2>)

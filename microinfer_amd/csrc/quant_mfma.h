@@ -77,14 +77,12 @@ __device__ __forceinline__ bf16x8_t widen_operand(uint32_t lo, uint32_t hi) {
 template <int N, typename V>
 __device__ __forceinline__ void split8(const float* x, V* part) {
   using T = typename std::conditional<std::is_same<V, bf16x8_t>::value, __bf16, _Float16>::type;
+  // The compiler may fuse a product with its conversion to f16, which rounds
+  // once instead of twice, in one of its uses: parts would not fit each other.
+  static_assert(N == 1 || std::is_same<T, __bf16>::value, "parts are bf16");
   float rest[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    rest[i] = x[i];
-    // The compiler may fuse a product with its conversion to f16, which rounds
-    // once instead of twice, in one of its uses: the parts would not fit.
-    if constexpr (N > 1 && std::is_same<T, _Float16>::value) asm("" : "+v"(rest[i]));
-  }
+  for (int i = 0; i < 8; ++i) rest[i] = x[i];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
 #pragma unroll
@@ -130,7 +128,7 @@ int32_t launch_quant_prefill_mfma(const QuantAttnArgs& a, int32_t dtype, int32_t
 // the lengths of requests for its plan.
 bool quant_decode_mfma_takes(int32_t head_dim, int32_t block_size);
 bool quant_mfma_aligned(const QuantCache& c);
-int32_t quant_decode_row_groups(int32_t rows);
+int32_t quant_decode_row_groups(int32_t rows, int32_t head_dim);
 int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, int32_t code,
                                  hipStream_t stream);
 int32_t launch_few_rows(const int32_t* cu_q, const int32_t* cu_k, int32_t num_seqs, int32_t* lens,

@@ -21,9 +21,12 @@
 //  * O^T += V^T . P^T on the same instruction, V^T by transposing LDS reads. A
 //    weight e = 2^(score - m) meets V as e * vs * 2^(m - mo) in f16, of which mo
 //    keeps the largest of the row between 2^10 and 2^15: rounding takes 2^-11 of a
-//    weight (an eighth of what bf16 would, a quarter or less of the bf16 output's
-//    own), and what f16 cannot hold is 2^-35 of the largest. f16 queries, whose
-//    output is as fine, have two such parts; f32 ones three in bf16.
+//    weight (an eighth of what bf16 would, and half a step of an f16 output), and
+//    what f16 cannot hold is 2^-35 of the largest. Against float64 a bf16 output is
+//    off by its own rounding (2^-9.2 root mean square), an f16 one by 2^-11.9, of
+//    which its own makes 2^-12.2: a second part would take that away and a fifth
+//    more time (six prompts 468 us for four layers, 386 without). f32 queries have
+//    three parts in bf16.
 //  * Row blocks whose keys are split publish theirs; the last arrival merges
 //    them in order.
 #include <algorithm>
@@ -79,7 +82,7 @@ template <>
 struct Meets<F16> {
   using Query = f16x8_t;
   using Weight = f16x8_t;
-  static constexpr int kQueries = 1, kWeights = 2;
+  static constexpr int kQueries = 1, kWeights = 1;
 };
 template <>
 struct Meets<F32> {

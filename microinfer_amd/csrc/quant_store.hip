@@ -75,7 +75,7 @@ namespace {
 
 constexpr int kGatherThreads = 256;
 
-// store8 past the caches, for rows that are written once and are many.
+// Eight elements of a row, past the caches: rows are written once and are many.
 template <typename E>
 __device__ __forceinline__ void store8_past(typename E::raw* p, const float* x) {
   using R = typename E::raw;

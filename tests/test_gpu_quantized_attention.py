@@ -16,10 +16,10 @@ pytestmark = pytest.mark.gpu
 
 # How a softmax weight is held for its product with V (``check_attention``).
 # Decode: two bf16 parts for 16-bit queries (half a step of each: 2^-8 of 2^-8),
-# three for float32. Varlen: one f16 part for bf16 queries (half a step, 2^-11),
-# two for f16 ones, three bf16 parts for float32.
+# three for float32. Varlen: one f16 part for 16-bit queries (half a step, 2^-11),
+# three bf16 parts for float32.
 DECODE = {"bf16": (16, 0), "f16": (16, 0), "f32": (24, 0)}
-VARLEN = {"bf16": (11, 2.0 ** -35), "f16": (22, 2.0 ** -35), "f32": (24, 0)}
+VARLEN = {"bf16": (11, 2.0 ** -35), "f16": (11, 2.0 ** -35), "f32": (24, 0)}
 
 SHAPES = [  # Hq, Hkv, D, block, layout
     (16, 8, 128, 16, "paired"), (32, 8, 128, 32, "head_major"), (5, 5, 128, 64, "token_major"),
@@ -78,7 +78,8 @@ def test_what_the_context_ends_before_does_not_matter(kind):
     blocks that the table does not name."""
     rng = np.random.default_rng(2)
     contexts = [19, 5, 160, 513]
-    for shape in ((4, 2, 128, 16, "paired"), (4, 2, 64, 32, "paired"), (4, 4, 32, 16, "paired")):
+    for shape in ((4, 2, 128, 16, "paired"), (4, 2, 64, 32, "paired"), (4, 4, 32, 16, "paired"),
+                  (4, 2, 256, 16, "paired")):
         twin, tables, query = decode_case(rng, contexts, shape, kind, "bf16")
         block = shape[3]
         used = {tables[s][j] for s, c in enumerate(contexts) for j in range(-(-c // block))}
@@ -99,7 +100,8 @@ def test_what_the_context_ends_before_does_not_matter(kind):
 
 
 @pytest.mark.parametrize("shape", [(4, 2, 128, 16, "paired"), (4, 2, 64, 16, "paired"),
-                                   (4, 2, 128, 64, "paired"), (3, 3, 32, 16, "paired")])
+                                   (4, 2, 128, 64, "paired"), (3, 3, 32, 16, "paired"),
+                                   (4, 2, 256, 16, "paired")])
 def test_blocks_outside_the_pool_are_masked(shape):
     rng = np.random.default_rng(3)
     contexts = [100, 900, 40, 33]
@@ -116,7 +118,7 @@ def test_blocks_outside_the_pool_are_masked(shape):
                     DECODE["f16"])
 
 
-@pytest.mark.parametrize("dim", [128, 64, 32])
+@pytest.mark.parametrize("dim", [256, 128, 64, 32])
 def test_nan_reaches_the_output(dim):
     """A NaN code or scale inside a context makes its rows NaN, wherever the
     context is split, and no other sequence's."""
@@ -217,7 +219,8 @@ def test_prefill_lengths(kind, contexts, lengths):
     ((12, 2, 128, 16, "paired"), [10, 9, 1, 6, 3]),  # 60, in two groups
     ((3, 1, 64, 16, "token_major"), [11, 21, 5, 16, 13]),  # 63
     ((20, 1, 128, 64, "paired"), [1, 3, 2, 0, 3]),
-    ((17, 1, 64, 16, "paired"), [0, 0, 1, 1, 0])])
+    ((17, 1, 64, 16, "paired"), [0, 0, 1, 1, 0]),
+    ((6, 2, 256, 32, "head_major"), [3, 0, 5, 1, 4])])  # 18, of 256 dims
 def test_few_rows_a_request(kind, dtype, shape, lengths):
     """Requests laid out like decode steps: whole and in parts, rows in one
     group and in several, tokens that see less than the last, rows that see
@@ -262,7 +265,7 @@ def test_one_request_of_rows_in_several_groups(dtype, shape, length, context):
 
 
 @pytest.mark.parametrize("hq,hkv", [(17, 1), (32, 1), (64, 2), (66, 2), (40, 1)])
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [64, 128, 256])
 def test_decode_of_large_groups(hq, hkv, dim):
     rng = np.random.default_rng(hq)
     contexts = [1500, 1, 77]

@@ -45,6 +45,11 @@ bool decode_on_mfma(int32_t head_dim, int32_t group, int32_t block_size) {
 // 279, 8 of 16 on 4000 199 / 183, 32 of 16 on 2000 255 / 221.
 constexpr int32_t kFewRows = 32;
 constexpr int32_t kFewInAll = 128;
+// Of heads of 256, whose longer requests are the vector kernel's, up to so many of
+// a request, and so many of all for the workspace's size (8 requests of 30 tokens
+// on 4000 531 us, on the vector kernel 6420).
+constexpr int32_t kFewRows256 = 256;
+constexpr int32_t kFewInAll256 = 4096;
 
 // A varlen call's sizes and where its workspace holds what.
 struct VarlenLayout {
@@ -65,7 +70,9 @@ VarlenLayout varlen_layout(int32_t num_tokens, int32_t num_requests, int32_t max
     return l;
   const int32_t group = num_q_heads / num_kv_heads;
   const int64_t rows = static_cast<int64_t>(std::min(max_seqlen_q, num_tokens)) * group;
-  l.few = (rows <= kFewRows || rows * num_requests <= kFewInAll) &&
+  const int64_t in_all = rows * num_requests;
+  l.few = (rows <= kFewRows || in_all <= kFewInAll ||
+           (head_dim == 256 && rows <= kFewRows256 && in_all <= kFewInAll256)) &&
           num_requests <= kMaxPlanSeqs && quant_decode_mfma_takes(head_dim, block_size);
   if (!l.few) {
     l.total = quant_prefill_workspace(num_tokens, num_requests, group, num_kv_heads, head_dim,

@@ -253,7 +253,8 @@ def test_few_rows_a_request(kind, dtype, shape, lengths):
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("shape,length,context", [
     ((8, 2, 128, 16, "paired"), 30, 1900), ((3, 1, 64, 32, "head_major"), 42, 700),
-    ((128, 1, 128, 16, "paired"), 1, 2500), ((16, 2, 64, 16, "paired"), 16, 50)])
+    ((128, 1, 128, 16, "paired"), 1, 2500), ((16, 2, 64, 16, "paired"), 16, 50),
+    ((4, 1, 256, 16, "paired"), 61, 900)])
 def test_one_request_of_rows_in_several_groups(dtype, shape, length, context):
     rng = np.random.default_rng(length)
     hq, hkv, dim, block, _ = shape

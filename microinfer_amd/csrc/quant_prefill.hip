@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
   auto look_up = [&](int h) {
     const int pos = key0 + 16 * h;
     Half x{0x1p-126f, 0.f, 0.f, 0};
-    int64_t at = 0;  // an invalid block reads block 0
+    int64_t at = 1;  // not there: block 0 is read
     if (pos < key_end) {
       const int blk = table[pos >> c.log2_block];
       if (blk >= 0 && blk < c.num_blocks) {
@@ -211,36 +211,39 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
     s_half[h % kInfo] = x;
   };
   Word4 k_reg[kLoads], v_reg[kLoads];
+  bool there[kLoads];
   auto load_step = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
-      const int64_t at = s_at[(t * kHalves + (key + u * kSpread) / 16) % kInfo];
-      k_reg[u] = *reinterpret_cast<const Word4*>(kc + at);
-      v_reg[u] = *reinterpret_cast<const Word4*>(vc + at);
+      const int k = key + u * kSpread;
+      const int64_t at = s_at[(t * kHalves + k / 16) % kInfo];
+      there[u] = (at & 1) == 0 & key0 + t * kKeys + k < key_end;
+      k_reg[u] = *reinterpret_cast<const Word4*>(kc + (at & ~int64_t(1)));
+      v_reg[u] = *reinterpret_cast<const Word4*>(vc + (at & ~int64_t(1)));
     }
   };
-  // `first`: which of the two chunks goes first, for the banks.
-  auto put = [&](auto lo, auto hi, uint16_t* row, int swz, int first)
-      __attribute__((always_inline)) {
-    using V = decltype(lo);
-    *reinterpret_cast<V*>(row + ((chunk + first) ^ swz) * 8) = first ? hi : lo;
-    *reinterpret_cast<V*>(row + ((chunk + 1 - first) ^ swz) * 8) = first ? lo : hi;
-  };
+  // The second of a thread's two chunks of V goes first for odd keys, for the banks.
+  const int first = D == 128 ? key & 1 : 0;
   auto land_step = [&](int t, int buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const int k = key + u * kSpread;
       const Word4& w = k_reg[u];
-      put(widen<Query, C>(w.w[0], w.w[1]), widen<Query, C>(w.w[2], w.w[3]), s_k[buf] + k * D,
-          swz_k<D>(k), 0);
+      auto put = [&](auto x, uint16_t* row, int at) __attribute__((always_inline)) {
+        *reinterpret_cast<decltype(x)*>(row + at * 8) = x;
+      };
+      put(widen<Query, C>(w.w[0], w.w[1]), s_k[buf] + k * D, chunk ^ swz_k<D>(k));
+      put(widen<Query, C>(w.w[2], w.w[3]), s_k[buf] + k * D, (chunk + 1) ^ swz_k<D>(k));
       // Keys that nothing may see may be NaN, which 0 times does not make 0.
-      const bool there =
-          key0 + t * kKeys + k < key_end && s_half[(t * kHalves + k / 16) % kInfo].ok;
       Word4 v = v_reg[u];
+      if (__ballot(!there[u]) != 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v.w[i] = there ? v.w[i] : 0;
-      put(widen<Weight, C>(v.w[0], v.w[1]), widen<Weight, C>(v.w[2], v.w[3]), s_v[buf] + k * D,
-          swz_v<D>(k), D == 128 ? k & 1 : 0);
+        for (int i = 0; i < 4; ++i) v.w[i] = there[u] ? v.w[i] : 0;
+      }
+      put(widen<Weight, C>(first ? v.w[2] : v.w[0], first ? v.w[3] : v.w[1]), s_v[buf] + k * D,
+          (chunk + first) ^ swz_v<D>(k));
+      put(widen<Weight, C>(first ? v.w[0] : v.w[2], first ? v.w[1] : v.w[3]), s_v[buf] + k * D,
+          (chunk + 1 - first) ^ swz_v<D>(k));
     }
   };
 

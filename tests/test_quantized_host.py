@@ -72,8 +72,8 @@ def _args(order, over):
 
 def _append(lib, **over):
     order = dict(rows_k=4096, kts=256, khs=128, rows_v=8192, vts=256, vhs=128, **CACHE, slots=4096,
-                 is64=0, plan=None, plan_bytes=0, tokens=3, heads=2, dim=128, block=16, blocks=8, dtype=2,
-                 code=0)
+                 is64=0, plan=None, plan_bytes=0, tokens=3, heads=2, dim=128, block=16, blocks=8,
+                 dtype=2, code=0)
     return lib.mi_quant_append(*_args(order, over), None)
 
 

@@ -1,6 +1,7 @@
 """Decode and varlen attention over an 8-bit cache against float64."""
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -10,6 +11,8 @@ from microinfer_amd.layer.hip_quantized_attention import (hip_quantized_decode,
                                                           hip_quantized_prefill,
                                                           quantized_decode_plan,
                                                           quantized_prefill_plan)
+from microinfer_amd.worker.hip_quantized_kv import quantized_append, quantized_gather
+from microinfer_amd.worker.kv_cache import KVCache
 from tests.quantized_support import CODES, DTYPES, Twin, check_attention, ints, tables_of
 
 pytestmark = pytest.mark.gpu
@@ -474,3 +477,149 @@ def test_results_repeat():
     for _ in range(5):
         assert torch.equal(first, hip_quantized_decode(query, *twin.tensors, ints(tables),
                                                        ints(contexts)))
+
+
+def test_two_threads_with_the_same_plans():
+    """Plans made by one thread, called by two at once, each on a stream of its
+    own: workspaces and counters are not shared."""
+    rng = np.random.default_rng(31)
+    contexts = [1900, 40, 1300]
+    twin, tables, _ = decode_case(rng, contexts, (8, 2, 128, 16, "paired"), "fp8", "bf16")
+    at, lens = ints(tables), ints(contexts)
+    cu_k = ints(np.cumsum([0] + contexts).tolist())
+    sizes = dict(num_q_heads=8, num_kv_heads=2, head_dim=128, dtype=torch.bfloat16,
+                 block_size=16, block_table_width=at.shape[1])
+    news = [[1, 1, 1], [5, 1, 3], [150, 40, 90]]
+    offsets = [ints(np.cumsum([0] + new).tolist()) for new in news]
+    plans = [quantized_decode_plan(lens, **sizes)] + [
+        quantized_prefill_plan(cu_q, cu_k, num_tokens=sum(new), max_seqlen_q=max(new), **sizes)
+        for cu_q, new in zip(offsets[1:], news[1:])]
+
+    def run(i, q):
+        if i == 0:
+            return hip_quantized_decode(q, *twin.tensors, at, lens, plan=plans[0])
+        return hip_quantized_prefill(q, *twin.tensors, offsets[i], cu_k, at,
+                                     max_seqlen_q=max(news[i]), plan=plans[i])
+
+    queries = [[query_of(rng, sum(new), 8, 128, "bf16") for new in news] for _ in range(2)]
+    torch.cuda.synchronize()
+    results, errors = [None, None], []
+
+    def work(who):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    outs = [run(i, q) for i, q in enumerate(queries[who])]
+                torch.cuda.current_stream().synchronize()
+            results[who] = outs
+        except Exception as error:  # reported by the test's own thread
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(who,)) for who in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not errors
+    for who in range(2):
+        for got, q, cu_q in zip(results[who], queries[who], offsets):
+            check_attention(got, q, twin, tables, contexts, cu_q.tolist(), 128 ** -0.5,
+                            VARLEN["bf16"])
+
+
+@pytest.mark.parametrize("layout", ["paired", "token_major"])
+def test_offsets_past_32_bits(layout):
+    """Blocks that lie more than 2^31 bytes into a pool hold and give what those of
+    a small one do."""
+    rng = np.random.default_rng(32)
+    blocks, heads, dim, block = 150000, 8, 128, 16
+    contexts = [500, 37]
+    need = [-(-c // block) for c in contexts]
+    high = [[blocks - 1 - 7 * j - 1000 * s for j in range(n)] + [-1] * (max(need) - n)
+            for s, n in enumerate(need)]
+    low = [[j + 40 * s for j in range(n)] + [-1] * (max(need) - n) for s, n in enumerate(need)]
+    rows = [torch.from_numpy(rng.standard_normal((sum(contexts), heads, dim))).bfloat16().cuda()
+            for _ in range(2)]
+    query = query_of(rng, 3, 16, dim, "bf16")
+    chunk = query_of(rng, 200, 16, dim, "bf16")
+    cu_k = ints([0, contexts[0], sum(contexts)])
+    outs = []
+    for count, tables in ((blocks, high), (80, low)):
+        cache = KVCache(1, count, block, heads, dim, dtype=torch.float8_e4m3fn, device="cuda",
+                        layout=layout).layer(0)
+        tensors = cache.keys, cache.values, cache.key_scales, cache.value_scales
+        slots = [t[p // block] * block + p % block for t, c in zip(tables, contexts)
+                 for p in range(c)]
+        at = ints(tables)
+        for part in (slice(0, 400), slice(400, None)):  # planned, scanned
+            quantized_append(*tensors, torch.tensor(slots[part], device="cuda"),
+                             rows[0][part], rows[1][part])
+        outs.append([
+            *quantized_gather(*tensors, at, cu_k, sum(contexts)),
+            hip_quantized_decode(query[:2], *tensors, at, ints(contexts)),
+            hip_quantized_prefill(query, *tensors, ints([0, 2, 3]), cu_k, at, max_seqlen_q=2),
+            hip_quantized_prefill(chunk, *tensors, ints([0, 170, 200]), cu_k, at,
+                                  max_seqlen_q=170)])
+        del cache, tensors
+    for far, near in zip(*outs):
+        assert torch.equal(far, near)
+    assert not torch.equal(outs[0][0], torch.zeros_like(outs[0][0]))
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 128, 256, "paired"), (2, 1, 64, 1024, "head_major"),
+                                   (3, 1, 256, 128, "paired"), (2, 2, 32, 512, "token_major")])
+def test_large_blocks(shape):
+    rng = np.random.default_rng(shape[3])
+    contexts = [1500, 3, 1024, 700]
+    twin, tables, query = decode_case(rng, contexts, shape, "int8", "f16")
+    scale = 1 / math.sqrt(shape[2])
+    got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+    check_attention(got, query, twin, tables, contexts, list(range(5)), scale, DECODE["f16"])
+    for lengths in ([3, 1, 0, 2], [130, 3, 1, 64]):
+        query = query_of(rng, sum(lengths), shape[0], shape[2], "f16")
+        got, cu_q = prefill(query, twin, tables, contexts, lengths)
+        check_attention(got, query, twin, tables, contexts, cu_q, scale, VARLEN["f16"])
+
+
+def test_the_most_sequences():
+    rng = np.random.default_rng(33)
+    contexts = [int(c) for c in rng.integers(0, 40, 4096)]
+    shape = (2, 1, 64, 16, "paired")
+    twin, tables, query = decode_case(rng, contexts, shape, "fp8", "bf16")
+    got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+    check_attention(got, query, twin, tables, contexts, list(range(4097)), 0.125, DECODE["bf16"])
+    plan = quantized_prefill_plan(
+        ints(range(4097)), ints(np.cumsum([0] + contexts).tolist()), num_tokens=4096,
+        max_seqlen_q=1, num_q_heads=2, num_kv_heads=1, head_dim=64, dtype=query.dtype,
+        block_size=16, block_table_width=len(tables[0]))
+    got = hip_quantized_prefill(query, *twin.tensors, plan.cu_seqlens_q, plan.cu_seqlens_k,
+                                ints(tables), max_seqlen_q=1, plan=plan)
+    check_attention(got, query, twin, tables, contexts, list(range(4097)), 0.125, DECODE["bf16"])
+    more = [1] * 4097
+    with pytest.raises(ValueError, match="4096"):
+        hip_quantized_decode(query_of(rng, 4097, 2, 64, "bf16"), *twin.tensors,
+                             torch.zeros(4097, 1, dtype=torch.int32, device="cuda"), ints(more))
+
+
+@pytest.mark.parametrize("lengths", [[3, 0, 2], [60, 1, 90]])
+def test_rows_behind_the_last_request(lengths):
+    """Padded queries: the requests' rows are what they are without; tables and
+    offsets of other types and strides."""
+    rng = np.random.default_rng(34)
+    contexts = [300, 70, 95]
+    twin, tables, _ = decode_case(rng, contexts, (8, 2, 128, 16, "paired"), "fp8", "bf16")
+    rows = sum(lengths)
+    query = query_of(rng, rows + 40, 8, 128, "bf16")
+    cu_q = np.cumsum([0] + lengths).tolist()
+    cu_k = np.cumsum([0] + contexts).tolist()
+    wide = torch.full((3, 2 * len(tables[0])), -1, dtype=torch.int64, device="cuda")
+    wide[:, ::2] = ints(tables)
+    got = hip_quantized_prefill(query, *twin.tensors, torch.tensor(cu_q, device="cuda"),
+                                torch.tensor(cu_k, device="cuda"), wide[:, ::2],
+                                max_seqlen_q=max(lengths))
+    check_attention(got[:rows], query[:rows], twin, tables, contexts, cu_q, 128 ** -0.5,
+                    VARLEN["bf16"])
+    got = hip_quantized_decode(query[:3], *twin.tensors, wide[:, ::2],
+                               torch.tensor(contexts, device="cuda"))
+    check_attention(got, query[:3], twin, tables, contexts, [0, 1, 2, 3], 128 ** -0.5,
+                    DECODE["bf16"])

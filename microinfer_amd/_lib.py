@@ -219,6 +219,10 @@ def stream_handle(device: torch.device) -> int:
         torch.cuda.current_device() if index is None else index)
 
 
+# The same two for a device's index, where a call's own time counts.
+raw_stream = torch._C._cuda_getCurrentRawStream
+raw_device = torch._C._cuda_getDevice
+
 _SAME_DEVICE = contextlib.nullcontext()
 
 

@@ -23,10 +23,10 @@ MAX_SEQS = 4096
 _FLOAT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
-def _call_place(device: torch.device) -> tuple:
-    """What calls that run one after the other have in common: thread, stream and
-    the capture that they are in, if any."""
-    stream, capture = _lib.stream_handle(device), 0
+def _call_place(stream: int) -> tuple:
+    """What calls that run one after the other have in common: thread, stream (the
+    current one) and the capture that they are in, if any."""
+    capture = 0
     if torch.cuda.is_current_stream_capturing():
         number = ctypes.c_uint64()
         _lib.check(_lib.load().mi_stream_capture_id(stream, ctypes.addressof(number)),
@@ -39,28 +39,26 @@ def _call_place(device: torch.device) -> tuple:
 class QuantizedDecodePlan:
     """One step's work (``quantized_decode_plan``), for calls of its sizes."""
 
-    buffer: torch.Tensor
-    counters: torch.Tensor  # zero, for calls in the place that made the plan
+    buffer: torch.Tensor  # the plan, and a workspace for where it was made
     sizes: tuple  # sequences, Hq, Hkv, head_dim, dtype, block size, table width
-    place: tuple
     bytes: int
     workspace_bytes: int
-    _workspaces: dict = field(default_factory=dict, repr=False, compare=False)
+    _workspaces: dict = field(repr=False, compare=False)  # place -> addresses, memory
 
-    def workspace(self, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
-        """Partials and counters of a call from here: its thread's and stream's
-        own, a call's own where a graph holds it but not the plan."""
-        place = _call_place(device)
+    def workspace(self, stream: int) -> tuple:
+        """Addresses of the partials and counters of a call from here (then what
+        keeps them): its thread's and stream's own, a call's own where a graph
+        holds it but not the plan."""
+        place = _call_place(stream)
         have = self._workspaces.get(place)
         if have is None:
+            device = self.buffer.device
             partials = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
-            if place == self.place:
-                have = partials, self.counters
-            else:
-                have = partials, torch.zeros_like(self.counters)
-                if place[2]:
-                    return have
-            self._workspaces[place] = have
+            counters = torch.zeros(self.sizes[0] * self.sizes[2], dtype=torch.int32,
+                                   device=device)
+            have = partials.data_ptr(), counters.data_ptr(), partials, counters
+            if not place[2]:
+                self._workspaces[place] = have
         return have
 
 
@@ -86,18 +84,23 @@ def quantized_decode_plan(context_lens: torch.Tensor, *, num_q_heads: int, num_k
     lib = _lib.load()
     with _lib.on_device(device):
         nbytes = lib.mi_quant_decode_plan_bytes(num_seqs, num_kv_heads)
-        buffer = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        counters = torch.empty(num_seqs * num_kv_heads, dtype=torch.int32, device=device)
+        partial_bytes = lib.mi_quant_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads,
+                                                            head_dim)
+        # One allocation: plan, partials, counters.
+        partials = -(-nbytes // 256) * 256
+        counters = partials + -(-partial_bytes // 256) * 256
+        buffer = torch.empty(counters + 4 * num_seqs * num_kv_heads, dtype=torch.uint8,
+                             device=device)
+        at, stream = buffer.data_ptr(), _lib.stream_handle(device)
         status = lib.mi_quant_decode_plan(
             context_lens.data_ptr(), num_seqs, num_q_heads, num_kv_heads, head_dim, block_size,
-            block_table_width, _lib.DTYPE_CODES[dtype], buffer.data_ptr(), nbytes,
-            counters.data_ptr(), _lib.stream_handle(device))
+            block_table_width, _lib.DTYPE_CODES[dtype], at, nbytes, at + counters, stream)
         _lib.check(status, "mi_quant_decode_plan")
-        place = _call_place(device)
+        place = _call_place(stream)
     return QuantizedDecodePlan(
-        buffer, counters, (num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size,
-                           block_table_width), place, nbytes,
-        lib.mi_quant_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim))
+        buffer, (num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, block_size,
+                 block_table_width), nbytes, partial_bytes,
+        {place: (at + partials, at + counters)})
 
 
 def _check_query(query: torch.Tensor, key_cache: torch.Tensor, device: int, rows: str):
@@ -136,6 +139,10 @@ def hip_quantized_decode(query: torch.Tensor, key_cache: torch.Tensor,
     ((num_seqs, num_q_heads, head_dim),
      (num_blocks, block_size, num_kv_heads, _)) = _check_query(query, key_cache, device,
                                                                "requests")
+    if device != _lib.raw_device():
+        with torch.cuda.device(device):
+            return hip_quantized_decode(query, key_cache, value_cache, key_scales, value_scales,
+                                        block_tables, context_lens, scale=scale, plan=plan)
     if block_tables.ndim != 2 or block_tables.shape[0] != num_seqs:
         raise ValueError("block_tables must have one row per request")
     if context_lens.numel() != num_seqs:
@@ -157,17 +164,16 @@ def hip_quantized_decode(query: torch.Tensor, key_cache: torch.Tensor,
     out = query.new_empty((num_seqs, num_q_heads, head_dim))
     if num_seqs == 0:
         return out
-    strides = query.stride()
-    with _lib.on_device(query.device):
-        partials, counters = plan.workspace(query.device)
-        status = _lib.load().mi_quant_decode(
-            query.data_ptr(), strides[0], strides[1], *cache, tables.data_ptr(), width, width,
-            plan.buffer.data_ptr(), plan.bytes, out.data_ptr(), num_q_heads * head_dim, head_dim,
-            partials.data_ptr(), plan.workspace_bytes, counters.data_ptr(), num_seqs,
-            num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
-            head_dim ** -0.5 if scale is None else float(scale), _lib.DTYPE_CODES[dtype], code,
-            _lib.stream_handle(query.device))
-    _lib.check(status, "mi_quant_decode")
+    strides, stream = query.stride(), _lib.raw_stream(device)
+    workspace = plan.workspace(stream)
+    status = _lib.load().mi_quant_decode(
+        query.data_ptr(), strides[0], strides[1], *cache, tables.data_ptr(), width, width,
+        plan.buffer.data_ptr(), plan.bytes, out.data_ptr(), num_q_heads * head_dim, head_dim,
+        workspace[0], plan.workspace_bytes, workspace[1], num_seqs, num_q_heads, num_kv_heads,
+        head_dim, block_size, num_blocks, head_dim ** -0.5 if scale is None else float(scale),
+        _lib.DTYPE_CODES[dtype], code, stream)
+    if status:
+        _lib.check(status, "mi_quant_decode")
     return out
 
 
@@ -182,14 +188,15 @@ class QuantizedPrefillPlan:
     workspace_bytes: int
     _workspaces: dict = field(default_factory=dict, repr=False, compare=False)
 
-    def workspace(self, device: torch.device) -> torch.Tensor:
+    def workspace(self, stream: int) -> torch.Tensor:
         """The plan with room for the partials of a call from here: its
         thread's and stream's own, a call's own where a graph holds it but not
         the plan."""
-        place = _call_place(device)
+        place = _call_place(stream)
         have = self._workspaces.get(place)
         if have is None:
-            have = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=device)
+            have = torch.empty(self.workspace_bytes, dtype=torch.uint8,
+                               device=self.cu_seqlens_q.device)
             tokens, requests, *sizes = self.sizes
             status = _lib.load().mi_quant_prefill_plan(
                 self.cu_seqlens_q.data_ptr(), self.cu_seqlens_k.data_ptr(), tokens, requests,
@@ -232,7 +239,7 @@ def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tenso
                                 (num_tokens, requests, *sizes, block_table_width), longest,
                                 nbytes)
     with _lib.on_device(device):
-        plan.workspace(device)
+        plan.workspace(_lib.stream_handle(device))
     return plan
 
 
@@ -254,6 +261,11 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
                                                 value_scales, "hip_quantized_prefill")
     ((num_tokens, num_q_heads, head_dim),
      (num_blocks, block_size, num_kv_heads, _)) = _check_query(query, key_cache, device, "tokens")
+    if device != _lib.raw_device():
+        with torch.cuda.device(device):
+            return hip_quantized_prefill(query, key_cache, value_cache, key_scales, value_scales,
+                                         cu_seqlens_q, cu_seqlens_k, block_tables,
+                                         max_seqlen_q=max_seqlen_q, scale=scale, plan=plan)
     if block_tables.ndim != 2:
         raise ValueError("block_tables must have one row per request")
     num_requests, width = block_tables.shape
@@ -285,17 +297,18 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
             cu_q, cu_k, num_tokens=num_tokens, num_q_heads=num_q_heads,
             num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=query.dtype,
             block_size=block_size, block_table_width=width, max_seqlen_q=max_seqlen_q)
-    strides = query.stride()
-    with _lib.on_device(query.device):
-        workspace, nbytes = None, 0
-        if plan is not None:
-            workspace, nbytes = plan.workspace(query.device).data_ptr(), plan.workspace_bytes
-            longest = plan.max_seqlen_q
-        status = _lib.load().mi_quant_prefill(
-            query.data_ptr(), strides[0], strides[1], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
-            tables.data_ptr(), width, width, out.data_ptr(), num_q_heads * head_dim, head_dim,
-            workspace, nbytes, num_tokens, num_requests, longest, num_q_heads, num_kv_heads,
-            head_dim, block_size, num_blocks, head_dim ** -0.5 if scale is None else float(scale),
-            _lib.DTYPE_CODES[query.dtype], code, _lib.stream_handle(query.device))
-    _lib.check(status, "mi_quant_prefill")
+    strides, stream = query.stride(), _lib.raw_stream(device)
+    workspace, nbytes = None, 0
+    if plan is not None:
+        workspace, nbytes = plan.workspace(stream), plan.workspace_bytes
+        longest = plan.max_seqlen_q
+    status = _lib.load().mi_quant_prefill(
+        query.data_ptr(), strides[0], strides[1], *cache, cu_q.data_ptr(), cu_k.data_ptr(),
+        tables.data_ptr(), width, width, out.data_ptr(), num_q_heads * head_dim, head_dim,
+        None if workspace is None else workspace.data_ptr(), nbytes, num_tokens, num_requests,
+        longest, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+        head_dim ** -0.5 if scale is None else float(scale), _lib.DTYPE_CODES[query.dtype], code,
+        stream)
+    if status:
+        _lib.check(status, "mi_quant_prefill")
     return out

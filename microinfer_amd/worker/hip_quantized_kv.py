@@ -169,6 +169,10 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
         raise ValueError("8-bit caches are written in blocks of at most 1024 tokens")
     if tokens == 0:
         return
+    if device != _lib.raw_device():
+        with torch.cuda.device(device):
+            return quantized_append(key_cache, value_cache, key_scales, value_scales, slots,
+                                    keys, values, plan=plan)
     if plan is None:
         plan = quantized_append_plan(slots, block_size=block_size, num_blocks=num_blocks)
     elif not isinstance(plan, QuantizedAppendPlan) or plan.sizes != (tokens, block_size,
@@ -178,14 +182,14 @@ def quantized_append(key_cache: torch.Tensor, value_cache: torch.Tensor,
         raise ValueError("plan must be on the cache device")
     keys, values = whole_vectors(keys), whole_vectors(values)
     k_strides, v_strides = keys.stride(), values.stride()
-    with _lib.on_device(key_cache.device):
-        status = _lib.load().mi_quant_append(
-            keys.data_ptr(), k_strides[0], k_strides[1], values.data_ptr(), v_strides[0],
-            v_strides[1], *cache, slots.data_ptr(), slots.dtype == torch.int64,
-            None if plan.buffer is None else plan.buffer.data_ptr(), plan.bytes, tokens,
-            num_kv_heads, head_dim, block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
-            _lib.stream_handle(key_cache.device))
-    _lib.check(status, "mi_quant_append")
+    status = _lib.load().mi_quant_append(
+        keys.data_ptr(), k_strides[0], k_strides[1], values.data_ptr(), v_strides[0],
+        v_strides[1], *cache, slots.data_ptr(), slots.dtype == torch.int64,
+        None if plan.buffer is None else plan.buffer.data_ptr(), plan.bytes, tokens,
+        num_kv_heads, head_dim, block_size, num_blocks, _lib.DTYPE_CODES[dtype], code,
+        _lib.raw_stream(device))
+    if status:
+        _lib.check(status, "mi_quant_append")
 
 
 def quantized_gather(key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -206,6 +210,10 @@ def quantized_gather(key_cache: torch.Tensor, value_cache: torch.Tensor,
         raise ValueError("block_tables and cu_seqlens_k must be on the cache device")
     if type(total_rows) is not int or total_rows < 0:
         raise ValueError("total_rows must be a nonnegative integer")
+    if device != _lib.raw_device():
+        with torch.cuda.device(device):
+            return quantized_gather(key_cache, value_cache, key_scales, value_scales,
+                                    block_tables, cu_seqlens_k, total_rows, dtype=dtype)
     num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
     keys = key_cache.new_empty((total_rows, num_kv_heads, head_dim), dtype=dtype)
     values = torch.empty_like(keys)
@@ -215,10 +223,10 @@ def quantized_gather(key_cache: torch.Tensor, value_cache: torch.Tensor,
         raise ValueError("rows without requests")
     tables, offsets = index32(block_tables), index32(cu_seqlens_k)
     requests, width = tables.shape
-    with _lib.on_device(key_cache.device):
-        status = _lib.load().mi_quant_gather(
-            *cache, tables.data_ptr(), width, width, offsets.data_ptr(), requests, total_rows,
-            keys.data_ptr(), values.data_ptr(), num_kv_heads, head_dim, block_size, num_blocks,
-            _lib.DTYPE_CODES[dtype], code, _lib.stream_handle(key_cache.device))
-    _lib.check(status, "mi_quant_gather")
+    status = _lib.load().mi_quant_gather(
+        *cache, tables.data_ptr(), width, width, offsets.data_ptr(), requests, total_rows,
+        keys.data_ptr(), values.data_ptr(), num_kv_heads, head_dim, block_size, num_blocks,
+        _lib.DTYPE_CODES[dtype], code, _lib.raw_stream(device))
+    if status:
+        _lib.check(status, "mi_quant_gather")
     return keys, values

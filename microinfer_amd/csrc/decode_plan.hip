@@ -13,6 +13,8 @@
 // freed until well into the launch, so a small item in the first round
 // leaves its CU idle, while small items at the end of the grid fill the
 // tail.
+#include <algorithm>
+
 #include "paged_attention.h"
 
 namespace mi {
@@ -81,16 +83,17 @@ __device__ __forceinline__ int step_part_blocks(int64_t total_blocks, int longes
   return max(max(least, 1), static_cast<int>((want + target - 1) / target));
 }
 
-__device__ __forceinline__ int whole_blocks(int num_seqs, int num_kv_heads, int lb) {
-  const int positions =
-      num_seqs * num_kv_heads >= kManyItems ? kWholePositionsMany : kWholePositions;
-  return max(positions >> lb, min(kWholeBlocks, kMaxMinPart >> lb));
+// Blocks up to which a sequence is one item; `positions`: what the caller says.
+int32_t whole_blocks(int32_t num_seqs, int32_t num_kv_heads, int32_t lb, int32_t positions) {
+  if (positions <= 0)
+    positions = num_seqs * num_kv_heads >= kManyItems ? kWholePositionsMany : kWholePositions;
+  return std::max(positions >> lb, std::min(kWholeBlocks, kMaxMinPart >> lb));
 }
 
 __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(
     const int32_t* __restrict__ context_lens, int num_seqs, int num_kv_heads, int block_size,
-    int lb, int width, int split_k, int target, int min_part, int max_min_part, int max_items,
-    PlanItem* __restrict__ plan, int32_t* __restrict__ counters, int num_counters) {
+    int lb, int width, int split_k, int target, int min_part, int max_min_part, int whole,
+    int max_items, PlanItem* __restrict__ plan, int32_t* __restrict__ counters, int num_counters) {
   __shared__ int s_ctx[kMaxPlanSeqs];
   __shared__ int s_order[kMaxPlanSeqs];  // rank -> sequence
   __shared__ int s_first[kMaxPlanSeqs];  // rank -> first item index
@@ -100,7 +103,6 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(
   __shared__ int s_total_blocks;
   __shared__ int s_total_items;
   __shared__ int s_longest;
-  const int whole = whole_blocks(num_seqs, num_kv_heads, lb);
   const int tid = threadIdx.x;
   const int max_ctx = width * block_size;
 
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(
 // 128-2048 8.6 -> 4.5.
 __global__ __launch_bounds__(kPlanThreads) void decode_plan_wave_kernel(
     const int32_t* __restrict__ context_lens, int num_seqs, int num_kv_heads, int block_size,
-    int lb, int width, int target, int min_part, int max_min_part, int max_items,
+    int lb, int width, int target, int min_part, int max_min_part, int whole, int max_items,
     PlanItem* __restrict__ plan,
     int32_t* __restrict__ counters, int num_counters) {
   const int tid = threadIdx.x;
@@ -257,7 +259,7 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_wave_kernel(
   for (int o = 1; o < kWave; o <<= 1) longest = max(longest, __shfl_xor(longest, o, kWave));
   const int pb = step_part_blocks(wave_sum_int(nb), longest, lb, num_kv_heads, target,
                                     min_part, max_min_part);
-  const int np = nb <= whole_blocks(num_seqs, num_kv_heads, lb) ? 1 : (nb + pb - 1) / pb;
+  const int np = nb <= whole ? 1 : (nb + pb - 1) / pb;
   const int last = nb - (np - 1) * pb;  // blocks of the last part, the odd one
   // Over the sequences ahead of this lane's (longer, or as long and earlier
   // in the batch): items and full parts; and the odd parts dispatched before this lane's
@@ -333,18 +335,21 @@ int64_t decode_plan_bytes(int32_t num_seqs, int32_t num_kv_heads, int32_t split_
 int32_t launch_decode_plan(const int32_t* context_lens, int32_t num_seqs, int32_t num_kv_heads,
                            int32_t block_size, int32_t block_table_width, int32_t split_k,
                            bool vector, PlanItem* plan, int32_t* counters, hipStream_t stream,
-                           int32_t min_part) {
+                           int32_t min_part, int32_t whole_positions) {
+  const int32_t whole =
+      whole_blocks(num_seqs, num_kv_heads, ilog2(block_size), whole_positions);
   const int32_t max_min_part = vector ? kMaxMinPartVector : kMaxMinPart;
   if (num_seqs <= kWave && split_k == 0) {
     decode_plan_wave_kernel<<<1, kPlanThreads, 0, stream>>>(
         context_lens, num_seqs, num_kv_heads, block_size, ilog2(block_size), block_table_width,
-        kTargetItems, min_part, max_min_part, decode_max_items(num_seqs, num_kv_heads, split_k), plan,
-        counters, counters != nullptr ? num_seqs * num_kv_heads : 0);
+        kTargetItems, min_part, max_min_part, whole,
+        decode_max_items(num_seqs, num_kv_heads, split_k), plan, counters,
+        counters != nullptr ? num_seqs * num_kv_heads : 0);
     return check_launch("decode plan");
   }
   decode_plan_kernel<<<1, kPlanThreads, 0, stream>>>(
       context_lens, num_seqs, num_kv_heads, block_size, ilog2(block_size), block_table_width,
-      split_k, kTargetItems, min_part, max_min_part,
+      split_k, kTargetItems, min_part, max_min_part, whole,
       decode_max_items(num_seqs, num_kv_heads, split_k), plan, counters,
       counters != nullptr ? num_seqs * num_kv_heads : 0);
   return check_launch("decode plan");

@@ -121,12 +121,12 @@ int64_t decode_plan_bytes(int32_t num_seqs, int32_t num_kv_heads, int32_t split_
 // counters (optional): the (sequence, KV head) arrival counters of the
 // decode launch that follows, zeroed by the plan kernel. vector: the launch
 // runs on the vector kernel, not on MFMA. min_part: positions that a part has at
-// least.
+// least; whole_positions: of a sequence that is not cut (0: the plan's own rule).
 constexpr int32_t kMinPartPositions = 64;
 int32_t launch_decode_plan(const int32_t* context_lens, int32_t num_seqs, int32_t num_kv_heads,
                            int32_t block_size, int32_t block_table_width, int32_t split_k,
                            bool vector, PlanItem* plan, int32_t* counters, hipStream_t stream,
-                           int32_t min_part = kMinPartPositions);
+                           int32_t min_part = kMinPartPositions, int32_t whole_positions = 0);
 
 constexpr int32_t kMaxPlanSeqs = 4096;
 

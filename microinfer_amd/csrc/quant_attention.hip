@@ -29,6 +29,17 @@ int32_t check_table(const std::string& fn, const int32_t* tables, int32_t width,
 // 192 / 256 41.3 / 38.2 / 40.3 / 40.7 us, four of up to 600 37.7 / 36.5 / 38.7 /
 // 39.5).
 constexpr int32_t kMinPart = 128;
+// A sequence of up to so many is not cut at all: eight waves have two tiles of 32
+// in flight each, so 384 cost one memory round trip, and a merge two more (one of
+// 300 tokens 34.7 us whole, 36.4 in parts; of 500 38.7 and 36.6). Where sequences
+// and KV heads alone make workgroups for much of the chip, eight times their
+// number: 12 of 500 44 whole, 48 in parts, 16 of 900-1100 59 and 62, 24 of 500
+// 48 and 55, 24 of 1000 61 and 67. More is worse where lengths differ (16 of 100 to
+// 2000 with up to 1024 / 1536 / 2048 62 / 67 / 70).
+int32_t whole_positions(int32_t num_seqs, int32_t num_kv_heads) {
+  return static_cast<int32_t>(
+      std::min<int64_t>(std::max<int64_t>(int64_t(8) * num_seqs * num_kv_heads, 384), 1536));
+}
 
 // Whether decode steps go to the MFMA kernel, cache alignment aside.
 bool decode_on_mfma(int32_t head_dim, int32_t group, int32_t block_size) {
@@ -146,11 +157,12 @@ extern "C" int32_t mi_quant_decode_plan(const int32_t* context_lens, int32_t num
   if (plan_bytes < decode_plan_bytes(num_seqs, num_kv_heads, 0) ||
       reinterpret_cast<uintptr_t>(plan) % 32 != 0)
     return fail(MI_ERR_WORKSPACE, fn + ": plan buffer too small or misaligned");
+  const bool mfma = decode_on_mfma(head_dim, num_q_heads / num_kv_heads, block_size);
   return launch_decode_plan(context_lens, num_seqs, num_kv_heads, block_size, block_table_width,
-                            0,
-                            !decode_on_mfma(head_dim, num_q_heads / num_kv_heads, block_size),
-                            static_cast<PlanItem*>(plan), counters,
-                            static_cast<hipStream_t>(stream), kMinPart);
+                            0, !mfma, static_cast<PlanItem*>(plan), counters,
+                            static_cast<hipStream_t>(stream),
+                            mfma ? kMinPart : kMinPartPositions,
+                            mfma ? whole_positions(num_seqs, num_kv_heads) : 0);
 }
 
 extern "C" int32_t mi_quant_decode(
@@ -263,7 +275,7 @@ extern "C" int32_t mi_quant_prefill_plan(const int32_t* cu_seqlens_q,
   if (st != MI_OK) return st;
   return launch_decode_plan(lens, num_requests, num_kv_heads, block_size, block_table_width, 0,
                             false, reinterpret_cast<PlanItem*>(ws + l.plan), nullptr, s,
-                            kMinPart);
+                            kMinPart, whole_positions(num_requests, num_kv_heads));
 }
 
 extern "C" int32_t mi_quant_prefill(

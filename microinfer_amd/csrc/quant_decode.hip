@@ -14,9 +14,9 @@
 //    (waited for by count, so a slot per wave stays in flight), the four scales
 //    of a tile with them.
 //  * Scores S^T[pos][row] = K . Q^T on v_mfma_f32_16x16x32_bf16, a half at a
-//    time; codes are widened to bf16 on their way from LDS, which loses nothing,
-//    and a query comes in as many bf16 parts as hold all of its bits (1 for
-//    bf16, 2 for f16, 3 for f32). The K scale meets the score in float32.
+//    time, or f16 for f16 queries; codes are widened to that on their way from LDS,
+//    which loses nothing. f32 queries come in three bf16 parts, which hold all of
+//    their bits. The K scale meets the score in float32.
 //  * The lanes that hold a tile's scores hold the weights that
 //    O^T[dim][row] += V^T . P^T wants from them, with V's bytes transposed on
 //    their way out of LDS (ds_read_b64_tr_b8). A weight times the V scale goes
@@ -29,7 +29,7 @@
 //
 // Four layers with their plan, captured, 8 KV heads of 128, us (the 16-bit cache's
 // kernel): 64 contexts of 128-2048 with 32 heads 125 (218; 480 MB, 3.8 TB/s), two of
-// 62000 212 (363; 4.7 TB/s), 24 of 300-2500 in f16 88 (129), four of 150-500 36 (38),
+// 62000 212 (363; 4.7 TB/s), 24 of 300-2500 in f16 82 (129), four of 150-500 36 (38),
 // where launches and one chain of loads (item, table, tile, merge) are the time.
 // Targets of 256, 384 and 512 items where the plan has 192 took 131, 133 and 141 us
 // for the first, 226, 255 and 246 for the second: their last round is partly empty.
@@ -52,6 +52,13 @@ __device__ __forceinline__ float max16(float v) {
   v = fmaxf(v, dpp_move<0x4E>(v));
   v = fmaxf(v, dpp_move<0x141>(v));
   return fmaxf(v, dpp_move<0x140>(v));
+}
+
+__device__ __forceinline__ f32x4_t mma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma(f16x8_t a, f16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // LDS: a half's rows are D bytes, 16-byte chunk c of row r at cell
@@ -78,6 +85,7 @@ __global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kern
     const QuantAttnArgs a) {
   using R = typename E::raw;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
+  using Query = QueryOperand<E>;
   constexpr int kParts = kQueryParts<E>;
   constexpr int kWeights = std::is_same<E, F32>::value ? 3 : 2;
   constexpr int kHalfBytes = kHalf * D;           // K or V of a half
@@ -194,7 +202,7 @@ __global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kern
   auto token_of = [&](int r) { return static_cast<int>(uint32_t(r) * a.group_inverse >> 24); };
   // Query operand of MFMA step 2 j + h: dims 16 (quad + 4 j) + 8 h .. + 7 of
   // row `col`, the order in which a lane reads K.
-  bf16x8_t qf[NC][kParts][kSteps];
+  Query qf[NC][kParts][kSteps];
   int limit[NC];  // the row sees positions below
   auto load_q = [&]() {
 #pragma unroll
@@ -214,7 +222,7 @@ __global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kern
       for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[s][i] = there ? x[s][i] : 0.f;
-        bf16x8_t part[kParts];
+        Query part[kParts];
         split8<kParts>(x[s], part);
 #pragma unroll
         for (int p = 0; p < kParts; ++p) qf[n][p][s] = part[p];
@@ -259,13 +267,13 @@ __global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kern
       for (int n = 0; n < NC; ++n) s[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        const bf16x8_t kf =
-            widen_operand<C>(kw[j][i / 2].w[2 * (i % 2)], kw[j][i / 2].w[2 * (i % 2) + 1]);
+        const Query kf =
+            widen<Query, C>(kw[j][i / 2].w[2 * (i % 2)], kw[j][i / 2].w[2 * (i % 2) + 1]);
 #pragma unroll
         for (int n = 0; n < NC; ++n)
 #pragma unroll
           for (int q = 0; q < kParts; ++q)
-            s[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[n][q][i], s[n], 0, 0, 0);
+            s[n] = mma(kf, qf[n][q][i], s[n]);
       }
       const float factor = scales[j] * a.scale_log2;
 #pragma unroll
@@ -309,7 +317,7 @@ __global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kern
       for (int n = 0; n < NC; ++n)
 #pragma unroll
         for (int q = 0; q < kWeights; ++q)
-          o[n][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n][q], o[n][db], 0, 0, 0);
+          o[n][db] = mma(vf, pf[n][q], o[n][db]);
     }
   };
 
@@ -594,8 +602,8 @@ int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, i
     return fail(MI_ERR_UNSUPPORTED, "quantized attention: too many rows for one launch");
   // Many workgroups: two a CU with a slot a wave, where they fit the registers
   // that leaves them (four layers of 128 sequences of 500 tokens 144 us, 173 with
-  // one of two slots; 64 of 1000 with heads of 64 77 / 80, float32 80 / 84. Heads
-  // of 128 spill: f16 64 of 1000 166 / 136, float32 376 / 141).
+  // one of two slots; 64 of 1000 with heads of 64 77 / 80, float32 80 / 84. In
+  // float32 heads of 128 spill: 64 of 1000 376 / 141).
   const bool narrow =
       static_cast<int64_t>(a.num_seqs) * a.c.heads * a.row_groups > device_cus();
   return with_types(dtype, code, [&](auto e, auto co) {
@@ -611,7 +619,7 @@ int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, i
       return wide ? go(quant_decode_kernel<E, C, 128, 2, 8, 2>)
                   : go(quant_decode_kernel<E, C, 64, 2, 8, 2>);
     if (narrow && !wide) return go(quant_decode_kernel<E, C, 64, 1, 8, 1>);
-    if constexpr (std::is_same<E, BF16>::value)
+    if constexpr (!std::is_same<E, F32>::value)
       if (narrow) return go(quant_decode_kernel<E, C, 128, 1, 8, 1>);
     return wide ? go(quant_decode_kernel<E, C, 128, 1, 8, 2>)
                 : go(quant_decode_kernel<E, C, 64, 1, 8, 2>);

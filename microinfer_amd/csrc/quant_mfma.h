@@ -1,5 +1,5 @@
 // Matrix-instruction pieces shared by the attention kernels over an 8-bit K/V
-// cache: codes widened to bf16 (exactly: both types have at most eight
+// cache: codes widened to bf16 or f16 (exactly: both types have at most eight
 // significant bits), float32 values split into bf16 parts.
 #pragma once
 
@@ -12,11 +12,15 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef int int2v_t __attribute__((ext_vector_type(2)));
 
-// bf16 parts of a query: all of its bits (8, 11 and 24 of them).
-template <typename E>
-constexpr int kQueryParts = std::is_same<E, BF16>::value ? 1 : std::is_same<E, F16>::value ? 2 : 3;
-
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// What a query meets the codes as, with all of its bits: 16-bit ones as they are,
+// f32 ones in three bf16 parts.
+template <typename E>
+using QueryOperand =
+    typename std::conditional<std::is_same<E, F16>::value, f16x8_t, bf16x8_t>::type;
+template <typename E>
+constexpr int kQueryParts = std::is_same<E, F32>::value ? 3 : 1;
 
 struct Word4 {
   uint32_t w[4];
@@ -70,6 +74,15 @@ __device__ __forceinline__ bf16x8_t widen_operand(uint32_t lo, uint32_t hi) {
   r.w[2] = widen_pair<C, false>(hi);
   r.w[3] = widen_pair<C, true>(hi);
   return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// Eight codes as an operand of either type.
+template <typename V, typename C>
+__device__ __forceinline__ V widen(uint32_t lo, uint32_t hi) {
+  if constexpr (std::is_same<V, bf16x8_t>::value)
+    return widen_operand<C>(lo, hi);
+  else
+    return widen_operand_f16<C>(lo, hi);
 }
 
 // x = part[0] + part[1] + ... in bf16 (or f16), each what the ones before

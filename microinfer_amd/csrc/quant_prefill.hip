@@ -80,25 +80,12 @@ __device__ __forceinline__ int swz_v(int key) {
   return D == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 }
 
-// How an element type's queries meet K (parts of the query), and its weights V.
+// How an element type's weights meet V, and in how many parts.
 template <typename E>
-struct Meets {
-  using Query = bf16x8_t;
-  using Weight = f16x8_t;
-  static constexpr int kQueries = 1, kWeights = 1;
-};
-template <>
-struct Meets<F16> {
-  using Query = f16x8_t;
-  using Weight = f16x8_t;
-  static constexpr int kQueries = 1, kWeights = 1;
-};
-template <>
-struct Meets<F32> {
-  using Query = bf16x8_t;
-  using Weight = bf16x8_t;
-  static constexpr int kQueries = 3, kWeights = 3;
-};
+using WeightOperand =
+    typename std::conditional<std::is_same<E, F32>::value, bf16x8_t, f16x8_t>::type;
+template <typename E>
+constexpr int kWeightParts = std::is_same<E, F32>::value ? 3 : 1;
 
 // What is known of 16 keys: the factor of their scores, the V scale and its
 // logarithm, whether they are in a block of the pool.
@@ -115,14 +102,6 @@ __device__ __forceinline__ f32x16_t mma(f16x8_t a, f16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-template <typename V, typename C>
-__device__ __forceinline__ V widen(uint32_t lo, uint32_t hi) {
-  if constexpr (std::is_same<V, bf16x8_t>::value)
-    return widen_operand<C>(lo, hi);
-  else
-    return widen_operand_f16<C>(lo, hi);
-}
-
 // Tiles of a step, by the registers of the query's parts.
 template <typename E, int D>
 constexpr int kTiles = std::is_same<E, F32>::value && D == 128 ? 1 : 2;
@@ -133,9 +112,9 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
   using R = typename E::raw;
   using ConstI32 = __attribute__((address_space(4))) const int32_t;
   using ConstF32 = __attribute__((address_space(4))) const float;
-  using Query = typename Meets<E>::Query;
-  using Weight = typename Meets<E>::Weight;
-  constexpr int kQueries = Meets<E>::kQueries, kWeights = Meets<E>::kWeights;
+  using Query = QueryOperand<E>;
+  using Weight = WeightOperand<E>;
+  constexpr int kQueries = kQueryParts<E>, kWeights = kWeightParts<E>;
   constexpr int NT = kTiles<E, D>;
   constexpr int kKeys = NT * kTile, kHalves = 2 * NT;
   constexpr int kAccFloats = D / 32 * 16;  // of a lane

@@ -50,8 +50,8 @@ bool decode_on_mfma(int32_t head_dim, int32_t group, int32_t block_size) {
 // Varlen calls of at most kFewRows rows of a request at a KV head, or kFewInAll of
 // all requests, are laid out and run like decode steps. Four layers of 32 query
 // and 8 KV heads of 128, us like that / as longer ones: a token on 16000
-// positions (one query head a KV head) 72 / 248, 8 tokens 122 / 249, 16 on 8000
-// 108 / 200, 32 on 8000 159 / 202, 64 on 8000 260 / 212; 16 requests of 4 tokens
+// positions (one query head a KV head) 72 / 248, 8 tokens 117 / 249, 16 on 8000
+// 105 / 200, 32 on 8000 154 / 202, 64 on 8000 260 / 212; 16 requests of 4 tokens
 // on 4000 155 / 200, 32 of 8 on 2000 160 / 193, 64 of 4 234 / 277, 64 of 8 295 /
 // 279, 8 of 16 on 4000 199 / 183, 32 of 16 on 2000 255 / 221.
 constexpr int32_t kFewRows = 32;

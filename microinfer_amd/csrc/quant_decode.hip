@@ -606,13 +606,16 @@ int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, i
   // that leaves them (four layers of 128 sequences of 500 tokens 144 us, 173 with
   // one of two slots; 64 of 1000 with heads of 64 77 / 80, float32 80 / 84. In
   // float32 heads of 128 spill: 64 of 1000 376 / 141).
-  const bool narrow =
-      static_cast<int64_t>(a.num_seqs) * a.c.heads * a.row_groups > device_cus();
+  // Four of four waves where there are so many: their starts and ends overlap (128
+  // sequences of 200 tokens 92 / 80 us, of 500 144 / 135, of 2000 403 / 412; at
+  // three a CU, 96 of 200-400 87 / 77, but of 100-2500 238 / 248).
+  const int64_t groups = static_cast<int64_t>(a.num_seqs) * a.c.heads * a.row_groups;
+  const bool narrow = groups > device_cus(), small = groups >= 4 * device_cus();
   return with_types(dtype, code, [&](auto e, auto co) {
     using E = decltype(e);
     using C = decltype(co);
-    auto go = [&](auto kernel) {
-      kernel<<<static_cast<uint32_t>(grid), kWave * 8, 0, stream>>>(a);
+    auto go = [&](auto kernel, int waves = 8) {
+      kernel<<<static_cast<uint32_t>(grid), kWave * waves, 0, stream>>>(a);
       return check_launch("quantized decode");
     };
     if (a.c.dim == 256) return go(quant_decode_kernel<E, C, 256, 1, 8, 1>);
@@ -620,9 +623,13 @@ int32_t launch_quant_decode_mfma(QuantAttnArgs a, int32_t rows, int32_t dtype, i
     if (rows > kCols)
       return wide ? go(quant_decode_kernel<E, C, 128, 2, 8, 2>)
                   : go(quant_decode_kernel<E, C, 64, 2, 8, 2>);
-    if (narrow && !wide) return go(quant_decode_kernel<E, C, 64, 1, 8, 1>);
+    if (narrow && !wide)
+      return small ? go(quant_decode_kernel<E, C, 64, 1, 4, 1>, 4)
+                   : go(quant_decode_kernel<E, C, 64, 1, 8, 1>);
     if constexpr (!std::is_same<E, F32>::value)
-      if (narrow) return go(quant_decode_kernel<E, C, 128, 1, 8, 1>);
+      if (narrow)
+        return small ? go(quant_decode_kernel<E, C, 128, 1, 4, 1>, 4)
+                     : go(quant_decode_kernel<E, C, 128, 1, 8, 1>);
     return wide ? go(quant_decode_kernel<E, C, 128, 1, 8, 2>)
                 : go(quant_decode_kernel<E, C, 64, 1, 8, 2>);
   });

@@ -601,6 +601,18 @@ def test_the_most_sequences():
                              torch.zeros(4097, 1, dtype=torch.int32, device="cuda"), ints(more))
 
 
+@pytest.mark.parametrize("shape,dtype", [
+    ((4, 2, 128, 16, "paired"), "bf16"), ((16, 2, 128, 16, "paired"), "f16"),
+    ((16, 2, 64, 16, "paired"), "f32"), ((32, 2, 64, 16, "head_major"), "bf16")])
+def test_many_short_sequences_and_a_few_long_ones(shape, dtype):
+    rng = np.random.default_rng(35)
+    contexts = [3000, 900] + [int(c) for c in rng.integers(0, 30, 600)] + [1500]
+    twin, tables, query = decode_case(rng, contexts, shape, "int8", dtype)
+    scale = 1 / math.sqrt(shape[2])
+    got = hip_quantized_decode(query, *twin.tensors, ints(tables), ints(contexts))
+    check_attention(got, query, twin, tables, contexts, list(range(604)), scale, DECODE[dtype])
+
+
 @pytest.mark.parametrize("lengths", [[3, 0, 2], [60, 1, 90]])
 def test_rows_behind_the_last_request(lengths):
     """Padded queries: the requests' rows are what they are without; tables and

@@ -55,6 +55,13 @@ constexpr int kBlockRows = kRows * kWaves;
 constexpr float kRescaleSlack = 15.f;
 // A row's largest weight lies between 2^kTopWeight and 2^kMostWeight.
 constexpr float kTopWeight = 10.f, kMostWeight = 15.f;
+// V of zeros has the scale 2^-126. Where a row has seen little else, mo lies that far
+// below the scores, and the factor 2^(m - mo) vs of another half, if only of keys that
+// the row does not see, would be infinite, which 0 times is NaN. So m stays within
+// kMostApart of mo, below the row's maximum by up to kMostAbove (l, a sum of so much
+// larger terms, is far from its range's end), and the factor below 2^kMostUp. Only V
+// beyond 2^62 of such a scale meets that last bound, in weights of less than 2^-111.
+constexpr float kMostApart = 64.f, kMostAbove = 80.f, kMostUp = 126.f;
 
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
@@ -323,9 +330,6 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
       wmax = fmaxf(wmax, x + hf[h].log_vs);
     }
     if (__ballot(smax > m + kRescaleSlack || wmax > mo + kMostWeight) != 0) {
-      const float mnew = fmaxf(m, fmaxf(smax, lane_xor32(smax, lane)));
-      l *= mnew == -INFINITY ? 1.f : fast_exp2(m - mnew);
-      m = mnew;
       const float monew = fmaxf(mo, fmaxf(wmax, lane_xor32(wmax, lane)) - kTopWeight);
       const float alpha = monew == -INFINITY ? 1.f : fast_exp2(mo - monew);
 #pragma unroll
@@ -333,6 +337,10 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
       mo = monew;
+      const float stop = fmaxf(smax, lane_xor32(smax, lane));
+      const float mnew = fmaxf(fmaxf(m, stop - kMostAbove), fminf(stop, mo + kMostApart));
+      l *= mnew == -INFINITY ? 1.f : fast_exp2(m - mnew);
+      m = mnew;
     }
     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
       for (int h = 0; h < 2; ++h) {
         const Half& x = hf[2 * n + h];
         // Without a reference all scales were 0 or NaN so far, and so it stays.
-        float up = fast_exp2(x.log_vs + (base - mo));
+        float up = fast_exp2(fminf(x.log_vs + (base - mo), kMostUp));
         up = mo > -INFINITY ? up : x.vs;
         up = x.ok ? up : 0.f;
         float weight[8];

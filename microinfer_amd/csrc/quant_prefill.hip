@@ -360,7 +360,8 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
       for (int h = 0; h < 2; ++h) {
         const Half& x = hf[2 * n + h];
         // Without a reference all scales were 0 or NaN so far, and so it stays.
-        float up = fast_exp2(fminf(x.log_vs + (base - mo), kMostUp));
+        const float rise = x.log_vs + (base - mo);
+        float up = fast_exp2(rise > kMostUp ? kMostUp : rise);  // NaN stays
         up = mo > -INFINITY ? up : x.vs;
         up = x.ok ? up : 0.f;
         float weight[8];

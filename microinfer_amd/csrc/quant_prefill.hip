@@ -100,6 +100,9 @@ struct alignas(16) Half {
   float factor, vs, log_vs;
   int ok;
 };
+// `ok` of a block whose K scale is NaN: its factor is a number, so that scores which
+// a row does not see stay -infinity, and the scores that it sees become NaN.
+constexpr int kOkNan = 2;
 constexpr int kInfo = 256;  // halves looked up, a ring of two parts
 
 __device__ __forceinline__ f32x16_t mma(bf16x8_t a, bf16x8_t b, f32x16_t c) {
@@ -195,11 +198,11 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
         at = blk * c.bs + (pos & (c.block_size - 1)) * c.ts;
         const int64_t s = blk * c.s_bs + head * c.s_hs;
         x.factor = c.ks[s] * scale_log2;
-        // Masked scores are -inf, which 0 would make NaN.
-        if (x.factor == 0.f) x.factor = 0x1p-126f;
+        x.ok = x.factor == x.factor ? 1 : kOkNan;
+        // Masked scores are -inf, which 0 or NaN would make NaN.
+        if (!(x.factor > 0.f)) x.factor = 0x1p-126f;
         x.vs = c.vs[s];
         x.log_vs = __builtin_amdgcn_logf(x.vs);
-        x.ok = 1;
       }
     }
     s_at[h % kInfo] = at;
@@ -308,15 +311,17 @@ __global__ __launch_bounds__(kThreads, 2) void quant_prefill_kernel(
       }
     int all = 1;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) all &= hf[h].ok;
+    for (int h = 0; h < kHalves; ++h) all &= hf[h].ok;  // not those of kOkNan
     if (t >= nint || !__builtin_amdgcn_readfirstlane(all)) {
       const int last = min(qpos, key_end - 1) - key0 - t * kKeys - half * 4;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[n][i] = 32 * n + i / 4 * 8 + i % 4 <= last && hf[2 * n + i / 8].ok ? s[n][i]
-                                                                               : -INFINITY;
+        for (int i = 0; i < 16; ++i) {
+          const int ok = hf[2 * n + i / 8].ok;
+          const float seen = ok == kOkNan ? NAN : s[n][i];
+          s[n][i] = 32 * n + i / 4 * 8 + i % 4 <= last && ok ? seen : -INFINITY;
+        }
     }
     // The references move where the step's scores lie too far above them.
     float smax = -INFINITY, wmax = -INFINITY;

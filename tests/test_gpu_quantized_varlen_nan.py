@@ -2,10 +2,11 @@
 reaches (more than 32 query rows a KV head, so that the kernel of long requests
 runs; the other kernels are tested with decode steps).
 
-A NaN in V makes NaN of the rows that see it, may do so to earlier rows of its
-request, and reaches no other. What lies behind a context, in unused blocks or
-outside the pool reaches no row. Rows that no NaN reaches are checked against
-float64 with the bounds of ``check_attention``.
+A NaN in K or V makes NaN of the rows that see it. One in V may do so to earlier
+rows of its request too; one in K does not, and none reaches another request. What
+lies behind a context, in unused blocks or outside the pool reaches no row. Rows
+that no NaN reaches are checked against float64 with the bounds of
+``check_attention``.
 """
 
 import numpy as np
@@ -13,6 +14,7 @@ import pytest
 import torch
 
 from microinfer_amd.layer.hip_quantized_attention import hip_quantized_prefill
+from microinfer_amd.worker.hip_quantized_kv import quantized_append
 from tests.quantized_support import DTYPES, Twin, check_attention, ints, tables_of
 
 pytestmark = pytest.mark.gpu
@@ -50,6 +52,35 @@ class Case:
         seen[self.cu_q[request] + first:self.cu_q[request + 1],
              head * share:(head + 1) * share] = True
         return seen
+
+
+@pytest.mark.parametrize("kind", ["fp8", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("request_,position", [(0, 70), (0, 33), (1, 64), (1, 15), (1, 88),
+                                               (2, 39)])
+def test_nan_in_k_reaches_the_rows_that_see_it(kind, dtype, dim, request_, position):
+    case = Case(kind, dtype, dim, position)
+    clean = case()
+    case.check(clean)
+    page = case.tables[request_][position // BLOCK]
+    held = [t.clone() for t in case.twin.tensors]
+    for what in ("scale", "code"):
+        if what == "code" and kind == "int8":
+            continue
+        if what == "scale":  # of the position's whole block
+            case.twin.layer.key_scales[page, 1] = float("nan")
+            seen = case.seeing(request_, position // BLOCK * BLOCK, 1)
+        else:
+            case.twin.layer.keys[page, position % BLOCK, 1, 3:4].view(torch.uint8).fill_(0x7f)
+            seen = case.seeing(request_, position, 1)
+        got = case()
+        assert got[seen].isnan().all()
+        case.check(torch.where(seen[..., None], clean, got))
+        for t, was in zip(case.twin.tensors, held):
+            if t.dtype != torch.float32:
+                t, was = t.view(torch.uint8), was.view(torch.uint8)
+            t.copy_(was)
 
 
 @pytest.mark.parametrize("kind", ["fp8", "int8"])
@@ -99,3 +130,33 @@ def test_what_no_row_sees_may_be_nan(kind, dtype, dim):
     case.tables[1][2] = twin.k.shape[0] + 5
     case.tables[0][0] = -7
     case.check(case())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_written_values_that_are_not_finite(dtype, dim):
+    """As appends write them: an infinite K value in an int8 cache makes its
+    block's scale NaN, and the rows ahead of the block do not see it."""
+    rng = np.random.default_rng(dim)
+    rows = 96
+    twin = Twin(rows // BLOCK, BLOCK, HKV, dim, "int8")
+    keys, values = (torch.from_numpy(rng.standard_normal((rows, HKV, dim))).bfloat16().cuda()
+                    for _ in range(2))
+    table = rng.permutation(rows // BLOCK).tolist()
+    slots = [table[p // BLOCK] * BLOCK + p % BLOCK for p in range(rows)]
+    query = torch.from_numpy(rng.standard_normal((rows, HQ, dim))).to(DTYPES[dtype]).cuda()
+
+    def run():
+        return hip_quantized_prefill(query, *twin.tensors, ints([0, rows]), ints([0, rows]),
+                                     ints([table]), max_seqlen_q=rows)
+
+    quantized_append(*twin.tensors, ints(slots), keys, values)
+    twin.expect(slots, keys, values)
+    clean = run()
+    keys[70, 0, 4] = float("inf")
+    quantized_append(*twin.tensors, ints(slots), keys, values)
+    got = run()
+    assert got[64:, :4].isnan().all()
+    assert not got[:64].isnan().any() and not got[:, 4:].isnan().any()
+    got[64:, :4] = clean[64:, :4]
+    check_attention(got, query, twin, [table], [rows], [0, rows], dim ** -0.5, VARLEN[dtype])

@@ -133,7 +133,8 @@ int32_t mi_quant_decode(const void* query, int64_t q_token_stride, int64_t q_hea
  * Varlen attention: mi_paged_prefill over an 8-bit cache. Request r's query
  * rows are cu_seqlens_q[r] .. cu_seqlens_q[r + 1], its context
  * cu_seqlens_k[r + 1] - cu_seqlens_k[r] positions, the mask causal and
- * bottom-right aligned. Rows that see no position give zeros. max_seqlen_q
+ * bottom-right aligned. Rows that see no position give zeros; rows of no request
+ * (behind the last, or ahead of the first) stay as they were. max_seqlen_q
  * bounds the query rows of any request: rows past it may stay unwritten. A NaN
  * makes NaN of the rows that see it; one in V may also do so to earlier rows of
  * its own request (0 times it is NaN), but to none of another, and what lies

@@ -53,8 +53,8 @@ __global__ __launch_bounds__(kThreads) void quant_vector_kernel(const QuantAttnA
     begin = 0;
     end = static_cast<int>(
         max(int64_t(0), min(seen, static_cast<int64_t>(a.t_width) * c.block_size)));
-    // Rows outside every request see nothing.
-    if (row < a.cu_q[lo] || row >= a.cu_q[lo + 1]) end = 0;
+    // Rows of no request stay as they were, as on the MFMA kernels (uniform).
+    if (row < a.cu_q[lo] || row >= a.cu_q[lo + 1]) return;
   } else {
     it = a.plan[w];
     if (it.seq < 0 || it.seq >= a.num_seqs || it.nparts < 1 || it.part < 0 ||

@@ -255,7 +255,9 @@ def hip_quantized_prefill(query: torch.Tensor, key_cache: torch.Tensor,
     context ``cu_seqlens_k[r+1] - cu_seqlens_k[r]`` (it includes the new rows,
     which the caller appended first). ``max_seqlen_q`` bounds the query rows of
     any request. ``plan``: of ``quantized_prefill_plan`` for these lengths and
-    sizes; without it the call makes its own. Rows that see nothing give zeros.
+    sizes; without it the call makes its own. Rows that see nothing give zeros;
+    rows of no request (behind the last one) are not computed: theirs is
+    uninitialised memory.
     """
     cache, code, device = check_quantized_cache(key_cache, value_cache, key_scales,
                                                 value_scales, "hip_quantized_prefill")

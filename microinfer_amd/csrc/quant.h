@@ -108,6 +108,13 @@ struct QuantAttnArgs {
   float scale_log2;
 };
 
+// Whether an item names a sequence and partials that are there: any memory may be
+// taken for a plan (one that a graph has not replayed yet), so no sum that can overflow.
+__device__ __forceinline__ bool item_fits(const PlanItem& it, const QuantAttnArgs& a) {
+  return it.seq >= 0 && it.seq < a.num_seqs && it.part >= 0 && it.part < it.nparts &&
+         it.first_item >= 0 && it.nparts <= a.max_items - it.first_item;
+}
+
 // Host side: checks of a cache's description. Returns an MI_* status.
 int32_t check_quant_cache(const std::string& fn, const void* key_cache, const void* value_cache,
                           int64_t block_stride, int64_t token_stride, int64_t head_stride,

@@ -120,14 +120,12 @@ __global__ __launch_bounds__(kWave * NW, waves_of(D, NS)) void quant_decode_kern
   typedef int32_t int8v __attribute__((ext_vector_type(8)));
   using ConstItem = __attribute__((address_space(4))) const int8v;
   const PlanItem it = __builtin_bit_cast(PlanItem, ((ConstItem*)(a.plan))[w]);
-  if (it.seq < 0 || it.seq >= a.num_seqs || it.nparts < 1 || it.part < 0 ||
-      it.part >= it.nparts || it.first_item < 0 || it.first_item + it.nparts > a.max_items)
-    return;  // unused slot (uniform across the workgroup)
+  if (!item_fits(it, a)) return;  // unused slot (uniform across the workgroup)
   const int seq = it.seq;
   const int lb = c.log2_block;
   const int ctx = min(max(it.ctx, 0), a.t_width << lb);
-  const int blk_begin = max(it.blk_begin, 0);
-  const int blk_end = min(it.blk_end, a.t_width);
+  const int blk_begin = min(max(it.blk_begin, 0), a.t_width);
+  const int blk_end = min(max(it.blk_end, 0), a.t_width);
   const int nparts = it.nparts;
   // The rows: of a decode step, or of a request's tokens, which see less of its
   // end the earlier they are.

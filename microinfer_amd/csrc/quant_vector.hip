@@ -57,13 +57,11 @@ __global__ __launch_bounds__(kThreads) void quant_vector_kernel(const QuantAttnA
     if (row < a.cu_q[lo] || row >= a.cu_q[lo + 1]) return;
   } else {
     it = a.plan[w];
-    if (it.seq < 0 || it.seq >= a.num_seqs || it.nparts < 1 || it.part < 0 ||
-        it.part >= it.nparts || it.first_item < 0 || it.first_item + it.nparts > a.max_items)
-      return;  // unused slot
+    if (!item_fits(it, a)) return;  // unused slot
     seq = row = it.seq;
     const int most = a.t_width << c.log2_block;
-    begin = max(it.blk_begin, 0) << c.log2_block;
-    end = min(min(max(it.ctx, 0), most), min(it.blk_end, a.t_width) << c.log2_block);
+    begin = min(max(it.blk_begin, 0), a.t_width) << c.log2_block;
+    end = min(min(max(it.ctx, 0), most), min(max(it.blk_end, 0), a.t_width) << c.log2_block);
   }
 
   float q[kHeads][8], acc[kHeads][8], m[kHeads], l[kHeads];

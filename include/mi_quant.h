@@ -70,7 +70,8 @@ int32_t mi_quant_append(const void* keys, int64_t key_token_stride, int64_t key_
 
 /*
  * The blocks that these slots write to, and their rows, found on the device.
- * plan: mi_quant_append_plan_bytes() bytes, 8-byte aligned, no initialisation.
+ * plan: mi_quant_append_plan_bytes() bytes (4 for each position of the pool, and
+ * 4 block_size + 8 for each token), 8-byte aligned, no initialisation.
  */
 int64_t mi_quant_append_plan_bytes(int32_t num_tokens, int32_t block_size, int32_t num_blocks);
 int32_t mi_quant_append_plan(const void* slots, int32_t slots_are_int64, int32_t num_tokens,
@@ -145,7 +146,15 @@ int32_t mi_quant_decode(const void* query, int64_t q_token_stride, int64_t q_hea
  * mi_quant_prefill_plan has laid out the step, on the device, from the
  * cu_seqlens, for the same sizes, max_seqlen_q and table width; the plan serves
  * all layers, one call after the other. Calls that may run concurrently need
- * workspaces of their own.
+ * workspaces of their own. Long requests take room for 1024 parts of row blocks:
+ * 71 MB with heads of 128, 38 MB with heads of 64, however few the tokens.
+ *
+ * Where it is 0, calls run without a plan or workspace on the vector kernel, 28 to
+ * 46 times slower than the MFMA kernel where both were measured: other head sizes
+ * and blocks of less than 16, groups of more than 128 query heads a KV head, heads of
+ * 256 with more than 256 rows a request (4096 in all), and steps of more than 2048
+ * requests or 4096 row blocks, of which a step has num_tokens / (128 / group) +
+ * num_requests (65000 tokens of groups of 8, 16000 of groups of 32): split those.
  */
 int64_t mi_quant_prefill_workspace_bytes(int32_t num_tokens, int32_t num_requests,
                                          int32_t max_seqlen_q, int32_t num_q_heads,

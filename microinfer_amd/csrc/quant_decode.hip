@@ -28,11 +28,12 @@
 //  * Waves are joined through LDS, partitions by their last arrival, in order.
 //
 // Four layers with their plan, captured, 8 KV heads of 128, us (the 16-bit cache's
-// kernel): 64 contexts of 128-2048 with 32 heads 125 (218; 480 MB, 3.8 TB/s), two of
-// 62000 212 (363; 4.7 TB/s), 24 of 300-2500 in f16 82 (129), four of 150-500 36 (38),
+// kernel): 64 contexts of 128-2048 with 32 heads 129 (218; 480 MB, 3.7 TB/s), two of
+// 62000 217 (363; 4.6 TB/s), 24 of 300-2500 in f16 82 (129), four of 150-500 36 (37),
 // where launches and one chain of loads (item, table, tile, merge) are the time.
-// Targets of 256, 384 and 512 items where the plan has 192 took 131, 133 and 141 us
-// for the first, 226, 255 and 246 for the second: their last round is partly empty.
+// Passes among others take 125 us of the first and 212 of the second: a replayed
+// graph's start is 4 us. Targets of 256, 384 and 512 items where the plan has 192 took
+// 131, 133 and 141 us there, 226, 255 and 246: their last round is partly empty.
 #include <algorithm>
 #include <climits>
 

@@ -27,15 +27,16 @@
 //    what f16 cannot hold is 2^-35 of the largest. Against float64 a bf16 output is
 //    off by its own rounding (2^-9.2 root mean square), an f16 one by 2^-11.9, of
 //    which its own makes 2^-12.2: a second part would take that away and a fifth
-//    more time (six prompts 468 us for four layers, 386 without). f32 queries have
-//    three parts in bf16.
+//    more time (six prompts 468 us for four layers, 386 without). The 16-bit cache's
+//    kernel, whose weights are of the query's type, is off by 2^-8.8 and 2^-11.8
+//    over the same values. f32 queries have three parts in bf16.
 //  * Row blocks whose keys are split publish theirs; the last arrival merges
 //    them in order.
 //
 // Four layers with their plan, captured, us (the 16-bit cache's kernel): 512 tokens
-// on 7700, 32 / 8 heads of 128, bf16 389 (426; 686 TFLOP/s, 58 % of a large library
-// product), six prompts of 40-1400 on up to 2000, 16 / 8 heads, f16 379 (307; 558
-// TFLOP/s), 300 tokens on 2000 in f32 218 (394), 500 on 4000 with heads of 64 168.
+// on 7700, 32 / 8 heads of 128, bf16 392 (426; 681 TFLOP/s, 58 % of a large library
+// product), six prompts of 40-1400 on up to 2000, 16 / 8 heads, f16 380 (307; 557
+// TFLOP/s), 300 tokens on 2000 in f32 219 (394), 500 on 4000 with heads of 64 168.
 // Not faster: scores of the next step beside the softmax, staging beside the
 // scores, LDS reads issued in fixed groups ahead of their products, wave
 // priorities, three workgroups a CU with steps of 32 keys.

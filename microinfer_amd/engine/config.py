@@ -59,8 +59,10 @@ class EngineConfig:
     # prompts) read them together; captures a second graph per bucket.
     shared_prefix_decode: bool = False
     # "fp8" or "int8": the K/V cache in 8 bits, half of a 16-bit one's memory,
-    # with a scale for each block and KV head. Sequences then read shared blocks
-    # each for itself.
+    # with a scale for each block and KV head. Decode steps get faster; chunks of
+    # prompts behind cached tokens may get slower (half precision, uneven lengths:
+    # by a quarter). Sequences read shared blocks each for itself:
+    # ``shared_prefix_decode`` has no effect.
     kv_cache_dtype: str | None = None
 
     def __post_init__(self):

@@ -215,9 +215,12 @@ def quantized_prefill_plan(cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tenso
                            max_seqlen_q: int | None = None) -> QuantizedPrefillPlan | None:
     """The plan of one step's ``hip_quantized_prefill`` calls (shared by its
     layers), from the cu_seqlens on the device (capture-safe). None: calls of
-    these sizes run without one. ``max_seqlen_q`` bounds the new tokens of any
+    these sizes run without one, row by row and many times slower (head sizes other
+    than 64 and 128, blocks of less than 16, the largest groups and steps:
+    ``mi_quant.h`` has the limits). ``max_seqlen_q`` bounds the new tokens of any
     request (``num_tokens`` by default): where it is small, the step is laid out
-    for few rows a request."""
+    for few rows a request. Plans of longer requests hold 38 MB (heads of 64) or
+    71 MB (128) of partials."""
     _lib.require_device(cu_seqlens_q, cu_seqlens_k, what="quantized_prefill_plan")
     if num_kv_heads <= 0 or num_q_heads <= 0 or num_q_heads % num_kv_heads:
         raise ValueError("Hq must be divisible by Hkv")

@@ -112,7 +112,7 @@ class QuantizedAppendPlan:
 def quantized_append_plan(slot_mapping: torch.Tensor, *, block_size: int,
                           num_blocks: int) -> QuantizedAppendPlan:
     """The plan of ``quantized_append`` calls with these slots, made on the
-    device (capture-safe)."""
+    device (capture-safe). It holds 4 bytes for each position of the pool."""
     slots = _slots(slot_mapping)
     if not slots.is_cuda:
         _lib.require_device(slots, what="quantized_append_plan")

@@ -85,3 +85,25 @@ def test_a_block_of_zeros_that_leads(kind, dtype, dim, lead):
     query = torch.from_numpy(query).to(DTYPES[dtype]).cuda()
     got = attend(query, twin, table, context)
     check_attention(got, query, twin, [table], [context], [0, new], scale, VARLEN[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lead,first", [(60, 0), (118, 896), (118, 1744), (200, 400)])
+def test_blocks_of_zeros_that_lead_in_one_part(dtype, dim, lead, first):
+    """The same among keys that are split, whose parts are merged: 60 rows on 1800."""
+    rng = np.random.default_rng(lead + dim + first)
+    hq, hkv = HEADS
+    context, new = 1800, 60
+    keys, values = 0.05 * rng.standard_normal((2, context, hkv, dim))
+    keys[:, :, 0] = -4
+    keys[first:first + 32, :, 0] = 4
+    values *= 40
+    values[first:first + 32] = 0
+    twin, table = written(rng, keys, values, "fp8", 16)
+    query = 0.05 * rng.standard_normal((new, hq, dim))
+    scale = dim ** -0.5
+    query[:, :, 0] = lead * np.log(2) / (8 * scale)
+    query = torch.from_numpy(query).to(DTYPES[dtype]).cuda()
+    got = attend(query, twin, table, context)
+    check_attention(got, query, twin, [table], [context], [0, new], scale, VARLEN[dtype])
